@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("EINSPARSE_LIB", os.path.join(HERE, "libeinsparse.so"))
 
 ES_OK, ES_ERR_INVALID, ES_ERR_INDEX, ES_ERR_WORKSPACE, ES_ERR_CUDA, ES_ERR_UNSUPPORTED, ES_ERR_TIMEOUT = range(7)
-ES_F32, ES_BF16, ES_F64, ES_I32, ES_I64 = range(5)
+ES_F32, ES_BF16, ES_F64, ES_I32, ES_I64, ES_F16 = range(6)
 ES_PREC_AUTO, ES_PREC_EXACT, ES_PREC_TC = range(3)
 ES_DUP_LAST, ES_DUP_SUM = range(2)
 
@@ -78,6 +78,23 @@ SIGNATURES = {
     "es_segsum_plan": (c_int, [c_vp, c_i64, c_int, c_i64p, c_vp, c_sz, c_vp, c_vp, c_vp]),
     "es_segsum_fill": (c_int, [c_vp, c_int, c_i64, c_i64, c_int, c_i64p, c_vp, c_sz, c_i64, c_vp, c_vp, c_int, c_vp]),
     "es_segsum_groups": (c_int, [c_i64, c_int, c_i64p, c_vp, c_sz, c_i64, c_vp, c_vp, c_vp]),
+    "es_route_experts": (c_int, [c_vp, c_int, c_i64, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp]),
+    "es_route_experts_grad": (c_int, [c_vp, c_int, c_i64, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "es_expert_plan_workspace_size": (c_sz, [c_i64, c_int]),
+    "es_expert_plan": (c_int, [c_vp, c_i64, c_int, c_vp, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "es_grouped_matmul_workspace_size": (c_sz, [c_int, c_int, c_i64, c_i64, c_i64]),
+    "es_grouped_matmul": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                                  c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
+    "es_grouped_matmul_wgrad_workspace_size": (c_sz, [c_int, c_int, c_i64, c_i64, c_i64]),
+    "es_grouped_matmul_wgrad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp,
+                                        c_int, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp, c_vp]),
+    "es_combine_experts": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_vp]),
+    "es_combine_experts_grad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp,
+                                        c_i64, c_vp, c_vp, c_vp]),
+    "es_quantize_rows": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "es_int8_matmul_workspace_size": (c_sz, [c_int, c_i64, c_i64, c_i64]),
+    "es_int8_matmul": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
+                               c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
     "es_scatter_add_workspace_size": (c_sz, [c_i64]),
     "es_scatter_add_rows": (c_int, [c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp, c_vp, c_vp]),
 }

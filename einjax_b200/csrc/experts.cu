@@ -1,0 +1,679 @@
+// Routing of tokens to experts, the row order of the routed choices, the
+// weighted sum of the experts' rows back to tokens, and the 8-bit rounding of
+// token rows. The products between routing and sum are in grouped.cu.
+//
+// T tokens choose k of E experts each; choice a = t * k + j. Row r of the
+// grouped order holds choice order[r]; expert e owns rows offsets[e] to
+// offsets[e + 1]; position[a] is the row of choice a. A choice of no expert
+// (-1) has no row, and the rows from offsets[E] on are empty.
+#include <cuda_fp16.h>
+
+#include <cfloat>
+
+#include "common.cuh"
+#include "experts.cuh"
+
+namespace es {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+
+// ------------------------------------------------------------------ routing
+//
+// One warp per token, the token's logits in registers (lane l holds experts
+// l, l + 32, ...). The k largest are found one after the other: a local
+// maximum, one warp reduction of the order-preserving bits, one of the lowest
+// index among equals. With m the largest logit, w_j = exp(l_j - m) / sum,
+// where the sum runs over the chosen (renorm) or over all experts. -inf is a
+// masked expert and is never chosen. NaN is never chosen either, and makes
+// every weight of its token NaN. Bound by launch latency for decode steps and
+// by the selection's reductions (2 per choice and warp) for long prompts.
+
+// Bits whose unsigned order is the order of the floats; 0 for -inf and NaN.
+// x + 0 makes -0 equal to +0, so that ties go by index alone.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  if (!(x > -INFINITY)) return 0u;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(const T* row, int E, float (&v)[PER]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = lane + 32 * i;
+    v[i] = e < E ? to_f32(row[e]) : -INFINITY;
+  }
+}
+
+template <int PER>
+__device__ __forceinline__ float row_max(const float (&v)[PER]) {
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) m = fmaxf(m, v[i]);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
+  return m;
+}
+
+__device__ __forceinline__ float warp_sum(float s) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+  return s;
+}
+
+template <typename T, int PER>
+__global__ void __launch_bounds__(128) route_kernel(const T* logits, int64_t ntok, int E, int64_t stride, int k,
+                                                    int renorm, float* weights, int32_t* experts) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  if (t >= ntok) return;
+  float v[PER];
+  load_logits<T, PER>(logits + t * stride, E, v);
+  uint32_t key[PER];
+  bool nan = false;
+  float all = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    key[i] = order_bits(v[i]);
+    nan |= v[i] != v[i];
+  }
+  const float m = row_max<PER>(v);
+  if (!renorm) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) all += key[i] ? expf(v[i] - m) : 0.0f;
+    all = warp_sum(all);
+  }
+  const bool poison = __any_sync(kFull, nan);
+  // choice j ends in lane j (k <= 32)
+  float mine = 0.0f;
+  int chosen = -1;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = 0;
+    int at = 0x7fffffff;
+    float val = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] > best) {
+        best = key[i];
+        at = lane + 32 * i;
+        val = v[i];
+      }
+    const uint32_t top = __reduce_max_sync(kFull, best);
+    if (top == 0) break;  // nothing left but masked experts
+    const int e = __reduce_min_sync(kFull, best == top ? at : 0x7fffffff);
+    const float x = __shfl_sync(kFull, val, e & 31);
+    if (lane == (e & 31)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i == (e >> 5)) key[i] = 0;
+    }
+    if (lane == j) {
+      chosen = e;
+      mine = expf(x - m);
+    }
+  }
+  const float total = renorm ? warp_sum(mine) : all;
+  if (lane < k) {
+    const float w = chosen >= 0 ? mine / total : 0.0f;
+    weights[t * k + lane] = poison ? NAN : w;
+    experts[t * k + lane] = chosen;
+  }
+}
+
+// dl_i = w_i (g_i - d), d = sum_j w_j g_j, over the chosen experts (renorm);
+// else dl_i = p_i (g_i [i chosen] - d) over all, with p recomputed from the
+// logits. Reads the logits (only for the second form), writes dlogits once.
+template <typename T, int PER>
+__global__ void __launch_bounds__(128) route_grad_kernel(const T* logits, int64_t ntok, int E, int64_t stride, int k,
+                                                         int renorm, const float* weights, const int32_t* experts,
+                                                         const float* dweights, T* dlogits) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x * 4LL + (threadIdx.x >> 5);
+  if (t >= ntok) return;
+  float w = 0.0f, g = 0.0f;
+  int e = -1;
+  if (lane < k) {
+    w = weights[t * k + lane];
+    e = experts[t * k + lane];
+    g = e >= 0 ? dweights[t * k + lane] : 0.0f;
+  }
+  const float d = warp_sum(w * g);
+  float out[PER];
+  if (renorm) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) out[i] = 0.0f;
+  } else {
+    float v[PER];
+    load_logits<T, PER>(logits + t * stride, E, v);
+    const float m = row_max<PER>(v);
+    float all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      // NaN logits keep their NaN here, masked ones add nothing
+      out[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - m);
+      all += out[i];
+    }
+    all = warp_sum(all);
+    const float f = all > 0.0f || all != all ? -d / all : 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) out[i] *= f;
+  }
+  const float mine = renorm ? w * (g - d) : w * g;
+  for (int j = 0; j < k; ++j) {
+    const int ej = __shfl_sync(kFull, e, j);
+    const float x = __shfl_sync(kFull, mine, j);
+    if (ej >= 0 && lane == (ej & 31)) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i == (ej >> 5)) out[i] += x;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int x = lane + 32 * i;
+    if (x < E) dlogits[t * static_cast<int64_t>(E) + x] = from_f32<T>(out[i]);
+  }
+}
+
+template <typename T>
+int route_typed(const void* logits, int64_t T_, int E, int64_t stride, int k, int renorm, float* weights,
+                int32_t* experts, const float* dweights, void* dlogits, cudaStream_t s) {
+  const T* x = static_cast<const T*>(logits);
+  const int64_t blocks = (T_ + 3) / 4;
+#define ES_ROUTE(PER)                                                                                            \
+  if (E <= 32 * PER) {                                                                                           \
+    if (dlogits)                                                                                                 \
+      ES_LAUNCH((route_grad_kernel<T, PER>), static_cast<unsigned>(blocks), 128, 0, s, x, T_, E, stride, k,       \
+                renorm, weights, experts, dweights, static_cast<T*>(dlogits));                                   \
+    else                                                                                                         \
+      ES_LAUNCH((route_kernel<T, PER>), static_cast<unsigned>(blocks), 128, 0, s, x, T_, E, stride, k, renorm,    \
+                weights, experts);                                                                               \
+    return ES_OK;                                                                                                \
+  }
+  ES_ROUTE(1)
+  ES_ROUTE(2)
+  ES_ROUTE(4)
+  ES_ROUTE(8)
+  ES_ROUTE(16)
+  ES_ROUTE(32)
+#undef ES_ROUTE
+  return ES_ERR_UNSUPPORTED;
+}
+
+// ----------------------------------------------------------------- row order
+//
+// A stable counting sort of the choices by expert ("no expert" sorts last, as
+// expert E). Few choices: one CTA, one launch. Else the choices are cut into
+// chunks: one launch counts each chunk's experts, and in a second every chunk
+// adds up the chunks before it and places its own. Within a CTA each warp owns
+// a consecutive run of choices; a choice's rank is its warp's start plus the
+// earlier choices of the warp with the same expert (match + popcount), so the
+// order never depends on the schedule.
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kPlanChunk = 4096;   // choices of one CTA; one CTA alone up to here
+constexpr int kPlanChunks = 1024;  // at most: every CTA reads every chunk's counts
+
+int64_t plan_chunk(int64_t n) {
+  const int64_t unit = static_cast<int64_t>(kPlanChunk) * kPlanChunks;
+  return kPlanChunk * (n > unit ? (n + unit - 1) / unit : 1);
+}
+
+__device__ __forceinline__ int expert_of(const int32_t* experts, int64_t a, int E, bool& bad) {
+  const int e = experts[a];
+  if (e < -1 || e >= E) bad = true;
+  return e >= 0 && e < E ? e : E;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const int32_t* experts, int64_t n, int64_t chunk,
+                                                                  int E, int32_t* counts) {
+  extern __shared__ int32_t hist[];
+  for (int i = threadIdx.x; i <= E; i += kPlanThreads) hist[i] = 0;
+  __syncthreads();
+  const int64_t c0 = blockIdx.x * chunk;
+  const int64_t c1 = min(n, c0 + chunk);
+  bool bad = false;
+  for (int64_t a = c0 + threadIdx.x; a < c1; a += kPlanThreads) atomicAdd(&hist[expert_of(experts, a, E, bad)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i <= E; i += kPlanThreads) counts[blockIdx.x * static_cast<int64_t>(E + 1) + i] = hist[i];
+}
+
+// counts: of every chunk (nullptr: this CTA is the only chunk).
+__global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const int32_t* experts, int64_t n, int64_t chunk,
+                                                                  int E, const int32_t* counts, int32_t* offsets,
+                                                                  int32_t* order, int32_t* position, int32_t* err) {
+  extern __shared__ int32_t sm[];
+  const int E1 = E + 1;
+  int32_t* cnt = sm;                      // [kPlanWarps][E1]: counts, then next row of (warp, expert)
+  int32_t* before = sm + kPlanWarps * E1;  // [E1] rows of this expert in the chunks before
+  int32_t* total = before + E1;            // [E1] rows of this expert in all, then its first row
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < kPlanWarps * E1; i += kPlanThreads) cnt[i] = 0;
+  __syncthreads();
+  const int64_t c0 = blockIdx.x * chunk;
+  const int m = static_cast<int>(min(n - c0, chunk));
+  const int per = ((m + kPlanWarps - 1) / kPlanWarps + 31) & ~31;  // a warp's run of choices
+  const int w0 = warp * per, w1 = min(m, w0 + per);
+  bool bad = false;
+  for (int i = w0 + lane; i < w1; i += 32) atomicAdd(&cnt[warp * E1 + expert_of(experts, c0 + i, E, bad)], 1);
+  if (bad && err) *static_cast<volatile int32_t*>(err) = ES_ERR_INDEX;
+  if (counts) {
+    for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+      int b = 0, all = 0;
+#pragma unroll 8
+      for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
+        const int v = counts[c * static_cast<int64_t>(E1) + e];
+        b += c < static_cast<int>(blockIdx.x) ? v : 0;
+        all += v;
+      }
+      before[e] = b;
+      total[e] = all;
+    }
+    __syncthreads();
+  } else {
+    __syncthreads();
+    for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+      int all = 0;
+      for (int w = 0; w < kPlanWarps; ++w) all += cnt[w * E1 + e];
+      before[e] = 0;
+      total[e] = all;
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {  // exclusive sum of the totals: each expert's first row
+    int run = 0;
+    for (int e0 = 0; e0 < E1; e0 += 32) {
+      const int e = e0 + lane;
+      const int v = e < E1 ? total[e] : 0;
+      int s = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFull, s, o);
+        if (lane >= o) s += u;
+      }
+      if (e < E1) {
+        total[e] = run + s - v;
+        if (blockIdx.x == 0) offsets[e] = run + s - v;
+      }
+      run += __shfl_sync(kFull, s, 31);
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+    int at = total[e] + before[e];
+    for (int w = 0; w < kPlanWarps; ++w) {
+      const int v = cnt[w * E1 + e];
+      cnt[w * E1 + e] = at;
+      at += v;
+    }
+  }
+  __syncthreads();
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const bool live = i < w1;
+    const int e = live ? expert_of(experts, c0 + i, E, bad) : E1;
+    const unsigned same = __match_any_sync(kFull, e);
+    int row = 0;
+    if (live) row = cnt[warp * E1 + e] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (live) {
+      if (lane == __ffs(same) - 1) cnt[warp * E1 + e] = row + __popc(same);
+      order[row] = e < E ? static_cast<int32_t>(c0 + i) : -1;
+      position[c0 + i] = e < E ? row : -1;
+    }
+    __syncwarp();
+  }
+}
+
+size_t plan_smem(int E) { return static_cast<size_t>(kPlanWarps + 2) * (E + 1) * sizeof(int32_t); }
+
+// --------------------------------------------------- weighted sum to tokens
+//
+// out_t = sum_j w_tj y_pos(t,j), in fp32, rounded once. Backward in one pass:
+// dy_pos(t,j) = w_tj dout_t and dw_tj = <dout_t, y_pos(t,j)>. Both are bound
+// by memory: every row is read (and written) once, in 16-byte pieces, by TP
+// threads per token; all the token's rows are in flight together.
+
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Piece {
+  T v[VEC];
+};
+
+constexpr int kCombineThreads = 256;
+constexpr int kRowsAhead = 8;  // choices of a token that are in flight together
+
+__device__ __forceinline__ int row_of(const int32_t* position, int64_t a, int64_t rows) {
+  const int p = position[a];
+  return p >= 0 && p < rows ? p : -1;
+}
+
+template <typename T, typename U, int VEC>
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(const T* y, int64_t rows, int64_t stride,
+                                                                  const float* weights, const int32_t* position,
+                                                                  int64_t ntok, int k, int64_t D, U* out, int tp) {
+  const int64_t t = blockIdx.x * static_cast<int64_t>(kCombineThreads / tp) + threadIdx.x / tp;
+  if (t >= ntok) return;
+  const int64_t pieces = D / VEC;
+  for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
+    float acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
+    for (int j0 = 0; j0 < k; j0 += kRowsAhead) {
+      Piece<T, VEC> p[kRowsAhead];
+      float w[kRowsAhead];
+#pragma unroll
+      for (int j = 0; j < kRowsAhead; ++j) {
+        const int r = j0 + j < k ? row_of(position, t * k + j0 + j, rows) : -1;
+        w[j] = 0.0f;
+        if (r >= 0) {
+          w[j] = weights ? weights[t * k + j0 + j] : 1.0f;
+          p[j] = reinterpret_cast<const Piece<T, VEC>*>(y + r * stride)[c];
+        } else {
+          p[j] = Piece<T, VEC>{};
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kRowsAhead; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[j], to_f32(p[j].v[i]), acc[i]);
+    }
+    Piece<U, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<U>(acc[i]);
+    reinterpret_cast<Piece<U, VEC>*>(out + t * D)[c] = o;
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kCombineThreads) combine_grad_kernel(
+    const T* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position, const int32_t* kept,
+    int64_t ntok, int k, int64_t D, const T* dout, int64_t dstride, T* dy, float* dweights, int tp) {
+  __shared__ float part[kCombineThreads / 32][kRowsAhead];
+  const int group = threadIdx.x / tp, lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x * static_cast<int64_t>(kCombineThreads / tp) + group;
+  const bool live = t < ntok;
+  const int64_t pieces = D / VEC;
+  for (int j0 = 0; j0 < k; j0 += kRowsAhead) {
+    float dot[kRowsAhead];
+    int r[kRowsAhead];
+    float w[kRowsAhead];
+#pragma unroll
+    for (int j = 0; j < kRowsAhead; ++j) {
+      dot[j] = 0.0f;
+      r[j] = live && j0 + j < k ? row_of(position, t * k + j0 + j, rows) : -1;
+      w[j] = r[j] >= 0 ? weights[t * k + j0 + j] : 0.0f;
+    }
+    if (live) {
+      for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
+        const Piece<T, VEC> g = reinterpret_cast<const Piece<T, VEC>*>(dout + t * dstride)[c];
+        Piece<T, VEC> p[kRowsAhead];
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j)
+          if (r[j] >= 0) p[j] = reinterpret_cast<const Piece<T, VEC>*>(y + r[j] * stride)[c];
+#pragma unroll
+        for (int j = 0; j < kRowsAhead; ++j)
+          if (r[j] >= 0) {
+            Piece<T, VEC> o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const float gi = to_f32(g.v[i]);
+              dot[j] = fmaf(gi, to_f32(p[j].v[i]), dot[j]);
+              o.v[i] = from_f32<T>(w[j] * gi);
+            }
+            reinterpret_cast<Piece<T, VEC>*>(dy + r[j] * D)[c] = o;
+          }
+      }
+    }
+    // the group's threads are whole warps (tp is a multiple of 32)
+#pragma unroll
+    for (int j = 0; j < kRowsAhead; ++j) dot[j] = warp_sum(dot[j]);
+    if (lane == 0) {
+#pragma unroll
+      for (int j = 0; j < kRowsAhead; ++j) part[threadIdx.x >> 5][j] = dot[j];
+    }
+    __syncthreads();
+    const int j = threadIdx.x % tp;
+    if (live && j < kRowsAhead && j0 + j < k) {
+      float s = 0.0f;
+      for (int w8 = 0; w8 < tp / 32; ++w8) s += part[group * (tp / 32) + w8][j];
+      dweights[t * k + j0 + j] = row_of(position, t * k + j0 + j, rows) >= 0 ? s : 0.0f;
+    }
+    __syncthreads();
+  }
+  // rows of no choice
+  const int64_t first = min(max(static_cast<int64_t>(*kept), int64_t{0}), rows);
+  for (int64_t r = first + blockIdx.x; r < rows; r += gridDim.x)
+    for (int64_t c = threadIdx.x; c < pieces; c += kCombineThreads)
+      reinterpret_cast<Piece<T, VEC>*>(dy + r * D)[c] = Piece<T, VEC>{};
+}
+
+// Threads per token: enough that each takes one or two pieces, in whole warps.
+int token_threads(int64_t pieces) {
+  int tp = 32;
+  while (tp < kCombineThreads && tp < pieces) tp *= 2;
+  return tp;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, typename U, int VEC>
+int combine_vec(const void* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position, int64_t T_,
+                int k, int64_t D, void* out, cudaStream_t s) {
+  const int tp = token_threads(D / VEC);
+  const int64_t per = kCombineThreads / tp;
+  ES_LAUNCH((combine_kernel<T, U, VEC>), static_cast<unsigned>((T_ + per - 1) / per), kCombineThreads, 0, s,
+            static_cast<const T*>(y), rows, stride, weights, position, T_, k, D, static_cast<U*>(out), tp);
+  return ES_OK;
+}
+
+template <typename T, typename U>
+int combine_typed(const void* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position,
+                  int64_t T_, int k, int64_t D, void* out, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (D % VEC == 0 && stride % VEC == 0 && aligned16(y) && aligned16(out))
+    return combine_vec<T, U, VEC>(y, rows, stride, weights, position, T_, k, D, out, s);
+  return combine_vec<T, U, 1>(y, rows, stride, weights, position, T_, k, D, out, s);
+}
+
+template <typename T, int VEC>
+int combine_grad_vec(const void* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position,
+                     const int32_t* kept, int64_t T_, int k, int64_t D, const void* dout, int64_t dstride, void* dy,
+                     float* dweights, cudaStream_t s) {
+  const int tp = token_threads(D / VEC);
+  const int64_t per = kCombineThreads / tp;
+  ES_LAUNCH((combine_grad_kernel<T, VEC>), static_cast<unsigned>((T_ + per - 1) / per), kCombineThreads, 0, s,
+            static_cast<const T*>(y), rows, stride, weights, position, kept, T_, k, D, static_cast<const T*>(dout),
+            dstride, static_cast<T*>(dy), dweights, tp);
+  return ES_OK;
+}
+
+template <typename T>
+int combine_grad_typed(const void* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position,
+                       const int32_t* kept, int64_t T_, int k, int64_t D, const void* dout, int64_t dstride, void* dy,
+                       float* dweights, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (D % VEC == 0 && stride % VEC == 0 && dstride % VEC == 0 && aligned16(y) && aligned16(dout) && aligned16(dy))
+    return combine_grad_vec<T, VEC>(y, rows, stride, weights, position, kept, T_, k, D, dout, dstride, dy, dweights, s);
+  return combine_grad_vec<T, 1>(y, rows, stride, weights, position, kept, T_, k, D, dout, dstride, dy, dweights, s);
+}
+
+// ------------------------------------------------------------ 8-bit rounding
+//
+// scale_t = max_i |x_ti| / 127 (one division rounded to nearest), q_ti =
+// rint(x_ti / scale_t), kept within +-127. A row of zeros has scale 0 and q 0;
+// a row with an infinity or NaN has scale NaN, so that its products are NaN
+// and not a finite guess. Bound by memory: a row is read once from HBM (the
+// second reading hits the L1) and its 8-bit copy written once.
+
+constexpr int kQuantThreads = 256;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const T* x, int64_t rows, int64_t K, int64_t stride,
+                                                                 int8_t* q, float* scale, int tp) {
+  __shared__ float part[kQuantThreads / 32];
+  const int group = threadIdx.x / tp;
+  const int64_t t = blockIdx.x * static_cast<int64_t>(kQuantThreads / tp) + group;
+  const bool live = t < rows;
+  const int64_t pieces = K / VEC;
+  float peak = 0.0f;
+  bool odd = false;  // an infinity or NaN
+  if (live) {
+    const Piece<T, VEC>* row = reinterpret_cast<const Piece<T, VEC>*>(x + t * stride);
+    for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
+      const Piece<T, VEC> p = row[c];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float a = fabsf(to_f32(p.v[i]));
+        odd |= !(a <= FLT_MAX);
+        peak = fmaxf(peak, a);
+      }
+    }
+  }
+  if (odd) peak = INFINITY;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(kFull, peak, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = peak;
+  __syncthreads();
+  if (!live) return;
+  for (int w = 0; w < tp / 32; ++w) peak = fmaxf(peak, part[group * (tp / 32) + w]);
+  const bool finite = peak <= FLT_MAX;
+  const float s = finite ? __fdiv_rn(peak, 127.0f) : NAN;
+  if (threadIdx.x % tp == 0) scale[t] = s;
+  const Piece<T, VEC>* row = reinterpret_cast<const Piece<T, VEC>*>(x + t * stride);
+  for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
+    const Piece<T, VEC> p = row[c];
+    Piece<int8_t, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float v = s > 0.0f ? rintf(__fdiv_rn(to_f32(p.v[i]), s)) : 0.0f;
+      o.v[i] = static_cast<int8_t>(fminf(fmaxf(v, -127.0f), 127.0f));
+    }
+    reinterpret_cast<Piece<int8_t, VEC>*>(q + t * K)[c] = o;
+  }
+}
+
+template <typename T, int VEC>
+int quantize_vec(const void* x, int64_t rows, int64_t K, int64_t stride, int8_t* q, float* scale, cudaStream_t s) {
+  const int tp = token_threads(K / VEC);
+  const int64_t per = kQuantThreads / tp;
+  ES_LAUNCH((quantize_kernel<T, VEC>), static_cast<unsigned>((rows + per - 1) / per), kQuantThreads, 0, s,
+            static_cast<const T*>(x), rows, K, stride, q, scale, tp);
+  return ES_OK;
+}
+
+template <typename T>
+int quantize_typed(const void* x, int64_t rows, int64_t K, int64_t stride, int8_t* q, float* scale, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (K % VEC == 0 && stride % VEC == 0 && aligned16(x) && aligned16(q))
+    return quantize_vec<T, VEC>(x, rows, K, stride, q, scale, s);
+  return quantize_vec<T, 1>(x, rows, K, stride, q, scale, s);
+}
+
+// Largest sizes: a row index fits 31 bits, a grid dimension too.
+bool rows_ok(int64_t n) { return n >= 0 && n <= 0x7fffff00LL; }
+
+}  // namespace
+}  // namespace es
+
+using namespace es;
+
+extern "C" int es_route_experts(const void* logits, int dtype, int64_t num_tokens, int num_experts,
+                                int64_t row_stride, int top_k, int renormalize, float* weights, int32_t* experts,
+                                void* stream) {
+  if (num_experts < 1 || top_k < 1 || top_k > num_experts || num_tokens < 0) return ES_ERR_INVALID;
+  if (num_experts > kMaxExperts || top_k > kMaxTopK || !rows_ok(num_tokens * top_k)) return ES_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return ES_OK;
+  if (!logits || !weights || !experts) return ES_ERR_INVALID;
+  ES_BY_TYPE(dtype, return route_typed<T>(logits, num_tokens, num_experts, row_stride, top_k, renormalize, weights,
+                                          experts, nullptr, nullptr, as_stream(stream)));
+  return ES_ERR_UNSUPPORTED;
+}
+
+extern "C" int es_route_experts_grad(const void* logits, int dtype, int64_t num_tokens, int num_experts,
+                                     int64_t row_stride, int top_k, int renormalize, const float* weights,
+                                     const int32_t* experts, const float* dweights, void* dlogits, void* stream) {
+  if (num_experts < 1 || top_k < 1 || top_k > num_experts || num_tokens < 0) return ES_ERR_INVALID;
+  if (num_experts > kMaxExperts || top_k > kMaxTopK || !rows_ok(num_tokens * top_k)) return ES_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return ES_OK;
+  if (!logits || !weights || !experts || !dweights || !dlogits) return ES_ERR_INVALID;
+  ES_BY_TYPE(dtype, return route_typed<T>(logits, num_tokens, num_experts, row_stride, top_k, renormalize,
+                                          const_cast<float*>(weights), const_cast<int32_t*>(experts), dweights,
+                                          dlogits, as_stream(stream)));
+  return ES_ERR_UNSUPPORTED;
+}
+
+extern "C" size_t es_expert_plan_workspace_size(int64_t num_choices, int num_experts) {
+  if (num_choices <= kPlanChunk || num_experts < 1) return 0;
+  const int64_t chunk = plan_chunk(num_choices);
+  return static_cast<size_t>((num_choices + chunk - 1) / chunk) * (num_experts + 1) * sizeof(int32_t);
+}
+
+extern "C" int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts, void* workspace,
+                              size_t workspace_bytes, int32_t* offsets, int32_t* order, int32_t* position,
+                              int32_t* status, void* stream) {
+  if (num_choices < 0 || num_experts < 1 || !offsets) return ES_ERR_INVALID;
+  if (num_experts > kMaxExperts || !rows_ok(num_choices)) return ES_ERR_UNSUPPORTED;
+  if (num_choices > 0 && (!experts || !order || !position)) return ES_ERR_INVALID;
+  if (workspace_bytes < es_expert_plan_workspace_size(num_choices, num_experts)) return ES_ERR_WORKSPACE;
+  cudaStream_t s = as_stream(stream);
+  const size_t smem = plan_smem(num_experts);
+  if (smem > 48 * 1024)
+    if (cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(smem)) != cudaSuccess)
+      return ES_ERR_CUDA;
+  const int64_t chunk = plan_chunk(num_choices);
+  const int64_t chunks = num_choices > 0 ? (num_choices + chunk - 1) / chunk : 1;
+  int32_t* counts = nullptr;
+  if (chunks > 1) {
+    counts = static_cast<int32_t*>(workspace);
+    ES_LAUNCH(plan_count_kernel, static_cast<unsigned>(chunks), kPlanThreads, (num_experts + 1) * sizeof(int32_t), s,
+              experts, num_choices, chunk, num_experts, counts);
+  }
+  ES_LAUNCH(plan_place_kernel, static_cast<unsigned>(chunks), kPlanThreads, smem, s, experts, num_choices,
+            chunk, num_experts, static_cast<const int32_t*>(counts), offsets, order, position, status);
+  return ES_OK;
+}
+
+extern "C" int es_combine_experts(const void* y, int dtype, int64_t num_rows, int64_t row_stride,
+                                  const float* weights, const int32_t* position, int64_t num_tokens, int top_k,
+                                  int64_t width, void* out, int out_dtype, void* stream) {
+  if (num_rows < 0 || num_tokens < 0 || top_k < 1 || width < 0) return ES_ERR_INVALID;
+  if (!rows_ok(num_rows) || !rows_ok(num_tokens * top_k)) return ES_ERR_UNSUPPORTED;
+  if (num_tokens == 0 || width == 0) return ES_OK;
+  if ((!y && num_rows) || !position || !out) return ES_ERR_INVALID;
+  cudaStream_t s = as_stream(stream);
+  if (dtype == out_dtype)
+    ES_BY_TYPE(dtype, return (combine_typed<T, T>(y, num_rows, row_stride, weights, position, num_tokens, top_k,
+                                                  width, out, s)));
+  if (dtype == ES_F32)  // the sum of fp32 rows in the operands' type
+    ES_BY_TYPE(out_dtype, return (combine_typed<float, T>(y, num_rows, row_stride, weights, position, num_tokens,
+                                                          top_k, width, out, s)));
+  return ES_ERR_UNSUPPORTED;
+}
+
+extern "C" int es_combine_experts_grad(const void* y, int dtype, int64_t num_rows, int64_t row_stride,
+                                       const float* weights, const int32_t* position, const int32_t* kept_rows,
+                                       int64_t num_tokens, int top_k, int64_t width, const void* dout,
+                                       int64_t dout_stride, void* dy, float* dweights, void* stream) {
+  if (num_rows < 0 || num_tokens < 0 || top_k < 1 || width < 0) return ES_ERR_INVALID;
+  if (!rows_ok(num_rows) || !rows_ok(num_tokens * top_k)) return ES_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return ES_OK;
+  if (!weights || !position || !kept_rows || !dweights || (width && (!dout || (num_rows && (!y || !dy)))))
+    return ES_ERR_INVALID;
+  ES_BY_TYPE(dtype, return combine_grad_typed<T>(y, num_rows, row_stride, weights, position, kept_rows, num_tokens,
+                                                 top_k, width, dout, dout_stride, dy, dweights, as_stream(stream)));
+  return ES_ERR_UNSUPPORTED;
+}
+
+extern "C" int es_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t width, int64_t row_stride,
+                                int8_t* q, float* scale, void* stream) {
+  if (num_rows < 0 || width < 0) return ES_ERR_INVALID;
+  if (!rows_ok(num_rows)) return ES_ERR_UNSUPPORTED;
+  if (num_rows == 0) return ES_OK;
+  if ((width && (!x || !q)) || !scale) return ES_ERR_INVALID;
+  ES_BY_TYPE(dtype, return quantize_typed<T>(x, num_rows, width, row_stride, q, scale, as_stream(stream)));
+  return ES_ERR_UNSUPPORTED;
+}

@@ -1,0 +1,473 @@
+"""Mixture of experts: routing, products grouped by expert, the weighted sum back to tokens, 8-bit products.
+
+A layer of experts is the contraction ``te,td,edf->tf`` with a token x expert
+matrix of ``top_k`` nonzeros a row. Its blocks are ragged in the token axis,
+so it runs beside the tile-COO path instead of on it:
+
+* ``route_experts``: the chosen experts of each token and their weights;
+* ``plan_experts``: the order that groups the choices by expert;
+* ``grouped_matmul``: each group's rows times its expert's matrix;
+* ``combine_experts``: the weighted sum of a token's rows;
+* ``quantize_rows``, ``quantize_experts``, ``int8_matmul``: the serving form
+  in 8-bit integers with a scale for each token and output channel;
+* ``expert_mlp``: a gated layer made of these.
+
+All of it runs on torch's current CUDA stream with no wait of the host. What
+only the device can see (a choice of an expert that does not exist, a bounded
+wait that ran out) is raised by ``check_device_errors``.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib as L
+from .sparse import _STATUS, stream_ptr
+
+MAX_EXPERTS, MAX_TOP_K, MAX_INT8_DEPTH = 1024, 32, 133152
+
+_DTYPES = {torch.float32: L.ES_F32, torch.bfloat16: L.ES_BF16, torch.float16: L.ES_F16}
+
+
+def _code(fn: str, name: str, dtype) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{fn}: {name} must be float32, bfloat16 or float16, got {dtype}")
+    return code
+
+
+def _on_gpu(fn: str, **tensors):
+    """The one CUDA device of the tensors."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{fn}: {name} must be a torch tensor, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise ValueError(f"{fn}: {name} must be a CUDA tensor")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{fn}: {name} is on {t.device}, the other operands on {dev}")
+    return dev
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` (2-D) with a contiguous last dimension and rows that do not overlap."""
+    if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t
+    return t.contiguous()
+
+
+class _on_device:
+    """Makes ``dev`` current for the launches inside, at no cost when it is already."""
+
+    def __init__(self, dev):
+        self.dev = dev.index if dev.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.dev is not None:
+            self.prev = torch.cuda.current_device()
+            torch.cuda.set_device(self.dev)
+
+    def __exit__(self, *exc):
+        if self.dev is not None:
+            torch.cuda.set_device(self.prev)
+
+
+@dataclass(eq=False)
+class ExpertPlan:
+    """Row order of the routed choices, all int32 on the device.
+
+    Expert ``e`` owns rows ``offsets[e]`` to ``offsets[e + 1]``; row ``r``
+    holds choice ``order[r]`` (``token * top_k + j``); ``position[token, j]``
+    is the row of that choice. -1: no row, no choice. The rows from
+    ``offsets[num_experts]`` on belong to no expert and are zero in every
+    output."""
+
+    offsets: torch.Tensor   # (num_experts + 1,)
+    order: torch.Tensor     # (num_tokens * top_k,)
+    position: torch.Tensor  # (num_tokens, top_k)
+
+    def __post_init__(self):
+        o, r, p = self.offsets, self.order, self.position
+        if o.dtype != torch.int32 or r.dtype != torch.int32 or p.dtype != torch.int32:
+            raise TypeError("ExpertPlan: offsets, order and position must be int32")
+        if o.dim() != 1 or r.dim() != 1 or p.dim() != 2 or o.shape[0] < 2 or p.shape[1] < 1 or \
+                p.shape[0] * p.shape[1] != r.shape[0]:
+            raise ValueError(f"ExpertPlan: shapes {tuple(o.shape)}, {tuple(r.shape)} and {tuple(p.shape)} are not "
+                             "(num_experts + 1,), (num_tokens * top_k,) and (num_tokens, top_k)")
+        if o.shape[0] - 1 > MAX_EXPERTS:
+            raise ValueError(f"ExpertPlan: at most {MAX_EXPERTS} experts, got {o.shape[0] - 1}")
+        if not (o.is_contiguous() and r.is_contiguous() and p.is_contiguous()):
+            raise ValueError("ExpertPlan: offsets, order and position must be contiguous")
+        _on_gpu("ExpertPlan", offsets=o, order=r, position=p)
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def num_tokens(self) -> int:
+        return self.position.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.position.shape[1]
+
+    @property
+    def num_rows(self) -> int:
+        return self.order.shape[0]
+
+    @property
+    def counts(self) -> torch.Tensor:
+        """Rows of each expert, int32 (num_experts,)."""
+        return self.offsets[1:] - self.offsets[:-1]
+
+
+# ------------------------------------------------------------------- routing
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, renormalize):
+        T, E = logits.shape
+        dev = logits.device
+        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        with _on_device(dev):
+            L.check("es_route_experts", L.lib().es_route_experts(
+                logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), top_k, renormalize,
+                weights.data_ptr(), experts.data_ptr(), stream_ptr(dev)))
+        ctx.mark_non_differentiable(experts)
+        if logits.requires_grad:
+            ctx.save_for_backward(logits, weights, experts)
+            ctx.renormalize = renormalize
+        return weights, experts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dweights, _):
+        logits, weights, experts = ctx.saved_tensors
+        T, E = logits.shape
+        dev = logits.device
+        dweights = dweights.to(torch.float32).contiguous()
+        dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
+        with _on_device(dev):
+            L.check("es_route_experts_grad", L.lib().es_route_experts_grad(
+                logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), experts.shape[1], ctx.renormalize,
+                weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), stream_ptr(dev)))
+        return dlogits, None, None
+
+
+def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True):
+    """The ``top_k`` experts of each token and their softmax weights.
+
+    ``logits`` (num_tokens, num_experts). Returns ``(weights, experts)``,
+    float32 and int32 (num_tokens, top_k), largest logit first, ties to the
+    lowest expert. The softmax runs over the chosen experts (``renormalize``)
+    or over all of them. ``-inf`` masks an expert: it is never chosen, and a
+    token with fewer than ``top_k`` experts left gets -1 with weight 0. The
+    type's lowest finite value is a logit like any other. A NaN logit is never
+    chosen and makes all weights of its token NaN. ``weights`` carries a
+    gradient to ``logits``."""
+    _on_gpu("route_experts", logits=logits)
+    if logits.dim() != 2:
+        raise ValueError(f"route_experts: logits must be (num_tokens, num_experts), got {tuple(logits.shape)}")
+    _code("route_experts", "logits", logits.dtype)
+    E, top_k = logits.shape[1], int(top_k)
+    if not 1 <= top_k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS:
+        raise ValueError(f"route_experts: top_k={top_k} of {E} experts; 1 <= top_k <= min(num_experts, {MAX_TOP_K}) "
+                         f"and num_experts <= {MAX_EXPERTS}")
+    return _Route.apply(_rows(logits), top_k, 1 if renormalize else 0)
+
+
+def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
+    """Groups the choices ``experts`` (num_tokens, top_k; -1: none) by expert,
+    in ascending token and choice inside an expert. An entry outside
+    ``[-1, num_experts)`` counts as -1 and is raised as ``ValueError`` by the
+    next ``check_device_errors``."""
+    dev = _on_gpu("plan_experts", experts=experts)
+    if experts.dim() != 2 or experts.shape[1] < 1:
+        raise ValueError(f"plan_experts: experts must be (num_tokens, top_k), got {tuple(experts.shape)}")
+    if experts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"plan_experts: experts must be int32 or int64, got {experts.dtype}")
+    E = int(num_experts)
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"plan_experts: num_experts={E} is not in [1, {MAX_EXPERTS}]")
+    lib = L.lib()
+    if experts.dtype == torch.int64:  # a value past 32 bits must not wrap into the range
+        experts = experts.clamp(-2, E).to(torch.int32)
+    experts = experts.contiguous()
+    n = experts.numel()
+    offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    position = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    nbytes = lib.es_expert_plan_workspace_size(n, E)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _on_device(dev):
+        L.check("es_expert_plan", lib.es_expert_plan(
+            experts.data_ptr(), n, E, ws.data_ptr() if ws is not None else None, nbytes, offsets.data_ptr(), order.data_ptr(), position.data_ptr(),
+            _STATUS.address("es_expert_plan", dev.index), stream_ptr(dev)))
+    return ExpertPlan(offsets, order, position)
+
+
+# ---------------------------------------------------------- grouped products
+
+def _plan_args(plan, gather):
+    return plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None
+
+
+def _grouped(x, w, plan, gather, out_dtype):
+    """``w`` (num_experts, K, N), any strides."""
+    dev = x.device
+    K, N, R = w.shape[1], w.shape[2], plan.num_rows
+    y = torch.empty((R, N), dtype=out_dtype, device=dev)
+    lib = L.lib()
+    code = _DTYPES[x.dtype]
+    nbytes = lib.es_grouped_matmul_workspace_size(code, plan.num_experts, K, N, R)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    off, order = _plan_args(plan, gather)
+    se, sk, sn = w.stride()
+    with _on_device(dev):
+        L.check("es_grouped_matmul", lib.es_grouped_matmul(
+            x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), plan.num_experts, K, N, se, sk, sn, off, order,
+            plan.top_k, R, y.data_ptr(), _DTYPES[out_dtype], ws.data_ptr() if ws is not None else None, nbytes,
+            _STATUS.address("es_grouped_matmul", dev.index), stream_ptr(dev)))
+    return y
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, plan, gather):
+        if x.requires_grad or w.requires_grad:
+            ctx.save_for_backward(x, w)
+            ctx.plan, ctx.gather = plan, gather
+        return _grouped(x, w, plan, gather, x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        plan, gather = ctx.plan, ctx.gather
+        dy = _rows(dy)
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            # a token's rows are summed before its gradient is rounded
+            dx = _grouped(dy, w.transpose(1, 2), plan, False, torch.float32 if gather else x.dtype)
+            if gather:
+                dx = _combine(dx, None, plan, x.dtype)
+        if ctx.needs_input_grad[1]:
+            dw = _wgrad(x, dy, w, plan, gather)
+        return dx, dw, None, None
+
+
+def _wgrad(x, dy, w, plan, gather):
+    dev = x.device
+    E, K, N = w.shape
+    # the gradient takes w's layout when it is a transposed view
+    dw = torch.empty((E, N, K), dtype=w.dtype, device=dev).transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 \
+        else torch.empty((E, K, N), dtype=w.dtype, device=dev)
+    lib = L.lib()
+    code = _DTYPES[x.dtype]
+    nbytes = lib.es_grouped_matmul_wgrad_workspace_size(code, E, K, N, plan.num_rows)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    off, order = _plan_args(plan, gather)
+    with _on_device(dev):
+        L.check("es_grouped_matmul_wgrad", lib.es_grouped_matmul_wgrad(
+            x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E, K, N, off, order, plan.top_k,
+            plan.num_rows, dw.data_ptr(), *dw.stride(), ws.data_ptr() if ws is not None else None, nbytes,
+            _STATUS.address("es_grouped_matmul_wgrad", dev.index), stream_ptr(dev)))
+    return dw
+
+
+def _check_rows(fn, x, name, plan, gather, K):
+    want = plan.num_tokens if gather else plan.num_rows
+    if x.dim() != 2 or x.shape[0] != want or (K is not None and x.shape[1] != K):
+        raise ValueError(f"{fn}: {name} has shape {tuple(x.shape)}, the plan's {'tokens' if gather else 'rows'} and "
+                         f"the weights want ({want}, {'...' if K is None else K})")
+
+
+def grouped_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan, gather: bool = False) -> torch.Tensor:
+    """Each expert's rows times its matrix: ``y[r] = x[r] @ w[e]`` for the rows
+    ``r`` of expert ``e``, ragged group sizes, sums in fp32, rounded once.
+
+    ``w`` (num_experts, K, N) of x's type (float32, bfloat16, float16), with
+    any strides (a transposed view is read as it lies). ``x``: (num_rows, K)
+    in the plan's order, or with ``gather`` (num_tokens, K), where row ``r`` is
+    the token of its choice. Returns (num_rows, N); rows of no expert are
+    zero. Differentiable in ``x`` and ``w``."""
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError(f"grouped_matmul: plan must be an ExpertPlan, got {type(plan).__name__}")
+    _on_gpu("grouped_matmul", x=x, w=w, plan=plan.offsets)
+    _code("grouped_matmul", "x", x.dtype)
+    if w.dtype != x.dtype:
+        raise TypeError(f"grouped_matmul: x is {x.dtype}, w is {w.dtype}")
+    if w.dim() != 3 or w.shape[0] != plan.num_experts:
+        raise ValueError(f"grouped_matmul: w has shape {tuple(w.shape)}, wanted ({plan.num_experts}, K, N)")
+    _check_rows("grouped_matmul", x, "x", plan, gather, w.shape[1])
+    return _GroupedMatmul.apply(_rows(x), w, plan, bool(gather))
+
+
+# ------------------------------------------------------ weighted sum to tokens
+
+def _combine(y, weights, plan, out_dtype):
+    dev = y.device
+    out = torch.empty((plan.num_tokens, y.shape[1]), dtype=out_dtype, device=dev)
+    with _on_device(dev):
+        L.check("es_combine_experts", L.lib().es_combine_experts(
+            y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), weights.data_ptr() if weights is not None else None,
+            plan.position.data_ptr(), plan.num_tokens, plan.top_k, y.shape[1], out.data_ptr(), _DTYPES[out_dtype],
+            stream_ptr(dev)))
+    return out
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, plan):
+        if y.requires_grad or weights.requires_grad:
+            ctx.save_for_backward(y, weights)
+            ctx.plan = plan
+        return _combine(y, weights, plan, y.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        y, weights = ctx.saved_tensors
+        plan = ctx.plan
+        dev = y.device
+        dout = _rows(dout.to(y.dtype))
+        dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
+        dweights = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+        with _on_device(dev):
+            L.check("es_combine_experts_grad", L.lib().es_combine_experts_grad(
+                y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), weights.data_ptr(), plan.position.data_ptr(),
+                plan.offsets.data_ptr() + 4 * plan.num_experts, plan.num_tokens, plan.top_k, y.shape[1],
+                dout.data_ptr(), dout.stride(0), dy.data_ptr(), dweights.data_ptr(), stream_ptr(dev)))
+        return dy, dweights, None
+
+
+def combine_experts(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
+    """``out[t] = sum_j weights[t, j] * y[position[t, j]]``: the weighted sum
+    of each token's rows of ``y`` (num_rows, width), in fp32, rounded once to
+    y's type. ``weights`` float32 (num_tokens, top_k). A choice without a row
+    adds nothing. Differentiable in ``y`` and ``weights``."""
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError(f"combine_experts: plan must be an ExpertPlan, got {type(plan).__name__}")
+    _on_gpu("combine_experts", y=y, weights=weights, plan=plan.offsets)
+    _code("combine_experts", "y", y.dtype)
+    if weights.dtype != torch.float32:
+        raise TypeError(f"combine_experts: weights must be float32, got {weights.dtype}")
+    _check_rows("combine_experts", y, "y", plan, False, None)
+    if weights.shape != plan.position.shape:
+        raise ValueError(f"combine_experts: weights have shape {tuple(weights.shape)}, the plan's choices "
+                         f"{tuple(plan.position.shape)}")
+    return _Combine.apply(_rows(y), weights.contiguous(), plan)
+
+
+# ------------------------------------------------------------ 8-bit products
+
+def quantize_rows(x: torch.Tensor):
+    """``(q, scale)``: each row of ``x`` (rows, width) in 8-bit integers with
+    ``scale = max |x| / 127`` (float32), ``q = rint(x / scale)``. A row of
+    zeros has scale 0; a row with an infinity or NaN has scale NaN."""
+    dev = _on_gpu("quantize_rows", x=x)
+    code = _code("quantize_rows", "x", x.dtype)
+    if x.dim() != 2:
+        raise ValueError(f"quantize_rows: x must be (rows, width), got {tuple(x.shape)}")
+    x = _rows(x.detach())
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    scale = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        L.check("es_quantize_rows", L.lib().es_quantize_rows(
+            x.data_ptr(), code, x.shape[0], x.shape[1], x.stride(0), q.data_ptr(), scale.data_ptr(), stream_ptr(dev)))
+    return q, scale
+
+
+def quantize_experts(w: torch.Tensor):
+    """Weights ``w`` (..., K, N) as ``int8_matmul`` takes them: ``(wq, scale)``
+    with ``wq`` int8 (..., N, K), contiguous along K, and a float32 scale for
+    each output channel (..., N)."""
+    if not isinstance(w, torch.Tensor) or w.dim() < 2:
+        raise ValueError("quantize_experts: w must be a tensor (..., K, N)")
+    wt = w.detach().transpose(-1, -2).contiguous()
+    q, scale = quantize_rows(wt.reshape(-1, wt.shape[-1]))
+    return q.reshape(wt.shape), scale.reshape(wt.shape[:-1])
+
+
+def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: torch.Tensor,
+                plan: ExpertPlan | None = None, gather: bool = False, out_dtype=torch.bfloat16) -> torch.Tensor:
+    """Product of 8-bit integers with scales: ``y[r, n] = scale[r] *
+    wscale[n] * sum_k q[r, k] * wq[n, k]``, the sum exact in 32-bit integers.
+
+    ``q`` int8 (rows, K) and ``scale`` float32 (rows,) as from
+    ``quantize_rows``; ``wq`` int8 (N, K), ``wscale`` float32 (N,). With a
+    ``plan`` the products are grouped by expert as in ``grouped_matmul``:
+    ``wq`` (num_experts, N, K), ``wscale`` (num_experts, N), and with
+    ``gather`` ``q`` and ``scale`` are by token. Returns (rows, N) of
+    ``out_dtype`` (float32, bfloat16, float16). K is at most 133,152."""
+    dev = _on_gpu("int8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=plan.offsets if plan is not None else None)
+    code = _code("int8_matmul", "out_dtype", out_dtype)
+    if q.dtype != torch.int8 or wq.dtype != torch.int8:
+        raise TypeError(f"int8_matmul: q and wq must be int8, got {q.dtype} and {wq.dtype}")
+    if scale.dtype != torch.float32 or wscale.dtype != torch.float32:
+        raise TypeError(f"int8_matmul: scale and wscale must be float32, got {scale.dtype} and {wscale.dtype}")
+    E = plan.num_experts if plan is not None else 0
+    if wq.dim() != (3 if E else 2) or (E and wq.shape[0] != E) or wscale.shape != wq.shape[:-1]:
+        raise ValueError(f"int8_matmul: wq {tuple(wq.shape)} and wscale {tuple(wscale.shape)} are not "
+                         + (f"({E}, N, K) and ({E}, N)" if E else "(N, K) and (N,)"))
+    N, K = wq.shape[-2], wq.shape[-1]
+    if plan is not None:
+        _check_rows("int8_matmul", q, "q", plan, gather, K)
+    elif gather or q.dim() != 2 or q.shape[1] != K:
+        raise ValueError(f"int8_matmul: q has shape {tuple(q.shape)}, wanted (rows, {K}); gather needs a plan")
+    if scale.dim() != 1 or scale.shape[0] != q.shape[0]:
+        raise ValueError(f"int8_matmul: scale has shape {tuple(scale.shape)}, wanted ({q.shape[0]},)")
+    if K > MAX_INT8_DEPTH:
+        raise ValueError(f"int8_matmul: K={K} is over {MAX_INT8_DEPTH}, where 32-bit sums can overflow")
+    q, scale, wscale = _rows(q), scale.contiguous(), wscale.contiguous()
+    if wq.stride(-1) != 1 or wq.stride(-2) < K:
+        wq = wq.contiguous()
+    R = plan.num_rows if plan is not None else q.shape[0]
+    y = torch.empty((R, N), dtype=out_dtype, device=dev)
+    lib = L.lib()
+    nbytes = lib.es_int8_matmul_workspace_size(E, K, N, R)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    off, order = _plan_args(plan, gather) if plan is not None else (None, None)
+    with _on_device(dev):
+        L.check("es_int8_matmul", lib.es_int8_matmul(
+            q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(), wscale.data_ptr(), E, K, N,
+            wq.stride(0) if E else 0, wq.stride(-2), off, order, plan.top_k if plan is not None else 1, R,
+            y.data_ptr(), code, ws.data_ptr() if ws is not None else None, nbytes,
+            _STATUS.address("es_int8_matmul", dev.index), stream_ptr(dev)))
+    return y
+
+
+# ----------------------------------------------------------- a layer of experts
+
+def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, renormalize: bool = True):
+    """A gated layer of experts: for each token ``x`` (num_tokens, D) the
+    weighted sum, over its ``top_k`` experts ``e``, of
+    ``(silu(x @ gate_e) * (x @ up_e)) @ w_out_e``.
+
+    ``router`` (D, num_experts). ``w_in`` (num_experts, D, 2 F) holds gate and
+    up side by side, ``w_out`` (num_experts, F, D): tensors of x's type for
+    training (differentiable in everything), or both ``(wq, scale)`` pairs
+    of ``quantize_experts`` for serving in 8-bit integers."""
+    quantized = isinstance(w_in, (tuple, list))
+    if quantized != isinstance(w_out, (tuple, list)):
+        raise TypeError("expert_mlp: w_in and w_out must both be tensors or both be (wq, scale) pairs")
+    logits = x.float() @ router.float()
+    weights, experts = route_experts(logits, top_k, renormalize)
+    plan = plan_experts(experts, router.shape[1])
+    if quantized:
+        h = int8_matmul(*quantize_rows(x), *w_in, plan, gather=True, out_dtype=x.dtype)
+    else:
+        h = grouped_matmul(x, w_in, plan, gather=True)
+    gate, up = h.chunk(2, dim=1)
+    h = torch.nn.functional.silu(gate) * up
+    y = int8_matmul(*quantize_rows(h), *w_out, plan, out_dtype=x.dtype) if quantized else \
+        grouped_matmul(h, w_out, plan)
+    return combine_experts(y, weights, plan)

@@ -127,6 +127,43 @@ class _DeferredErrors:
 _DEFERRED = _DeferredErrors()
 
 
+class _StatusWords:
+    """One pinned int32 per operator that its kernels write when they fail (a
+    choice of an expert that does not exist, a bounded wait that ran out) and
+    leave alone otherwise: no copy, event or wait of a call's own.
+    ``check_device_errors`` waits for the devices that ran such calls and
+    raises for the first word that is set."""
+
+    def __init__(self):
+        self.words = {}  # function name -> (pinned tensor, address)
+        self.devices = set()
+
+    def address(self, fn: str, device_index: int) -> int:
+        self.devices.add(device_index)
+        try:
+            return self.words[fn][1]
+        except KeyError:
+            word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            self.words[fn] = (word, word.data_ptr())
+            return self.words[fn][1]
+
+    def flush(self) -> None:
+        devices, self.devices = self.devices, set()
+        for d in devices:
+            torch.cuda.synchronize(d)
+        first = None
+        for fn, (word, _) in self.words.items():
+            e = int(word[0])
+            word[0] = 0
+            if e and first is None:
+                first = (fn, e)
+        if first is not None:
+            L.check(first[0] + " (device)", first[1])
+
+
+_STATUS = _StatusWords()
+
+
 def defer_device_error(fn: str, err: torch.Tensor) -> None:
     """Check ``err`` (device int32 status) at the next count read or
     ``check_device_errors`` instead of now."""
@@ -138,6 +175,7 @@ def check_device_errors() -> None:
     for the first failure (``ValueError`` for bad input, ``EinsparseError``
     otherwise, e.g. a bounded wait that ran out)."""
     _DEFERRED.flush()
+    _STATUS.flush()
 
 
 class _PendingFills:

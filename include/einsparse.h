@@ -39,7 +39,7 @@ typedef enum es_status {
   ES_ERR_TIMEOUT = 6      /* a bounded device-side wait ran out; outputs are invalid */
 } es_status;
 
-typedef enum es_dtype { ES_F32 = 0, ES_BF16 = 1, ES_F64 = 2, ES_I32 = 3, ES_I64 = 4 } es_dtype;
+typedef enum es_dtype { ES_F32 = 0, ES_BF16 = 1, ES_F64 = 2, ES_I32 = 3, ES_I64 = 4, ES_F16 = 5 } es_dtype;
 
 /* Arithmetic of the tile contraction. EXACT: fp32 FFMA (SIMT); TC: tensor
  * cores (bf16 inputs: kind::f16; fp32 inputs: 3-pass split TF32, fp32-level
@@ -366,6 +366,93 @@ int es_sparsity_stats(const int32_t* indices, const void* values, int values_dty
                       const int64_t* shape, const int64_t* tile_shapes, int num_schemes, void* workspace,
                       size_t workspace_bytes, int64_t* num_tuples_dev, int64_t* value_count_dev,
                       int32_t* error_dev, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Mixture of experts: a contraction with a token x expert matrix of top_k
+ * nonzeros a row, whose blocks are ragged in the token axis. No reference
+ * counterpart (its relations have fixed tiles).
+ *
+ * num_tokens tokens choose top_k (<= 32) of num_experts (<= 1024) experts;
+ * choice a = token * top_k + j. Row r of the grouped order belongs to choice
+ * order[r]; expert e owns the rows offsets[e] to offsets[e + 1] (int32,
+ * num_experts + 1); position[a] is the row of choice a. A choice of no expert
+ * (-1) has no row (position -1); the rows from offsets[num_experts] on are
+ * empty (order -1) and are zero in every output. Value types: ES_F32,
+ * ES_BF16, ES_F16; sums in fp32, rounded once. Row strides are in elements,
+ * the last dimension is contiguous. Offsets, orders and positions are bounded
+ * on the device: what points outside is left out. `status` (may be NULL) is
+ * an int32 that the device can write, pinned host memory included: it is left
+ * alone unless the call fails on the device (ES_ERR_INDEX, ES_ERR_TIMEOUT).
+ * ------------------------------------------------------------------------- */
+
+/* The top_k largest logits of each token, largest first, ties to the lowest
+ * expert, and their weights: exp(logit - max) over its sum, over the chosen
+ * experts (renormalize != 0) or over all. -inf masks an expert: where fewer
+ * than top_k are left the choice is -1 with weight 0. A NaN logit is never
+ * chosen and makes every weight of its token NaN. */
+int es_route_experts(const void* logits, int dtype, int64_t num_tokens, int num_experts, int64_t row_stride,
+                     int top_k, int renormalize, float* weights, int32_t* experts, void* stream);
+/* dlogits (num_tokens, num_experts) contiguous, of the logits' type, from the
+ * weights and experts of es_route_experts on the same logits. */
+int es_route_experts_grad(const void* logits, int dtype, int64_t num_tokens, int num_experts, int64_t row_stride,
+                          int top_k, int renormalize, const float* weights, const int32_t* experts,
+                          const float* dweights, void* dlogits, void* stream);
+
+/* offsets, order and position of num_choices choices (int32, -1: none), in
+ * ascending choice inside an expert. A choice outside [-1, num_experts) counts
+ * as -1 and sets *status to ES_ERR_INDEX. */
+size_t es_expert_plan_workspace_size(int64_t num_choices, int num_experts);
+int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts, void* workspace,
+                   size_t workspace_bytes, int32_t* offsets, int32_t* order, int32_t* position, int32_t* status,
+                   void* stream);
+
+/* y[r] = x[row(r)] w[e(r)] for the num_rows grouped rows: w[e] is (K, N) with
+ * any element strides, row(r) = order[r] / top_k when order is given (x by
+ * token), else r. y (num_rows, N) contiguous, of out_dtype (ES_F32 or the
+ * operands' type). */
+size_t es_grouped_matmul_workspace_size(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows);
+int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w, int num_experts,
+                      int64_t K, int64_t N, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
+                      const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, void* y,
+                      int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* dw[e] = sum over e's rows of x[row(r)]^T dy[r], with dw's element strides;
+ * zero for an expert without rows. dw has the operands' type. */
+size_t es_grouped_matmul_wgrad_workspace_size(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows);
+int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* dy,
+                            int64_t dy_stride, int num_experts, int64_t K, int64_t N, const int32_t* offsets,
+                            const int32_t* order, int top_k, int64_t num_rows, void* dw, int64_t dw_expert_stride,
+                            int64_t dw_k_stride, int64_t dw_n_stride, void* workspace, size_t workspace_bytes,
+                            int32_t* status, void* stream);
+
+/* out[t] = sum_j weights[t, j] y[position[t, j]] (weights NULL: 1), y
+ * (num_rows, width). out (num_tokens, width) contiguous, of out_dtype: y's
+ * type, or any when y is ES_F32. */
+int es_combine_experts(const void* y, int dtype, int64_t num_rows, int64_t row_stride, const float* weights,
+                       const int32_t* position, int64_t num_tokens, int top_k, int64_t width, void* out,
+                       int out_dtype, void* stream);
+/* dy[position[t, j]] = weights[t, j] dout[t] and dweights[t, j] = <dout[t],
+ * y[position[t, j]]>, zero for -1; kept_rows: device int32, the rows that
+ * have a choice (offsets + num_experts), the rows from there on are zeroed.
+ * Every row below *kept_rows is the position of one choice. dy contiguous. */
+int es_combine_experts_grad(const void* y, int dtype, int64_t num_rows, int64_t row_stride, const float* weights,
+                            const int32_t* position, const int32_t* kept_rows, int64_t num_tokens, int top_k,
+                            int64_t width, const void* dout, int64_t dout_stride, void* dy, float* dweights,
+                            void* stream);
+
+/* q[r, i] = rint(x[r, i] / scale[r]), scale[r] = max |x[r]| / 127 in fp32. A
+ * row of zeros has scale 0; a row with an infinity or NaN has scale NaN. */
+int es_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t width, int64_t row_stride, int8_t* q,
+                     float* scale, void* stream);
+
+/* y[r, n] = x_scale[row(r)] w_scale[e(r), n] sum_k q[row(r), k] wq[e(r), n, k],
+ * the sum exact in 32-bit integers (K <= 133152). wq: (num_experts, N, K) int8
+ * with contiguous k, w_scale (num_experts, N). num_experts == 0: one matrix
+ * for all rows (offsets and order NULL). y (num_rows, N) contiguous. */
+size_t es_int8_matmul_workspace_size(int num_experts, int64_t K, int64_t N, int64_t num_rows);
+int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride, const int8_t* wq,
+                   const float* w_scale, int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
+                   int64_t w_n_stride, const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows,
+                   void* y, int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }
