@@ -238,6 +238,7 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
   if (num_rows == 0 || N == 0) return ES_OK;
   if (!y || (K && ((x_rows && !x) || !w))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
+  if (grouped_rows_tc_ok(g, dtype, x, w)) return grouped_rows_tc(g, dtype, x, w, y, out_dtype, status, s);
   if (out_dtype == dtype) ES_BY_TYPE(dtype, return (rows_simt<T, T>(g, x, w, y, s)));
   ES_BY_TYPE(dtype, return (rows_simt<T, float>(g, x, w, y, s)));
   return ES_ERR_UNSUPPORTED;
@@ -259,6 +260,8 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
   ES_TRY(check_args(g));
   if (K == 0 || N == 0) return ES_OK;
   if (!dw || (num_rows && (!dy || (x_rows && !x)))) return ES_ERR_INVALID;
+  if (grouped_wgrad_tc_ok(g, dtype, x, dy, dy_stride))
+    return grouped_wgrad_tc(g, dtype, x, dy, dy_stride, dw, status, as_stream(stream));
   const int64_t kt = (K + kTile - 1) / kTile, nt = (N + kTile - 1) / kTile;
   if (nt > 65535) return ES_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(kt), static_cast<unsigned>(nt), static_cast<unsigned>(num_experts));
@@ -285,6 +288,8 @@ extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_r
   if (num_rows == 0 || N == 0) return ES_OK;
   if (!y || !w_scale || (x_rows && !x_scale) || (K && ((x_rows && !q) || !wq))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
+  if (out_dtype != ES_F32 && out_dtype != ES_BF16 && out_dtype != ES_F16) return ES_ERR_UNSUPPORTED;
+  if (grouped_rows_tc_ok(g, kInt8, q, wq)) return grouped_rows_tc(g, kInt8, q, wq, y, out_dtype, status, s);
   ES_BY_TYPE(out_dtype, return (rows_simt<int8_t, T>(g, q, wq, y, s)));
   return ES_ERR_UNSUPPORTED;
 }

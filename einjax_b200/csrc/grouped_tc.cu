@@ -1,0 +1,993 @@
+// Products grouped by expert on the tensor cores (tcgen05 + TMEM + TMA), with
+// ragged group sizes: the rows' product (forward, and the gradient of the
+// rows with the weights read transposed), the weights' gradient, and the
+// product of 8-bit integers.
+//
+// Orientation. The 128 lanes of the accumulator (256 for a pair of CTAs) are
+// the dimension that never is ragged, the output channels; the columns are a
+// group's rows:  D[channel, row] = sum_k W[channel, k] X[row, k].  The width
+// of an MMA (a multiple of 16, or 32 for a pair) is set tile by tile to the
+// rows that are left, so a group of 3 rows costs a 16-wide MMA and no padding,
+// and one kernel serves a decode step and a long prompt. For the weights'
+// gradient lanes and columns are its two dimensions and the sum runs over the
+// group's rows; of a group's last block only whole 16-row steps that hold rows
+// are multiplied, and TMA gathers that block row by row with the missing rows
+// pointing outside of the tensor, which reads zeros (so that infinities of the
+// next group stay out of it).
+//
+// Operands are read as they lie: K-major or MN-major, through 128-byte
+// swizzled TMA boxes; routed tokens by TMA row gathers (tile::gather4), with
+// no copy of the rows in between.
+//
+// Roles (8 warps): warp 0 issues the TMA loads, warp 1 the MMAs (one lane),
+// warps 2-3 clear the output rows of no expert, warps 4-7 read the
+// accumulator (TMEM lane quadrant = warp % 4) and write the output. Tiles are
+// dealt to the CTAs in turn; the accumulator is double buffered, so a tile's
+// epilogue runs under the next tile's MMAs. Every wait is bounded: when one
+// runs out the CTA sets ES_ERR_TIMEOUT, drains its copies and MMAs, frees
+// TMEM and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cstring>
+
+#include "grouped.cuh"
+#include "tc_ptx.cuh"
+
+namespace es {
+namespace {
+
+constexpr int kTcThreads = 256;
+constexpr int kEpiWarps = 4;
+constexpr int kABytes = 16384;  // 128 lanes x 128 bytes of depth
+constexpr int kSwizzleRow = 128;
+constexpr int kBoxRows = 32;    // rows of one TMA box of X
+constexpr int kTileBlock = 8;   // row tiles that share a channel tile's weights in L2
+constexpr int kMaxTcStages = 8;
+constexpr uint64_t kTcWaitNs = 2000000000ull;
+constexpr uint64_t kTcDrainNs = 100000000ull;
+
+enum { kKindF16 = 0, kKindI8 = 1 };
+
+struct TcArgs {
+  GroupedArgs g;
+  void* out;
+  int out_dtype;
+  int64_t lanes;      // extent of the lane dimension
+  int64_t cols;       // extent of the column dimension (weights' gradient)
+  int64_t out_col;    // output stride of a column (rows: of a row)
+  int64_t out_expert; // output stride of an expert (weights' gradient)
+  int lane_tiles, col_tiles;
+  int expert_step;    // 0: every expert has the same matrix
+  int gather_a, gather_b;  // operands that are gathered through g.order
+  int a_rows, b_rows;      // rows of the gathered tensors: this index reads zeros
+  uint32_t idesc;     // instruction descriptor without N
+  int pairs;          // two neighbouring lanes may be stored together
+  int32_t* status;
+};
+
+struct TcCtl {
+  uint64_t full[kMaxTcStages];
+  uint64_t empty[kMaxTcStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t red_full, red_empty;
+  uint64_t drain;
+  uint32_t tmem;
+  int abort;
+  uint32_t progress;
+};
+
+// ------------------------------------------------------------------ PTX glue
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Address of this CTA's shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t at_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ float load_at(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// Bounded wait; false when this CTA has given up. `progress`: a counter whose
+// movement shows that the wait is long and not stuck.
+__device__ bool tc_wait(uint64_t* bar, uint32_t parity, TcCtl* ctl, int32_t* status, bool progress = false) {
+  if (try_wait_cluster(bar, parity)) return true;
+  uint64_t t0 = global_ns();
+  uint32_t seen = *reinterpret_cast<volatile uint32_t*>(&ctl->progress);
+  for (uint32_t i = 1;; ++i) {
+    if (try_wait_cluster(bar, parity)) return true;
+    if ((i & 31) == 0) {
+      if (*reinterpret_cast<volatile int*>(&ctl->abort)) return false;
+      const uint64_t now = global_ns();
+      const uint32_t cur = *reinterpret_cast<volatile uint32_t*>(&ctl->progress);
+      if (progress && cur != seen) {
+        seen = cur;
+        t0 = now;
+      }
+      if (now - t0 > kTcWaitNs) break;
+    }
+  }
+  *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
+  if (status) *reinterpret_cast<volatile int32_t*>(status) = ES_ERR_TIMEOUT;
+  return false;
+}
+
+__device__ void tc_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = global_ns();
+  for (uint32_t i = 0;; ++i) {
+    if (try_wait_cluster(bar, parity)) return;
+    if ((i & 31) == 0 && global_ns() - t0 > kTcDrainNs) return;
+  }
+}
+
+// TMA loads; bar is a shared::cluster address (the leader's barrier, for a
+// pair of CTAs), which needs the cta_group::2 form.
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+// Four rows of a tensor into four consecutive 128-byte rows.
+template <int CG>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int x, const int (&r)[4],
+                                          uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(bar)
+        : "memory");
+}
+
+template <int CG, int KIND>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+#define ES_MMA(group, kind)                                                                            \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                       \
+               "tcgen05.mma.cta_group::" #group ".kind::" #kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+               "l"(a), "l"(b), "r"(idesc), "r"(accum)                                                  \
+               : "memory")
+  if constexpr (CG == 2 && KIND == kKindF16) ES_MMA(2, f16);
+  if constexpr (CG == 2 && KIND == kKindI8) ES_MMA(2, i8);
+  if constexpr (CG == 1 && KIND == kKindF16) ES_MMA(1, f16);
+  if constexpr (CG == 1 && KIND == kKindI8) ES_MMA(1, i8);
+#undef ES_MMA
+}
+
+// Arrives on the barrier (of both CTAs of a pair) when the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+  else
+    umma_commit(bar);
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_alloc(uint32_t* slot, uint32_t ncols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(slot, ncols);
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tc_dealloc(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+  else
+    tmem_dealloc(taddr, ncols);
+}
+
+// Descriptor of an operand in 128-byte swizzled rows. K-major: rows of depth,
+// 8-row groups 1024 bytes apart. MN-major: rows of 64 lanes, one row for each
+// k; 8-k groups 1024 bytes apart, the next 64 lanes one box (64 k) on.
+__device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
+  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(mn ? 8192 >> 4 : 1) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// ------------------------------------------------------------------- kernel
+
+template <int CG_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_>
+struct TcShape {
+  static constexpr int CG = CG_;        // CTAs of one MMA
+  static constexpr int NT = NT_;        // widest MMA
+  static constexpr int KIND = KIND_;
+  static constexpr bool A_MN = A_MN_;   // lanes contiguous in memory
+  static constexpr bool WGRAD = WGRAD_;
+  static constexpr bool SPLIT = SPLIT_; // the cluster's CTAs share one tile's depth
+  static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
+  static constexpr int kLanes = 128 * CG;
+  static constexpr int kStageBytes = kABytes + NT / CG * kSwizzleRow;
+  static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
+  static constexpr int kStages =
+      (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
+};
+
+// One output tile, and what of its depth this CTA multiplies.
+struct TileAt {
+  int expert;
+  int64_t lane0;
+  int row0;    // first row (rows) or first column (weights' gradient)
+  int rows;    // rows or columns of the tile
+  int first;   // weights' gradient: the group's first row
+  int depth;   // depth of the product
+  int kb0, kb1;
+};
+
+template <typename S>
+struct Tiles {
+  const TcArgs& p;
+  const int* pre;   // [groups + 1] tiles before each group
+  const int* lo;    // [groups]
+  const int* cnt;   // [groups]
+  int total;
+
+  __device__ __forceinline__ TileAt at(int t, uint32_t rank, uint32_t split) const {
+    TileAt r;
+    int depth;
+    int group, idx, tt;
+    if constexpr (S::WGRAD) {
+      const int per = p.lane_tiles * p.col_tiles;
+      group = t / per;
+      idx = t - group * per;
+      tt = p.col_tiles;
+    } else {
+      int a = 0, b = p.g.groups();
+      while (b - a > 1) {
+        const int m = (a + b) >> 1;
+        if (pre[m] <= t) a = m;
+        else b = m;
+      }
+      group = a;
+      idx = t - pre[a];
+      tt = (cnt[a] + S::NT - 1) / S::NT;
+    }
+    // blocks of kTileBlock column tiles walk the lane tiles together
+    const int block = idx / (kTileBlock * p.lane_tiles);
+    const int in = idx - block * kTileBlock * p.lane_tiles;
+    const int w = min(kTileBlock, tt - block * kTileBlock);
+    const int lane_tile = in / w, col_tile = block * kTileBlock + in % w;
+    r.expert = group;
+    r.lane0 = static_cast<int64_t>(lane_tile) * S::kLanes;
+    if constexpr (S::WGRAD) {
+      r.row0 = col_tile * S::NT;
+      r.rows = static_cast<int>(min(p.cols - r.row0, static_cast<int64_t>(S::NT)));
+      r.first = lo[group];
+      depth = cnt[group];
+    } else {
+      r.row0 = lo[group] + col_tile * S::NT;
+      r.rows = min(cnt[group] - col_tile * S::NT, S::NT);
+      r.first = 0;
+      depth = static_cast<int>(p.g.K);
+    }
+    r.depth = depth;
+    const int nkb = (depth + S::BK - 1) / S::BK;
+    if constexpr (S::SPLIT) {
+      r.kb0 = static_cast<int>(static_cast<int64_t>(nkb) * rank / split);
+      r.kb1 = static_cast<int>(static_cast<int64_t>(nkb) * (rank + 1) / split);
+    } else {
+      r.kb0 = 0;
+      r.kb1 = nkb;
+    }
+    return r;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// Stores v[c] (lane = this thread's channel) to out + c * stride, c < n. In
+// 16 bits two neighbouring lanes trade values, so that each stores two
+// channels of every other column: 4-byte stores, half as many.
+template <typename T>
+__device__ __forceinline__ void store_cols(T* out, int64_t stride, const float (&v)[32], int n, bool live,
+                                           bool pairs) {
+  if constexpr (sizeof(T) == 2) {
+    if (pairs) {
+      const int odd = threadIdx.x & 1;
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const float give = odd ? v[c] : v[c + 1];
+        const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+        if (live && c + odd < n) {
+          const uint32_t two = odd ? pack2<T>(got, v[c + 1]) : pack2<T>(v[c], got);
+          *reinterpret_cast<uint32_t*>(out - odd + (c + odd) * stride) = two;
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 32; ++c)
+    if (live && c < n) out[c * stride] = from_f32<T>(v[c]);
+}
+
+__device__ __forceinline__ void store_typed(void* out, int dtype, int64_t at, int64_t stride, const float (&v)[32],
+                                            int n, bool live, bool pairs) {
+  if (dtype == ES_BF16)
+    store_cols(static_cast<__nv_bfloat16*>(out) + at, stride, v, n, live, pairs);
+  else if (dtype == ES_F16)
+    store_cols(static_cast<__half*>(out) + at, stride, v, n, live, pairs);
+  else
+    store_cols(static_cast<float*>(out) + at, stride, v, n, live, false);
+}
+
+__device__ __forceinline__ void store_one(void* out, int dtype, int64_t at, float v) {
+  if (dtype == ES_BF16)
+    static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16(v);
+  else if (dtype == ES_F16)
+    static_cast<__half*>(out)[at] = __float2half(v);
+  else
+    static_cast<float*>(out)[at] = v;
+}
+
+// Clears the output rows [from, to) with the threads `t` of `nt`.
+__device__ __forceinline__ void clear_rows(const TcArgs& p, int64_t from, int64_t to, int64_t t, int64_t nt) {
+  const int64_t esz = p.out_dtype == ES_F32 ? 4 : 2;
+  char* a = static_cast<char*>(p.out) + from * p.g.N * esz;
+  char* b = static_cast<char*>(p.out) + to * p.g.N * esz;
+  const int64_t halves = (b - a) / 2;
+  const int64_t head = min(halves, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(a) & 15)) & 15) / 2);
+  for (int64_t i = t; i < head; i += nt) reinterpret_cast<uint16_t*>(a)[i] = 0;
+  uint4* mid = reinterpret_cast<uint4*>(a + head * 2);
+  const int64_t n = (halves - head) / 8;
+  for (int64_t i = t; i < n; i += nt) mid[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t i = head + n * 8 + t; i < halves; i += nt) reinterpret_cast<uint16_t*>(a)[i] = 0;
+}
+
+template <typename S>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    grouped_tc_kernel(const __grid_constant__ TcArgs p, const __grid_constant__ CUtensorMap map_a,
+                      const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap rows_a,
+                      const __grid_constant__ CUtensorMap rows_b) {
+  constexpr int CG = S::CG, NT = S::NT, BK = S::BK, STAGES = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ TcCtl ctl;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  float* part = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + STAGES * S::kStageBytes);
+  int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(part) + S::kPartBytes);
+  const int groups = p.g.groups();
+  int* lo = pre + groups + 1;
+  int* cnt = lo + groups;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank(), csize = cluster_size();
+  const uint32_t pair_rank = CG == 2 ? rank : 0;
+  const bool leader = pair_rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ctl.acc_full[b], 1);
+      mbar_init(&ctl.acc_empty[b], CG * kEpiWarps);
+    }
+    mbar_init(&ctl.red_full, csize * kEpiWarps);
+    mbar_init(&ctl.red_empty, csize * kEpiWarps);
+    mbar_init(&ctl.drain, 1);
+    ctl.abort = 0;
+    ctl.progress = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc_alloc<CG>(&ctl.tmem, 2 * NT);
+  if (warp == 2) {  // tiles of each group
+    int run = 0;
+    for (int e0 = 0; e0 < groups; e0 += 32) {
+      const int e = e0 + lane;
+      int64_t a = 0, b = 0;
+      if (e < groups) p.g.bounds(e, a, b);
+      const int n = static_cast<int>(b - a);
+      const int tiles = S::WGRAD ? 0 : (n + NT - 1) / NT * p.lane_tiles;
+      int s = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += u;
+      }
+      if (e < groups) {
+        pre[e] = run + s - tiles;
+        lo[e] = static_cast<int>(a);
+        cnt[e] = n;
+      }
+      run += __shfl_sync(0xffffffffu, s, 31);
+    }
+    if (lane == 0) pre[groups] = run;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (csize > 1) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = ctl.tmem;
+  const Tiles<S> tiles{p, pre, lo, cnt, S::WGRAD ? groups * p.lane_tiles * p.col_tiles : pre[groups]};
+  const int step = static_cast<int>(gridDim.x / csize), t0 = static_cast<int>(blockIdx.x / csize);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA loads
+    int stage = 0, used = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = t0; t < tiles.total && ok; t += step) {
+      const TileAt at = tiles.at(t, rank, csize);
+      const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
+      const int half = width / CG;  // columns of this CTA's part of B
+      const int64_t lane0 = at.lane0 + pair_rank * 128;
+      const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
+      int src[4];  // rows (gathered): this lane's four tokens
+      if constexpr (!S::WGRAD)
+        if (p.gather_b) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int c = lane * 4 + i;
+            int64_t r = -1;
+            if (c < half && static_cast<int>(pair_rank) * half + c < at.rows) r = p.g.source(col0 + c);
+            src[i] = r < 0 ? p.b_rows : static_cast<int>(r);
+          }
+        }
+      for (int kb = at.kb0; kb < at.kb1; ++kb) {
+        int valid = BK, rows16 = BK;
+        int ra[4], rb[4];  // weights' gradient: rows of a gathered block
+        bool ga = false, gb = false;
+        if constexpr (S::WGRAD) {
+          valid = min(at.depth - kb * BK, BK);
+          rows16 = (valid + 15) & ~15;
+          ga = p.gather_a || valid < BK;
+          gb = p.gather_b || valid < BK;
+          if (ga || gb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = (lane & 15) * 4 + i;
+              const int64_t row = at.first + static_cast<int64_t>(kb) * BK + r;
+              int64_t sa = -1;
+              if (r < valid) sa = (p.gather_a || p.gather_b) ? p.g.source(row) : row;
+              ra[i] = r < valid ? static_cast<int>(p.gather_a ? (sa < 0 ? p.a_rows : sa) : row) : p.a_rows;
+              rb[i] = r < valid ? static_cast<int>(p.gather_b ? (sa < 0 ? p.b_rows : sa) : row) : p.b_rows;
+            }
+          }
+        }
+        uint32_t bytes;
+        if constexpr (S::WGRAD) {
+          const int boxes_b = (half + 63) / 64;
+          bytes = 2u * (ga ? rows16 : BK) * 128 + boxes_b * (gb ? rows16 : BK) * 128u;
+        } else {
+          bytes = kABytes + (p.gather_b ? (half + 3) / 4 * 512u : (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u));
+        }
+        int go = 0;
+        if (lane == 0) {
+          go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+          if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
+          if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+        }
+        go = __shfl_sync(0xffffffffu, go, 0);
+        if (!go) {
+          ok = false;
+          break;
+        }
+        const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
+        const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
+        if constexpr (S::WGRAD) {
+          // operand boxes of 64 lanes (columns) by 64 rows; a gathered box
+          // is 16 loads of four rows, dealt to half a warp
+          const int row = at.first + kb * BK;
+          const int half16 = lane >> 4, quad = lane & 15;
+          if (ga) {
+            if (quad * 4 < rows16)
+              load_rows<CG>(sa + half16 * 8192 + quad * 512, &rows_a, static_cast<int>(lane0) + half16 * 64, ra, bar);
+          } else if (lane < 2) {
+            load_2d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, row, bar);
+          }
+          const int boxes = (half + 63) / 64;
+          if (gb) {
+            for (int b = half16; b < boxes; b += 2)
+              if (quad * 4 < rows16) load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
+          } else if (lane >= 2 && lane - 2 < boxes) {
+            load_2d<CG>(sb + (lane - 2) * 8192, &map_b, col0 + (lane - 2) * 64, row, bar);
+          }
+        } else {
+          const int z = at.expert * p.expert_step;
+          if constexpr (S::A_MN) {
+            if (lane < 2) load_3d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, kb * BK, z, bar);
+          } else {
+            if (lane == 0) load_3d<CG>(sa, &map_a, kb * BK, static_cast<int>(lane0), z, bar);
+          }
+          if (p.gather_b) {
+            if (lane * 4 < half) load_rows<CG>(sb + lane * 512, &rows_b, kb * BK, src, bar);
+          } else if (lane * kBoxRows < half) {
+            load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK, col0 + lane * kBoxRows, bar);
+          }
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (lane == 0) {
+      // the stages still held: their MMAs have arrived here before this CTA may end
+      for (int s = 0; s < STAGES && ok; ++s) {
+        if (s < used) {
+          const int last = (stage + STAGES - 1 - s) % STAGES;
+          const uint32_t ph = last < stage ? phase : phase ^ 1;
+          ok = tc_wait(&ctl.empty[last], ph, &ctl, p.status);
+        }
+      }
+      if (!ok && leader)
+        for (int s = 0; s < STAGES && s < used; ++s) {
+          const int last = (stage + STAGES - 1 - s) % STAGES;
+          tc_drain(&ctl.full[last], last < stage ? phase : phase ^ 1);
+        }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMAs
+    if (leader && lane == 0) {
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = t0; t < tiles.total && ok; t += step) {
+        const TileAt at = tiles.at(t, rank, csize);
+        if (at.kb0 == at.kb1) continue;
+        const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
+        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
+        ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * NT;
+        for (int kb = at.kb0; kb < at.kb1; ++kb) {
+          ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sa = base + stage * S::kStageBytes;
+          const uint64_t da = operand(sa, S::A_MN), db = operand(sa + kABytes, S::WGRAD);
+          constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
+          int steps = 4;
+          if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+          if (steps == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, kb > at.kb0 || i > 0);
+          } else {
+            for (int i = 0; i < steps; ++i)
+              mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, kb > at.kb0 || i > 0);
+          }
+          commit<CG>(&ctl.empty[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        commit<CG>(&ctl.acc_full[buf]);
+        if (++buf == 2) {
+          buf = 0;
+          acc_phase ^= 1;
+        }
+      }
+      if (!ok) {
+        commit<CG>(&ctl.drain);
+        tc_drain(&ctl.drain, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    if constexpr (!S::WGRAD)  // rows of no expert
+      clear_rows(p, p.g.kept(), p.g.rows, blockIdx.x * 64LL + (threadIdx.x - 64), gridDim.x * 64LL);
+  } else {
+    // ------------------------------------------------------------- epilogue
+    const int quad = warp & 3;
+    int buf = 0;
+    uint32_t acc_phase = 0, red_phase = 0;
+    for (int t = t0; t < tiles.total; t += step) {
+      const TileAt at = tiles.at(t, rank, csize);
+      const int64_t ch = at.lane0 + pair_rank * 128 + quad * 32 + lane;
+      const bool live = ch < p.lanes;
+      const bool any = at.kb0 < at.kb1;
+      if (any) {
+        int go = 0;
+        if (lane == 0) go = tc_wait(&ctl.acc_full[buf], acc_phase, &ctl, p.status, true) ? 1 : 0;
+        if (!__shfl_sync(0xffffffffu, go, 0)) break;
+        tc_fence_after();
+      }
+      float wscale = 1.0f;
+      if constexpr (S::KIND == kKindI8) wscale = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
+      const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16);
+      if constexpr (S::SPLIT) {
+        // this CTA's part of the sum into shared memory, [column][lane]
+        int go = 1;
+        if (lane == 0) go = tc_wait(&ctl.red_empty, red_phase ^ 1, &ctl, p.status, true) ? 1 : 0;
+        if (!__shfl_sync(0xffffffffu, go, 0)) break;
+        for (int c0 = 0; c0 < at.rows; c0 += 32) {
+          float v[32];
+          if (any) {
+            tmem_ld32(acc + c0, v);
+            if constexpr (S::KIND == kKindI8) {
+              // the parts stay integers (their bits travel as floats): the sum is exact
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c0 + i < at.rows) part[(c0 + i) * 128 + quad * 32 + lane] = v[i];
+        }
+        if (any) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), rank));
+        }
+        __syncwarp();
+        if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_full), lane));
+        go = 1;
+        if (lane == 0) go = tc_wait(&ctl.red_full, red_phase, &ctl, p.status, true) ? 1 : 0;
+        if (!__shfl_sync(0xffffffffu, go, 0)) break;
+        // columns rank, rank + csize, ...: the parts are added in the CTAs' order
+        for (int c = rank; c < at.rows; c += csize) {
+          const uint32_t mine = smem_u32(part + c * 128 + quad * 32 + lane);
+          float v = 0.0f;
+          if constexpr (S::KIND == kKindI8) {
+            int sum = 0;
+            for (uint32_t r = 0; r < csize; ++r) sum += __float_as_int(load_at(at_rank(mine, r)));
+            const int64_t tok = p.g.source(at.row0 + c);
+            v = tok >= 0 ? static_cast<float>(sum) * p.g.x_scale[tok] * wscale : 0.0f;
+          } else {
+            for (uint32_t r = 0; r < csize; ++r) v += load_at(at_rank(mine, r));
+          }
+          if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch, v);
+        }
+        __syncwarp();
+        if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
+        red_phase ^= 1;
+      } else {
+        const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col + ch;
+        for (int c0 = 0; c0 < at.rows; c0 += 32) {
+          float v[32];
+          if (any) {
+            tmem_ld32(acc + c0, v);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+          }
+          if constexpr (S::KIND == kKindI8) {
+            float xs = 0.0f;  // lane l holds the scale of column c0 + l
+            bool row = false;
+            if (c0 + lane < at.rows) {
+              const int64_t tok = p.g.source(at.row0 + c0 + lane);
+              row = tok >= 0;
+              if (row) xs = p.g.x_scale[tok];
+            }
+            const unsigned rows = __ballot_sync(0xffffffffu, row);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float s = __shfl_sync(0xffffffffu, xs, i);
+              v[i] = (rows >> i) & 1 ? static_cast<float>(__float_as_int(v[i])) * s * wscale : 0.0f;
+            }
+          }
+          store_typed(p.out, p.out_dtype, out0 + c0 * p.out_col, p.out_col, v, at.rows - c0, live, p.pairs != 0);
+        }
+        if (any) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
+        }
+      }
+      if (any && ++buf == 2) {
+        buf = 0;
+        acc_phase ^= 1;
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (csize > 1) cluster_sync();
+  tc_fence_after();
+  if (warp == 1) tc_dealloc<CG>(tmem, 2 * NT);
+}
+
+// --------------------------------------------------------------------- host
+
+using Encode = PFN_cuTensorMapEncodeTiled_v12000;
+
+Encode encoder() {
+  static const Encode fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  return fn;
+}
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == ES_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+         : dtype == ES_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                           : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+}
+
+struct MapSpec {
+  const void* p;
+  int dtype;  // ES_BF16, ES_F16, or anything else for bytes
+  int64_t d0, d1, d2;
+  int64_t s1, s2;  // strides in bytes
+  int b0, b1;
+};
+
+bool encode_map(const MapSpec& m, int rank, CUtensorMap* map) {
+  std::memset(map, 0, sizeof(*map));
+  Encode fn = encoder();
+  if (!fn) return false;
+  cuuint64_t dim[3] = {static_cast<cuuint64_t>(m.d0), static_cast<cuuint64_t>(m.d1), static_cast<cuuint64_t>(m.d2)};
+  cuuint64_t stride[2] = {static_cast<cuuint64_t>(m.s1), static_cast<cuuint64_t>(m.s2)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(m.b0), static_cast<cuuint32_t>(m.b1), 1};
+  cuuint32_t one[3] = {1, 1, 1};
+  return fn(map, map_type(m.dtype), static_cast<cuuint32_t>(rank), const_cast<void*>(m.p), dim, stride, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a TMA map asks of an address and of the strides (in bytes).
+bool tma_ok(const void* p, int64_t s1, int64_t s2 = 16) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s1 > 0 && s1 % 16 == 0 && s1 < (1LL << 40) && s2 > 0 &&
+         s2 % 16 == 0 && s2 < (1LL << 40);
+}
+
+int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
+
+template <typename S>
+int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int csize, cudaStream_t stream) {
+  const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kPartBytes +
+                      (3 * p.g.groups() + 1) * sizeof(int);
+  static std::atomic<bool> raised[kMaxAttrDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ES_ERR_CUDA;
+  const bool tracked = dev >= 0 && dev < kMaxAttrDevices;
+  if (!tracked || !raised[dev].load(std::memory_order_relaxed)) {
+    const size_t most = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kPartBytes +
+                        (3 * kMaxExperts + 1) * sizeof(int);
+    if (cudaFuncSetAttribute(grouped_tc_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(most)) != cudaSuccess)
+      return ES_ERR_CUDA;
+    if (tracked) raised[dev].store(true, std::memory_order_relaxed);
+  }
+  int64_t clusters = kSMs / csize;
+  if (clusters > max_tiles) clusters = max_tiles;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * csize));
+  cfg.blockDim = dim3(kTcThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = csize;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, grouped_tc_kernel<S>, p, m[0], m[1], m[2], m[3]) != cudaSuccess) {
+    cudaGetLastError();
+    return ES_ERR_CUDA;
+  }
+  count_launch();
+  return ES_OK;
+}
+
+constexpr int64_t kMaxTiles = 0x7fffffffLL;
+
+template <int KIND, bool A_MN>
+int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
+  const int64_t R = p.g.rows, groups = p.g.groups();
+  const int64_t live = groups < R ? groups : R;  // groups that can have rows
+  const int64_t mean = R / live;
+  auto tiles = [&](int cg, int nt) {
+    p.lane_tiles = static_cast<int>((p.lanes + 128 * cg - 1) / (128 * cg));
+    return (R / nt + live) * p.lane_tiles;
+  };
+  if (mean > 128) {
+    const int64_t n = tiles(2, 256);
+    p.idesc |= 16u << 24;
+    return launch<TcShape<2, 256, KIND, A_MN, false, false>>(p, m, n, 2, stream);
+  }
+  p.idesc |= 8u << 24;
+  if (mean > 64) return launch<TcShape<1, 128, KIND, A_MN, false, false>>(p, m, tiles(1, 128), 1, stream);
+  // few rows: the weights' bytes are the time; a tile's depth is shared by a
+  // cluster while the tiles alone do not fill the SMs
+  const int64_t n = tiles(1, 64);
+  const int64_t nkb = (p.g.K + TcShape<1, 64, KIND, A_MN, false, true>::BK - 1) /
+                      TcShape<1, 64, KIND, A_MN, false, true>::BK;
+  int split = 1;
+  while (split < 8 && n * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
+  if (split > 1) return launch<TcShape<1, 64, KIND, A_MN, false, true>>(p, m, n, split, stream);
+  return launch<TcShape<1, 64, KIND, A_MN, false, false>>(p, m, n, 1, stream);
+}
+
+uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
+  // D format (f32 1, s32 2), A and B formats (f16 0, bf16 1, s8 1), majors
+  const uint32_t d = dtype == ES_BF16 || dtype == ES_F16 ? 1u : 2u;
+  const uint32_t ab = dtype == ES_F16 ? 0u : 1u;
+  return (d << 4) | (ab << 7) | (ab << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16);
+}
+
+}  // namespace
+
+// Whether the tensor-core kernel takes these operands (dtype 0x100: 8-bit).
+bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* w) {
+  if (dtype != ES_BF16 && dtype != ES_F16 && dtype != kInt8) return false;
+  const int64_t esz = dtype == kInt8 ? 1 : 2;
+  const int64_t xs = g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
+  if (g.K < 1 || g.x_rows < 1 || !tma_ok(x, xs)) return false;
+  const bool mn = g.w_n == 1 && g.N > 1;
+  if (mn ? dtype == kInt8 : g.w_k != 1 && g.K > 1) return false;
+  const int64_t row = mn ? g.w_k : g.w_n, rows = mn ? g.K : g.N;
+  const int64_t ws = rows == 1 ? 16 : row * esz, we = g.groups() == 1 || g.w_e == 0 ? 16 : g.w_e * esz;
+  return tma_ok(w, ws, we) && (g.rows / 64 + g.groups()) * ((g.N + 127) / 128) < kMaxTiles;
+}
+
+int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
+                    int32_t* status, cudaStream_t stream) {
+  const int64_t esz = dtype == kInt8 ? 1 : 2;
+  const int bk = static_cast<int>(128 / esz);
+  const bool mn = g.w_n == 1 && g.N > 1;
+  TcArgs p{};
+  p.g = g;
+  p.out = y;
+  p.out_dtype = out_dtype;
+  p.lanes = g.N;
+  p.out_col = g.N;
+  p.expert_step = g.groups() == 1 || g.w_e == 0 ? 0 : 1;
+  p.gather_b = g.order != nullptr;
+  p.b_rows = static_cast<int>(g.x_rows);
+  p.idesc = idesc_of(dtype, mn, false);
+  p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0;
+  p.status = status;
+  const int64_t xs = g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
+  const int64_t experts = p.expert_step ? g.num_experts : 1, we = p.expert_step ? g.w_e * esz : 16;
+  CUtensorMap m[4];
+  const bool ok =
+      encode_map(mn ? MapSpec{w, dtype, g.N, g.K, experts, g.K == 1 ? round16(g.N * esz) : g.w_k * esz, we, 64, 64}
+                    : MapSpec{w, dtype, g.K, g.N, experts, g.N == 1 ? round16(g.K * esz) : g.w_n * esz, we, bk, 128},
+                 3, &m[0]) &&
+      encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, bk, g.order ? 1 : kBoxRows}, 2, &m[1]);
+  if (!ok) return ES_ERR_CUDA;
+  m[2] = m[1];
+  m[3] = m[1];
+  if (dtype == kInt8) return rows_launch<kKindI8, false>(p, m, stream);
+  return mn ? rows_launch<kKindF16, true>(p, m, stream) : rows_launch<kKindF16, false>(p, m, stream);
+}
+
+bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride) {
+  if (dtype != ES_BF16 && dtype != ES_F16) return false;
+  if (g.rows < 1 || g.x_rows < 1 || (g.w_n != 1 && g.w_k != 1)) return false;
+  const int64_t xs = g.x_rows == 1 ? round16(g.K * 2) : g.x_stride * 2;
+  const int64_t ds = g.rows == 1 ? round16(g.N * 2) : dy_stride * 2;
+  return tma_ok(x, xs) && tma_ok(dy, ds) &&
+         g.groups() * ((g.N + 127) / 128) * ((g.K + 127) / 128) < kMaxTiles;
+}
+
+int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
+                     int32_t* status, cudaStream_t stream) {
+  // lanes: the dimension that is contiguous in dw
+  const bool n_lanes = g.w_n == 1;
+  TcArgs p{};
+  p.g = g;
+  p.out = dw;
+  p.out_dtype = dtype;
+  p.lanes = n_lanes ? g.N : g.K;
+  p.cols = n_lanes ? g.K : g.N;
+  p.out_col = n_lanes ? g.w_k : g.w_n;
+  p.out_expert = g.w_e;
+  p.gather_a = !n_lanes && g.order;
+  p.gather_b = n_lanes && g.order;
+  p.a_rows = static_cast<int>(n_lanes ? g.rows : g.x_rows);
+  p.b_rows = static_cast<int>(n_lanes ? g.x_rows : g.rows);
+  p.idesc = idesc_of(dtype, true, true) | (16u << 24);
+  p.pairs = p.lanes % 2 == 0 && p.out_col % 2 == 0 && p.out_expert % 2 == 0 &&
+            (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
+  p.status = status;
+  p.lane_tiles = static_cast<int>((p.lanes + 255) / 256);
+  p.col_tiles = static_cast<int>((p.cols + 255) / 256);
+  const int64_t xs = g.x_rows == 1 ? round16(g.K * 2) : g.x_stride * 2;
+  const int64_t ds = g.rows == 1 ? round16(g.N * 2) : dy_stride * 2;
+  CUtensorMap m[4];
+  const int a = n_lanes ? 1 : 0, b = 1 - a;  // place of x among (A, B)
+  const bool ok = encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, 64, 64}, 2, &m[a]) &&
+                  encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, 64, 1}, 2, &m[2 + a]) &&
+                  encode_map(MapSpec{dy, dtype, g.N, g.rows, 1, ds, 16, 64, 64}, 2, &m[b]) &&
+                  encode_map(MapSpec{dy, dtype, g.N, g.rows, 1, ds, 16, 64, 1}, 2, &m[2 + b]);
+  if (!ok) return ES_ERR_CUDA;
+  return launch<TcShape<2, 256, kKindF16, true, true, false>>(
+      p, m, static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles, 2, stream);
+}
+
+}  // namespace es
