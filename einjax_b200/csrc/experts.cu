@@ -343,40 +343,41 @@ struct alignas(VEC * sizeof(T)) Piece {
 };
 
 constexpr int kCombineThreads = 256;
-constexpr int kRowsAhead = 8;  // choices of a token that are in flight together
 
 __device__ __forceinline__ int row_of(const int32_t* position, int64_t a, int64_t rows) {
   const int p = position[a];
   return p >= 0 && p < rows ? p : -1;
 }
 
-template <typename T, typename U, int VEC>
+// AHEAD: choices of a token that are in flight together (4 or 8; more go
+// round again).
+template <typename T, typename U, int VEC, int AHEAD>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const T* y, int64_t rows, int64_t stride,
                                                                   const float* weights, const int32_t* position,
                                                                   int64_t ntok, int k, int64_t D, U* out, int tp) {
   const int64_t t = blockIdx.x * static_cast<int64_t>(kCombineThreads / tp) + threadIdx.x / tp;
   if (t >= ntok) return;
   const int64_t pieces = D / VEC;
+  const Piece<T, VEC>* from[AHEAD];
+  float w[AHEAD];
   for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.0f;
-    for (int j0 = 0; j0 < k; j0 += kRowsAhead) {
-      Piece<T, VEC> p[kRowsAhead];
-      float w[kRowsAhead];
+    for (int j0 = 0; j0 < k; j0 += AHEAD) {
+      if (k > AHEAD || c < tp) {  // the rows of these choices: once, where they all fit
 #pragma unroll
-      for (int j = 0; j < kRowsAhead; ++j) {
-        const int r = j0 + j < k ? row_of(position, t * k + j0 + j, rows) : -1;
-        w[j] = 0.0f;
-        if (r >= 0) {
-          w[j] = weights ? weights[t * k + j0 + j] : 1.0f;
-          p[j] = reinterpret_cast<const Piece<T, VEC>*>(y + r * stride)[c];
-        } else {
-          p[j] = Piece<T, VEC>{};
+        for (int j = 0; j < AHEAD; ++j) {
+          const int r = j0 + j < k ? row_of(position, t * k + j0 + j, rows) : -1;
+          w[j] = r >= 0 ? (weights ? weights[t * k + j0 + j] : 1.0f) : 0.0f;
+          from[j] = r >= 0 ? reinterpret_cast<const Piece<T, VEC>*>(y + r * stride) : nullptr;
         }
       }
+      Piece<T, VEC> p[AHEAD];
 #pragma unroll
-      for (int j = 0; j < kRowsAhead; ++j)
+      for (int j = 0; j < AHEAD; ++j) p[j] = from[j] ? from[j][c] : Piece<T, VEC>{};
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w[j], to_f32(p[j].v[i]), acc[i]);
     }
@@ -387,21 +388,21 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(const T* y, in
   }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int AHEAD>
 __global__ void __launch_bounds__(kCombineThreads) combine_grad_kernel(
     const T* y, int64_t rows, int64_t stride, const float* weights, const int32_t* position, const int32_t* kept,
     int64_t ntok, int k, int64_t D, const T* dout, int64_t dstride, T* dy, float* dweights, int tp) {
-  __shared__ float part[kCombineThreads / 32][kRowsAhead];
+  __shared__ float part[kCombineThreads / 32][AHEAD];
   const int group = threadIdx.x / tp, lane = threadIdx.x & 31;
   const int64_t t = blockIdx.x * static_cast<int64_t>(kCombineThreads / tp) + group;
   const bool live = t < ntok;
   const int64_t pieces = D / VEC;
-  for (int j0 = 0; j0 < k; j0 += kRowsAhead) {
-    float dot[kRowsAhead];
-    int r[kRowsAhead];
-    float w[kRowsAhead];
+  for (int j0 = 0; j0 < k; j0 += AHEAD) {
+    float dot[AHEAD];
+    int r[AHEAD];
+    float w[AHEAD];
 #pragma unroll
-    for (int j = 0; j < kRowsAhead; ++j) {
+    for (int j = 0; j < AHEAD; ++j) {
       dot[j] = 0.0f;
       r[j] = live && j0 + j < k ? row_of(position, t * k + j0 + j, rows) : -1;
       w[j] = r[j] >= 0 ? weights[t * k + j0 + j] : 0.0f;
@@ -409,12 +410,12 @@ __global__ void __launch_bounds__(kCombineThreads) combine_grad_kernel(
     if (live) {
       for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
         const Piece<T, VEC> g = reinterpret_cast<const Piece<T, VEC>*>(dout + t * dstride)[c];
-        Piece<T, VEC> p[kRowsAhead];
+        Piece<T, VEC> p[AHEAD];
 #pragma unroll
-        for (int j = 0; j < kRowsAhead; ++j)
+        for (int j = 0; j < AHEAD; ++j)
           if (r[j] >= 0) p[j] = reinterpret_cast<const Piece<T, VEC>*>(y + r[j] * stride)[c];
 #pragma unroll
-        for (int j = 0; j < kRowsAhead; ++j)
+        for (int j = 0; j < AHEAD; ++j)
           if (r[j] >= 0) {
             Piece<T, VEC> o;
 #pragma unroll
@@ -429,14 +430,14 @@ __global__ void __launch_bounds__(kCombineThreads) combine_grad_kernel(
     }
     // the group's threads are whole warps (tp is a multiple of 32)
 #pragma unroll
-    for (int j = 0; j < kRowsAhead; ++j) dot[j] = warp_sum(dot[j]);
+    for (int j = 0; j < AHEAD; ++j) dot[j] = warp_sum(dot[j]);
     if (lane == 0) {
 #pragma unroll
-      for (int j = 0; j < kRowsAhead; ++j) part[threadIdx.x >> 5][j] = dot[j];
+      for (int j = 0; j < AHEAD; ++j) part[threadIdx.x >> 5][j] = dot[j];
     }
     __syncthreads();
     const int j = threadIdx.x % tp;
-    if (live && j < kRowsAhead && j0 + j < k) {
+    if (live && j < AHEAD && j0 + j < k) {
       float s = 0.0f;
       for (int w8 = 0; w8 < tp / 32; ++w8) s += part[group * (tp / 32) + w8][j];
       dweights[t * k + j0 + j] = row_of(position, t * k + j0 + j, rows) >= 0 ? s : 0.0f;
@@ -464,8 +465,13 @@ int combine_vec(const void* y, int64_t rows, int64_t stride, const float* weight
                 int k, int64_t D, void* out, cudaStream_t s) {
   const int tp = token_threads(D / VEC);
   const int64_t per = kCombineThreads / tp;
-  ES_LAUNCH((combine_kernel<T, U, VEC>), static_cast<unsigned>((T_ + per - 1) / per), kCombineThreads, 0, s,
-            static_cast<const T*>(y), rows, stride, weights, position, T_, k, D, static_cast<U*>(out), tp);
+  const unsigned blocks = static_cast<unsigned>((T_ + per - 1) / per);
+  if (k <= 4)
+    ES_LAUNCH((combine_kernel<T, U, VEC, 4>), blocks, kCombineThreads, 0, s, static_cast<const T*>(y), rows, stride,
+              weights, position, T_, k, D, static_cast<U*>(out), tp);
+  else
+    ES_LAUNCH((combine_kernel<T, U, VEC, 8>), blocks, kCombineThreads, 0, s, static_cast<const T*>(y), rows, stride,
+              weights, position, T_, k, D, static_cast<U*>(out), tp);
   return ES_OK;
 }
 
@@ -484,9 +490,15 @@ int combine_grad_vec(const void* y, int64_t rows, int64_t stride, const float* w
                      float* dweights, cudaStream_t s) {
   const int tp = token_threads(D / VEC);
   const int64_t per = kCombineThreads / tp;
-  ES_LAUNCH((combine_grad_kernel<T, VEC>), static_cast<unsigned>((T_ + per - 1) / per), kCombineThreads, 0, s,
-            static_cast<const T*>(y), rows, stride, weights, position, kept, T_, k, D, static_cast<const T*>(dout),
-            dstride, static_cast<T*>(dy), dweights, tp);
+  const unsigned blocks = static_cast<unsigned>((T_ + per - 1) / per);
+  if (k <= 4)
+    ES_LAUNCH((combine_grad_kernel<T, VEC, 4>), blocks, kCombineThreads, 0, s, static_cast<const T*>(y), rows, stride,
+              weights, position, kept, T_, k, D, static_cast<const T*>(dout), dstride, static_cast<T*>(dy), dweights,
+              tp);
+  else
+    ES_LAUNCH((combine_grad_kernel<T, VEC, 8>), blocks, kCombineThreads, 0, s, static_cast<const T*>(y), rows, stride,
+              weights, position, kept, T_, k, D, static_cast<const T*>(dout), dstride, static_cast<T*>(dy), dweights,
+              tp);
   return ES_OK;
 }
 

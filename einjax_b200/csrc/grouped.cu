@@ -221,8 +221,8 @@ int check_args(const GroupedArgs& g) {
 using namespace es;
 
 extern "C" size_t es_grouped_matmul_workspace_size(int dtype, int num_experts, int64_t K, int64_t N,
-                                                   int64_t num_rows) {
-  return 0;
+                                                   int64_t num_rows, int gather) {
+  return gather_bytes(gather && (dtype == ES_BF16 || dtype == ES_F16), num_rows, K, 2);
 }
 
 extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
@@ -236,17 +236,19 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
   ES_TRY(check_args(g));
   if (out_dtype != dtype && out_dtype != ES_F32) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
+  if (workspace_bytes < es_grouped_matmul_workspace_size(dtype, num_experts, K, N, num_rows, order != nullptr))
+    return ES_ERR_WORKSPACE;
   if (!y || (K && ((x_rows && !x) || !w))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
-  if (grouped_rows_tc_ok(g, dtype, x, w)) return grouped_rows_tc(g, dtype, x, w, y, out_dtype, status, s);
+  if (grouped_rows_tc_ok(g, dtype, x, w)) return grouped_rows_tc(g, dtype, x, w, y, out_dtype, workspace, status, s);
   if (out_dtype == dtype) ES_BY_TYPE(dtype, return (rows_simt<T, T>(g, x, w, y, s)));
   ES_BY_TYPE(dtype, return (rows_simt<T, float>(g, x, w, y, s)));
   return ES_ERR_UNSUPPORTED;
 }
 
 extern "C" size_t es_grouped_matmul_wgrad_workspace_size(int dtype, int num_experts, int64_t K, int64_t N,
-                                                         int64_t num_rows) {
-  return 0;
+                                                         int64_t num_rows, int gather) {
+  return es_grouped_matmul_workspace_size(dtype, num_experts, K, N, num_rows, gather);
 }
 
 extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* dy,
@@ -259,9 +261,11 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
   if (num_experts < 1) return ES_ERR_INVALID;
   ES_TRY(check_args(g));
   if (K == 0 || N == 0) return ES_OK;
+  if (workspace_bytes < es_grouped_matmul_wgrad_workspace_size(dtype, num_experts, K, N, num_rows, order != nullptr))
+    return ES_ERR_WORKSPACE;
   if (!dw || (num_rows && (!dy || (x_rows && !x)))) return ES_ERR_INVALID;
   if (grouped_wgrad_tc_ok(g, dtype, x, dy, dy_stride))
-    return grouped_wgrad_tc(g, dtype, x, dy, dy_stride, dw, status, as_stream(stream));
+    return grouped_wgrad_tc(g, dtype, x, dy, dy_stride, dw, workspace, status, as_stream(stream));
   const int64_t kt = (K + kTile - 1) / kTile, nt = (N + kTile - 1) / kTile;
   if (nt > 65535) return ES_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(kt), static_cast<unsigned>(nt), static_cast<unsigned>(num_experts));
@@ -274,7 +278,9 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
   return ES_ERR_UNSUPPORTED;
 }
 
-extern "C" size_t es_int8_matmul_workspace_size(int num_experts, int64_t K, int64_t N, int64_t num_rows) { return 0; }
+extern "C" size_t es_int8_matmul_workspace_size(int num_experts, int64_t K, int64_t N, int64_t num_rows, int gather) {
+  return gather_bytes(gather, num_rows, K, 1);
+}
 
 extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,
                               const int8_t* wq, const float* w_scale, int num_experts, int64_t K, int64_t N,
@@ -286,10 +292,12 @@ extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_r
   ES_TRY(check_args(g));
   if (K > kMaxInt8Depth) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
+  if (workspace_bytes < es_int8_matmul_workspace_size(num_experts, K, N, num_rows, order != nullptr))
+    return ES_ERR_WORKSPACE;
   if (!y || !w_scale || (x_rows && !x_scale) || (K && ((x_rows && !q) || !wq))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
   if (out_dtype != ES_F32 && out_dtype != ES_BF16 && out_dtype != ES_F16) return ES_ERR_UNSUPPORTED;
-  if (grouped_rows_tc_ok(g, kInt8, q, wq)) return grouped_rows_tc(g, kInt8, q, wq, y, out_dtype, status, s);
+  if (grouped_rows_tc_ok(g, kInt8, q, wq)) return grouped_rows_tc(g, kInt8, q, wq, y, out_dtype, workspace, status, s);
   ES_BY_TYPE(out_dtype, return (rows_simt<int8_t, T>(g, q, wq, y, s)));
   return ES_ERR_UNSUPPORTED;
 }

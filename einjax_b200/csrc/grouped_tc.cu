@@ -16,8 +16,10 @@
 // next group stay out of it).
 //
 // Operands are read as they lie: K-major or MN-major, through 128-byte
-// swizzled TMA boxes; routed tokens by TMA row gathers (tile::gather4), with
-// no copy of the rows in between.
+// swizzled TMA boxes. Routed tokens are first copied into the rows' order: TMA
+// row gathers in the main loop (tile::gather4, four rows an instruction) took
+// 2.76 ms where the copy and box loads take 1.0 ms (16384 rows, 4096 x 8192,
+// bf16).
 //
 // Roles (8 warps): warp 0 issues the TMA loads, warp 1 the MMAs (one lane),
 // warps 2-3 clear the output rows of no expert, warps 4-7 read the
@@ -59,8 +61,7 @@ struct TcArgs {
   int64_t out_expert; // output stride of an expert (weights' gradient)
   int lane_tiles, col_tiles;
   int expert_step;    // 0: every expert has the same matrix
-  int gather_a, gather_b;  // operands that are gathered through g.order
-  int a_rows, b_rows;      // rows of the gathered tensors: this index reads zeros
+  int src_rows;       // rows of the weights' gradient's operands: this row index reads zeros
   uint32_t idesc;     // instruction descriptor without N
   int pairs;          // two neighbouring lanes may be stored together
   int32_t* status;
@@ -506,44 +507,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int half = width / CG;  // columns of this CTA's part of B
       const int64_t lane0 = at.lane0 + pair_rank * 128;
       const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
-      int src[4];  // rows (gathered): this lane's four tokens
-      if constexpr (!S::WGRAD)
-        if (p.gather_b) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int c = lane * 4 + i;
-            int64_t r = -1;
-            if (c < half && static_cast<int>(pair_rank) * half + c < at.rows) r = p.g.source(col0 + c);
-            src[i] = r < 0 ? p.b_rows : static_cast<int>(r);
-          }
-        }
       for (int kb = at.kb0; kb < at.kb1; ++kb) {
-        int valid = BK, rows16 = BK;
-        int ra[4], rb[4];  // weights' gradient: rows of a gathered block
-        bool ga = false, gb = false;
+        uint32_t bytes;
+        int src[4];            // weights' gradient, last block: four rows of a gather
+        int rows16 = BK;       // rows of the block in whole MMA steps
+        bool tail = false;
         if constexpr (S::WGRAD) {
-          valid = min(at.depth - kb * BK, BK);
-          rows16 = (valid + 15) & ~15;
-          ga = p.gather_a || valid < BK;
-          gb = p.gather_b || valid < BK;
-          if (ga || gb) {
+          const int valid = min(at.depth - kb * BK, BK);
+          tail = valid < BK;
+          if (tail) {
+            rows16 = (valid + 15) & ~15;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = (lane & 15) * 4 + i;
-              const int64_t row = at.first + static_cast<int64_t>(kb) * BK + r;
-              int64_t sa = -1;
-              if (r < valid) sa = (p.gather_a || p.gather_b) ? p.g.source(row) : row;
-              ra[i] = r < valid ? static_cast<int>(p.gather_a ? (sa < 0 ? p.a_rows : sa) : row) : p.a_rows;
-              rb[i] = r < valid ? static_cast<int>(p.gather_b ? (sa < 0 ? p.b_rows : sa) : row) : p.b_rows;
+              src[i] = r < valid ? at.first + kb * BK + r : p.src_rows;
             }
           }
-        }
-        uint32_t bytes;
-        if constexpr (S::WGRAD) {
-          const int boxes_b = (half + 63) / 64;
-          bytes = 2u * (ga ? rows16 : BK) * 128 + boxes_b * (gb ? rows16 : BK) * 128u;
+          bytes = (2 + (half + 63) / 64) * rows16 * 128u;
         } else {
-          bytes = kABytes + (p.gather_b ? (half + 3) / 4 * 512u : (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u));
+          bytes = kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
         }
         int go = 0;
         if (lane == 0) {
@@ -559,21 +541,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
         const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
         if constexpr (S::WGRAD) {
-          // operand boxes of 64 lanes (columns) by 64 rows; a gathered box
-          // is 16 loads of four rows, dealt to half a warp
+          // operand boxes of 64 lanes (columns) by 64 rows; of the last block
+          // loads of four rows, dealt to half a warp a box
           const int row = at.first + kb * BK;
-          const int half16 = lane >> 4, quad = lane & 15;
-          if (ga) {
-            if (quad * 4 < rows16)
-              load_rows<CG>(sa + half16 * 8192 + quad * 512, &rows_a, static_cast<int>(lane0) + half16 * 64, ra, bar);
+          const int boxes = (half + 63) / 64;
+          if (tail) {
+            const int quad = lane & 15;
+            if (quad * 4 < rows16) {
+              load_rows<CG>(sa + (lane >> 4) * 8192 + quad * 512, &rows_a, static_cast<int>(lane0) + (lane >> 4) * 64,
+                            src, bar);
+              for (int b = lane >> 4; b < boxes; b += 2)
+                load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, src, bar);
+            }
           } else if (lane < 2) {
             load_2d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, row, bar);
-          }
-          const int boxes = (half + 63) / 64;
-          if (gb) {
-            for (int b = half16; b < boxes; b += 2)
-              if (quad * 4 < rows16) load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
-          } else if (lane >= 2 && lane - 2 < boxes) {
+          } else if (lane - 2 < boxes) {
             load_2d<CG>(sb + (lane - 2) * 8192, &map_b, col0 + (lane - 2) * 64, row, bar);
           }
         } else {
@@ -583,11 +565,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           } else {
             if (lane == 0) load_3d<CG>(sa, &map_a, kb * BK, static_cast<int>(lane0), z, bar);
           }
-          if (p.gather_b) {
-            if (lane * 4 < half) load_rows<CG>(sb + lane * 512, &rows_b, kb * BK, src, bar);
-          } else if (lane * kBoxRows < half) {
+          if (lane * kBoxRows < half)
             load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK, col0 + lane * kBoxRows, bar);
-          }
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -826,6 +805,49 @@ bool tma_ok(const void* p, int64_t s1, int64_t s2 = 16) {
 
 int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
 
+int64_t x_row_bytes(const GroupedArgs& g, int64_t esz) {
+  return g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
+}
+
+bool rows_ok(const GroupedArgs& g, int64_t esz, const void* x) {
+  return tma_ok(x, x_row_bytes(g, esz)) && (!g.order || g.K * esz % 16 == 0);
+}
+
+// ------------------------------------------------------- rows in their order
+//
+// Copies the routed tokens' rows into the grouped order, 16 bytes a load.
+// Bound by memory: each copied row is written once, each token read from HBM
+// once (its other choices from L2).
+constexpr int kCopyThreads = 256;
+
+__global__ void __launch_bounds__(kCopyThreads) gather_rows_kernel(GroupedArgs g, const uint4* x, int64_t stride,
+                                                                   int64_t pieces, uint4* out, int tp) {
+  const int64_t kept = g.kept();
+  const int64_t r = blockIdx.x * static_cast<int64_t>(kCopyThreads / tp) + threadIdx.x / tp;
+  if (r >= kept) return;
+  const int64_t t = g.source(r);
+  const uint4* from = x + t * stride;
+  uint4* to = out + r * pieces;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+  for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) to[c] = t >= 0 ? from[c] : zero;
+}
+
+// Replaces routed rows of x by their copy in the workspace.
+int gather_rows(GroupedArgs& g, int64_t esz, const void*& x, void* workspace, cudaStream_t stream) {
+  if (!g.order) return ES_OK;
+  const int64_t pieces = g.K * esz / 16;
+  int tp = 32;
+  while (tp < kCopyThreads && tp * 4 < pieces) tp *= 2;
+  const int64_t per = kCopyThreads / tp;
+  ES_LAUNCH(gather_rows_kernel, static_cast<unsigned>((g.rows + per - 1) / per), kCopyThreads, 0, stream, g,
+            static_cast<const uint4*>(x), x_row_bytes(g, esz) / 16, pieces, static_cast<uint4*>(workspace), tp);
+  x = workspace;
+  g.x_rows = g.rows;
+  g.x_stride = g.K;
+  return ES_OK;
+}
+
 template <typename S>
 int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int csize, cudaStream_t stream) {
   const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kPartBytes +
@@ -901,12 +923,11 @@ uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
 
 }  // namespace
 
-// Whether the tensor-core kernel takes these operands (dtype 0x100: 8-bit).
+// Whether the tensor-core kernel takes these operands.
 bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* w) {
   if (dtype != ES_BF16 && dtype != ES_F16 && dtype != kInt8) return false;
   const int64_t esz = dtype == kInt8 ? 1 : 2;
-  const int64_t xs = g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
-  if (g.K < 1 || g.x_rows < 1 || !tma_ok(x, xs)) return false;
+  if (g.K < 1 || g.x_rows < 1 || !rows_ok(g, esz, x)) return false;
   const bool mn = g.w_n == 1 && g.N > 1;
   if (mn ? dtype == kInt8 : g.w_k != 1 && g.K > 1) return false;
   const int64_t row = mn ? g.w_k : g.w_n, rows = mn ? g.K : g.N;
@@ -914,31 +935,30 @@ bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype, const void* x, const vo
   return tma_ok(w, ws, we) && (g.rows / 64 + g.groups()) * ((g.N + 127) / 128) < kMaxTiles;
 }
 
-int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
-                    int32_t* status, cudaStream_t stream) {
+int grouped_rows_tc(const GroupedArgs& args, int dtype, const void* x, const void* w, void* y, int out_dtype,
+                    void* workspace, int32_t* status, cudaStream_t stream) {
   const int64_t esz = dtype == kInt8 ? 1 : 2;
+  GroupedArgs g = args;
+  ES_TRY(gather_rows(g, esz, x, workspace, stream));
   const int bk = static_cast<int>(128 / esz);
   const bool mn = g.w_n == 1 && g.N > 1;
   TcArgs p{};
-  p.g = g;
+  p.g = args;  // the scales of 8-bit rows go by token
   p.out = y;
   p.out_dtype = out_dtype;
   p.lanes = g.N;
   p.out_col = g.N;
   p.expert_step = g.groups() == 1 || g.w_e == 0 ? 0 : 1;
-  p.gather_b = g.order != nullptr;
-  p.b_rows = static_cast<int>(g.x_rows);
   p.idesc = idesc_of(dtype, mn, false);
   p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0;
   p.status = status;
-  const int64_t xs = g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
   const int64_t experts = p.expert_step ? g.num_experts : 1, we = p.expert_step ? g.w_e * esz : 16;
   CUtensorMap m[4];
   const bool ok =
       encode_map(mn ? MapSpec{w, dtype, g.N, g.K, experts, g.K == 1 ? round16(g.N * esz) : g.w_k * esz, we, 64, 64}
                     : MapSpec{w, dtype, g.K, g.N, experts, g.N == 1 ? round16(g.K * esz) : g.w_n * esz, we, bk, 128},
                  3, &m[0]) &&
-      encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, bk, g.order ? 1 : kBoxRows}, 2, &m[1]);
+      encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, x_row_bytes(g, esz), 16, bk, kBoxRows}, 2, &m[1]);
   if (!ok) return ES_ERR_CUDA;
   m[2] = m[1];
   m[3] = m[1];
@@ -949,14 +969,14 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride) {
   if (dtype != ES_BF16 && dtype != ES_F16) return false;
   if (g.rows < 1 || g.x_rows < 1 || (g.w_n != 1 && g.w_k != 1)) return false;
-  const int64_t xs = g.x_rows == 1 ? round16(g.K * 2) : g.x_stride * 2;
-  const int64_t ds = g.rows == 1 ? round16(g.N * 2) : dy_stride * 2;
-  return tma_ok(x, xs) && tma_ok(dy, ds) &&
+  return rows_ok(g, 2, x) && tma_ok(dy, g.rows == 1 ? round16(g.N * 2) : dy_stride * 2) &&
          g.groups() * ((g.N + 127) / 128) * ((g.K + 127) / 128) < kMaxTiles;
 }
 
-int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
-                     int32_t* status, cudaStream_t stream) {
+int grouped_wgrad_tc(const GroupedArgs& args, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
+                     void* workspace, int32_t* status, cudaStream_t stream) {
+  GroupedArgs g = args;
+  ES_TRY(gather_rows(g, 2, x, workspace, stream));
   // lanes: the dimension that is contiguous in dw
   const bool n_lanes = g.w_n == 1;
   TcArgs p{};
@@ -967,17 +987,14 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
   p.cols = n_lanes ? g.K : g.N;
   p.out_col = n_lanes ? g.w_k : g.w_n;
   p.out_expert = g.w_e;
-  p.gather_a = !n_lanes && g.order;
-  p.gather_b = n_lanes && g.order;
-  p.a_rows = static_cast<int>(n_lanes ? g.rows : g.x_rows);
-  p.b_rows = static_cast<int>(n_lanes ? g.x_rows : g.rows);
+  p.src_rows = static_cast<int>(g.rows);
   p.idesc = idesc_of(dtype, true, true) | (16u << 24);
   p.pairs = p.lanes % 2 == 0 && p.out_col % 2 == 0 && p.out_expert % 2 == 0 &&
             (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
   p.status = status;
   p.lane_tiles = static_cast<int>((p.lanes + 255) / 256);
   p.col_tiles = static_cast<int>((p.cols + 255) / 256);
-  const int64_t xs = g.x_rows == 1 ? round16(g.K * 2) : g.x_stride * 2;
+  const int64_t xs = x_row_bytes(g, 2);
   const int64_t ds = g.rows == 1 ? round16(g.N * 2) : dy_stride * 2;
   CUtensorMap m[4];
   const int a = n_lanes ? 1 : 0, b = 1 - a;  // place of x among (A, B)

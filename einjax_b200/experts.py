@@ -19,14 +19,14 @@ wait that ran out) is raised by ``check_device_errors``.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from . import _lib as L
-from .sparse import _STATUS, stream_ptr
+from .sparse import _STATUS, _raw_stream
 
 MAX_EXPERTS, MAX_TOP_K, MAX_INT8_DEPTH = 1024, 32, 133152
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 _DTYPES = {torch.float32: L.ES_F32, torch.bfloat16: L.ES_BF16, torch.float16: L.ES_F16}
 
@@ -39,11 +39,9 @@ def _code(fn: str, name: str, dtype) -> int:
 
 
 def _on_gpu(fn: str, **tensors):
-    """The one CUDA device of the tensors."""
+    """Raises unless all are CUDA tensors of one device."""
     dev = None
     for name, t in tensors.items():
-        if t is None:
-            continue
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{fn}: {name} must be a torch tensor, got {type(t).__name__}")
         if not t.is_cuda:
@@ -52,7 +50,6 @@ def _on_gpu(fn: str, **tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError(f"{fn}: {name} is on {t.device}, the other operands on {dev}")
-    return dev
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -62,65 +59,65 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-class _on_device:
-    """Makes ``dev`` current for the launches inside, at no cost when it is already."""
+def _call(fn: str, dev, *args):
+    """Calls the entry point on ``dev`` and its current stream (the last argument)."""
+    index = dev.index
+    here = _current_device()
+    if here != index:
+        torch.cuda.set_device(index)
+    try:
+        status = getattr(L.lib(), fn)(*args, _raw_stream(index))
+    finally:
+        if here != index:
+            torch.cuda.set_device(here)
+    if status:
+        L.check(fn, status)
 
-    def __init__(self, dev):
-        self.dev = dev.index if dev.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.dev is not None:
-            self.prev = torch.cuda.current_device()
-            torch.cuda.set_device(self.dev)
-
-    def __exit__(self, *exc):
-        if self.dev is not None:
-            torch.cuda.set_device(self.prev)
+def _scratch(nbytes: int, dev):
+    """A workspace that is held until the call is queued (torch's allocator
+    hands it out again only behind that on the stream), or None."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-@dataclass(eq=False)
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
 class ExpertPlan:
-    """Row order of the routed choices, all int32 on the device.
+    """Row order of the routed choices, all int32 and contiguous on the device.
 
     Expert ``e`` owns rows ``offsets[e]`` to ``offsets[e + 1]``; row ``r``
     holds choice ``order[r]`` (``token * top_k + j``); ``position[token, j]``
     is the row of that choice. -1: no row, no choice. The rows from
     ``offsets[num_experts]`` on belong to no expert and are zero in every
-    output."""
+    output. ``plan_experts`` makes one; so does a caller that has the three
+    arrays (offsets that ascend from 0, ``position`` the inverse of ``order``)."""
 
-    offsets: torch.Tensor   # (num_experts + 1,)
-    order: torch.Tensor     # (num_tokens * top_k,)
-    position: torch.Tensor  # (num_tokens, top_k)
+    __slots__ = ("offsets", "order", "position", "device", "num_experts", "num_tokens", "top_k", "num_rows")
 
-    def __post_init__(self):
-        o, r, p = self.offsets, self.order, self.position
-        if o.dtype != torch.int32 or r.dtype != torch.int32 or p.dtype != torch.int32:
-            raise TypeError("ExpertPlan: offsets, order and position must be int32")
-        if o.dim() != 1 or r.dim() != 1 or p.dim() != 2 or o.shape[0] < 2 or p.shape[1] < 1 or \
-                p.shape[0] * p.shape[1] != r.shape[0]:
-            raise ValueError(f"ExpertPlan: shapes {tuple(o.shape)}, {tuple(r.shape)} and {tuple(p.shape)} are not "
+    def __init__(self, offsets: torch.Tensor, order: torch.Tensor, position: torch.Tensor):
+        _on_gpu("ExpertPlan", offsets=offsets, order=order, position=position)
+        for t in (offsets, order, position):
+            if t.dtype != torch.int32:
+                raise TypeError("ExpertPlan: offsets, order and position must be int32")
+            if not t.is_contiguous():
+                raise ValueError("ExpertPlan: offsets, order and position must be contiguous")
+        E, R, P = offsets.shape, order.shape, position.shape
+        if len(E) != 1 or len(R) != 1 or len(P) != 2 or E[0] < 2 or P[1] < 1 or P[0] * P[1] != R[0]:
+            raise ValueError(f"ExpertPlan: shapes {tuple(E)}, {tuple(R)} and {tuple(P)} are not "
                              "(num_experts + 1,), (num_tokens * top_k,) and (num_tokens, top_k)")
-        if o.shape[0] - 1 > MAX_EXPERTS:
-            raise ValueError(f"ExpertPlan: at most {MAX_EXPERTS} experts, got {o.shape[0] - 1}")
-        if not (o.is_contiguous() and r.is_contiguous() and p.is_contiguous()):
-            raise ValueError("ExpertPlan: offsets, order and position must be contiguous")
-        _on_gpu("ExpertPlan", offsets=o, order=r, position=p)
+        if E[0] - 1 > MAX_EXPERTS:
+            raise ValueError(f"ExpertPlan: at most {MAX_EXPERTS} experts, got {E[0] - 1}")
+        self._set(offsets, order, position)
 
-    @property
-    def num_experts(self) -> int:
-        return self.offsets.shape[0] - 1
-
-    @property
-    def num_tokens(self) -> int:
-        return self.position.shape[0]
-
-    @property
-    def top_k(self) -> int:
-        return self.position.shape[1]
-
-    @property
-    def num_rows(self) -> int:
-        return self.order.shape[0]
+    def _set(self, offsets, order, position):
+        self.offsets, self.order, self.position = offsets, order, position
+        self.device = offsets.device
+        self.num_experts = offsets.shape[0] - 1
+        self.num_tokens, self.top_k = position.shape
+        self.num_rows = order.shape[0]
+        return self
 
     @property
     def counts(self) -> torch.Tensor:
@@ -130,35 +127,39 @@ class ExpertPlan:
 
 # ------------------------------------------------------------------- routing
 
+def _route(logits, top_k, renormalize):
+    dev = logits.device
+    T, E = logits.shape
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    _call("es_route_experts", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), top_k,
+          renormalize, weights.data_ptr(), experts.data_ptr())
+    return weights, experts
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, renormalize):
-        T, E = logits.shape
-        dev = logits.device
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-        experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-        with _on_device(dev):
-            L.check("es_route_experts", L.lib().es_route_experts(
-                logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), top_k, renormalize,
-                weights.data_ptr(), experts.data_ptr(), stream_ptr(dev)))
+        weights, experts = _route(logits, top_k, renormalize)
         ctx.mark_non_differentiable(experts)
-        if logits.requires_grad:
-            ctx.save_for_backward(logits, weights, experts)
-            ctx.renormalize = renormalize
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, weights, experts)
+        ctx.renormalize = renormalize
         return weights, experts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dweights, _):
+        if dweights is None:
+            return None, None, None
         logits, weights, experts = ctx.saved_tensors
-        T, E = logits.shape
         dev = logits.device
-        dweights = dweights.to(torch.float32).contiguous()
+        T, E = logits.shape
+        dweights = dweights.contiguous()
         dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
-        with _on_device(dev):
-            L.check("es_route_experts_grad", L.lib().es_route_experts_grad(
-                logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), experts.shape[1], ctx.renormalize,
-                weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), stream_ptr(dev)))
+        _call("es_route_experts_grad", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0),
+              experts.shape[1], ctx.renormalize, weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(),
+              dlogits.data_ptr())
         return dlogits, None, None
 
 
@@ -181,7 +182,8 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     if not 1 <= top_k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS:
         raise ValueError(f"route_experts: top_k={top_k} of {E} experts; 1 <= top_k <= min(num_experts, {MAX_TOP_K}) "
                          f"and num_experts <= {MAX_EXPERTS}")
-    return _Route.apply(_rows(logits), top_k, 1 if renormalize else 0)
+    run = _Route.apply if logits.requires_grad and torch.is_grad_enabled() else _route
+    return run(_rows(logits), top_k, 1 if renormalize else 0)
 
 
 def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
@@ -189,7 +191,7 @@ def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     in ascending token and choice inside an expert. An entry outside
     ``[-1, num_experts)`` counts as -1 and is raised as ``ValueError`` by the
     next ``check_device_errors``."""
-    dev = _on_gpu("plan_experts", experts=experts)
+    _on_gpu("plan_experts", experts=experts)
     if experts.dim() != 2 or experts.shape[1] < 1:
         raise ValueError(f"plan_experts: experts must be (num_tokens, top_k), got {tuple(experts.shape)}")
     if experts.dtype not in (torch.int32, torch.int64):
@@ -197,54 +199,56 @@ def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     E = int(num_experts)
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"plan_experts: num_experts={E} is not in [1, {MAX_EXPERTS}]")
-    lib = L.lib()
     if experts.dtype == torch.int64:  # a value past 32 bits must not wrap into the range
         experts = experts.clamp(-2, E).to(torch.int32)
     experts = experts.contiguous()
-    n = experts.numel()
+    dev, n = experts.device, experts.numel()
     offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
     order = torch.empty(n, dtype=torch.int32, device=dev)
     position = torch.empty(experts.shape, dtype=torch.int32, device=dev)
-    nbytes = lib.es_expert_plan_workspace_size(n, E)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    with _on_device(dev):
-        L.check("es_expert_plan", lib.es_expert_plan(
-            experts.data_ptr(), n, E, ws.data_ptr() if ws is not None else None, nbytes, offsets.data_ptr(), order.data_ptr(), position.data_ptr(),
-            _STATUS.address("es_expert_plan", dev.index), stream_ptr(dev)))
-    return ExpertPlan(offsets, order, position)
+    nbytes = L.lib().es_expert_plan_workspace_size(n, E)
+    ws = _scratch(nbytes, dev)
+    _call("es_expert_plan", dev, experts.data_ptr(), n, E, _ptr(ws), nbytes, offsets.data_ptr(), order.data_ptr(),
+          position.data_ptr(), _STATUS.address("es_expert_plan", dev.index))
+    return ExpertPlan.__new__(ExpertPlan)._set(offsets, order, position)
 
 
 # ---------------------------------------------------------- grouped products
 
-def _plan_args(plan, gather):
-    return plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None
-
-
 def _grouped(x, w, plan, gather, out_dtype):
     """``w`` (num_experts, K, N), any strides."""
     dev = x.device
-    K, N, R = w.shape[1], w.shape[2], plan.num_rows
+    E, K, N = w.shape
+    R, code = plan.num_rows, _DTYPES[x.dtype]
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
-    lib = L.lib()
-    code = _DTYPES[x.dtype]
-    nbytes = lib.es_grouped_matmul_workspace_size(code, plan.num_experts, K, N, R)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    off, order = _plan_args(plan, gather)
-    se, sk, sn = w.stride()
-    with _on_device(dev):
-        L.check("es_grouped_matmul", lib.es_grouped_matmul(
-            x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), plan.num_experts, K, N, se, sk, sn, off, order,
-            plan.top_k, R, y.data_ptr(), _DTYPES[out_dtype], ws.data_ptr() if ws is not None else None, nbytes,
-            _STATUS.address("es_grouped_matmul", dev.index), stream_ptr(dev)))
+    nbytes = L.lib().es_grouped_matmul_workspace_size(code, E, K, N, R, gather)
+    ws = _scratch(nbytes, dev)
+    _call("es_grouped_matmul", dev, x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(),
+          plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, R, y.data_ptr(),
+          _DTYPES[out_dtype], _ptr(ws), nbytes, _STATUS.address("es_grouped_matmul", dev.index))
     return y
+
+
+def _wgrad(x, dy, w, plan, gather):
+    dev = x.device
+    E, K, N = w.shape
+    # the gradient takes w's layout when it is a transposed view
+    dw = torch.empty((E, N, K), dtype=w.dtype, device=dev).transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 \
+        else torch.empty((E, K, N), dtype=w.dtype, device=dev)
+    R, code = plan.num_rows, _DTYPES[x.dtype]
+    nbytes = L.lib().es_grouped_matmul_wgrad_workspace_size(code, E, K, N, R, gather)
+    ws = _scratch(nbytes, dev)
+    _call("es_grouped_matmul_wgrad", dev, x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E,
+          K, N, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, R, dw.data_ptr(),
+          *dw.stride(), _ptr(ws), nbytes, _STATUS.address("es_grouped_matmul_wgrad", dev.index))
+    return dw
 
 
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, plan, gather):
-        if x.requires_grad or w.requires_grad:
-            ctx.save_for_backward(x, w)
-            ctx.plan, ctx.gather = plan, gather
+        ctx.save_for_backward(x, w)
+        ctx.plan, ctx.gather = plan, gather
         return _grouped(x, w, plan, gather, x.dtype)
 
     @staticmethod
@@ -262,25 +266,6 @@ class _GroupedMatmul(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dw = _wgrad(x, dy, w, plan, gather)
         return dx, dw, None, None
-
-
-def _wgrad(x, dy, w, plan, gather):
-    dev = x.device
-    E, K, N = w.shape
-    # the gradient takes w's layout when it is a transposed view
-    dw = torch.empty((E, N, K), dtype=w.dtype, device=dev).transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 \
-        else torch.empty((E, K, N), dtype=w.dtype, device=dev)
-    lib = L.lib()
-    code = _DTYPES[x.dtype]
-    nbytes = lib.es_grouped_matmul_wgrad_workspace_size(code, E, K, N, plan.num_rows)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    off, order = _plan_args(plan, gather)
-    with _on_device(dev):
-        L.check("es_grouped_matmul_wgrad", lib.es_grouped_matmul_wgrad(
-            x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E, K, N, off, order, plan.top_k,
-            plan.num_rows, dw.data_ptr(), *dw.stride(), ws.data_ptr() if ws is not None else None, nbytes,
-            _STATUS.address("es_grouped_matmul_wgrad", dev.index), stream_ptr(dev)))
-    return dw
 
 
 def _check_rows(fn, x, name, plan, gather, K):
@@ -308,44 +293,41 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan, gather: b
     if w.dim() != 3 or w.shape[0] != plan.num_experts:
         raise ValueError(f"grouped_matmul: w has shape {tuple(w.shape)}, wanted ({plan.num_experts}, K, N)")
     _check_rows("grouped_matmul", x, "x", plan, gather, w.shape[1])
-    return _GroupedMatmul.apply(_rows(x), w, plan, bool(gather))
+    x, gather = _rows(x), bool(gather)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _GroupedMatmul.apply(x, w, plan, gather)
+    return _grouped(x, w, plan, gather, x.dtype)
 
 
 # ------------------------------------------------------ weighted sum to tokens
 
 def _combine(y, weights, plan, out_dtype):
-    dev = y.device
-    out = torch.empty((plan.num_tokens, y.shape[1]), dtype=out_dtype, device=dev)
-    with _on_device(dev):
-        L.check("es_combine_experts", L.lib().es_combine_experts(
-            y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), weights.data_ptr() if weights is not None else None,
-            plan.position.data_ptr(), plan.num_tokens, plan.top_k, y.shape[1], out.data_ptr(), _DTYPES[out_dtype],
-            stream_ptr(dev)))
+    dev, D = y.device, y.shape[1]
+    out = torch.empty((plan.num_tokens, D), dtype=out_dtype, device=dev)
+    _call("es_combine_experts", dev, y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), _ptr(weights),
+          plan.position.data_ptr(), plan.num_tokens, plan.top_k, D, out.data_ptr(), _DTYPES[out_dtype])
     return out
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, plan):
-        if y.requires_grad or weights.requires_grad:
-            ctx.save_for_backward(y, weights)
-            ctx.plan = plan
+        ctx.save_for_backward(y, weights)
+        ctx.plan = plan
         return _combine(y, weights, plan, y.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
-        plan = ctx.plan
-        dev = y.device
-        dout = _rows(dout.to(y.dtype))
+        plan, dev = ctx.plan, y.device
+        dout = _rows(dout)
         dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
         dweights = torch.empty(weights.shape, dtype=torch.float32, device=dev)
-        with _on_device(dev):
-            L.check("es_combine_experts_grad", L.lib().es_combine_experts_grad(
-                y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), weights.data_ptr(), plan.position.data_ptr(),
-                plan.offsets.data_ptr() + 4 * plan.num_experts, plan.num_tokens, plan.top_k, y.shape[1],
-                dout.data_ptr(), dout.stride(0), dy.data_ptr(), dweights.data_ptr(), stream_ptr(dev)))
+        _call("es_combine_experts_grad", dev, y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0),
+              weights.data_ptr(), plan.position.data_ptr(), plan.offsets.data_ptr() + 4 * plan.num_experts,
+              plan.num_tokens, plan.top_k, y.shape[1], dout.data_ptr(), dout.stride(0), dy.data_ptr(),
+              dweights.data_ptr())
         return dy, dweights, None
 
 
@@ -364,7 +346,10 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) ->
     if weights.shape != plan.position.shape:
         raise ValueError(f"combine_experts: weights have shape {tuple(weights.shape)}, the plan's choices "
                          f"{tuple(plan.position.shape)}")
-    return _Combine.apply(_rows(y), weights.contiguous(), plan)
+    y, weights = _rows(y), weights.contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
+        return _Combine.apply(y, weights, plan)
+    return _combine(y, weights, plan, y.dtype)
 
 
 # ------------------------------------------------------------ 8-bit products
@@ -373,16 +358,15 @@ def quantize_rows(x: torch.Tensor):
     """``(q, scale)``: each row of ``x`` (rows, width) in 8-bit integers with
     ``scale = max |x| / 127`` (float32), ``q = rint(x / scale)``. A row of
     zeros has scale 0; a row with an infinity or NaN has scale NaN."""
-    dev = _on_gpu("quantize_rows", x=x)
+    _on_gpu("quantize_rows", x=x)
     code = _code("quantize_rows", "x", x.dtype)
     if x.dim() != 2:
         raise ValueError(f"quantize_rows: x must be (rows, width), got {tuple(x.shape)}")
-    x = _rows(x.detach())
+    dev, x = x.device, _rows(x.detach())
     q = torch.empty(x.shape, dtype=torch.int8, device=dev)
     scale = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
-    with _on_device(dev):
-        L.check("es_quantize_rows", L.lib().es_quantize_rows(
-            x.data_ptr(), code, x.shape[0], x.shape[1], x.stride(0), q.data_ptr(), scale.data_ptr(), stream_ptr(dev)))
+    _call("es_quantize_rows", dev, x.data_ptr(), code, x.shape[0], x.shape[1], x.stride(0), q.data_ptr(),
+          scale.data_ptr())
     return q, scale
 
 
@@ -408,7 +392,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     ``wq`` (num_experts, N, K), ``wscale`` (num_experts, N), and with
     ``gather`` ``q`` and ``scale`` are by token. Returns (rows, N) of
     ``out_dtype`` (float32, bfloat16, float16). K is at most 133,152."""
-    dev = _on_gpu("int8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=plan.offsets if plan is not None else None)
+    _on_gpu("int8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=q if plan is None else plan.offsets)
     code = _code("int8_matmul", "out_dtype", out_dtype)
     if q.dtype != torch.int8 or wq.dtype != torch.int8:
         raise TypeError(f"int8_matmul: q and wq must be int8, got {q.dtype} and {wq.dtype}")
@@ -430,18 +414,15 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     q, scale, wscale = _rows(q), scale.contiguous(), wscale.contiguous()
     if wq.stride(-1) != 1 or wq.stride(-2) < K:
         wq = wq.contiguous()
+    dev = q.device
     R = plan.num_rows if plan is not None else q.shape[0]
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
-    lib = L.lib()
-    nbytes = lib.es_int8_matmul_workspace_size(E, K, N, R)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    off, order = _plan_args(plan, gather) if plan is not None else (None, None)
-    with _on_device(dev):
-        L.check("es_int8_matmul", lib.es_int8_matmul(
-            q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(), wscale.data_ptr(), E, K, N,
-            wq.stride(0) if E else 0, wq.stride(-2), off, order, plan.top_k if plan is not None else 1, R,
-            y.data_ptr(), code, ws.data_ptr() if ws is not None else None, nbytes,
-            _STATUS.address("es_int8_matmul", dev.index), stream_ptr(dev)))
+    nbytes = L.lib().es_int8_matmul_workspace_size(E, K, N, R, bool(gather))
+    ws = _scratch(nbytes, dev)
+    _call("es_int8_matmul", dev, q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(),
+          wscale.data_ptr(), E, K, N, wq.stride(0) if E else 0, wq.stride(-2),
+          plan.offsets.data_ptr() if E else None, plan.order.data_ptr() if gather else None, plan.top_k if E else 1, R,
+          y.data_ptr(), code, _ptr(ws), nbytes, _STATUS.address("es_int8_matmul", dev.index))
     return y
 
 
