@@ -82,17 +82,20 @@ SIGNATURES = {
     "es_route_experts_grad": (c_int, [c_vp, c_int, c_i64, c_int, c_i64, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "es_expert_plan_workspace_size": (c_sz, [c_i64, c_int]),
     "es_expert_plan": (c_int, [c_vp, c_i64, c_int, c_vp, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp]),
-    "es_grouped_matmul_workspace_size": (c_sz, [c_int, c_int, c_i64, c_i64, c_i64, c_int]),
+    "es_grouped_matmul_workspace_size": (c_sz, [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64,
+                                                 c_i64, c_vp, c_vp, c_int, c_i64]),
     "es_grouped_matmul": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
                                   c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
-    "es_grouped_matmul_wgrad_workspace_size": (c_sz, [c_int, c_int, c_i64, c_i64, c_i64, c_int]),
+    "es_grouped_matmul_wgrad_workspace_size": (c_sz, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_i64, c_i64,
+                                                       c_vp, c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_i64]),
     "es_grouped_matmul_wgrad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp,
                                         c_int, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp, c_vp]),
     "es_combine_experts": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_vp]),
     "es_combine_experts_grad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp,
                                         c_i64, c_vp, c_vp, c_vp]),
     "es_quantize_rows": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
-    "es_int8_matmul_workspace_size": (c_sz, [c_int, c_i64, c_i64, c_i64, c_int]),
+    "es_int8_matmul_workspace_size": (c_sz, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64,
+                                              c_vp, c_vp, c_int, c_i64]),
     "es_int8_matmul": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
     "es_scatter_add_workspace_size": (c_sz, [c_i64]),

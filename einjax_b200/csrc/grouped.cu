@@ -215,14 +215,23 @@ int check_args(const GroupedArgs& g) {
   return ES_OK;
 }
 
+bool value_type(int dtype) { return dtype == ES_F32 || dtype == ES_BF16 || dtype == ES_F16; }
+
+bool use_tc(const GroupedArgs& g, int dtype, const void* x, const void* w) { return grouped_rows_tc_ok(g, dtype); }
+
 }  // namespace
 }  // namespace es
 
 using namespace es;
 
-extern "C" size_t es_grouped_matmul_workspace_size(int dtype, int num_experts, int64_t K, int64_t N,
-                                                   int64_t num_rows, int gather) {
-  return gather_bytes(gather && (dtype == ES_BF16 || dtype == ES_F16), num_rows, K, 2);
+extern "C" size_t es_grouped_matmul_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride,
+                                                   const void* w, int num_experts, int64_t K, int64_t N,
+                                                   int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
+                                                   const int32_t* offsets, const int32_t* order, int top_k,
+                                                   int64_t num_rows) {
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
+                      w_k_stride, w_n_stride, nullptr, nullptr};
+  return check_args(g) == ES_OK && use_tc(g, dtype, x, w) ? grouped_rows_tc_workspace(g, dtype, x, w) : 0;
 }
 
 extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
@@ -230,25 +239,33 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
                                  int64_t w_n_stride, const int32_t* offsets, const int32_t* order, int top_k,
                                  int64_t num_rows, void* y, int out_dtype, void* workspace, size_t workspace_bytes,
                                  int32_t* status, void* stream) {
-  GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, w_k_stride,
-                w_n_stride, nullptr, nullptr};
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
+                      w_k_stride, w_n_stride, nullptr, nullptr};
   if (num_experts < 1) return ES_ERR_INVALID;
   ES_TRY(check_args(g));
-  if (out_dtype != dtype && out_dtype != ES_F32) return ES_ERR_UNSUPPORTED;
+  if (!value_type(dtype) || (out_dtype != dtype && out_dtype != ES_F32)) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
-  if (workspace_bytes < es_grouped_matmul_workspace_size(dtype, num_experts, K, N, num_rows, order != nullptr))
-    return ES_ERR_WORKSPACE;
   if (!y || (K && ((x_rows && !x) || !w))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
-  if (grouped_rows_tc_ok(g, dtype, x, w)) return grouped_rows_tc(g, dtype, x, w, y, out_dtype, workspace, status, s);
+  if (use_tc(g, dtype, x, w)) {
+    if (workspace_bytes < grouped_rows_tc_workspace(g, dtype, x, w)) return ES_ERR_WORKSPACE;
+    return grouped_rows_tc(g, dtype, x, w, y, out_dtype, workspace, status, s);
+  }
   if (out_dtype == dtype) ES_BY_TYPE(dtype, return (rows_simt<T, T>(g, x, w, y, s)));
   ES_BY_TYPE(dtype, return (rows_simt<T, float>(g, x, w, y, s)));
   return ES_ERR_UNSUPPORTED;
 }
 
-extern "C" size_t es_grouped_matmul_wgrad_workspace_size(int dtype, int num_experts, int64_t K, int64_t N,
-                                                         int64_t num_rows, int gather) {
-  return es_grouped_matmul_workspace_size(dtype, num_experts, K, N, num_rows, gather);
+extern "C" size_t es_grouped_matmul_wgrad_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride,
+                                                         const void* dy, int64_t dy_stride, int num_experts, int64_t K,
+                                                         int64_t N, const int32_t* offsets, const int32_t* order,
+                                                         int top_k, int64_t num_rows, void* dw,
+                                                         int64_t dw_expert_stride, int64_t dw_k_stride,
+                                                         int64_t dw_n_stride) {
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride,
+                      dw_k_stride, dw_n_stride, nullptr, nullptr};
+  return check_args(g) == ES_OK && grouped_wgrad_tc_ok(g, dtype)
+             ? grouped_wgrad_tc_workspace(g, dtype, x, dy, dy_stride) : 0;
 }
 
 extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* dy,
@@ -256,20 +273,21 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
                                        const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows,
                                        void* dw, int64_t dw_expert_stride, int64_t dw_k_stride, int64_t dw_n_stride,
                                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride, dw_k_stride,
-                dw_n_stride, nullptr, nullptr};
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride,
+                      dw_k_stride, dw_n_stride, nullptr, nullptr};
   if (num_experts < 1) return ES_ERR_INVALID;
   ES_TRY(check_args(g));
+  if (!value_type(dtype)) return ES_ERR_UNSUPPORTED;
   if (K == 0 || N == 0) return ES_OK;
-  if (workspace_bytes < es_grouped_matmul_wgrad_workspace_size(dtype, num_experts, K, N, num_rows, order != nullptr))
-    return ES_ERR_WORKSPACE;
   if (!dw || (num_rows && (!dy || (x_rows && !x)))) return ES_ERR_INVALID;
-  if (grouped_wgrad_tc_ok(g, dtype, x, dy, dy_stride))
-    return grouped_wgrad_tc(g, dtype, x, dy, dy_stride, dw, workspace, status, as_stream(stream));
+  cudaStream_t s = as_stream(stream);
+  if (grouped_wgrad_tc_ok(g, dtype)) {
+    if (workspace_bytes < grouped_wgrad_tc_workspace(g, dtype, x, dy, dy_stride)) return ES_ERR_WORKSPACE;
+    return grouped_wgrad_tc(g, dtype, x, dy, dy_stride, dw, workspace, status, s);
+  }
   const int64_t kt = (K + kTile - 1) / kTile, nt = (N + kTile - 1) / kTile;
   if (nt > 65535) return ES_ERR_UNSUPPORTED;
   const dim3 grid(static_cast<unsigned>(kt), static_cast<unsigned>(nt), static_cast<unsigned>(num_experts));
-  cudaStream_t s = as_stream(stream);
   ES_BY_TYPE(dtype, {
     ES_LAUNCH((wgrad_kernel<T>), grid, kThreads, 0, s, g, static_cast<const T*>(x), static_cast<const T*>(dy),
               dy_stride, static_cast<T*>(dw));
@@ -278,8 +296,14 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
   return ES_ERR_UNSUPPORTED;
 }
 
-extern "C" size_t es_int8_matmul_workspace_size(int num_experts, int64_t K, int64_t N, int64_t num_rows, int gather) {
-  return gather_bytes(gather, num_rows, K, 1);
+extern "C" size_t es_int8_matmul_workspace_size(const int8_t* q, const float* x_scale, int64_t x_rows,
+                                                int64_t x_stride, const int8_t* wq, const float* w_scale,
+                                                int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
+                                                int64_t w_n_stride, const int32_t* offsets, const int32_t* order,
+                                                int top_k, int64_t num_rows) {
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, 1,
+                      w_n_stride, x_scale, w_scale};
+  return check_args(g) == ES_OK && use_tc(g, kInt8, q, wq) ? grouped_rows_tc_workspace(g, kInt8, q, wq) : 0;
 }
 
 extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,
@@ -287,17 +311,17 @@ extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_r
                               int64_t w_expert_stride, int64_t w_n_stride, const int32_t* offsets,
                               const int32_t* order, int top_k, int64_t num_rows, void* y, int out_dtype,
                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
-  GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, 1, w_n_stride,
-                x_scale, w_scale};
+  const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, 1,
+                      w_n_stride, x_scale, w_scale};
   ES_TRY(check_args(g));
-  if (K > kMaxInt8Depth) return ES_ERR_UNSUPPORTED;
+  if (K > kMaxInt8Depth || !value_type(out_dtype)) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
-  if (workspace_bytes < es_int8_matmul_workspace_size(num_experts, K, N, num_rows, order != nullptr))
-    return ES_ERR_WORKSPACE;
   if (!y || !w_scale || (x_rows && !x_scale) || (K && ((x_rows && !q) || !wq))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
-  if (out_dtype != ES_F32 && out_dtype != ES_BF16 && out_dtype != ES_F16) return ES_ERR_UNSUPPORTED;
-  if (grouped_rows_tc_ok(g, kInt8, q, wq)) return grouped_rows_tc(g, kInt8, q, wq, y, out_dtype, workspace, status, s);
+  if (use_tc(g, kInt8, q, wq)) {
+    if (workspace_bytes < grouped_rows_tc_workspace(g, kInt8, q, wq)) return ES_ERR_WORKSPACE;
+    return grouped_rows_tc(g, kInt8, q, wq, y, out_dtype, workspace, status, s);
+  }
   ES_BY_TYPE(out_dtype, return (rows_simt<int8_t, T>(g, q, wq, y, s)));
   return ES_ERR_UNSUPPORTED;
 }

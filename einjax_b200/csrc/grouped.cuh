@@ -51,15 +51,14 @@ struct GroupedArgs {
 
 constexpr int kInt8 = 0x100;  // operand type of the 8-bit product
 
-// Tensor-core forms (grouped_tc.cu), for 16-bit and 8-bit operands whose
-// addresses and strides TMA can read. workspace: gather_bytes of the call.
-inline size_t gather_bytes(bool gather, int64_t rows, int64_t K, int64_t esz) {
-  return gather ? static_cast<size_t>(rows) * K * esz : 0;
-}
-bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* w);
+// Tensor-core forms (grouped_tc.cu). The workspace holds copies of what TMA
+// cannot read as it lies.
+bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype);
+size_t grouped_rows_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w);
 int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
                     void* workspace, int32_t* status, cudaStream_t stream);
-bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride);
+bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype);
+size_t grouped_wgrad_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride);
 int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
                      void* workspace, int32_t* status, cudaStream_t stream);
 

@@ -19,7 +19,13 @@
 // swizzled TMA boxes. Routed tokens are first copied into the rows' order: TMA
 // row gathers in the main loop (tile::gather4, four rows an instruction) took
 // 2.76 ms where the copy and box loads take 1.0 ms (16384 rows, 4096 x 8192,
-// bf16).
+// bf16). What TMA cannot read (odd addresses or strides) is copied too.
+//
+// fp32 operands are cut into three bf16 planes, x = b0 + b1 + b2 exactly, and
+// the six products b_i b_j with i + j <= 2 are added, the smallest first; what
+// is left out is at most 2^-24 of a product. The accumulator truncates each step's sum (measured: a relative
+// error of 1e-9 a unit of depth), so a sum is cut into chains of 512 that the
+// epilogue adds in fp32.
 //
 // Roles (8 warps): warp 0 issues the TMA loads, warp 1 the MMAs (one lane),
 // warps 2-3 clear the output rows of no expert, warps 4-7 read the
@@ -61,6 +67,8 @@ struct TcArgs {
   int64_t out_expert; // output stride of an expert (weights' gradient)
   int lane_tiles, col_tiles;
   int expert_step;    // 0: every expert has the same matrix
+  int plane_experts;  // matrices of one plane of W
+  int plane_rows;     // rows of one plane of X (and dY)
   int src_rows;       // rows of the weights' gradient's operands: this row index reads zeros
   uint32_t idesc;     // instruction descriptor without N
   int pairs;          // two neighbouring lanes may be stored together
@@ -270,8 +278,14 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 
 // ------------------------------------------------------------------- kernel
 
-template <int CG_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_>
+// Planes of the six products of fp32 operands, in the order they are added.
+__host__ __device__ constexpr int term_a(int t) { return t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0; }
+__host__ __device__ constexpr int term_b(int t) { return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0; }
+
+template <int CG_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
 struct TcShape {
+  static constexpr int kTerms = PLANES_ == 3 ? 6 : 1;
+  static constexpr int kChain = PLANES_ == 3 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int CG = CG_;        // CTAs of one MMA
   static constexpr int NT = NT_;        // widest MMA
   static constexpr int KIND = KIND_;
@@ -507,70 +521,85 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int half = width / CG;  // columns of this CTA's part of B
       const int64_t lane0 = at.lane0 + pair_rank * 128;
       const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
-      for (int kb = at.kb0; kb < at.kb1; ++kb) {
-        uint32_t bytes;
-        int src[4];            // weights' gradient, last block: four rows of a gather
-        int rows16 = BK;       // rows of the block in whole MMA steps
-        bool tail = false;
-        if constexpr (S::WGRAD) {
-          const int valid = min(at.depth - kb * BK, BK);
-          tail = valid < BK;
-          if (tail) {
-            rows16 = (valid + 15) & ~15;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = (lane & 15) * 4 + i;
-              src[i] = r < valid ? at.first + kb * BK + r : p.src_rows;
+      for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
+        const int s1 = s0 + min(S::kChain, at.kb1 - s0);
+        for (int term = 0; term < S::kTerms && ok; ++term) {
+          const int plane_a = S::kTerms > 1 ? term_a(term) : 0, plane_b = S::kTerms > 1 ? term_b(term) : 0;
+          for (int kb = s0; kb < s1; ++kb) {
+            uint32_t bytes;
+            int src[4];            // weights' gradient, last block: four rows of a gather
+            int rows16 = BK;       // rows of the block in whole MMA steps
+            bool tail = false;
+            if constexpr (S::WGRAD) {
+              const int valid = min(at.depth - kb * BK, BK);
+              tail = valid < BK;
+              if (tail) {
+                rows16 = (valid + 15) & ~15;
+    #pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int r = (lane & 15) * 4 + i;
+                  src[i] = r < valid ? at.first + kb * BK + r : -1;
+                }
+              }
+              bytes = (2 + (half + 63) / 64) * rows16 * 128u;
+            } else {
+              bytes = kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
+            }
+            int go = 0;
+            if (lane == 0) {
+              go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+              if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
+              if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+            }
+            go = __shfl_sync(0xffffffffu, go, 0);
+            if (!go) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
+            const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
+            if constexpr (S::WGRAD) {
+              // operand boxes of 64 lanes (columns) by 64 rows; of the last block
+              // loads of four rows, dealt to half a warp a box
+              const int row_a = at.first + kb * BK + plane_a * p.plane_rows;
+              const int row_b = at.first + kb * BK + plane_b * p.plane_rows;
+              const int boxes = (half + 63) / 64;
+              if (tail) {
+                const int quad = lane & 15;
+                if (quad * 4 < rows16) {
+                  int ra[4], rb[4];
+    #pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    ra[i] = src[i] < 0 ? p.src_rows : src[i] + plane_a * p.plane_rows;
+                    rb[i] = src[i] < 0 ? p.src_rows : src[i] + plane_b * p.plane_rows;
+                  }
+                  load_rows<CG>(sa + (lane >> 4) * 8192 + quad * 512, &rows_a,
+                                static_cast<int>(lane0) + (lane >> 4) * 64, ra, bar);
+                  for (int b = lane >> 4; b < boxes; b += 2)
+                    load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
+                }
+              } else if (lane < 2) {
+                load_2d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, row_a, bar);
+              } else if (lane - 2 < boxes) {
+                load_2d<CG>(sb + (lane - 2) * 8192, &map_b, col0 + (lane - 2) * 64, row_b, bar);
+              }
+            } else {
+              const int z = at.expert * p.expert_step + plane_a * p.plane_experts;
+              if constexpr (S::A_MN) {
+                if (lane < 2)
+                  load_3d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, kb * BK, z, bar);
+              } else {
+                if (lane == 0) load_3d<CG>(sa, &map_a, kb * BK, static_cast<int>(lane0), z, bar);
+              }
+              if (lane * kBoxRows < half)
+                load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK,
+                            col0 + lane * kBoxRows + plane_b * p.plane_rows, bar);
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
             }
           }
-          bytes = (2 + (half + 63) / 64) * rows16 * 128u;
-        } else {
-          bytes = kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
-        }
-        int go = 0;
-        if (lane == 0) {
-          go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
-          if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
-          if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
-        }
-        go = __shfl_sync(0xffffffffu, go, 0);
-        if (!go) {
-          ok = false;
-          break;
-        }
-        const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
-        const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
-        if constexpr (S::WGRAD) {
-          // operand boxes of 64 lanes (columns) by 64 rows; of the last block
-          // loads of four rows, dealt to half a warp a box
-          const int row = at.first + kb * BK;
-          const int boxes = (half + 63) / 64;
-          if (tail) {
-            const int quad = lane & 15;
-            if (quad * 4 < rows16) {
-              load_rows<CG>(sa + (lane >> 4) * 8192 + quad * 512, &rows_a, static_cast<int>(lane0) + (lane >> 4) * 64,
-                            src, bar);
-              for (int b = lane >> 4; b < boxes; b += 2)
-                load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, src, bar);
-            }
-          } else if (lane < 2) {
-            load_2d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, row, bar);
-          } else if (lane - 2 < boxes) {
-            load_2d<CG>(sb + (lane - 2) * 8192, &map_b, col0 + (lane - 2) * 64, row, bar);
-          }
-        } else {
-          const int z = at.expert * p.expert_step;
-          if constexpr (S::A_MN) {
-            if (lane < 2) load_3d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, kb * BK, z, bar);
-          } else {
-            if (lane == 0) load_3d<CG>(sa, &map_a, kb * BK, static_cast<int>(lane0), z, bar);
-          }
-          if (lane * kBoxRows < half)
-            load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK, col0 + lane * kBoxRows, bar);
-        }
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
         }
       }
     }
@@ -600,38 +629,43 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (at.kb0 == at.kb1) continue;
         const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
-        ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t d = tmem + buf * NT;
-        for (int kb = at.kb0; kb < at.kb1; ++kb) {
-          ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
+        for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
+          const int s1 = s0 + min(S::kChain, at.kb1 - s0);
+          ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = base + stage * S::kStageBytes;
-          const uint64_t da = operand(sa, S::A_MN), db = operand(sa + kABytes, S::WGRAD);
-          constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
-          int steps = 4;
-          if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
-          if (steps == 4) {
+          const uint32_t d = tmem + buf * NT;
+          uint32_t more = 0;
+          for (int term = 0; term < S::kTerms && ok; ++term)
+            for (int kb = s0; kb < s1; ++kb) {
+              ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t sa = base + stage * S::kStageBytes;
+              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + kABytes, S::WGRAD);
+              constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
+              int steps = 4;
+              if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+              if (steps == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, kb > at.kb0 || i > 0);
-          } else {
-            for (int i = 0; i < steps; ++i)
-              mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, kb > at.kb0 || i > 0);
+                for (int i = 0; i < 4; ++i) mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, more | i);
+              } else {
+                for (int i = 0; i < steps; ++i)
+                  mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, more | i);
+              }
+              more = 1;
+              commit<CG>(&ctl.empty[stage]);
+              if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
+          if (!ok) break;
+          commit<CG>(&ctl.acc_full[buf]);
+          if (++buf == 2) {
+            buf = 0;
+            acc_phase ^= 1;
           }
-          commit<CG>(&ctl.empty[stage]);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-        if (!ok) break;
-        commit<CG>(&ctl.acc_full[buf]);
-        if (++buf == 2) {
-          buf = 0;
-          acc_phase ^= 1;
         }
       }
       if (!ok) {
@@ -652,44 +686,88 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const TileAt at = tiles.at(t, rank, csize);
       const int64_t ch = at.lane0 + pair_rank * 128 + quad * 32 + lane;
       const bool live = ch < p.lanes;
-      const bool any = at.kb0 < at.kb1;
-      if (any) {
-        int go = 0;
-        if (lane == 0) go = tc_wait(&ctl.acc_full[buf], acc_phase, &ctl, p.status, true) ? 1 : 0;
-        if (!__shfl_sync(0xffffffffu, go, 0)) break;
-        tc_fence_after();
-      }
       float wscale = 1.0f;
       if constexpr (S::KIND == kKindI8) wscale = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
-      const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16);
-      if constexpr (S::SPLIT) {
-        // this CTA's part of the sum into shared memory, [column][lane]
+      if constexpr (S::SPLIT) {  // the last tile's parts have been read by the whole cluster
         int go = 1;
         if (lane == 0) go = tc_wait(&ctl.red_empty, red_phase ^ 1, &ctl, p.status, true) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      }
+      const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col + ch;
+      bool ok = true;
+      int s0 = at.kb0;
+      do {  // the chains of the sum; one pass over zeros where there is no depth
+        const bool any = s0 < at.kb1, first = s0 == at.kb0;
+        if (any) {
+          int go = 0;
+          if (lane == 0) go = tc_wait(&ctl.acc_full[buf], acc_phase, &ctl, p.status, true) ? 1 : 0;
+          ok = __shfl_sync(0xffffffffu, go, 0) != 0;
+          if (!ok) break;
+          tc_fence_after();
+        }
+        const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16);
         for (int c0 = 0; c0 < at.rows; c0 += 32) {
           float v[32];
           if (any) {
             tmem_ld32(acc + c0, v);
-            if constexpr (S::KIND == kKindI8) {
-              // the parts stay integers (their bits travel as floats): the sum is exact
-            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.0f;
           }
+          const int n = at.rows - c0;
+          if constexpr (S::SPLIT) {
+            // this CTA's part of the sum into shared memory, [column][lane];
+            // 8-bit products stay integers (their bits travel as floats)
+            float* mine = part + c0 * 128 + quad * 32 + lane;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c0 + i < at.rows) part[(c0 + i) * 128 + quad * 32 + lane] = v[i];
+            for (int i = 0; i < 32; ++i)
+              if (i < n) mine[i * 128] = first ? v[i] : mine[i * 128] + v[i];
+          } else {
+            if constexpr (S::KIND == kKindI8) {
+              float xs = 0.0f;  // lane l holds the scale of column c0 + l
+              bool row = false;
+              if (lane < n) {
+                const int64_t tok = p.g.source(at.row0 + c0 + lane);
+                row = tok >= 0;
+                if (row) xs = p.g.x_scale[tok];
+              }
+              const unsigned rows = __ballot_sync(0xffffffffu, row);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float s = __shfl_sync(0xffffffffu, xs, i);
+                v[i] = (rows >> i) & 1 ? static_cast<float>(__float_as_int(v[i])) * s * wscale : 0.0f;
+              }
+            }
+            const int64_t at0 = out0 + c0 * p.out_col;
+            if constexpr (S::kTerms > 1) {
+              float* o = static_cast<float*>(p.out) + at0;
+              if (!first && live) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (i < n) v[i] += o[i * p.out_col];
+              }
+              store_cols(o, p.out_col, v, n, live, false);
+            } else {
+              store_typed(p.out, p.out_dtype, at0, p.out_col, v, n, live, p.pairs != 0);
+            }
+          }
         }
         if (any) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), rank));
+          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
+          if (++buf == 2) {
+            buf = 0;
+            acc_phase ^= 1;
+          }
+          s0 += min(S::kChain, at.kb1 - s0);
         }
+      } while (s0 < at.kb1);
+      if (!ok) break;
+      if constexpr (S::SPLIT) {
         __syncwarp();
         if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_full), lane));
-        go = 1;
+        int go = 1;
         if (lane == 0) go = tc_wait(&ctl.red_full, red_phase, &ctl, p.status, true) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
         // columns rank, rank + csize, ...: the parts are added in the CTAs' order
@@ -709,42 +787,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
         red_phase ^= 1;
-      } else {
-        const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col + ch;
-        for (int c0 = 0; c0 < at.rows; c0 += 32) {
-          float v[32];
-          if (any) {
-            tmem_ld32(acc + c0, v);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-          }
-          if constexpr (S::KIND == kKindI8) {
-            float xs = 0.0f;  // lane l holds the scale of column c0 + l
-            bool row = false;
-            if (c0 + lane < at.rows) {
-              const int64_t tok = p.g.source(at.row0 + c0 + lane);
-              row = tok >= 0;
-              if (row) xs = p.g.x_scale[tok];
-            }
-            const unsigned rows = __ballot_sync(0xffffffffu, row);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float s = __shfl_sync(0xffffffffu, xs, i);
-              v[i] = (rows >> i) & 1 ? static_cast<float>(__float_as_int(v[i])) * s * wscale : 0.0f;
-            }
-          }
-          store_typed(p.out, p.out_dtype, out0 + c0 * p.out_col, p.out_col, v, at.rows - c0, live, p.pairs != 0);
-        }
-        if (any) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
-        }
-      }
-      if (any && ++buf == 2) {
-        buf = 0;
-        acc_phase ^= 1;
       }
     }
   }
@@ -803,49 +845,161 @@ bool tma_ok(const void* p, int64_t s1, int64_t s2 = 16) {
          s2 % 16 == 0 && s2 < (1LL << 40);
 }
 
-int64_t round16(int64_t v) { return (v + 15) / 16 * 16; }
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-int64_t x_row_bytes(const GroupedArgs& g, int64_t esz) {
-  return g.x_rows == 1 ? round16(g.K * esz) : g.x_stride * esz;
-}
-
-bool rows_ok(const GroupedArgs& g, int64_t esz, const void* x) {
-  return tma_ok(x, x_row_bytes(g, esz)) && (!g.order || g.K * esz % 16 == 0);
-}
-
-// ------------------------------------------------------- rows in their order
+// ------------------------------------------------- operands laid out for TMA
 //
-// Copies the routed tokens' rows into the grouped order, 16 bytes a load.
-// Bound by memory: each copied row is written once, each token read from HBM
-// once (its other choices from L2).
+// Copies a (depth, rows, cols) tensor of any strides into rows that TMA can
+// read: 16-byte pitch, routed rows in the grouped order, fp32 cut into three
+// bf16 planes. A thread writes 16 bytes of one row (of each plane). Bound by
+// memory. Matrices of experts without rows are left out.
 constexpr int kCopyThreads = 256;
 
-__global__ void __launch_bounds__(kCopyThreads) gather_rows_kernel(GroupedArgs g, const uint4* x, int64_t stride,
-                                                                   int64_t pieces, uint4* out, int tp) {
-  const int64_t kept = g.kept();
-  const int64_t r = blockIdx.x * static_cast<int64_t>(kCopyThreads / tp) + threadIdx.x / tp;
-  if (r >= kept) return;
-  const int64_t t = g.source(r);
-  const uint4* from = x + t * stride;
-  uint4* to = out + r * pieces;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) to[c] = t >= 0 ? from[c] : zero;
+struct LayoutArgs {
+  GroupedArgs g;
+  const void* src;
+  int64_t s_z, s_row, s_col;  // source strides in elements
+  int64_t rows, cols, pitch;  // pitch: elements of a row of the copy
+  int64_t depth;              // matrices of one plane
+  void* out;
+  int by_row;   // rows are grouped rows: the source row is theirs, those of no expert are left out
+  int by_expert;
+  int wide;     // 16-byte loads
+};
+
+// b0 + b1 + b2 == x exactly: each plane is what is left, rounded to 8 bits
+// (to nearest: a rest is at most 2^-8 of its number, twice less than after
+// truncation, which the products left out have in their square). A value that
+// would round past the type's largest is truncated; an infinity or NaN is its
+// first plane alone, so that its products are infinite or NaN.
+__device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
+  const uint32_t u = __float_as_uint(x);
+  const bool finite = (u & 0x7f800000u) != 0x7f800000u;
+  __nv_bfloat16 b0 = __float2bfloat16_rn(x);
+  if (finite && __hisinf(b0)) b0 = __ushort_as_bfloat16(static_cast<uint16_t>(u >> 16));
+  const float r1 = finite ? x - __bfloat162float(b0) : 0.0f;
+  const __nv_bfloat16 b1 = __float2bfloat16_rn(r1);
+  b[0] = __bfloat16_as_ushort(b0);
+  b[1] = __bfloat16_as_ushort(b1);
+  b[2] = __bfloat16_as_ushort(__float2bfloat16_rn(r1 - __bfloat162float(b1)));
 }
 
-// Replaces routed rows of x by their copy in the workspace.
-int gather_rows(GroupedArgs& g, int64_t esz, const void*& x, void* workspace, cudaStream_t stream) {
-  if (!g.order) return ES_OK;
-  const int64_t pieces = g.K * esz / 16;
-  int tp = 32;
-  while (tp < kCopyThreads && tp * 4 < pieces) tp *= 2;
-  const int64_t per = kCopyThreads / tp;
-  ES_LAUNCH(gather_rows_kernel, static_cast<unsigned>((g.rows + per - 1) / per), kCopyThreads, 0, stream, g,
-            static_cast<const uint4*>(x), x_row_bytes(g, esz) / 16, pieces, static_cast<uint4*>(workspace), tp);
-  x = workspace;
-  g.x_rows = g.rows;
-  g.x_stride = g.K;
+template <typename T>
+__global__ void __launch_bounds__(kCopyThreads) layout_kernel(const __grid_constant__ LayoutArgs p) {
+  constexpr bool kSplit = std::is_same<T, float>::value;
+  constexpr int VEC = kSplit ? 8 : 16 / sizeof(T);  // elements of a 16-byte store
+  const int64_t z = blockIdx.y;
+  if (p.by_expert) {
+    int64_t lo, hi;
+    p.g.bounds(static_cast<int>(z), lo, hi);
+    if (hi <= lo) return;
+  }
+  const int64_t pieces = p.pitch / VEC;
+  const int64_t at = blockIdx.x * static_cast<int64_t>(kCopyThreads) + threadIdx.x;
+  const int64_t row = at / pieces, c0 = (at - row * pieces) * VEC;
+  if (row >= p.rows) return;
+  int64_t from = row;
+  if (p.by_row) {
+    if (row >= p.g.kept()) return;
+    from = p.g.source(row);
+  }
+  const T* src = static_cast<const T*>(p.src) + z * p.s_z + from * p.s_row;
+  alignas(16) T v[VEC];
+  if (p.wide && from >= 0 && c0 + VEC <= p.cols) {
+    constexpr int LOADS = VEC * sizeof(T) / 16;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(src + c0)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = from >= 0 && c0 + i < p.cols ? src[(c0 + i) * p.s_col] : T(0);
+  }
+  if constexpr (kSplit) {
+    uint16_t b[3][VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      uint16_t s[3];
+      split3(v[i], s);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) b[k][i] = s[k];
+    }
+    uint16_t* out = static_cast<uint16_t*>(p.out);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint4 q;
+      q.x = b[k][0] | b[k][1] << 16;
+      q.y = b[k][2] | b[k][3] << 16;
+      q.z = b[k][4] | b[k][5] << 16;
+      q.w = b[k][6] | b[k][7] << 16;
+      *reinterpret_cast<uint4*>(out + ((k * p.depth + z) * p.rows + row) * p.pitch + c0) = q;
+    }
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (z * p.rows + row) * p.pitch + c0) =
+        *reinterpret_cast<const uint4*>(v);
+  }
+}
+
+// One operand: where it lies, or where it is copied to.
+struct Operand {
+  const void* p;
+  int64_t rows, cols, depth;   // of one plane; cols contiguous
+  int64_t s_z, s_row, s_col;   // in elements of the source
+  bool copy;
+  int64_t pitch;               // of the copy, in elements
+  size_t bytes;                // of the copy
+
+  int64_t row_bytes(int64_t esz) const {
+    if (copy) return pitch * esz;
+    return rows == 1 ? round_up(cols * esz, 16) : s_row * esz;
+  }
+  int64_t z_bytes(int64_t esz) const {
+    if (copy) return rows * pitch * esz;
+    return depth == 1 ? round_up(rows * row_bytes(esz), 16) : s_z * esz;
+  }
+};
+
+// Element size on the tensor cores: planes of fp32 are 16-bit.
+int64_t tc_size(int dtype) { return dtype == kInt8 ? 1 : 2; }
+int planes_of(int dtype) { return dtype == ES_F32 ? 3 : 1; }
+
+Operand operand_of(const void* p, int dtype, int64_t depth, int64_t rows, int64_t cols, int64_t s_z, int64_t s_row,
+                   int64_t s_col, bool must_copy) {
+  const int64_t esz = tc_size(dtype);
+  Operand o{p, rows, cols, depth, s_z, s_row, s_col, false, 0, 0};
+  o.copy = must_copy || dtype == ES_F32 || (s_col != 1 && cols > 1) ||
+           !tma_ok(p, o.row_bytes(esz), o.z_bytes(esz));
+  if (o.copy) {
+    o.pitch = round_up(cols, 16 / esz);
+    o.bytes = round_up(planes_of(dtype) * depth * rows * o.pitch * esz, 256);
+  }
+  return o;
+}
+
+int lay_out(const GroupedArgs& g, Operand& o, int dtype, bool by_row, bool by_expert, void* to, cudaStream_t stream) {
+  if (!o.copy) return ES_OK;
+  LayoutArgs a{g, o.p, o.s_z, o.s_row, o.s_col, o.rows, o.cols, o.pitch, o.depth, to, by_row, by_expert, 0};
+  const int64_t esz = dtype == ES_F32 ? 4 : tc_size(dtype);
+  a.wide = (o.s_col == 1 || o.cols == 1) && (reinterpret_cast<uintptr_t>(o.p) & 15) == 0 &&
+           (o.s_row * esz % 16 == 0 || (o.rows == 1 && !by_row)) && (o.s_z * esz % 16 == 0 || o.depth == 1);
+  const int64_t vec = dtype == ES_F32 ? 8 : 16 / esz;
+  const dim3 grid(static_cast<unsigned>((o.rows * (o.pitch / vec) + kCopyThreads - 1) / kCopyThreads),
+                  static_cast<unsigned>(o.depth));
+  if (dtype == ES_F32)
+    ES_LAUNCH((layout_kernel<float>), grid, kCopyThreads, 0, stream, a);
+  else if (dtype == kInt8)
+    ES_LAUNCH((layout_kernel<int8_t>), grid, kCopyThreads, 0, stream, a);
+  else
+    ES_LAUNCH((layout_kernel<uint16_t>), grid, kCopyThreads, 0, stream, a);
+  o.p = to;
   return ES_OK;
+}
+
+bool encode_operand(const Operand& o, int dtype, int box_cols, int box_rows, int rank, CUtensorMap* map) {
+  const int64_t esz = tc_size(dtype), planes = planes_of(dtype);
+  const int64_t rows = rank == 2 ? planes * o.rows : o.rows, depth = rank == 3 ? planes * o.depth : 1;
+  return encode_map(MapSpec{o.p, dtype == ES_F32 ? ES_BF16 : dtype, o.cols, rows, depth, o.row_bytes(esz),
+                            o.z_bytes(esz), box_cols, box_rows},
+                    rank, map);
 }
 
 template <typename S>
@@ -887,7 +1041,7 @@ int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int cs
 
 constexpr int64_t kMaxTiles = 0x7fffffffLL;
 
-template <int KIND, bool A_MN>
+template <int KIND, bool A_MN, int PLANES>
 int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
   const int64_t R = p.g.rows, groups = p.g.groups();
   const int64_t live = groups < R ? groups : R;  // groups that can have rows
@@ -899,84 +1053,120 @@ int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
   if (mean > 128) {
     const int64_t n = tiles(2, 256);
     p.idesc |= 16u << 24;
-    return launch<TcShape<2, 256, KIND, A_MN, false, false>>(p, m, n, 2, stream);
+    return launch<TcShape<2, 256, KIND, A_MN, false, false, PLANES>>(p, m, n, 2, stream);
   }
   p.idesc |= 8u << 24;
-  if (mean > 64) return launch<TcShape<1, 128, KIND, A_MN, false, false>>(p, m, tiles(1, 128), 1, stream);
+  if (mean > 64) return launch<TcShape<1, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(1, 128), 1, stream);
   // few rows: the weights' bytes are the time; a tile's depth is shared by a
   // cluster while the tiles alone do not fill the SMs
   const int64_t n = tiles(1, 64);
-  const int64_t nkb = (p.g.K + TcShape<1, 64, KIND, A_MN, false, true>::BK - 1) /
-                      TcShape<1, 64, KIND, A_MN, false, true>::BK;
+  const int64_t nkb = (p.g.K + TcShape<1, 64, KIND, A_MN, false, true, PLANES>::BK - 1) /
+                      TcShape<1, 64, KIND, A_MN, false, true, PLANES>::BK;
   int split = 1;
   while (split < 8 && n * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
-  if (split > 1) return launch<TcShape<1, 64, KIND, A_MN, false, true>>(p, m, n, split, stream);
-  return launch<TcShape<1, 64, KIND, A_MN, false, false>>(p, m, n, 1, stream);
+  if (split > 1) return launch<TcShape<1, 64, KIND, A_MN, false, true, PLANES>>(p, m, n, split, stream);
+  return launch<TcShape<1, 64, KIND, A_MN, false, false, PLANES>>(p, m, n, 1, stream);
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
   // D format (f32 1, s32 2), A and B formats (f16 0, bf16 1, s8 1), majors
-  const uint32_t d = dtype == ES_BF16 || dtype == ES_F16 ? 1u : 2u;
+  const uint32_t d = dtype == kInt8 ? 2u : 1u;
   const uint32_t ab = dtype == ES_F16 ? 0u : 1u;
   return (d << 4) | (ab << 7) | (ab << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16);
 }
 
-}  // namespace
+// The operands of the rows' product: X (rows, K) and the matrices, lanes
+// contiguous (MN-major: K rows of N) or depth contiguous (N rows of K).
+struct RowsOperands {
+  bool mn;
+  Operand x, w;
+};
 
-// Whether the tensor-core kernel takes these operands.
-bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* w) {
-  if (dtype != ES_BF16 && dtype != ES_F16 && dtype != kInt8) return false;
-  const int64_t esz = dtype == kInt8 ? 1 : 2;
-  if (g.K < 1 || g.x_rows < 1 || !rows_ok(g, esz, x)) return false;
-  const bool mn = g.w_n == 1 && g.N > 1;
-  if (mn ? dtype == kInt8 : g.w_k != 1 && g.K > 1) return false;
-  const int64_t row = mn ? g.w_k : g.w_n, rows = mn ? g.K : g.N;
-  const int64_t ws = rows == 1 ? 16 : row * esz, we = g.groups() == 1 || g.w_e == 0 ? 16 : g.w_e * esz;
-  return tma_ok(w, ws, we) && (g.rows / 64 + g.groups()) * ((g.N + 127) / 128) < kMaxTiles;
+RowsOperands rows_operands(const GroupedArgs& g, int dtype, const void* x, const void* w) {
+  RowsOperands o;
+  o.mn = dtype != kInt8 && (g.w_n == 1 || g.w_k != 1) && g.N > 1;
+  const int64_t depth = g.groups() == 1 || g.w_e == 0 ? 1 : g.num_experts;
+  o.x = operand_of(x, dtype, 1, g.order ? g.rows : g.x_rows, g.K, 0, g.x_stride, 1, g.order != nullptr);
+  o.w = o.mn ? operand_of(w, dtype, depth, g.K, g.N, g.w_e, g.w_k, g.w_n, false)
+             : operand_of(w, dtype, depth, g.N, g.K, g.w_e, g.w_n, g.w_k, false);
+  return o;
 }
 
-int grouped_rows_tc(const GroupedArgs& args, int dtype, const void* x, const void* w, void* y, int out_dtype,
+// The operands of the weights' gradient, (rows, K) and (rows, N).
+struct WgradOperands {
+  Operand x, dy;
+};
+
+WgradOperands wgrad_operands(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride) {
+  WgradOperands o;
+  o.x = operand_of(x, dtype, 1, g.order ? g.rows : g.x_rows, g.K, 0, g.x_stride, 1, g.order != nullptr);
+  o.dy = operand_of(dy, dtype, 1, g.rows, g.N, 0, dy_stride, 1, false);
+  return o;
+}
+
+bool sizes_ok(const GroupedArgs& g, int dtype) {
+  return (dtype == ES_F32 || dtype == ES_BF16 || dtype == ES_F16 || dtype == kInt8) && g.K > 0 && g.N > 0 &&
+         g.rows > 0 && g.x_rows > 0 && g.rows * planes_of(dtype) < kMaxTiles;
+}
+
+}  // namespace
+
+bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype) {
+  return sizes_ok(g, dtype) && (g.rows / 64 + g.groups()) * ((g.N + 127) / 128) < kMaxTiles;
+}
+
+size_t grouped_rows_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w) {
+  const RowsOperands o = rows_operands(g, dtype, x, w);
+  return o.x.bytes + o.w.bytes;
+}
+
+int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
                     void* workspace, int32_t* status, cudaStream_t stream) {
-  const int64_t esz = dtype == kInt8 ? 1 : 2;
-  GroupedArgs g = args;
-  ES_TRY(gather_rows(g, esz, x, workspace, stream));
-  const int bk = static_cast<int>(128 / esz);
-  const bool mn = g.w_n == 1 && g.N > 1;
+  RowsOperands o = rows_operands(g, dtype, x, w);
+  ES_TRY(lay_out(g, o.x, dtype, true, false, workspace, stream));
+  ES_TRY(lay_out(g, o.w, dtype, false, o.w.depth > 1, static_cast<char*>(workspace) + o.x.bytes, stream));
   TcArgs p{};
-  p.g = args;  // the scales of 8-bit rows go by token
+  p.g = g;
   p.out = y;
   p.out_dtype = out_dtype;
   p.lanes = g.N;
   p.out_col = g.N;
-  p.expert_step = g.groups() == 1 || g.w_e == 0 ? 0 : 1;
-  p.idesc = idesc_of(dtype, mn, false);
+  p.expert_step = o.w.depth > 1 ? 1 : 0;
+  p.plane_experts = static_cast<int>(o.w.depth);
+  p.plane_rows = static_cast<int>(o.x.rows);
+  p.idesc = idesc_of(dtype, o.mn, false);
   p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0;
   p.status = status;
-  const int64_t experts = p.expert_step ? g.num_experts : 1, we = p.expert_step ? g.w_e * esz : 16;
   CUtensorMap m[4];
-  const bool ok =
-      encode_map(mn ? MapSpec{w, dtype, g.N, g.K, experts, g.K == 1 ? round16(g.N * esz) : g.w_k * esz, we, 64, 64}
-                    : MapSpec{w, dtype, g.K, g.N, experts, g.N == 1 ? round16(g.K * esz) : g.w_n * esz, we, bk, 128},
-                 3, &m[0]) &&
-      encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, x_row_bytes(g, esz), 16, bk, kBoxRows}, 2, &m[1]);
-  if (!ok) return ES_ERR_CUDA;
-  m[2] = m[1];
+  const int bk = static_cast<int>(128 / tc_size(dtype));
+  if (!encode_operand(o.w, dtype, o.mn ? 64 : bk, o.mn ? 64 : 128, 3, &m[0]) ||
+      !encode_operand(o.x, dtype, bk, kBoxRows, 2, &m[1]))
+    return ES_ERR_CUDA;
+  m[2] = m[0];
   m[3] = m[1];
-  if (dtype == kInt8) return rows_launch<kKindI8, false>(p, m, stream);
-  return mn ? rows_launch<kKindF16, true>(p, m, stream) : rows_launch<kKindF16, false>(p, m, stream);
+  if (dtype == kInt8) return rows_launch<kKindI8, false, 1>(p, m, stream);
+  if (dtype == ES_F32)
+    return o.mn ? rows_launch<kKindF16, true, 3>(p, m, stream) : rows_launch<kKindF16, false, 3>(p, m, stream);
+  return o.mn ? rows_launch<kKindF16, true, 1>(p, m, stream) : rows_launch<kKindF16, false, 1>(p, m, stream);
 }
 
-bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride) {
-  if (dtype != ES_BF16 && dtype != ES_F16) return false;
-  if (g.rows < 1 || g.x_rows < 1 || (g.w_n != 1 && g.w_k != 1)) return false;
-  return rows_ok(g, 2, x) && tma_ok(dy, g.rows == 1 ? round16(g.N * 2) : dy_stride * 2) &&
+bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype) {
+  return sizes_ok(g, dtype) && (g.w_n == 1 || g.w_k == 1) &&
          g.groups() * ((g.N + 127) / 128) * ((g.K + 127) / 128) < kMaxTiles;
 }
 
-int grouped_wgrad_tc(const GroupedArgs& args, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
+size_t grouped_wgrad_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride) {
+  const WgradOperands o = wgrad_operands(g, dtype, x, dy, dy_stride);
+  return o.x.bytes + o.dy.bytes;
+}
+
+int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,
                      void* workspace, int32_t* status, cudaStream_t stream) {
-  GroupedArgs g = args;
-  ES_TRY(gather_rows(g, 2, x, workspace, stream));
+  WgradOperands o = wgrad_operands(g, dtype, x, dy, dy_stride);
+  ES_TRY(lay_out(g, o.x, dtype, true, false, workspace, stream));
+  GroupedArgs plain = g;
+  plain.order = nullptr;
+  ES_TRY(lay_out(plain, o.dy, dtype, true, false, static_cast<char*>(workspace) + o.x.bytes, stream));
   // lanes: the dimension that is contiguous in dw
   const bool n_lanes = g.w_n == 1;
   TcArgs p{};
@@ -987,24 +1177,22 @@ int grouped_wgrad_tc(const GroupedArgs& args, int dtype, const void* x, const vo
   p.cols = n_lanes ? g.K : g.N;
   p.out_col = n_lanes ? g.w_k : g.w_n;
   p.out_expert = g.w_e;
-  p.src_rows = static_cast<int>(g.rows);
+  p.plane_rows = static_cast<int>(g.rows);
+  p.src_rows = static_cast<int>(g.rows * planes_of(dtype));
   p.idesc = idesc_of(dtype, true, true) | (16u << 24);
   p.pairs = p.lanes % 2 == 0 && p.out_col % 2 == 0 && p.out_expert % 2 == 0 &&
             (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
   p.status = status;
   p.lane_tiles = static_cast<int>((p.lanes + 255) / 256);
   p.col_tiles = static_cast<int>((p.cols + 255) / 256);
-  const int64_t xs = x_row_bytes(g, 2);
-  const int64_t ds = g.rows == 1 ? round16(g.N * 2) : dy_stride * 2;
   CUtensorMap m[4];
-  const int a = n_lanes ? 1 : 0, b = 1 - a;  // place of x among (A, B)
-  const bool ok = encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, 64, 64}, 2, &m[a]) &&
-                  encode_map(MapSpec{x, dtype, g.K, g.x_rows, 1, xs, 16, 64, 1}, 2, &m[2 + a]) &&
-                  encode_map(MapSpec{dy, dtype, g.N, g.rows, 1, ds, 16, 64, 64}, 2, &m[b]) &&
-                  encode_map(MapSpec{dy, dtype, g.N, g.rows, 1, ds, 16, 64, 1}, 2, &m[2 + b]);
-  if (!ok) return ES_ERR_CUDA;
-  return launch<TcShape<2, 256, kKindF16, true, true, false>>(
-      p, m, static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles, 2, stream);
+  const Operand &a = n_lanes ? o.dy : o.x, &b = n_lanes ? o.x : o.dy;
+  if (!encode_operand(a, dtype, 64, 64, 2, &m[0]) || !encode_operand(b, dtype, 64, 64, 2, &m[1]) ||
+      !encode_operand(a, dtype, 64, 1, 2, &m[2]) || !encode_operand(b, dtype, 64, 1, 2, &m[3]))
+    return ES_ERR_CUDA;
+  const int64_t tiles = static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles;
+  if (dtype == ES_F32) return launch<TcShape<2, 256, kKindF16, true, true, false, 3>>(p, m, tiles, 2, stream);
+  return launch<TcShape<2, 256, kKindF16, true, true, false, 1>>(p, m, tiles, 2, stream);
 }
 
 }  // namespace es

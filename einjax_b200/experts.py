@@ -221,11 +221,12 @@ def _grouped(x, w, plan, gather, out_dtype):
     E, K, N = w.shape
     R, code = plan.num_rows, _DTYPES[x.dtype]
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
-    nbytes = L.lib().es_grouped_matmul_workspace_size(code, E, K, N, R, gather)
+    args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), plan.offsets.data_ptr(),
+            plan.order.data_ptr() if gather else None, plan.top_k, R)
+    nbytes = L.lib().es_grouped_matmul_workspace_size(*args)
     ws = _scratch(nbytes, dev)
-    _call("es_grouped_matmul", dev, x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(),
-          plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, R, y.data_ptr(),
-          _DTYPES[out_dtype], _ptr(ws), nbytes, _STATUS.address("es_grouped_matmul", dev.index))
+    _call("es_grouped_matmul", dev, *args, y.data_ptr(), _DTYPES[out_dtype], _ptr(ws), nbytes,
+          _STATUS.address("es_grouped_matmul", dev.index))
     return y
 
 
@@ -236,11 +237,12 @@ def _wgrad(x, dy, w, plan, gather):
     dw = torch.empty((E, N, K), dtype=w.dtype, device=dev).transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 \
         else torch.empty((E, K, N), dtype=w.dtype, device=dev)
     R, code = plan.num_rows, _DTYPES[x.dtype]
-    nbytes = L.lib().es_grouped_matmul_wgrad_workspace_size(code, E, K, N, R, gather)
+    args = (x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E, K, N, plan.offsets.data_ptr(),
+            plan.order.data_ptr() if gather else None, plan.top_k, R, dw.data_ptr(), *dw.stride())
+    nbytes = L.lib().es_grouped_matmul_wgrad_workspace_size(*args)
     ws = _scratch(nbytes, dev)
-    _call("es_grouped_matmul_wgrad", dev, x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E,
-          K, N, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k, R, dw.data_ptr(),
-          *dw.stride(), _ptr(ws), nbytes, _STATUS.address("es_grouped_matmul_wgrad", dev.index))
+    _call("es_grouped_matmul_wgrad", dev, *args, _ptr(ws), nbytes,
+          _STATUS.address("es_grouped_matmul_wgrad", dev.index))
     return dw
 
 
@@ -417,12 +419,13 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     dev = q.device
     R = plan.num_rows if plan is not None else q.shape[0]
     y = torch.empty((R, N), dtype=out_dtype, device=dev)
-    nbytes = L.lib().es_int8_matmul_workspace_size(E, K, N, R, bool(gather))
+    args = (q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(), wscale.data_ptr(), E, K, N,
+            wq.stride(0) if E else 0, wq.stride(-2), plan.offsets.data_ptr() if E else None,
+            plan.order.data_ptr() if gather else None, plan.top_k if E else 1, R)
+    nbytes = L.lib().es_int8_matmul_workspace_size(*args)
     ws = _scratch(nbytes, dev)
-    _call("es_int8_matmul", dev, q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(),
-          wscale.data_ptr(), E, K, N, wq.stride(0) if E else 0, wq.stride(-2),
-          plan.offsets.data_ptr() if E else None, plan.order.data_ptr() if gather else None, plan.top_k if E else 1, R,
-          y.data_ptr(), code, _ptr(ws), nbytes, _STATUS.address("es_int8_matmul", dev.index))
+    _call("es_int8_matmul", dev, *args, y.data_ptr(), code, _ptr(ws), nbytes,
+          _STATUS.address("es_int8_matmul", dev.index))
     return y
 
 

@@ -409,17 +409,22 @@ int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts,
 /* y[r] = x[row(r)] w[e(r)] for the num_rows grouped rows: w[e] is (K, N) with
  * any element strides, row(r) = order[r] / top_k when order is given (x by
  * token), else r. y (num_rows, N) contiguous, of out_dtype (ES_F32 or the
- * operands' type). The workspace depends on whether order is given (gather). */
-size_t es_grouped_matmul_workspace_size(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows,
-                                        int gather);
+ * operands' type). The workspace's size goes by the call's own arguments. */
+size_t es_grouped_matmul_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
+                                        int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
+                                        int64_t w_k_stride, int64_t w_n_stride, const int32_t* offsets,
+                                        const int32_t* order, int top_k, int64_t num_rows);
 int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w, int num_experts,
                       int64_t K, int64_t N, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
                       const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, void* y,
                       int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 /* dw[e] = sum over e's rows of x[row(r)]^T dy[r], with dw's element strides;
  * zero for an expert without rows. dw has the operands' type. */
-size_t es_grouped_matmul_wgrad_workspace_size(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows,
-                                              int gather);
+size_t es_grouped_matmul_wgrad_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride,
+                                              const void* dy, int64_t dy_stride, int num_experts, int64_t K,
+                                              int64_t N, const int32_t* offsets, const int32_t* order, int top_k,
+                                              int64_t num_rows, void* dw, int64_t dw_expert_stride,
+                                              int64_t dw_k_stride, int64_t dw_n_stride);
 int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* dy,
                             int64_t dy_stride, int num_experts, int64_t K, int64_t N, const int32_t* offsets,
                             const int32_t* order, int top_k, int64_t num_rows, void* dw, int64_t dw_expert_stride,
@@ -450,7 +455,10 @@ int es_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t width, 
  * the sum exact in 32-bit integers (K <= 133152). wq: (num_experts, N, K) int8
  * with contiguous k, w_scale (num_experts, N). num_experts == 0: one matrix
  * for all rows (offsets and order NULL). y (num_rows, N) contiguous. */
-size_t es_int8_matmul_workspace_size(int num_experts, int64_t K, int64_t N, int64_t num_rows, int gather);
+size_t es_int8_matmul_workspace_size(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,
+                                     const int8_t* wq, const float* w_scale, int num_experts, int64_t K, int64_t N,
+                                     int64_t w_expert_stride, int64_t w_n_stride, const int32_t* offsets,
+                                     const int32_t* order, int top_k, int64_t num_rows);
 int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride, const int8_t* wq,
                    const float* w_scale, int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
                    int64_t w_n_stride, const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows,
