@@ -45,8 +45,8 @@
 namespace es {
 namespace {
 
-constexpr int kTcThreads = 256;
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;
+constexpr int kTcThreads = 128 + 32 * kEpiWarps;
 constexpr int kABytes = 16384;  // 128 lanes x 128 bytes of depth
 constexpr int kSwizzleRow = 128;
 constexpr int kBoxRows = 32;    // rows of one TMA box of X
@@ -282,8 +282,9 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 __host__ __device__ constexpr int term_a(int t) { return t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0; }
 __host__ __device__ constexpr int term_b(int t) { return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0; }
 
-template <int CG_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
+template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
 struct TcShape {
+  static constexpr int MT = MT_;  // accumulators of 128 lanes (of each CTA) that share B
   static constexpr int kTerms = PLANES_ == 3 ? 6 : 1;
   static constexpr int kChain = PLANES_ == 3 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int CG = CG_;        // CTAs of one MMA
@@ -293,8 +294,9 @@ struct TcShape {
   static constexpr bool WGRAD = WGRAD_;
   static constexpr bool SPLIT = SPLIT_; // the cluster's CTAs share one tile's depth
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
-  static constexpr int kLanes = 128 * CG;
-  static constexpr int kStageBytes = kABytes + NT / CG * kSwizzleRow;
+  static constexpr int kLanes = 128 * MT * CG;
+  static constexpr int kBufs = 2 * MT * NT <= 512 ? 2 : 1;  // tiles in TMEM
+  static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     grouped_tc_kernel(const __grid_constant__ TcArgs p, const __grid_constant__ CUtensorMap map_a,
                       const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap rows_a,
                       const __grid_constant__ CUtensorMap rows_b) {
-  constexpr int CG = S::CG, NT = S::NT, BK = S::BK, STAGES = S::kStages;
+  constexpr int CG = S::CG, MT = S::MT, NT = S::NT, BK = S::BK, STAGES = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcCtl ctl;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -478,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ctl.progress = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc_alloc<CG>(&ctl.tmem, 2 * NT);
+  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kBufs * MT * NT);
   if (warp == 2) {  // tiles of each group
     int run = 0;
     for (int e0 = 0; e0 < groups; e0 += 32) {
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const TileAt at = tiles.at(t, rank, csize);
       const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
       const int half = width / CG;  // columns of this CTA's part of B
-      const int64_t lane0 = at.lane0 + pair_rank * 128;
+      const int lane0 = static_cast<int>(at.lane0) + static_cast<int>(pair_rank) * 128;
       const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
       for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
         const int s1 = s0 + min(S::kChain, at.kb1 - s0);
@@ -541,9 +543,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   src[i] = r < valid ? at.first + kb * BK + r : -1;
                 }
               }
-              bytes = (2 + (half + 63) / 64) * rows16 * 128u;
+              bytes = (2 * MT + (half + 63) / 64) * rows16 * 128u;
             } else {
-              bytes = kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
+              bytes = MT * kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
             }
             int go = 0;
             if (lane == 0) {
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               ok = false;
               break;
             }
-            const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
+            const uint32_t sa = base + stage * S::kStageBytes, sb = sa + MT * kABytes;
             const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
             if constexpr (S::WGRAD) {
               // operand boxes of 64 lanes (columns) by 64 rows; of the last block
@@ -573,23 +575,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ra[i] = src[i] < 0 ? p.src_rows : src[i] + plane_a * p.plane_rows;
                     rb[i] = src[i] < 0 ? p.src_rows : src[i] + plane_b * p.plane_rows;
                   }
-                  load_rows<CG>(sa + (lane >> 4) * 8192 + quad * 512, &rows_a,
-                                static_cast<int>(lane0) + (lane >> 4) * 64, ra, bar);
+#pragma unroll
+                  for (int m = 0; m < MT; ++m)
+                    load_rows<CG>(sa + m * kABytes + (lane >> 4) * 8192 + quad * 512, &rows_a,
+                                  lane0 + m * 128 * CG + (lane >> 4) * 64, ra, bar);
                   for (int b = lane >> 4; b < boxes; b += 2)
                     load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
                 }
-              } else if (lane < 2) {
-                load_2d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, row_a, bar);
-              } else if (lane - 2 < boxes) {
-                load_2d<CG>(sb + (lane - 2) * 8192, &map_b, col0 + (lane - 2) * 64, row_b, bar);
+              } else if (lane < 2 * MT) {
+                load_2d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, row_a, bar);
+              } else if (lane - 2 * MT < boxes) {
+                load_2d<CG>(sb + (lane - 2 * MT) * 8192, &map_b, col0 + (lane - 2 * MT) * 64, row_b, bar);
               }
             } else {
               const int z = at.expert * p.expert_step + plane_a * p.plane_experts;
               if constexpr (S::A_MN) {
-                if (lane < 2)
-                  load_3d<CG>(sa + lane * 8192, &map_a, static_cast<int>(lane0) + lane * 64, kb * BK, z, bar);
+                if (lane < 2 * MT)
+                  load_3d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
+                              bar);
               } else {
-                if (lane == 0) load_3d<CG>(sa, &map_a, kb * BK, static_cast<int>(lane0), z, bar);
+                if (lane < MT) load_3d<CG>(sa + lane * kABytes, &map_a, kb * BK, lane0 + lane * 128 * CG, z, bar);
               }
               if (lane * kBoxRows < half)
                 load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK,
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + buf * NT;
+          const uint32_t d = tmem + buf * MT * NT;
           uint32_t more = 0;
           for (int term = 0; term < S::kTerms && ok; ++term)
             for (int kb = s0; kb < s1; ++kb) {
@@ -642,16 +647,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (!ok) break;
               tc_fence_after();
               const uint32_t sa = base + stage * S::kStageBytes;
-              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + kABytes, S::WGRAD);
+              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + MT * kABytes, S::WGRAD);
               constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
               int steps = 4;
               if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
-              if (steps == 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, more | i);
-              } else {
-                for (int i = 0; i < steps; ++i)
-                  mma<CG, S::KIND>(d, da + i * step_a, db + i * step_b, idesc, more | i);
+              for (int m = 0; m < MT; ++m) {
+                const uint64_t dm = da + m * (kABytes >> 4);
+                if (steps == 4) {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
+                } else {
+                  for (int i = 0; i < steps; ++i)
+                    mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
+                }
               }
               more = 1;
               commit<CG>(&ctl.empty[stage]);
@@ -662,7 +672,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           if (!ok) break;
           commit<CG>(&ctl.acc_full[buf]);
-          if (++buf == 2) {
+          if (++buf == S::kBufs) {
             buf = 0;
             acc_phase ^= 1;
           }
@@ -679,21 +689,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       clear_rows(p, p.g.kept(), p.g.rows, blockIdx.x * 64LL + (threadIdx.x - 64), gridDim.x * 64LL);
   } else {
     // ------------------------------------------------------------- epilogue
-    const int quad = warp & 3;
+    // two sets of four warps share the tile's 32-column blocks
+    const int quad = warp & 3, set = (warp - 4) >> 2;
     int buf = 0;
     uint32_t acc_phase = 0, red_phase = 0;
     for (int t = t0; t < tiles.total; t += step) {
       const TileAt at = tiles.at(t, rank, csize);
-      const int64_t ch = at.lane0 + pair_rank * 128 + quad * 32 + lane;
-      const bool live = ch < p.lanes;
-      float wscale = 1.0f;
-      if constexpr (S::KIND == kKindI8) wscale = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
+      const int64_t ch0 = at.lane0 + pair_rank * 128 + quad * 32 + lane;
+      const int blocks = (at.rows + 31) / 32;
       if constexpr (S::SPLIT) {  // the last tile's parts have been read by the whole cluster
         int go = 1;
         if (lane == 0) go = tc_wait(&ctl.red_empty, red_phase ^ 1, &ctl, p.status, true) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
       }
-      const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col + ch;
+      const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col;
       bool ok = true;
       int s0 = at.kb0;
       do {  // the chains of the sum; one pass over zeros where there is no depth
@@ -705,16 +714,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!ok) break;
           tc_fence_after();
         }
-        const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16);
-        for (int c0 = 0; c0 < at.rows; c0 += 32) {
+        const uint32_t acc = tmem + buf * MT * NT + (static_cast<uint32_t>(quad * 32) << 16);
+        for (int b = set; b < MT * blocks; b += 2) {
+          const int m = b / blocks, c0 = (b - m * blocks) * 32, n = at.rows - c0;
+          const int64_t ch = ch0 + m * 128 * CG;
+          const bool live = ch < p.lanes;
           float v[32];
           if (any) {
-            tmem_ld32(acc + c0, v);
+            tmem_ld32(acc + m * NT + c0, v);
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.0f;
           }
-          const int n = at.rows - c0;
           if constexpr (S::SPLIT) {
             // this CTA's part of the sum into shared memory, [column][lane];
             // 8-bit products stay integers (their bits travel as floats)
@@ -724,6 +735,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (i < n) mine[i * 128] = first ? v[i] : mine[i * 128] + v[i];
           } else {
             if constexpr (S::KIND == kKindI8) {
+              const float wscale = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
               float xs = 0.0f;  // lane l holds the scale of column c0 + l
               bool row = false;
               if (lane < n) {
@@ -738,7 +750,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 v[i] = (rows >> i) & 1 ? static_cast<float>(__float_as_int(v[i])) * s * wscale : 0.0f;
               }
             }
-            const int64_t at0 = out0 + c0 * p.out_col;
+            const int64_t at0 = out0 + c0 * p.out_col + ch;
             if constexpr (S::kTerms > 1) {
               float* o = static_cast<float*>(p.out) + at0;
               if (!first && live) {
@@ -756,7 +768,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
-          if (++buf == 2) {
+          if (++buf == S::kBufs) {
             buf = 0;
             acc_phase ^= 1;
           }
@@ -770,8 +782,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int go = 1;
         if (lane == 0) go = tc_wait(&ctl.red_full, red_phase, &ctl, p.status, true) ? 1 : 0;
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
-        // columns rank, rank + csize, ...: the parts are added in the CTAs' order
-        for (int c = rank; c < at.rows; c += csize) {
+        const bool live = ch0 < p.lanes;
+        float wscale = 1.0f;
+        if constexpr (S::KIND == kKindI8) wscale = live ? p.g.w_scale[at.expert * p.lanes + ch0] : 0.0f;
+        // every (2 csize)-th column: the parts are added in the CTAs' order
+        for (int c = rank * 2 + set; c < at.rows; c += 2 * csize) {
           const uint32_t mine = smem_u32(part + c * 128 + quad * 32 + lane);
           float v = 0.0f;
           if constexpr (S::KIND == kKindI8) {
@@ -782,7 +797,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           } else {
             for (uint32_t r = 0; r < csize; ++r) v += load_at(at_rank(mine, r));
           }
-          if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch, v);
+          if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch0, v);
         }
         __syncwarp();
         if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
@@ -795,7 +810,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   if (csize > 1) cluster_sync();
   tc_fence_after();
-  if (warp == 1) tc_dealloc<CG>(tmem, 2 * NT);
+  if (warp == 1) tc_dealloc<CG>(tmem, S::kBufs * MT * NT);
 }
 
 // --------------------------------------------------------------------- host
@@ -1046,26 +1061,26 @@ int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
   const int64_t R = p.g.rows, groups = p.g.groups();
   const int64_t live = groups < R ? groups : R;  // groups that can have rows
   const int64_t mean = R / live;
-  auto tiles = [&](int cg, int nt) {
-    p.lane_tiles = static_cast<int>((p.lanes + 128 * cg - 1) / (128 * cg));
+  auto tiles = [&](int lanes, int nt) {
+    p.lane_tiles = static_cast<int>((p.lanes + lanes - 1) / lanes);
     return (R / nt + live) * p.lane_tiles;
   };
   if (mean > 128) {
-    const int64_t n = tiles(2, 256);
+    const int64_t n = tiles(512, 256);
     p.idesc |= 16u << 24;
-    return launch<TcShape<2, 256, KIND, A_MN, false, false, PLANES>>(p, m, n, 2, stream);
+    return launch<TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>>(p, m, n, 2, stream);
   }
   p.idesc |= 8u << 24;
-  if (mean > 64) return launch<TcShape<1, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(1, 128), 1, stream);
+  if (mean > 64) return launch<TcShape<1, 1, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(128, 128), 1, stream);
   // few rows: the weights' bytes are the time; a tile's depth is shared by a
   // cluster while the tiles alone do not fill the SMs
-  const int64_t n = tiles(1, 64);
-  const int64_t nkb = (p.g.K + TcShape<1, 64, KIND, A_MN, false, true, PLANES>::BK - 1) /
-                      TcShape<1, 64, KIND, A_MN, false, true, PLANES>::BK;
+  const int64_t n = tiles(128, 64);
+  const int64_t nkb = (p.g.K + TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>::BK - 1) /
+                      TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>::BK;
   int split = 1;
   while (split < 8 && n * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
-  if (split > 1) return launch<TcShape<1, 64, KIND, A_MN, false, true, PLANES>>(p, m, n, split, stream);
-  return launch<TcShape<1, 64, KIND, A_MN, false, false, PLANES>>(p, m, n, 1, stream);
+  if (split > 1) return launch<TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>>(p, m, n, split, stream);
+  return launch<TcShape<1, 1, 64, KIND, A_MN, false, false, PLANES>>(p, m, n, 1, stream);
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
@@ -1183,7 +1198,7 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
   p.pairs = p.lanes % 2 == 0 && p.out_col % 2 == 0 && p.out_expert % 2 == 0 &&
             (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
   p.status = status;
-  p.lane_tiles = static_cast<int>((p.lanes + 255) / 256);
+  p.lane_tiles = static_cast<int>((p.lanes + 511) / 512);
   p.col_tiles = static_cast<int>((p.cols + 255) / 256);
   CUtensorMap m[4];
   const Operand &a = n_lanes ? o.dy : o.x, &b = n_lanes ? o.x : o.dy;
@@ -1191,8 +1206,8 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
       !encode_operand(a, dtype, 64, 1, 2, &m[2]) || !encode_operand(b, dtype, 64, 1, 2, &m[3]))
     return ES_ERR_CUDA;
   const int64_t tiles = static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles;
-  if (dtype == ES_F32) return launch<TcShape<2, 256, kKindF16, true, true, false, 3>>(p, m, tiles, 2, stream);
-  return launch<TcShape<2, 256, kKindF16, true, true, false, 1>>(p, m, tiles, 2, stream);
+  if (dtype == ES_F32) return launch<TcShape<2, 2, 256, kKindF16, true, true, false, 3>>(p, m, tiles, 2, stream);
+  return launch<TcShape<2, 2, 256, kKindF16, true, true, false, 1>>(p, m, tiles, 2, stream);
 }
 
 }  // namespace es
