@@ -385,24 +385,37 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Stores v[c] (lane = this thread's channel) to out + c * stride, c < n. In
-// 16 bits two neighbouring lanes trade values, so that each stores two
-// channels of every other column: 4-byte stores, half as many.
+// Two neighbouring lanes (channels) trade values, so that the even one holds
+// both channels of the even columns and the odd one of the odd columns.
+template <typename T>
+__device__ __forceinline__ void pack_cols(const float (&v)[32], uint32_t (&two)[16]) {
+  const int odd = threadIdx.x & 1;
+#pragma unroll
+  for (int c = 0; c < 32; c += 2) {
+    const float got = __shfl_xor_sync(0xffffffffu, odd ? v[c] : v[c + 1], 1);
+    two[c / 2] = odd ? pack2<T>(got, v[c + 1]) : pack2<T>(v[c], got);
+  }
+}
+
+// Stores packed columns c < n to out + c * stride (out: this lane's channel).
+template <typename T>
+__device__ __forceinline__ void store_packed(T* out, int64_t stride, const uint32_t (&two)[16], int n, bool live) {
+  const int odd = threadIdx.x & 1;
+  T* o = out - odd + odd * stride;
+#pragma unroll
+  for (int c = 0; c < 32; c += 2)
+    if (live && c + odd < n) *reinterpret_cast<uint32_t*>(o + c * stride) = two[c / 2];
+}
+
+// Stores v[c] (lane = this thread's channel) to out + c * stride, c < n.
 template <typename T>
 __device__ __forceinline__ void store_cols(T* out, int64_t stride, const float (&v)[32], int n, bool live,
                                            bool pairs) {
   if constexpr (sizeof(T) == 2) {
     if (pairs) {
-      const int odd = threadIdx.x & 1;
-#pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        const float give = odd ? v[c] : v[c + 1];
-        const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-        if (live && c + odd < n) {
-          const uint32_t two = odd ? pack2<T>(got, v[c + 1]) : pack2<T>(v[c], got);
-          *reinterpret_cast<uint32_t*>(out - odd + (c + odd) * stride) = two;
-        }
-      }
+      uint32_t two[16];
+      pack_cols<T>(v, two);
+      store_packed(out, stride, two, n, live);
       return;
     }
   }
@@ -442,6 +455,37 @@ __device__ __forceinline__ void clear_rows(const TcArgs& p, int64_t from, int64_
   const int64_t n = (halves - head) / 8;
   for (int64_t i = t; i < n; i += nt) mid[i] = make_uint4(0, 0, 0, 0);
   for (int64_t i = head + n * 8 + t; i < halves; i += nt) reinterpret_cast<uint16_t*>(a)[i] = 0;
+}
+
+// Reads one accumulator of a 16-bit output tile. TMEM holds a single tile of
+// this size, so the next tile's MMAs wait for this: all but the first blocks of
+// 32 columns are packed in registers and stored after the accumulator has been
+// handed back. `scale(v, b)` finishes block b, `release` hands back.
+constexpr int kAtOnce = 2;  // blocks stored at once: eight held ones would spill
+
+template <typename T, typename Scale, typename Release>
+__device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, Scale scale,
+                                           Release release) {
+  uint32_t held[8 - kAtOnce][16];
+  const int blocks = (rows + 31) / 32;
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    if (b >= blocks) continue;
+    float v[32];
+    tmem_ld32(acc + b * 32, v);
+    scale(v, b);
+    if (b < kAtOnce) {
+      uint32_t two[16];
+      pack_cols<T>(v, two);
+      store_packed(out + b * 32 * stride, stride, two, rows - b * 32, live);
+    } else {
+      pack_cols<T>(v, held[b - kAtOnce]);
+    }
+  }
+  release();
+#pragma unroll
+  for (int b = kAtOnce; b < 8; ++b)
+    if (b < blocks) store_packed(out + b * 32 * stride, stride, held[b - kAtOnce], rows - b * 32, live);
 }
 
 template <typename S>
@@ -703,6 +747,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
       }
       const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col;
+      // scales of 8-bit operands, loaded under the MMAs: lane l has those of
+      // columns l, l + 32, ...
+      float xs[S::KIND == kKindI8 ? NT / 32 : 1], ws[MT];
+      if constexpr (S::KIND == kKindI8 && !S::SPLIT) {
+#pragma unroll
+        for (int b = 0; b < NT / 32; ++b) {
+          xs[b] = 0.0f;
+          if (b * 32 + lane < at.rows) {
+            const int64_t tok = p.g.source(at.row0 + b * 32 + lane);
+            if (tok >= 0) xs[b] = p.g.x_scale[tok];
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          ws[m] = ch0 + m * 128 * CG < p.lanes ? p.g.w_scale[at.expert * p.lanes + ch0 + m * 128 * CG] : 0.0f;
+      }
+      auto scale = [&](float (&v)[32], float x, float w) {
+        if constexpr (S::KIND == kKindI8) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = static_cast<float>(__float_as_int(v[i])) * __shfl_sync(0xffffffffu, x, i) * w;
+        }
+      };
       bool ok = true;
       int s0 = at.kb0;
       do {  // the chains of the sum; one pass over zeros where there is no depth
@@ -715,7 +782,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           tc_fence_after();
         }
         const uint32_t acc = tmem + buf * MT * NT + (static_cast<uint32_t>(quad * 32) << 16);
-        for (int b = set; b < MT * blocks; b += 2) {
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
+        };
+        bool released = !any;
+        if constexpr (S::kBufs == 1 && S::kTerms == 1) {
+          if (any && p.pairs && p.out_dtype != ES_F32) {
+            const int64_t ch = ch0 + set * 128 * CG;
+            const uint32_t mine = acc + set * NT;
+            auto finish = [&](float (&v)[32], int b) {
+              if constexpr (S::KIND == kKindI8) scale(v, xs[b], set ? ws[MT - 1] : ws[0]);
+            };
+            if (p.out_dtype == ES_BF16)
+              drain_held(mine, static_cast<__nv_bfloat16*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes,
+                         finish, release);
+            else
+              drain_held(mine, static_cast<__half*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes, finish,
+                         release);
+            released = true;
+          }
+        }
+        for (int b = set; b < MT * blocks && (!released || !any); b += 2) {
           const int m = b / blocks, c0 = (b - m * blocks) * 32, n = at.rows - c0;
           const int64_t ch = ch0 + m * 128 * CG;
           const bool live = ch < p.lanes;
@@ -735,20 +824,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               if (i < n) mine[i * 128] = first ? v[i] : mine[i * 128] + v[i];
           } else {
             if constexpr (S::KIND == kKindI8) {
-              const float wscale = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
-              float xs = 0.0f;  // lane l holds the scale of column c0 + l
-              bool row = false;
-              if (lane < n) {
-                const int64_t tok = p.g.source(at.row0 + c0 + lane);
-                row = tok >= 0;
-                if (row) xs = p.g.x_scale[tok];
-              }
-              const unsigned rows = __ballot_sync(0xffffffffu, row);
+              float x = xs[0], w = ws[0];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float s = __shfl_sync(0xffffffffu, xs, i);
-                v[i] = (rows >> i) & 1 ? static_cast<float>(__float_as_int(v[i])) * s * wscale : 0.0f;
-              }
+              for (int i = 1; i < NT / 32; ++i)
+                if (c0 == i * 32) x = xs[i];
+              if (m > 0) w = ws[MT - 1];
+              scale(v, x, w);
             }
             const int64_t at0 = out0 + c0 * p.out_col + ch;
             if constexpr (S::kTerms > 1) {
@@ -764,10 +845,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
+        if (!released) release();
         if (any) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
           if (++buf == S::kBufs) {
             buf = 0;
             acc_phase ^= 1;
