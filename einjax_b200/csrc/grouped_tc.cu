@@ -296,6 +296,7 @@ struct TcShape {
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
   static constexpr int kLanes = 128 * MT * CG;
   static constexpr int kBufs = 2 * MT * NT <= 512 ? 2 : 1;  // tiles in TMEM
+  static constexpr bool kHeld = kBufs == 1 && PLANES_ == 1;  // tiles are held in registers, see drain_held
   static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
@@ -385,26 +386,32 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// Two neighbouring lanes (channels) trade values, so that the even one holds
-// both channels of the even columns and the odd one of the odd columns.
+// Keeps the compiler from computing a stride's multiples ahead of the loop over
+// tiles: they took 60 registers that the held accumulators need.
+__device__ __forceinline__ void keep_here(int64_t& stride) { asm volatile("" : "+l"(stride)); }
+
 template <typename T>
 __device__ __forceinline__ void pack_cols(const float (&v)[32], uint32_t (&two)[16]) {
-  const int odd = threadIdx.x & 1;
 #pragma unroll
-  for (int c = 0; c < 32; c += 2) {
-    const float got = __shfl_xor_sync(0xffffffffu, odd ? v[c] : v[c + 1], 1);
-    two[c / 2] = odd ? pack2<T>(got, v[c + 1]) : pack2<T>(v[c], got);
-  }
+  for (int i = 0; i < 16; ++i) two[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
 }
 
-// Stores packed columns c < n to out + c * stride (out: this lane's channel).
+// Stores columns c < n, packed two to a register, to out + c * stride (out:
+// this lane's channel). Two neighbouring lanes (channels) trade registers, so
+// that the even one stores both channels of the even columns and the odd one
+// of the odd columns, in 4-byte stores.
 template <typename T>
 __device__ __forceinline__ void store_packed(T* out, int64_t stride, const uint32_t (&two)[16], int n, bool live) {
+  keep_here(stride);
   const int odd = threadIdx.x & 1;
   T* o = out - odd + odd * stride;
+  const uint32_t take = odd ? 0x3276u : 0x5410u;  // the high halves (theirs, mine), or the low ones (mine, theirs)
 #pragma unroll
-  for (int c = 0; c < 32; c += 2)
-    if (live && c + odd < n) *reinterpret_cast<uint32_t*>(o + c * stride) = two[c / 2];
+  for (int c = 0; c < 32; c += 2) {
+    const uint32_t theirs = __shfl_xor_sync(0xffffffffu, two[c / 2], 1);
+    if (live && c + odd < n) *reinterpret_cast<uint32_t*>(o) = __byte_perm(two[c / 2], theirs, take);
+    o += 2 * stride;
+  }
 }
 
 // Stores v[c] (lane = this thread's channel) to out + c * stride, c < n.
@@ -419,9 +426,12 @@ __device__ __forceinline__ void store_cols(T* out, int64_t stride, const float (
       return;
     }
   }
+  keep_here(stride);
 #pragma unroll
-  for (int c = 0; c < 32; ++c)
-    if (live && c < n) out[c * stride] = from_f32<T>(v[c]);
+  for (int c = 0; c < 32; ++c) {
+    if (live && c < n) *out = from_f32<T>(v[c]);
+    out += stride;
+  }
 }
 
 __device__ __forceinline__ void store_typed(void* out, int dtype, int64_t at, int64_t stride, const float (&v)[32],
@@ -457,36 +467,80 @@ __device__ __forceinline__ void clear_rows(const TcArgs& p, int64_t from, int64_
   for (int64_t i = head + n * 8 + t; i < halves; i += nt) reinterpret_cast<uint16_t*>(a)[i] = 0;
 }
 
-// Reads one accumulator of a 16-bit output tile. TMEM holds a single tile of
-// this size, so the next tile's MMAs wait for this: all but the first blocks of
-// 32 columns are packed in registers and stored after the accumulator has been
-// handed back. `scale(v, b)` finishes block b, `release` hands back.
-constexpr int kAtOnce = 2;  // blocks stored at once: eight held ones would spill
-
-template <typename T, typename Scale, typename Release>
-__device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, Scale scale,
-                                           Release release) {
-  uint32_t held[8 - kAtOnce][16];
-  const int blocks = (rows + 31) / 32;
+// The 8-bit product's sums times the scales of their rows (xs) and channel.
+__device__ __forceinline__ void scale_block(float (&v)[32], const float* xs, float w) {
 #pragma unroll
-  for (int b = 0; b < 8; ++b) {
-    if (b >= blocks) continue;
-    float v[32];
-    tmem_ld32(acc + b * 32, v);
-    scale(v, b);
-    if (b < kAtOnce) {
-      uint32_t two[16];
-      pack_cols<T>(v, two);
-      store_packed(out + b * 32 * stride, stride, two, rows - b * 32, live);
-    } else {
-      pack_cols<T>(v, held[b - kAtOnce]);
+  for (int i = 0; i < 32; i += 4) {
+    const float4 x = *reinterpret_cast<const float4*>(xs + i);
+    v[i] = static_cast<float>(__float_as_int(v[i])) * x.x * w;
+    v[i + 1] = static_cast<float>(__float_as_int(v[i + 1])) * x.y * w;
+    v[i + 2] = static_cast<float>(__float_as_int(v[i + 2])) * x.z * w;
+    v[i + 3] = static_cast<float>(__float_as_int(v[i + 3])) * x.w * w;
+  }
+}
+
+// Reads one accumulator of an output tile. TMEM holds a single tile of this
+// size, so the next tile's MMAs wait for this: the last blocks of 32 columns
+// are held in registers (16-bit ones packed) and stored after the accumulator has been
+// handed back (`release`). xs, w: scales of 8-bit operands (I8).
+constexpr int kAtOnce = 0;   // blocks stored at once, 16-bit tiles
+constexpr int kAtOnce32 = 3; // and fp32 tiles: the rest fits the registers
+
+template <typename T, bool I8, typename Release>
+__device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, const float* xs,
+                                           float w, Release release) {
+  // all of the accumulator, whatever `rows`: no branch parts the registers' lives
+  if constexpr (sizeof(T) == 2) {
+    uint32_t held[8 - kAtOnce][16];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      float v[32];
+      tmem_ld32(acc + b * 32, v);
+      if constexpr (I8) scale_block(v, xs + b * 32, w);
+      if (b < kAtOnce) {
+        uint32_t two[16];
+        pack_cols<T>(v, two);
+        store_packed(out, stride, two, rows - b * 32, live);
+        out += 32 * stride;
+      } else {
+        pack_cols<T>(v, held[b - kAtOnce]);
+      }
+    }
+    release();
+#pragma unroll
+    for (int b = kAtOnce; b < 8; ++b) {
+      store_packed(out, stride, held[b - kAtOnce], rows - b * 32, live);
+      out += 32 * stride;
+    }
+  } else {
+    float held[8 - kAtOnce32][32];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      if (b < kAtOnce32) {
+        float v[32];
+        tmem_ld32(acc + b * 32, v);
+        if constexpr (I8) scale_block(v, xs + b * 32, w);
+        store_cols(out, stride, v, rows - b * 32, live, false);
+        out += 32 * stride;
+      } else {
+        tmem_ld32(acc + b * 32, held[b - kAtOnce32]);
+        if constexpr (I8) scale_block(held[b - kAtOnce32], xs + b * 32, w);
+      }
+    }
+    release();
+#pragma unroll
+    for (int b = kAtOnce32; b < 8; ++b) {
+      store_cols(out, stride, held[b - kAtOnce32], rows - b * 32, live, false);
+      out += 32 * stride;
     }
   }
-  release();
-#pragma unroll
-  for (int b = kAtOnce; b < 8; ++b)
-    if (b < blocks) store_packed(out + b * 32 * stride, stride, held[b - kAtOnce], rows - b * 32, live);
 }
+
+// Registers: the epilogue's two warpgroups take over what the first does not
+// need. 128 * kRoleRegs + 256 * kEpiRegs = 384 * kLaunchRegs, which the launch
+// has (checked there: a split of more would wait for ever).
+constexpr int kRoleRegs = 72, kEpiRegs = 216, kLaunchRegs = 168;
+static_assert(128 * kRoleRegs + 256 * kEpiRegs == kTcThreads * kLaunchRegs, "register split");
 
 template <typename S>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -496,6 +550,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int CG = S::CG, MT = S::MT, NT = S::NT, BK = S::BK, STAGES = S::kStages;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcCtl ctl;
+  __shared__ alignas(16) float x_scales[S::KIND == kKindI8 ? 2 : 1][S::KIND == kKindI8 ? NT : 4];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* part = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + STAGES * S::kStageBytes);
   int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(part) + S::kPartBytes);
@@ -556,187 +611,191 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const Tiles<S> tiles{p, pre, lo, cnt, S::WGRAD ? groups * p.lane_tiles * p.col_tiles : pre[groups]};
   const int step = static_cast<int>(gridDim.x / csize), t0 = static_cast<int>(blockIdx.x / csize);
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA loads
-    int stage = 0, used = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    for (int t = t0; t < tiles.total && ok; t += step) {
-      const TileAt at = tiles.at(t, rank, csize);
-      const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
-      const int half = width / CG;  // columns of this CTA's part of B
-      const int lane0 = static_cast<int>(at.lane0) + static_cast<int>(pair_rank) * 128;
-      const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
-      for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
-        const int s1 = s0 + min(S::kChain, at.kb1 - s0);
-        for (int term = 0; term < S::kTerms && ok; ++term) {
-          const int plane_a = S::kTerms > 1 ? term_a(term) : 0, plane_b = S::kTerms > 1 ? term_b(term) : 0;
-          for (int kb = s0; kb < s1; ++kb) {
-            uint32_t bytes;
-            int src[4];            // weights' gradient, last block: four rows of a gather
-            int rows16 = BK;       // rows of the block in whole MMA steps
-            bool tail = false;
-            if constexpr (S::WGRAD) {
-              const int valid = min(at.depth - kb * BK, BK);
-              tail = valid < BK;
-              if (tail) {
-                rows16 = (valid + 15) & ~15;
-    #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int r = (lane & 15) * 4 + i;
-                  src[i] = r < valid ? at.first + kb * BK + r : -1;
-                }
-              }
-              bytes = (2 * MT + (half + 63) / 64) * rows16 * 128u;
-            } else {
-              bytes = MT * kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
-            }
-            int go = 0;
-            if (lane == 0) {
-              go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
-              if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
-              if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
-            }
-            go = __shfl_sync(0xffffffffu, go, 0);
-            if (!go) {
-              ok = false;
-              break;
-            }
-            const uint32_t sa = base + stage * S::kStageBytes, sb = sa + MT * kABytes;
-            const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
-            if constexpr (S::WGRAD) {
-              // operand boxes of 64 lanes (columns) by 64 rows; of the last block
-              // loads of four rows, dealt to half a warp a box
-              const int row_a = at.first + kb * BK + plane_a * p.plane_rows;
-              const int row_b = at.first + kb * BK + plane_b * p.plane_rows;
-              const int boxes = (half + 63) / 64;
-              if (tail) {
-                const int quad = lane & 15;
-                if (quad * 4 < rows16) {
-                  int ra[4], rb[4];
-    #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    ra[i] = src[i] < 0 ? p.src_rows : src[i] + plane_a * p.plane_rows;
-                    rb[i] = src[i] < 0 ? p.src_rows : src[i] + plane_b * p.plane_rows;
-                  }
-#pragma unroll
-                  for (int m = 0; m < MT; ++m)
-                    load_rows<CG>(sa + m * kABytes + (lane >> 4) * 8192 + quad * 512, &rows_a,
-                                  lane0 + m * 128 * CG + (lane >> 4) * 64, ra, bar);
-                  for (int b = lane >> 4; b < boxes; b += 2)
-                    load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
-                }
-              } else if (lane < 2 * MT) {
-                load_2d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, row_a, bar);
-              } else if (lane - 2 * MT < boxes) {
-                load_2d<CG>(sb + (lane - 2 * MT) * 8192, &map_b, col0 + (lane - 2 * MT) * 64, row_b, bar);
-              }
-            } else {
-              const int z = at.expert * p.expert_step + plane_a * p.plane_experts;
-              if constexpr (S::A_MN) {
-                if (lane < 2 * MT)
-                  load_3d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
-                              bar);
-              } else {
-                if (lane < MT) load_3d<CG>(sa + lane * kABytes, &map_a, kb * BK, lane0 + lane * 128 * CG, z, bar);
-              }
-              if (lane * kBoxRows < half)
-                load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK,
-                            col0 + lane * kBoxRows + plane_b * p.plane_rows, bar);
-            }
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1;
-            }
-          }
-        }
-      }
-    }
-    if (lane == 0) {
-      // the stages still held: their MMAs have arrived here before this CTA may end
-      for (int s = 0; s < STAGES && ok; ++s) {
-        if (s < used) {
-          const int last = (stage + STAGES - 1 - s) % STAGES;
-          const uint32_t ph = last < stage ? phase : phase ^ 1;
-          ok = tc_wait(&ctl.empty[last], ph, &ctl, p.status);
-        }
-      }
-      if (!ok && leader)
-        for (int s = 0; s < STAGES && s < used; ++s) {
-          const int last = (stage + STAGES - 1 - s) % STAGES;
-          tc_drain(&ctl.full[last], last < stage ? phase : phase ^ 1);
-        }
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- MMAs
-    if (leader && lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, acc_phase = 0;
+  if (warp < 4) {
+    if constexpr (S::kHeld) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA loads
+      int stage = 0, used = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int t = t0; t < tiles.total && ok; t += step) {
         const TileAt at = tiles.at(t, rank, csize);
-        if (at.kb0 == at.kb1) continue;
         const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
-        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
+        const int half = width / CG;  // columns of this CTA's part of B
+        const int lane0 = static_cast<int>(at.lane0) + static_cast<int>(pair_rank) * 128;
+        const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
         for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
           const int s1 = s0 + min(S::kChain, at.kb1 - s0);
-          ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t d = tmem + buf * MT * NT;
-          uint32_t more = 0;
-          for (int term = 0; term < S::kTerms && ok; ++term)
+          for (int term = 0; term < S::kTerms && ok; ++term) {
+            const int plane_a = S::kTerms > 1 ? term_a(term) : 0, plane_b = S::kTerms > 1 ? term_b(term) : 0;
             for (int kb = s0; kb < s1; ++kb) {
-              ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t sa = base + stage * S::kStageBytes;
-              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + MT * kABytes, S::WGRAD);
-              constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
-              int steps = 4;
-              if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                const uint64_t dm = da + m * (kABytes >> 4);
-                if (steps == 4) {
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
-                } else {
-                  for (int i = 0; i < steps; ++i)
-                    mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
+              uint32_t bytes;
+              int src[4];            // weights' gradient, last block: four rows of a gather
+              int rows16 = BK;       // rows of the block in whole MMA steps
+              bool tail = false;
+              if constexpr (S::WGRAD) {
+                const int valid = min(at.depth - kb * BK, BK);
+                tail = valid < BK;
+                if (tail) {
+                  rows16 = (valid + 15) & ~15;
+      #pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int r = (lane & 15) * 4 + i;
+                    src[i] = r < valid ? at.first + kb * BK + r : -1;
+                  }
                 }
+                bytes = (2 * MT + (half + 63) / 64) * rows16 * 128u;
+              } else {
+                bytes = MT * kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
               }
-              more = 1;
-              commit<CG>(&ctl.empty[stage]);
+              int go = 0;
+              if (lane == 0) {
+                go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+                if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
+                if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+              }
+              go = __shfl_sync(0xffffffffu, go, 0);
+              if (!go) {
+                ok = false;
+                break;
+              }
+              const uint32_t sa = base + stage * S::kStageBytes, sb = sa + MT * kABytes;
+              const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
+              if constexpr (S::WGRAD) {
+                // operand boxes of 64 lanes (columns) by 64 rows; of the last block
+                // loads of four rows, dealt to half a warp a box
+                const int row_a = at.first + kb * BK + plane_a * p.plane_rows;
+                const int row_b = at.first + kb * BK + plane_b * p.plane_rows;
+                const int boxes = (half + 63) / 64;
+                if (tail) {
+                  const int quad = lane & 15;
+                  if (quad * 4 < rows16) {
+                    int ra[4], rb[4];
+      #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      ra[i] = src[i] < 0 ? p.src_rows : src[i] + plane_a * p.plane_rows;
+                      rb[i] = src[i] < 0 ? p.src_rows : src[i] + plane_b * p.plane_rows;
+                    }
+  #pragma unroll
+                    for (int m = 0; m < MT; ++m)
+                      load_rows<CG>(sa + m * kABytes + (lane >> 4) * 8192 + quad * 512, &rows_a,
+                                    lane0 + m * 128 * CG + (lane >> 4) * 64, ra, bar);
+                    for (int b = lane >> 4; b < boxes; b += 2)
+                      load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
+                  }
+                } else if (lane < 2 * MT) {
+                  load_2d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, row_a, bar);
+                } else if (lane - 2 * MT < boxes) {
+                  load_2d<CG>(sb + (lane - 2 * MT) * 8192, &map_b, col0 + (lane - 2 * MT) * 64, row_b, bar);
+                }
+              } else {
+                const int z = at.expert * p.expert_step + plane_a * p.plane_experts;
+                if constexpr (S::A_MN) {
+                  if (lane < 2 * MT)
+                    load_3d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
+                                bar);
+                } else {
+                  if (lane < MT) load_3d<CG>(sa + lane * kABytes, &map_a, kb * BK, lane0 + lane * 128 * CG, z, bar);
+                }
+                if (lane * kBoxRows < half)
+                  load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK,
+                              col0 + lane * kBoxRows + plane_b * p.plane_rows, bar);
+              }
               if (++stage == STAGES) {
                 stage = 0;
                 phase ^= 1;
               }
             }
-          if (!ok) break;
-          commit<CG>(&ctl.acc_full[buf]);
-          if (++buf == S::kBufs) {
-            buf = 0;
-            acc_phase ^= 1;
           }
         }
       }
-      if (!ok) {
-        commit<CG>(&ctl.drain);
-        tc_drain(&ctl.drain, 0);
+      if (lane == 0) {
+        // the stages still held: their MMAs have arrived here before this CTA may end
+        for (int s = 0; s < STAGES && ok; ++s) {
+          if (s < used) {
+            const int last = (stage + STAGES - 1 - s) % STAGES;
+            const uint32_t ph = last < stage ? phase : phase ^ 1;
+            ok = tc_wait(&ctl.empty[last], ph, &ctl, p.status);
+          }
+        }
+        if (!ok && leader)
+          for (int s = 0; s < STAGES && s < used; ++s) {
+            const int last = (stage + STAGES - 1 - s) % STAGES;
+            tc_drain(&ctl.full[last], last < stage ? phase : phase ^ 1);
+          }
       }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMAs
+      if (leader && lane == 0) {
+        int stage = 0, buf = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for (int t = t0; t < tiles.total && ok; t += step) {
+          const TileAt at = tiles.at(t, rank, csize);
+          if (at.kb0 == at.kb1) continue;
+          const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
+          const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
+          for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
+            const int s1 = s0 + min(S::kChain, at.kb1 - s0);
+            ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + buf * MT * NT;
+            uint32_t more = 0;
+            for (int term = 0; term < S::kTerms && ok; ++term)
+              for (int kb = s0; kb < s1; ++kb) {
+                ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t sa = base + stage * S::kStageBytes;
+                const uint64_t da = operand(sa, S::A_MN), db = operand(sa + MT * kABytes, S::WGRAD);
+                constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
+                int steps = 4;
+                if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+  #pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                  const uint64_t dm = da + m * (kABytes >> 4);
+                  if (steps == 4) {
+  #pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
+                  } else {
+                    for (int i = 0; i < steps; ++i)
+                      mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
+                  }
+                }
+                more = 1;
+                commit<CG>(&ctl.empty[stage]);
+                if (++stage == STAGES) {
+                  stage = 0;
+                  phase ^= 1;
+                }
+              }
+            if (!ok) break;
+            commit<CG>(&ctl.acc_full[buf]);
+            if (++buf == S::kBufs) {
+              buf = 0;
+              acc_phase ^= 1;
+            }
+          }
+        }
+        if (!ok) {
+          commit<CG>(&ctl.drain);
+          tc_drain(&ctl.drain, 0);
+        }
+      }
+      __syncwarp();
+    } else if (warp < 4) {
+      if constexpr (!S::WGRAD)  // rows of no expert
+        clear_rows(p, p.g.kept(), p.g.rows, blockIdx.x * 64LL + (threadIdx.x - 64), gridDim.x * 64LL);
     }
-    __syncwarp();
-  } else if (warp < 4) {
-    if constexpr (!S::WGRAD)  // rows of no expert
-      clear_rows(p, p.g.kept(), p.g.rows, blockIdx.x * 64LL + (threadIdx.x - 64), gridDim.x * 64LL);
   } else {
+    if constexpr (S::kHeld) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ------------------------------------------------------------- epilogue
     // two sets of four warps share the tile's 32-column blocks
     const int quad = warp & 3, set = (warp - 4) >> 2;
     int buf = 0;
-    uint32_t acc_phase = 0, red_phase = 0;
+    uint32_t acc_phase = 0, red_phase = 0, nth = 0;
     for (int t = t0; t < tiles.total; t += step) {
       const TileAt at = tiles.at(t, rank, csize);
       const int64_t ch0 = at.lane0 + pair_rank * 128 + quad * 32 + lane;
@@ -747,29 +806,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!__shfl_sync(0xffffffffu, go, 0)) break;
       }
       const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col;
-      // scales of 8-bit operands, loaded under the MMAs: lane l has those of
-      // columns l, l + 32, ...
-      float xs[S::KIND == kKindI8 ? NT / 32 : 1], ws[MT];
+      // scales of 8-bit operands, loaded under the MMAs; two tiles' worth, so
+      // that one barrier a tile is enough
+      const float* xs = x_scales[nth & 1];
+      float ws[MT];
       if constexpr (S::KIND == kKindI8 && !S::SPLIT) {
-#pragma unroll
-        for (int b = 0; b < NT / 32; ++b) {
-          xs[b] = 0.0f;
-          if (b * 32 + lane < at.rows) {
-            const int64_t tok = p.g.source(at.row0 + b * 32 + lane);
-            if (tok >= 0) xs[b] = p.g.x_scale[tok];
-          }
+        const int c = threadIdx.x - 128;
+        if (c < NT) {
+          const int64_t tok = c < at.rows ? p.g.source(at.row0 + c) : -1;
+          x_scales[nth & 1][c] = tok >= 0 ? p.g.x_scale[tok] : 0.0f;
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           ws[m] = ch0 + m * 128 * CG < p.lanes ? p.g.w_scale[at.expert * p.lanes + ch0 + m * 128 * CG] : 0.0f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        ++nth;
       }
-      auto scale = [&](float (&v)[32], float x, float w) {
-        if constexpr (S::KIND == kKindI8) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            v[i] = static_cast<float>(__float_as_int(v[i])) * __shfl_sync(0xffffffffu, x, i) * w;
-        }
-      };
       bool ok = true;
       int s0 = at.kb0;
       do {  // the chains of the sum; one pass over zeros where there is no depth
@@ -788,19 +840,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
         };
         bool released = !any;
-        if constexpr (S::kBufs == 1 && S::kTerms == 1) {
-          if (any && p.pairs && p.out_dtype != ES_F32) {
+        if constexpr (S::kHeld) {
+          if (any && (p.pairs || p.out_dtype == ES_F32)) {
             const int64_t ch = ch0 + set * 128 * CG;
             const uint32_t mine = acc + set * NT;
-            auto finish = [&](float (&v)[32], int b) {
-              if constexpr (S::KIND == kKindI8) scale(v, xs[b], set ? ws[MT - 1] : ws[0]);
-            };
+            constexpr bool I8 = S::KIND == kKindI8;
+            const float w = I8 ? (set ? ws[MT - 1] : ws[0]) : 1.0f;
             if (p.out_dtype == ES_BF16)
-              drain_held(mine, static_cast<__nv_bfloat16*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes,
-                         finish, release);
+              drain_held<__nv_bfloat16, I8>(mine, static_cast<__nv_bfloat16*>(p.out) + out0 + ch, p.out_col, at.rows,
+                                            ch < p.lanes, xs, w, release);
+            else if (p.out_dtype == ES_F16)
+              drain_held<__half, I8>(mine, static_cast<__half*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes,
+                                     xs, w, release);
             else
-              drain_held(mine, static_cast<__half*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes, finish,
-                         release);
+              drain_held<float, I8>(mine, static_cast<float*>(p.out) + out0 + ch, p.out_col, at.rows, ch < p.lanes, xs,
+                                    w, release);
             released = true;
           }
         }
@@ -823,21 +877,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int i = 0; i < 32; ++i)
               if (i < n) mine[i * 128] = first ? v[i] : mine[i * 128] + v[i];
           } else {
-            if constexpr (S::KIND == kKindI8) {
-              float x = xs[0], w = ws[0];
-#pragma unroll
-              for (int i = 1; i < NT / 32; ++i)
-                if (c0 == i * 32) x = xs[i];
-              if (m > 0) w = ws[MT - 1];
-              scale(v, x, w);
-            }
+            if constexpr (S::KIND == kKindI8) scale_block(v, xs + c0, m ? ws[MT - 1] : ws[0]);
             const int64_t at0 = out0 + c0 * p.out_col + ch;
             if constexpr (S::kTerms > 1) {
               float* o = static_cast<float*>(p.out) + at0;
               if (!first && live) {
+                int64_t stride = p.out_col;
+                keep_here(stride);
+                const float* q = o;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (i < n) v[i] += o[i * p.out_col];
+                for (int i = 0; i < 32; ++i) {
+                  if (i < n) v[i] += *q;
+                  q += stride;
+                }
               }
               store_cols(o, p.out_col, v, n, live, false);
             } else {
@@ -1105,6 +1157,9 @@ int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int cs
   if (cudaGetDevice(&dev) != cudaSuccess) return ES_ERR_CUDA;
   const bool tracked = dev >= 0 && dev < kMaxAttrDevices;
   if (!tracked || !raised[dev].load(std::memory_order_relaxed)) {
+    cudaFuncAttributes attrs;
+    if (cudaFuncGetAttributes(&attrs, grouped_tc_kernel<S>) != cudaSuccess) return ES_ERR_CUDA;
+    if (S::kHeld && attrs.numRegs < kLaunchRegs) return ES_ERR_UNSUPPORTED;
     const size_t most = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kPartBytes +
                         (3 * kMaxExperts + 1) * sizeof(int);
     if (cudaFuncSetAttribute(grouped_tc_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
