@@ -37,6 +37,10 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
+__device__ __forceinline__ float from_order_bits(uint32_t u) {
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+
 template <typename T, int PER>
 __device__ __forceinline__ void load_logits(const T* row, int E, float (&v)[PER]) {
   const int lane = threadIdx.x & 31;
@@ -86,34 +90,38 @@ __global__ void __launch_bounds__(128) route_kernel(const T* logits, int64_t nto
     all = warp_sum(all);
   }
   const bool poison = __any_sync(kFull, nan);
-  // choice j ends in lane j (k <= 32)
-  float mine = 0.0f;
-  int chosen = -1;
-  for (int j = 0; j < k; ++j) {
-    uint32_t best = 0;
-    int at = 0x7fffffff;
-    float val = 0.0f;
+  // each lane offers its largest; the lane whose offer is taken looks again.
+  // Choice j ends in lane j (k <= 32).
+  uint32_t best = 0, mine_bits = 0;
+  int slot = 0, chosen = -1;
+  auto look = [&] {
+    best = key[0];
+    slot = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
+    for (int i = 1; i < PER; ++i)
       if (key[i] > best) {
         best = key[i];
-        at = lane + 32 * i;
-        val = v[i];
+        slot = i;
       }
+  };
+  look();
+  for (int j = 0; j < k; ++j) {
     const uint32_t top = __reduce_max_sync(kFull, best);
     if (top == 0) break;  // nothing left but masked experts
+    const int at = lane + 32 * slot;
     const int e = __reduce_min_sync(kFull, best == top ? at : 0x7fffffff);
-    const float x = __shfl_sync(kFull, val, e & 31);
-    if (lane == (e & 31)) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i == (e >> 5)) key[i] = 0;
-    }
     if (lane == j) {
       chosen = e;
-      mine = expf(x - m);
+      mine_bits = top;
+    }
+    if (at == e) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i == slot) key[i] = 0;
+      look();
     }
   }
+  const float mine = chosen >= 0 ? expf(from_order_bits(mine_bits) - m) : 0.0f;
   const float total = renorm ? warp_sum(mine) : all;
   if (lane < k) {
     const float w = chosen >= 0 ? mine / total : 0.0f;
@@ -122,9 +130,10 @@ __global__ void __launch_bounds__(128) route_kernel(const T* logits, int64_t nto
   }
 }
 
-// dl_i = w_i (g_i - d), d = sum_j w_j g_j, over the chosen experts (renorm);
-// else dl_i = p_i (g_i [i chosen] - d) over all, with p recomputed from the
-// logits. Reads the logits (only for the second form), writes dlogits once.
+// dl_i = w_i (g_i - d), d = sum_j w_j g_j, for the chosen experts (whose w_i
+// is p_i); for the others 0 (renorm), or -p_i d with p recomputed from the
+// logits. Every dlogit is written as if not chosen, in whole rows, and then
+// the chosen ones over it.
 template <typename T, int PER>
 __global__ void __launch_bounds__(128) route_grad_kernel(const T* logits, int64_t ntok, int E, int64_t stride, int k,
                                                          int renorm, const float* weights, const int32_t* experts,
@@ -140,10 +149,11 @@ __global__ void __launch_bounds__(128) route_grad_kernel(const T* logits, int64_
     g = e >= 0 ? dweights[t * k + lane] : 0.0f;
   }
   const float d = warp_sum(w * g);
-  float out[PER];
+  T* out = dlogits + t * static_cast<int64_t>(E);
   if (renorm) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) out[i] = 0.0f;
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(0.0f);
   } else {
     float v[PER];
     load_logits<T, PER>(logits + t * stride, E, v);
@@ -152,29 +162,17 @@ __global__ void __launch_bounds__(128) route_grad_kernel(const T* logits, int64_
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       // NaN logits keep their NaN here, masked ones add nothing
-      out[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - m);
-      all += out[i];
+      v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - m);
+      all += v[i];
     }
     all = warp_sum(all);
     const float f = all > 0.0f || all != all ? -d / all : 0.0f;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) out[i] *= f;
+    for (int i = 0; i < PER; ++i)
+      if (lane + 32 * i < E) out[lane + 32 * i] = from_f32<T>(v[i] * f);
   }
-  const float mine = renorm ? w * (g - d) : w * g;
-  for (int j = 0; j < k; ++j) {
-    const int ej = __shfl_sync(kFull, e, j);
-    const float x = __shfl_sync(kFull, mine, j);
-    if (ej >= 0 && lane == (ej & 31)) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i == (ej >> 5)) out[i] += x;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int x = lane + 32 * i;
-    if (x < E) dlogits[t * static_cast<int64_t>(E) + x] = from_f32<T>(out[i]);
-  }
+  __syncwarp();
+  if (e >= 0) out[e] = from_f32<T>(w * (g - d));
 }
 
 template <typename T>
@@ -205,22 +203,19 @@ int route_typed(const void* logits, int64_t T_, int E, int64_t stride, int k, in
 // ----------------------------------------------------------------- row order
 //
 // A stable counting sort of the choices by expert ("no expert" sorts last, as
-// expert E). Few choices: one CTA, one launch. Else the choices are cut into
-// chunks: one launch counts each chunk's experts, and in a second every chunk
-// adds up the chunks before it and places its own. Within a CTA each warp owns
-// a consecutive run of choices; a choice's rank is its warp's start plus the
-// earlier choices of the warp with the same expert (match + popcount), so the
-// order never depends on the schedule.
+// expert E). Up to 2048 choices: one CTA, one launch. Else the choices are cut
+// into chunks: one launch counts each chunk's experts, a second places them.
+// Every chunk adds up the counts of the chunks before it, while there are few
+// (kPlanDirect); else a launch in between does that for all. Within a CTA each
+// warp owns a consecutive run of choices, 32 at a time; a choice's rank is the
+// warp's earlier choices of the same expert (match + popcount), so the order
+// never depends on the schedule. Bound by latency: each choice is read once.
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
-constexpr int kPlanChunk = 4096;   // choices of one CTA; one CTA alone up to here
-constexpr int kPlanChunks = 1024;  // at most: every CTA reads every chunk's counts
-
-int64_t plan_chunk(int64_t n) {
-  const int64_t unit = static_cast<int64_t>(kPlanChunk) * kPlanChunks;
-  return kPlanChunk * (n > unit ? (n + unit - 1) / unit : 1);
-}
+constexpr int kPlanChunk = 2048;  // choices of one CTA
+constexpr int kPlanItems = kPlanChunk / kPlanThreads;
+constexpr int kPlanDirect = 64;   // chunks whose counts a CTA adds up by itself
 
 __device__ __forceinline__ int expert_of(const int32_t* experts, int64_t a, int E, bool& bad) {
   const int e = experts[a];
@@ -228,103 +223,146 @@ __device__ __forceinline__ int expert_of(const int32_t* experts, int64_t a, int 
   return e >= 0 && e < E ? e : E;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const int32_t* experts, int64_t n, int64_t chunk,
-                                                                  int E, int32_t* counts) {
+__global__ void __launch_bounds__(kPlanThreads) plan_count_kernel(const int32_t* experts, int64_t n, int E,
+                                                                  int32_t* counts) {
   extern __shared__ int32_t hist[];
   for (int i = threadIdx.x; i <= E; i += kPlanThreads) hist[i] = 0;
   __syncthreads();
-  const int64_t c0 = blockIdx.x * chunk;
-  const int64_t c1 = min(n, c0 + chunk);
+  const int64_t c0 = blockIdx.x * static_cast<int64_t>(kPlanChunk);
   bool bad = false;
-  for (int64_t a = c0 + threadIdx.x; a < c1; a += kPlanThreads) atomicAdd(&hist[expert_of(experts, a, E, bad)], 1);
+#pragma unroll
+  for (int i = 0; i < kPlanItems; ++i) {
+    const int64_t a = c0 + i * kPlanThreads + threadIdx.x;
+    if (a < n) atomicAdd(&hist[expert_of(experts, a, E, bad)], 1);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i <= E; i += kPlanThreads) counts[blockIdx.x * static_cast<int64_t>(E + 1) + i] = hist[i];
 }
 
-// counts: of every chunk (nullptr: this CTA is the only chunk).
-__global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const int32_t* experts, int64_t n, int64_t chunk,
-                                                                  int E, const int32_t* counts, int32_t* offsets,
-                                                                  int32_t* order, int32_t* position, int32_t* err) {
+// Replaces every chunk's count of expert blockIdx.x by the count of the chunks
+// before it, and writes the total behind the last chunk's.
+__global__ void __launch_bounds__(kPlanThreads) plan_scan_kernel(int32_t* counts, int64_t chunks, int E) {
+  __shared__ int32_t sums[kPlanWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.x;
+  int run = 0;
+  for (int64_t c0 = 0; c0 < chunks; c0 += kPlanThreads) {
+    const int64_t c = c0 + threadIdx.x;
+    const int v = c < chunks ? counts[c * (E + 1) + e] : 0;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(kFull, s, o);
+      if (lane >= o) s += u;
+    }
+    if (lane == 31) sums[warp] = s;
+    __syncthreads();
+    int before = run;
+    for (int w = 0; w < kPlanWarps; ++w) {
+      if (w < warp) before += sums[w];
+      run += sums[w];
+    }
+    if (c < chunks) counts[c * (E + 1) + e] = before + s - v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) counts[chunks * (E + 1) + e] = run;
+}
+
+// counts: of every chunk; nullptr: this CTA is the only chunk; scanned: as
+// plan_scan_kernel leaves them.
+__global__ void __launch_bounds__(kPlanThreads) plan_place_kernel(const int32_t* experts, int64_t n, int E,
+                                                                  const int32_t* counts, int scanned,
+                                                                  int32_t* offsets, int32_t* order,
+                                                                  int32_t* position, int32_t* err) {
   extern __shared__ int32_t sm[];
   const int E1 = E + 1;
-  int32_t* cnt = sm;                      // [kPlanWarps][E1]: counts, then next row of (warp, expert)
+  int32_t* cnt = sm;                       // [kPlanWarps][E1]: counts, then first row of (warp, expert)
   int32_t* before = sm + kPlanWarps * E1;  // [E1] rows of this expert in the chunks before
   int32_t* total = before + E1;            // [E1] rows of this expert in all, then its first row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < kPlanWarps * E1; i += kPlanThreads) cnt[i] = 0;
-  __syncthreads();
-  const int64_t c0 = blockIdx.x * chunk;
-  const int m = static_cast<int>(min(n - c0, chunk));
-  const int per = ((m + kPlanWarps - 1) / kPlanWarps + 31) & ~31;  // a warp's run of choices
-  const int w0 = warp * per, w1 = min(m, w0 + per);
+  const int64_t c0 = blockIdx.x * static_cast<int64_t>(kPlanChunk);
+  const int m = static_cast<int>(min(n - c0, static_cast<int64_t>(kPlanChunk)));
+  const int per = m <= kPlanThreads ? 32 : kPlanItems * 32;  // a warp's run of choices
+  int e[kPlanItems], rank[kPlanItems];
   bool bad = false;
-  for (int i = w0 + lane; i < w1; i += 32) atomicAdd(&cnt[warp * E1 + expert_of(experts, c0 + i, E, bad)], 1);
+#pragma unroll
+  for (int i = 0; i < kPlanItems; ++i) {
+    const int a = warp * per + i * 32 + lane;
+    e[i] = i * 32 < per && a < m ? expert_of(experts, c0 + a, E, bad) : E1;
+  }
+  for (int i = threadIdx.x; i < (kPlanWarps + 2) * E1; i += kPlanThreads) sm[i] = 0;
+  __syncthreads();
   if (bad && err) *static_cast<volatile int32_t*>(err) = ES_ERR_INDEX;
-  if (counts) {
-    for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
-      int b = 0, all = 0;
-#pragma unroll 8
-      for (int c = 0; c < static_cast<int>(gridDim.x); ++c) {
-        const int v = counts[c * static_cast<int64_t>(E1) + e];
-        b += c < static_cast<int>(blockIdx.x) ? v : 0;
-        all += v;
-      }
-      before[e] = b;
-      total[e] = all;
+#pragma unroll
+  for (int i = 0; i < kPlanItems; ++i) {
+    if (warp * per + i * 32 >= m || i * 32 >= per) break;  // the whole warp
+    const unsigned same = __match_any_sync(kFull, e[i]);
+    const int had = e[i] < E1 ? cnt[warp * E1 + e[i]] : 0;
+    rank[i] = had + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (e[i] < E1 && lane == __ffs(same) - 1) cnt[warp * E1 + e[i]] = had + __popc(same);
+    __syncwarp();
+  }
+  if (counts && scanned) {
+    for (int x = threadIdx.x; x < E1; x += kPlanThreads) {
+      before[x] = counts[blockIdx.x * static_cast<int64_t>(E1) + x];
+      total[x] = counts[gridDim.x * static_cast<int64_t>(E1) + x];
     }
-    __syncthreads();
-  } else {
-    __syncthreads();
-    for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
+  } else if (counts) {
+    for (int i = threadIdx.x; i < static_cast<int>(gridDim.x) * E1; i += kPlanThreads) {
+      const int v = counts[i];
+      if (v) {
+        atomicAdd(&total[i % E1], v);
+        if (i < static_cast<int>(blockIdx.x) * E1) atomicAdd(&before[i % E1], v);
+      }
+    }
+  }
+  __syncthreads();
+  if (!counts) {
+    for (int x = threadIdx.x; x < E1; x += kPlanThreads) {
       int all = 0;
-      for (int w = 0; w < kPlanWarps; ++w) all += cnt[w * E1 + e];
-      before[e] = 0;
-      total[e] = all;
+#pragma unroll
+      for (int w = 0; w < kPlanWarps; ++w) all += cnt[w * E1 + x];
+      total[x] = all;
     }
     __syncthreads();
   }
   if (warp == 0) {  // exclusive sum of the totals: each expert's first row
     int run = 0;
     for (int e0 = 0; e0 < E1; e0 += 32) {
-      const int e = e0 + lane;
-      const int v = e < E1 ? total[e] : 0;
+      const int x = e0 + lane;
+      const int v = x < E1 ? total[x] : 0;
       int s = v;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(kFull, s, o);
         if (lane >= o) s += u;
       }
-      if (e < E1) {
-        total[e] = run + s - v;
-        if (blockIdx.x == 0) offsets[e] = run + s - v;
+      if (x < E1) {
+        total[x] = run + s - v;
+        if (blockIdx.x == 0) offsets[x] = run + s - v;
       }
       run += __shfl_sync(kFull, s, 31);
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E1; e += kPlanThreads) {
-    int at = total[e] + before[e];
+  for (int x = threadIdx.x; x < E1; x += kPlanThreads) {
+    int at = total[x] + before[x];
+#pragma unroll
     for (int w = 0; w < kPlanWarps; ++w) {
-      const int v = cnt[w * E1 + e];
-      cnt[w * E1 + e] = at;
+      const int v = cnt[w * E1 + x];
+      cnt[w * E1 + x] = at;
       at += v;
     }
   }
   __syncthreads();
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const bool live = i < w1;
-    const int e = live ? expert_of(experts, c0 + i, E, bad) : E1;
-    const unsigned same = __match_any_sync(kFull, e);
-    int row = 0;
-    if (live) row = cnt[warp * E1 + e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (live) {
-      if (lane == __ffs(same) - 1) cnt[warp * E1 + e] = row + __popc(same);
-      order[row] = e < E ? static_cast<int32_t>(c0 + i) : -1;
-      position[c0 + i] = e < E ? row : -1;
-    }
-    __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kPlanItems; ++i) {
+    const int a = warp * per + i * 32 + lane;
+    if (i * 32 >= per || a >= m) break;
+    const int row = cnt[warp * E1 + e[i]] + rank[i];
+    order[row] = e[i] < E ? static_cast<int32_t>(c0 + a) : -1;
+    position[c0 + a] = e[i] < E ? row : -1;
   }
 }
 
@@ -547,62 +585,137 @@ int combine_grad_typed(const void* y, int64_t rows, int64_t stride, const float*
 // scale_t = max_i |x_ti| / 127 (one division rounded to nearest), q_ti =
 // rint(x_ti / scale_t), kept within +-127. A row of zeros has scale 0 and q 0;
 // a row with an infinity or NaN has scale NaN, so that its products are NaN
-// and not a finite guess. Bound by memory: a row is read once from HBM (the
-// second reading hits the L1) and its 8-bit copy written once.
+// and not a finite guess. Bound by memory: a row is read once and its 8-bit
+// copy written once.
 
 constexpr int kQuantThreads = 256;
 
+// The larger of two magnitudes; NaN where one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <int VEC>
+__device__ __forceinline__ float piece_peak(const Piece<float, VEC>& p) {
+  float m = fabsf(p.v[0]);
+#pragma unroll
+  for (int i = 1; i < VEC; ++i) m = max_nan(m, fabsf(p.v[i]));
+  return m;
+}
+template <int VEC>
+__device__ __forceinline__ float piece_peak(const Piece<__nv_bfloat16, VEC>& p) {
+  if constexpr (VEC == 1) {
+    return fabsf(to_f32(p.v[0]));
+  } else {
+    const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(p.v);
+    __nv_bfloat162 m = __habs2(v[0]);
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) m = __hmax2_nan(m, __habs2(v[i]));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+}
+template <int VEC>
+__device__ __forceinline__ float piece_peak(const Piece<__half, VEC>& p) {
+  if constexpr (VEC == 1) {
+    return fabsf(to_f32(p.v[0]));
+  } else {
+    const __half2* v = reinterpret_cast<const __half2*>(p.v);
+    __half2 m = __habs2(v[0]);
+#pragma unroll
+    for (int i = 1; i < VEC / 2; ++i) m = __hmax2_nan(m, __habs2(v[i]));
+    return max_nan(__low2float(m), __high2float(m));
+  }
+}
+
+// rint(x / s) as a division rounded to nearest gives it. x times the
+// reciprocal is at most a few units in the last place of 127 from that
+// quotient, so a piece is divided only where one of its values is next to a
+// tie (or the reciprocal overflows). Adding 1.5 * 2^23 rounds to the nearest
+// integer and leaves it in the low bits. (A division for every value took
+// three times as long.)
 template <typename T, int VEC>
+__device__ __forceinline__ Piece<int8_t, VEC> quantize_piece(const Piece<T, VEC>& p, float s, float inv) {
+  constexpr float kRound = 12582912.0f;
+  Piece<int8_t, VEC> o;
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const float q = to_f32(p.v[i]) * inv;
+    const float r = q + kRound;
+    off = max_nan(off, fabsf(q - (r - kRound)));
+    o.v[i] = static_cast<int8_t>(__float_as_int(r));
+  }
+  if (!(off < 0.4999f)) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float r = s > 0.0f ? rintf(__fdiv_rn(to_f32(p.v[i]), s)) : 0.0f;
+      o.v[i] = static_cast<int8_t>(fminf(fmaxf(r, -127.0f), 127.0f));
+    }
+  }
+  return o;
+}
+
+// A row for tp threads, its first NP pieces a thread held in registers between
+// the search for the largest and the rounding (what is beyond is read again).
+template <typename T, int VEC, int NP>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const T* x, int64_t rows, int64_t K, int64_t stride,
                                                                  int8_t* q, float* scale, int tp) {
+  let_next_grid_start();
   __shared__ float part[kQuantThreads / 32];
   const int group = threadIdx.x / tp;
   const int64_t t = blockIdx.x * static_cast<int64_t>(kQuantThreads / tp) + group;
   const bool live = t < rows;
   const int64_t pieces = K / VEC;
+  const Piece<T, VEC>* row = reinterpret_cast<const Piece<T, VEC>*>(x + t * stride);
+  Piece<T, VEC> held[NP];
   float peak = 0.0f;
-  bool odd = false;  // an infinity or NaN
-  if (live) {
-    const Piece<T, VEC>* row = reinterpret_cast<const Piece<T, VEC>*>(x + t * stride);
-    for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
-      const Piece<T, VEC> p = row[c];
+  const int64_t c0 = threadIdx.x % tp;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float a = fabsf(to_f32(p.v[i]));
-        odd |= !(a <= FLT_MAX);
-        peak = fmaxf(peak, a);
-      }
-    }
+  for (int n = 0; n < NP; ++n) {
+    const int64_t c = c0 + n * tp;
+    held[n] = live && c < pieces ? row[c] : Piece<T, VEC>{};
   }
-  if (odd) peak = INFINITY;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) peak = fmaxf(peak, __shfl_xor_sync(kFull, peak, o));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = peak;
-  __syncthreads();
+  for (int n = 0; n < NP; ++n) peak = max_nan(peak, piece_peak<VEC>(held[n]));
+  if (live)
+    for (int64_t c = c0 + NP * tp; c < pieces; c += tp) peak = max_nan(peak, piece_peak<VEC>(row[c]));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(kFull, peak, o));
+  if (tp > 32) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = peak;
+    __syncthreads();
+    for (int w = 0; w < tp / 32; ++w) peak = max_nan(peak, part[group * (tp / 32) + w]);
+  }
   if (!live) return;
-  for (int w = 0; w < tp / 32; ++w) peak = fmaxf(peak, part[group * (tp / 32) + w]);
   const bool finite = peak <= FLT_MAX;
   const float s = finite ? __fdiv_rn(peak, 127.0f) : NAN;
-  if (threadIdx.x % tp == 0) scale[t] = s;
-  const Piece<T, VEC>* row = reinterpret_cast<const Piece<T, VEC>*>(x + t * stride);
-  for (int64_t c = threadIdx.x % tp; c < pieces; c += tp) {
-    const Piece<T, VEC> p = row[c];
-    Piece<int8_t, VEC> o;
+  const float inv = __fdiv_rn(1.0f, s);
+  if (c0 == 0) scale[t] = s;
+  Piece<int8_t, VEC>* out = reinterpret_cast<Piece<int8_t, VEC>*>(q + t * K);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float v = s > 0.0f ? rintf(__fdiv_rn(to_f32(p.v[i]), s)) : 0.0f;
-      o.v[i] = static_cast<int8_t>(fminf(fmaxf(v, -127.0f), 127.0f));
-    }
-    reinterpret_cast<Piece<int8_t, VEC>*>(q + t * K)[c] = o;
-  }
+  for (int n = 0; n < NP; ++n)
+    if (c0 + n * tp < pieces) out[c0 + n * tp] = quantize_piece<T, VEC>(held[n], s, inv);
+  for (int64_t c = c0 + NP * tp; c < pieces; c += tp) out[c] = quantize_piece<T, VEC>(row[c], s, inv);
 }
 
 template <typename T, int VEC>
 int quantize_vec(const void* x, int64_t rows, int64_t K, int64_t stride, int8_t* q, float* scale, cudaStream_t s) {
-  const int tp = token_threads(K / VEC);
-  const int64_t per = kQuantThreads / tp;
-  ES_LAUNCH((quantize_kernel<T, VEC>), static_cast<unsigned>((rows + per - 1) / per), kQuantThreads, 0, s,
-            static_cast<const T*>(x), rows, K, stride, q, scale, tp);
+  // few rows: a CTA a row; else as few threads a row as hold it in registers
+  const int64_t pieces = K / VEC;
+  int tp = rows >= 4 * kSMs ? 32 : kQuantThreads;
+  while (tp < kQuantThreads && tp * 4 < pieces) tp *= 2;
+  const int64_t per = kQuantThreads / tp, np = (pieces + tp - 1) / tp;
+  const unsigned blocks = static_cast<unsigned>((rows + per - 1) / per);
+#define ES_QUANT(NP)                                                                                             \
+  ES_LAUNCH((quantize_kernel<T, VEC, NP>), blocks, kQuantThreads, 0, s, static_cast<const T*>(x), rows, K, stride, \
+            q, scale, tp)
+  if (np <= 2)
+    ES_QUANT(2);
+  else
+    ES_QUANT(4);
+#undef ES_QUANT
   return ES_OK;
 }
 
@@ -649,8 +762,8 @@ extern "C" int es_route_experts_grad(const void* logits, int dtype, int64_t num_
 
 extern "C" size_t es_expert_plan_workspace_size(int64_t num_choices, int num_experts) {
   if (num_choices <= kPlanChunk || num_experts < 1) return 0;
-  const int64_t chunk = plan_chunk(num_choices);
-  return static_cast<size_t>((num_choices + chunk - 1) / chunk) * (num_experts + 1) * sizeof(int32_t);
+  const int64_t chunks = (num_choices + kPlanChunk - 1) / kPlanChunk;
+  return static_cast<size_t>(chunks + 1) * (num_experts + 1) * sizeof(int32_t);
 }
 
 extern "C" int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts, void* workspace,
@@ -666,16 +779,19 @@ extern "C" int es_expert_plan(const int32_t* experts, int64_t num_choices, int n
     if (cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              static_cast<int>(smem)) != cudaSuccess)
       return ES_ERR_CUDA;
-  const int64_t chunk = plan_chunk(num_choices);
-  const int64_t chunks = num_choices > 0 ? (num_choices + chunk - 1) / chunk : 1;
+  const int64_t chunks = num_choices > kPlanChunk ? (num_choices + kPlanChunk - 1) / kPlanChunk : 1;
   int32_t* counts = nullptr;
   if (chunks > 1) {
     counts = static_cast<int32_t*>(workspace);
     ES_LAUNCH(plan_count_kernel, static_cast<unsigned>(chunks), kPlanThreads, (num_experts + 1) * sizeof(int32_t), s,
-              experts, num_choices, chunk, num_experts, counts);
+              experts, num_choices, num_experts, counts);
   }
+  const int scanned = chunks > kPlanDirect;
+  if (scanned)
+    ES_LAUNCH(plan_scan_kernel, static_cast<unsigned>(num_experts + 1), kPlanThreads, 0, s, counts, chunks,
+              num_experts);
   ES_LAUNCH(plan_place_kernel, static_cast<unsigned>(chunks), kPlanThreads, smem, s, experts, num_choices,
-            chunk, num_experts, static_cast<const int32_t*>(counts), offsets, order, position, status);
+            num_experts, static_cast<const int32_t*>(counts), scanned, offsets, order, position, status);
   return ES_OK;
 }
 

@@ -11,6 +11,12 @@ namespace es {
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopK = 32;
 
+// Programmatic dependent launch: the next kernel of the stream, if it was
+// launched for it, may start before this one is done; it waits for the earlier
+// ones' results before it touches memory.
+__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_earlier_grids() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }

@@ -81,6 +81,7 @@ struct TcCtl {
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t red_full, red_empty;
+  uint64_t scales;
   uint64_t drain;
   uint32_t tmem;
   int abort;
@@ -126,6 +127,22 @@ __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return ok != 0;
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+// Eight columns of this warp's TMEM lanes.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ float load_at(uint32_t cluster_addr) {
@@ -536,6 +553,84 @@ __device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride,
   }
 }
 
+// The epilogue of a tile whose depth the cluster's CTAs share: each CTA puts
+// its part of the sum into shared memory, [column][lane], and every CTA adds
+// up every csize-th column, the parts in the CTAs' order. 8-bit products stay
+// integers until then (their bits travel as floats). Few columns: the code is
+// short and rolled, since a decode step meets it cold. False: given up.
+template <typename S>
+__device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const TileAt& at, float* part, uint32_t tmem,
+                                           int64_t ch, uint32_t rank, uint32_t csize, int set, int quad, int& buf,
+                                           uint32_t& acc_phase, uint32_t& red_phase) {
+  constexpr bool I8 = S::KIND == kKindI8;
+  const int lane = threadIdx.x & 31;
+  const bool live = ch < p.lanes;
+  // lane i: the scale of the i-th column that this warp will add up
+  float xs = 0.0f, ws = 1.0f;
+  const int c_first = rank * 2 + set, c_step = 2 * csize;
+  if constexpr (I8) {
+    const int c = c_first + lane * c_step;
+    const int64_t tok = c < at.rows ? p.g.source(at.row0 + c) : -1;
+    if (tok >= 0) xs = p.g.x_scale[tok];
+    ws = live ? p.g.w_scale[at.expert * p.lanes + ch] : 0.0f;
+  }
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    int go = 1;
+    if (lane == 0) go = tc_wait(bar, parity, &ctl, p.status, true) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, go, 0) != 0;
+  };
+  // the last tile's parts have been read by the whole cluster
+  if (!wait(&ctl.red_empty, red_phase ^ 1)) return false;
+  float* mine = part + quad * 32 + lane;
+  for (int s0 = at.kb0; s0 < at.kb1; s0 += min(S::kChain, at.kb1 - s0)) {
+    if (!wait(&ctl.acc_full[buf], acc_phase)) return false;
+    tc_fence_after();
+    const uint32_t acc = tmem + buf * S::NT + (static_cast<uint32_t>(quad * 32) << 16);
+#pragma unroll 1
+    for (int c0 = set * 8; c0 < at.rows; c0 += 16) {
+      float v[8];
+      tmem_ld8(acc + c0, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // columns past the tile's are written and not read
+        if (S::kTerms > 1 && s0 > at.kb0) v[i] += mine[(c0 + i) * 128];
+        mine[(c0 + i) * 128] = v[i];
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), rank));
+    if (++buf == S::kBufs) {
+      buf = 0;
+      acc_phase ^= 1;
+    }
+  }
+  __syncwarp();
+  if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_full), lane));
+  if (!wait(&ctl.red_full, red_phase)) return false;
+#pragma unroll 1
+  for (int c = c_first, i = 0; c < at.rows; c += c_step, ++i) {
+    const uint32_t from = smem_u32(mine + c * 128);
+    float f[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) f[r] = r < static_cast<int>(csize) ? load_at(at_rank(from, r)) : 0.0f;
+    float v = 0.0f;
+    if constexpr (I8) {
+      int sum = 0;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) sum += __float_as_int(f[r]);
+      v = static_cast<float>(sum) * __shfl_sync(0xffffffffu, xs, i) * ws;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v += f[r];
+    }
+    if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch, v);
+  }
+  __syncwarp();
+  if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
+  red_phase ^= 1;
+  return true;
+}
+
 // Registers: the epilogue's two warpgroups take over what the first does not
 // need. 128 * kRoleRegs + 256 * kEpiRegs = 384 * kLaunchRegs, which the launch
 // has (checked there: a split of more would wait for ever).
@@ -564,6 +659,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const bool leader = pair_rank == 0;
 
   if (threadIdx.x == 0) {
+    prefetch_map(&map_a);
+    prefetch_map(&map_b);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ctl.full[s], 1);
       mbar_init(&ctl.empty[s], 1);
@@ -572,6 +669,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&ctl.acc_full[b], 1);
       mbar_init(&ctl.acc_empty[b], CG * kEpiWarps);
     }
+    mbar_init(&ctl.scales, kEpiWarps);
     mbar_init(&ctl.red_full, csize * kEpiWarps);
     mbar_init(&ctl.red_empty, csize * kEpiWarps);
     mbar_init(&ctl.drain, 1);
@@ -580,6 +678,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_mbar_init();
   }
   if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kBufs * MT * NT);
+  wait_for_earlier_grids();
   if (warp == 2) {  // tiles of each group
     int run = 0;
     for (int e0 = 0; e0 < groups; e0 += 32) {
@@ -800,17 +899,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const TileAt at = tiles.at(t, rank, csize);
       const int64_t ch0 = at.lane0 + pair_rank * 128 + quad * 32 + lane;
       const int blocks = (at.rows + 31) / 32;
-      if constexpr (S::SPLIT) {  // the last tile's parts have been read by the whole cluster
-        int go = 1;
-        if (lane == 0) go = tc_wait(&ctl.red_empty, red_phase ^ 1, &ctl, p.status, true) ? 1 : 0;
-        if (!__shfl_sync(0xffffffffu, go, 0)) break;
+      if constexpr (S::SPLIT) {
+        if (!split_tile<S>(p, ctl, at, part, tmem, ch0, rank, csize, set, quad, buf, acc_phase, red_phase)) break;
+        continue;
       }
       const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col;
       // scales of 8-bit operands, loaded under the MMAs; two tiles' worth, so
       // that one barrier a tile is enough
       const float* xs = x_scales[nth & 1];
       float ws[MT];
-      if constexpr (S::KIND == kKindI8 && !S::SPLIT) {
+      if constexpr (S::KIND == kKindI8) {
         const int c = threadIdx.x - 128;
         if (c < NT) {
           const int64_t tok = c < at.rows ? p.g.source(at.row0 + c) : -1;
@@ -819,7 +917,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int m = 0; m < MT; ++m)
           ws[m] = ch0 + m * 128 * CG < p.lanes ? p.g.w_scale[at.expert * p.lanes + ch0 + m * 128 * CG] : 0.0f;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        __syncwarp();
+        int go = 1;
+        if (lane == 0) {
+          mbar_arrive(&ctl.scales);
+          go = tc_wait(&ctl.scales, nth & 1, &ctl, p.status) ? 1 : 0;
+        }
+        if (!__shfl_sync(0xffffffffu, go, 0)) break;
         ++nth;
       }
       bool ok = true;
@@ -869,32 +973,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.0f;
           }
-          if constexpr (S::SPLIT) {
-            // this CTA's part of the sum into shared memory, [column][lane];
-            // 8-bit products stay integers (their bits travel as floats)
-            float* mine = part + c0 * 128 + quad * 32 + lane;
+          if constexpr (S::KIND == kKindI8) scale_block(v, xs + c0, m ? ws[MT - 1] : ws[0]);
+          const int64_t at0 = out0 + c0 * p.out_col + ch;
+          if constexpr (S::kTerms > 1) {
+            float* o = static_cast<float*>(p.out) + at0;
+            if (!first && live) {
+              int64_t stride = p.out_col;
+              keep_here(stride);
+              const float* q = o;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < n) mine[i * 128] = first ? v[i] : mine[i * 128] + v[i];
-          } else {
-            if constexpr (S::KIND == kKindI8) scale_block(v, xs + c0, m ? ws[MT - 1] : ws[0]);
-            const int64_t at0 = out0 + c0 * p.out_col + ch;
-            if constexpr (S::kTerms > 1) {
-              float* o = static_cast<float*>(p.out) + at0;
-              if (!first && live) {
-                int64_t stride = p.out_col;
-                keep_here(stride);
-                const float* q = o;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  if (i < n) v[i] += *q;
-                  q += stride;
-                }
+              for (int i = 0; i < 32; ++i) {
+                if (i < n) v[i] += *q;
+                q += stride;
               }
-              store_cols(o, p.out_col, v, n, live, false);
-            } else {
-              store_typed(p.out, p.out_dtype, at0, p.out_col, v, n, live, p.pairs != 0);
             }
+            store_cols(o, p.out_col, v, n, live, false);
+          } else {
+            store_typed(p.out, p.out_dtype, at0, p.out_col, v, n, live, p.pairs != 0);
           }
         }
         if (!released) release();
@@ -907,33 +1002,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       } while (s0 < at.kb1);
       if (!ok) break;
-      if constexpr (S::SPLIT) {
-        __syncwarp();
-        if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_full), lane));
-        int go = 1;
-        if (lane == 0) go = tc_wait(&ctl.red_full, red_phase, &ctl, p.status, true) ? 1 : 0;
-        if (!__shfl_sync(0xffffffffu, go, 0)) break;
-        const bool live = ch0 < p.lanes;
-        float wscale = 1.0f;
-        if constexpr (S::KIND == kKindI8) wscale = live ? p.g.w_scale[at.expert * p.lanes + ch0] : 0.0f;
-        // every (2 csize)-th column: the parts are added in the CTAs' order
-        for (int c = rank * 2 + set; c < at.rows; c += 2 * csize) {
-          const uint32_t mine = smem_u32(part + c * 128 + quad * 32 + lane);
-          float v = 0.0f;
-          if constexpr (S::KIND == kKindI8) {
-            int sum = 0;
-            for (uint32_t r = 0; r < csize; ++r) sum += __float_as_int(load_at(at_rank(mine, r)));
-            const int64_t tok = p.g.source(at.row0 + c);
-            v = tok >= 0 ? static_cast<float>(sum) * p.g.x_scale[tok] * wscale : 0.0f;
-          } else {
-            for (uint32_t r = 0; r < csize; ++r) v += load_at(at_rank(mine, r));
-          }
-          if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch0, v);
-        }
-        __syncwarp();
-        if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
-        red_phase ^= 1;
-      }
     }
   }
   __syncwarp();
@@ -1032,6 +1100,7 @@ __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
 
 template <typename T>
 __global__ void __launch_bounds__(kCopyThreads) layout_kernel(const __grid_constant__ LayoutArgs p) {
+  let_next_grid_start();
   constexpr bool kSplit = std::is_same<T, float>::value;
   constexpr int VEC = kSplit ? 8 : 16 / sizeof(T);  // elements of a 16-byte store
   const int64_t z = blockIdx.y;
@@ -1174,12 +1243,16 @@ int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int cs
   cfg.blockDim = dim3(kTcThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = csize;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = csize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  // the kernel sets up its barriers and TMEM while the one before it (the rows'
+  // copy, their rounding) still runs, and waits for it before its first read
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, grouped_tc_kernel<S>, p, m[0], m[1], m[2], m[3]) != cudaSuccess) {
     cudaGetLastError();
     return ES_ERR_CUDA;

@@ -74,6 +74,11 @@ def _call(fn: str, dev, *args):
         L.check(fn, status)
 
 
+def _empty(rows: int, cols: int, dtype, dev):
+    """``torch.empty((rows, cols))``, which takes twice as long from a tuple."""
+    return torch.empty_strided((rows, cols), (cols or 1, 1), dtype=dtype, device=dev)
+
+
 def _scratch(nbytes: int, dev):
     """A workspace that is held until the call is queued (torch's allocator
     hands it out again only behind that on the stream), or None."""
@@ -98,11 +103,11 @@ class ExpertPlan:
 
     def __init__(self, offsets: torch.Tensor, order: torch.Tensor, position: torch.Tensor):
         _on_gpu("ExpertPlan", offsets=offsets, order=order, position=position)
-        for t in (offsets, order, position):
-            if t.dtype != torch.int32:
-                raise TypeError("ExpertPlan: offsets, order and position must be int32")
-            if not t.is_contiguous():
-                raise ValueError("ExpertPlan: offsets, order and position must be contiguous")
+        i32 = torch.int32
+        if offsets.dtype != i32 or order.dtype != i32 or position.dtype != i32:
+            raise TypeError("ExpertPlan: offsets, order and position must be int32")
+        if not (offsets.is_contiguous() and order.is_contiguous() and position.is_contiguous()):
+            raise ValueError("ExpertPlan: offsets, order and position must be contiguous")
         E, R, P = offsets.shape, order.shape, position.shape
         if len(E) != 1 or len(R) != 1 or len(P) != 2 or E[0] < 2 or P[1] < 1 or P[0] * P[1] != R[0]:
             raise ValueError(f"ExpertPlan: shapes {tuple(E)}, {tuple(R)} and {tuple(P)} are not "
@@ -130,8 +135,8 @@ class ExpertPlan:
 def _route(logits, top_k, renormalize):
     dev = logits.device
     T, E = logits.shape
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-    experts = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    weights = _empty(T, top_k, torch.float32, dev)
+    experts = _empty(T, top_k, torch.int32, dev)
     _call("es_route_experts", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), top_k,
           renormalize, weights.data_ptr(), experts.data_ptr())
     return weights, experts
@@ -156,7 +161,7 @@ class _Route(torch.autograd.Function):
         dev = logits.device
         T, E = logits.shape
         dweights = dweights.contiguous()
-        dlogits = torch.empty((T, E), dtype=logits.dtype, device=dev)
+        dlogits = _empty(T, E, logits.dtype, dev)
         _call("es_route_experts_grad", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0),
               experts.shape[1], ctx.renormalize, weights.data_ptr(), experts.data_ptr(), dweights.data_ptr(),
               dlogits.data_ptr())
@@ -205,7 +210,7 @@ def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
     dev, n = experts.device, experts.numel()
     offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
     order = torch.empty(n, dtype=torch.int32, device=dev)
-    position = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    position = torch.empty_like(experts)
     nbytes = L.lib().es_expert_plan_workspace_size(n, E)
     ws = _scratch(nbytes, dev)
     _call("es_expert_plan", dev, experts.data_ptr(), n, E, _ptr(ws), nbytes, offsets.data_ptr(), order.data_ptr(),
@@ -220,7 +225,7 @@ def _grouped(x, w, plan, gather, out_dtype):
     dev = x.device
     E, K, N = w.shape
     R, code = plan.num_rows, _DTYPES[x.dtype]
-    y = torch.empty((R, N), dtype=out_dtype, device=dev)
+    y = _empty(R, N, out_dtype, dev)
     args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), plan.offsets.data_ptr(),
             plan.order.data_ptr() if gather else None, plan.top_k, R)
     nbytes = L.lib().es_grouped_matmul_workspace_size(*args)
@@ -305,7 +310,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan, gather: b
 
 def _combine(y, weights, plan, out_dtype):
     dev, D = y.device, y.shape[1]
-    out = torch.empty((plan.num_tokens, D), dtype=out_dtype, device=dev)
+    out = _empty(plan.num_tokens, D, out_dtype, dev)
     _call("es_combine_experts", dev, y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0), _ptr(weights),
           plan.position.data_ptr(), plan.num_tokens, plan.top_k, D, out.data_ptr(), _DTYPES[out_dtype])
     return out
@@ -324,8 +329,8 @@ class _Combine(torch.autograd.Function):
         y, weights = ctx.saved_tensors
         plan, dev = ctx.plan, y.device
         dout = _rows(dout)
-        dy = torch.empty(y.shape, dtype=y.dtype, device=dev)
-        dweights = torch.empty(weights.shape, dtype=torch.float32, device=dev)
+        dy = _empty(*y.shape, y.dtype, dev)
+        dweights = torch.empty_like(weights)
         _call("es_combine_experts_grad", dev, y.data_ptr(), _DTYPES[y.dtype], y.shape[0], y.stride(0),
               weights.data_ptr(), plan.position.data_ptr(), plan.offsets.data_ptr() + 4 * plan.num_experts,
               plan.num_tokens, plan.top_k, y.shape[1], dout.data_ptr(), dout.stride(0), dy.data_ptr(),
@@ -365,7 +370,7 @@ def quantize_rows(x: torch.Tensor):
     if x.dim() != 2:
         raise ValueError(f"quantize_rows: x must be (rows, width), got {tuple(x.shape)}")
     dev, x = x.device, _rows(x.detach())
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    q = _empty(*x.shape, torch.int8, dev)
     scale = torch.empty(x.shape[0], dtype=torch.float32, device=dev)
     _call("es_quantize_rows", dev, x.data_ptr(), code, x.shape[0], x.shape[1], x.stride(0), q.data_ptr(),
           scale.data_ptr())
@@ -418,7 +423,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
         wq = wq.contiguous()
     dev = q.device
     R = plan.num_rows if plan is not None else q.shape[0]
-    y = torch.empty((R, N), dtype=out_dtype, device=dev)
+    y = _empty(R, N, out_dtype, dev)
     args = (q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(), wscale.data_ptr(), E, K, N,
             wq.stride(0) if E else 0, wq.stride(-2), plan.offsets.data_ptr() if E else None,
             plan.order.data_ptr() if gather else None, plan.top_k if E else 1, R)
