@@ -175,6 +175,15 @@ __device__ bool tc_wait(uint64_t* bar, uint32_t parity, TcCtl* ctl, int32_t* sta
   return false;
 }
 
+// The wait of a whole warp: one look by all, then lane 0 waits for them.
+__device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, TcCtl* ctl, int32_t* status,
+                                             bool progress = false) {
+  if (__all_sync(0xffffffffu, try_wait_cluster(bar, parity))) return true;
+  int go = 0;
+  if ((threadIdx.x & 31) == 0) go = tc_wait(bar, parity, ctl, status, progress) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, go, 0) != 0;
+}
+
 __device__ void tc_drain(uint64_t* bar, uint32_t parity) {
   const uint64_t t0 = global_ns();
   for (uint32_t i = 0;; ++i) {
@@ -235,12 +244,13 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
         : "memory");
 }
 
+// One MMA, issued by an elected lane of a converged warp.
 template <int CG, int KIND>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
-#define ES_MMA(group, kind)                                                                            \
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                       \
-               "tcgen05.mma.cta_group::" #group ".kind::" #kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
-               "l"(a), "l"(b), "r"(idesc), "r"(accum)                                                  \
+#define ES_MMA(group, kind)                                                                               \
+  asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"        \
+               "@e tcgen05.mma.cta_group::" #group ".kind::" #kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d), \
+               "l"(a), "l"(b), "r"(idesc), "r"(accum)                                                     \
                : "memory")
   if constexpr (CG == 2 && KIND == kKindF16) ES_MMA(2, f16);
   if constexpr (CG == 2 && KIND == kKindI8) ES_MMA(2, i8);
@@ -249,17 +259,19 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 #undef ES_MMA
 }
 
-// Arrives on the barrier (of both CTAs of a pair) when the MMAs issued so far are done.
+// Arrives on the barrier (of both CTAs of a pair) when the MMAs that the
+// elected lane has issued so far are done; a converged warp.
 template <int CG>
 __device__ __forceinline__ void commit(uint64_t* bar) {
   if constexpr (CG == 2)
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+            "r"(smem_u32(bar)),
         "h"(static_cast<uint16_t>(3))
         : "memory");
   else
-    umma_commit(bar);
+    umma_commit_warp(bar);
 }
 
 template <int CG>
@@ -825,7 +837,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
-      if (leader && lane == 0) {
+      // the whole warp walks the loop and one elected lane issues: operands
+      // that are alike in all lanes go to the uniform registers that the
+      // instruction reads (issued by one lane's branch an MMA took 68 cycles)
+      if (leader) {
         int stage = 0, buf = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
@@ -836,14 +851,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
           for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
             const int s1 = s0 + min(S::kChain, at.kb1 - s0);
-            ok = tc_wait(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
+            ok = tc_wait_warp(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
             if (!ok) break;
             tc_fence_after();
             const uint32_t d = tmem + buf * MT * NT;
             uint32_t more = 0;
             for (int term = 0; term < S::kTerms && ok; ++term)
               for (int kb = s0; kb < s1; ++kb) {
-                ok = tc_wait(&ctl.full[stage], phase, &ctl, p.status);
+                ok = tc_wait_warp(&ctl.full[stage], phase, &ctl, p.status);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t sa = base + stage * S::kStageBytes;
@@ -851,17 +866,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
                 int steps = 4;
                 if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
-  #pragma unroll
+#pragma unroll
                 for (int m = 0; m < MT; ++m) {
                   const uint64_t dm = da + m * (kABytes >> 4);
-                  if (steps == 4) {
-  #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                      mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
-                  } else {
-                    for (int i = 0; i < steps; ++i)
-                      mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
-                  }
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (i < steps) mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
                 }
                 more = 1;
                 commit<CG>(&ctl.empty[stage]);
@@ -880,7 +890,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (!ok) {
           commit<CG>(&ctl.drain);
-          tc_drain(&ctl.drain, 0);
+          if (lane == 0) tc_drain(&ctl.drain, 0);
         }
       }
       __syncwarp();
