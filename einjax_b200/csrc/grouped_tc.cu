@@ -1288,7 +1288,7 @@ int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
     return launch<TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>>(p, m, n, 2, stream);
   }
   p.idesc |= 8u << 24;
-  if (mean > 64) return launch<TcShape<1, 1, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(128, 128), 1, stream);
+  if (mean > 64) return launch<TcShape<1, 2, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(256, 128), 1, stream);
   // few rows: the weights' bytes are the time; a tile's depth is shared by a
   // cluster while the tiles alone do not fill the SMs
   const int64_t n = tiles(128, 64);
