@@ -1275,6 +1275,10 @@ constexpr int64_t kMaxTiles = 0x7fffffffLL;
 
 template <int KIND, bool A_MN, int PLANES>
 int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
+  using Wide = TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>;
+  using Middle = TcShape<1, 2, 128, KIND, A_MN, false, false, PLANES>;
+  using Narrow = TcShape<1, 1, 64, KIND, A_MN, false, false, PLANES>;
+  using Split = TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>;
   const int64_t R = p.g.rows, groups = p.g.groups();
   const int64_t live = groups < R ? groups : R;  // groups that can have rows
   const int64_t mean = R / live;
@@ -1282,22 +1286,26 @@ int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
     p.lane_tiles = static_cast<int>((p.lanes + lanes - 1) / lanes);
     return (R / nt + live) * p.lane_tiles;
   };
-  if (mean > 128) {
-    const int64_t n = tiles(512, 256);
+  // By the rows of a group, where the tiles then fill the SMs. 60 experts,
+  // 2048 x 2816, bf16, us for Narrow, Middle, Wide: 8 rows 104, 107, 118; 24
+  // rows 118, 111, 119; 144 rows 339, 144, 154; 176 rows 397, 173, 160. In 8
+  // bits Wide gains from 300 rows (224: 105 and 111, 300: 142 and 126).
+  const int64_t wide = tiles(Wide::kLanes, Wide::NT);
+  if (mean > (KIND == kKindI8 ? 240 : 160) && wide >= kSMs / 2) {
     p.idesc |= 16u << 24;
-    return launch<TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>>(p, m, n, 2, stream);
+    return launch<Wide>(p, m, wide, 2, stream);
   }
   p.idesc |= 8u << 24;
-  if (mean > 64) return launch<TcShape<1, 2, 128, KIND, A_MN, false, false, PLANES>>(p, m, tiles(256, 128), 1, stream);
-  // few rows: the weights' bytes are the time; a tile's depth is shared by a
-  // cluster while the tiles alone do not fill the SMs
-  const int64_t n = tiles(128, 64);
-  const int64_t nkb = (p.g.K + TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>::BK - 1) /
-                      TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>::BK;
+  const int64_t middle = tiles(Middle::kLanes, Middle::NT);
+  if (mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
+  // few rows, or few tiles: a tile's depth is shared by a cluster while the
+  // tiles alone do not fill the SMs
+  const int64_t narrow = tiles(Narrow::kLanes, Narrow::NT);
+  const int64_t nkb = (p.g.K + Split::BK - 1) / Split::BK;
   int split = 1;
-  while (split < 8 && n * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
-  if (split > 1) return launch<TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>>(p, m, n, split, stream);
-  return launch<TcShape<1, 1, 64, KIND, A_MN, false, false, PLANES>>(p, m, n, 1, stream);
+  while (split < 8 && narrow * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
+  if (split > 1) return launch<Split>(p, m, narrow, split, stream);
+  return launch<Narrow>(p, m, narrow, 1, stream);
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
