@@ -687,6 +687,32 @@ def test_streams_and_graph():
     del graph
 
 
+def test_from_a_new_thread():
+    """A thread whose first CUDA work is the product (as autograd's threads)."""
+    import threading
+    g = gen(21)
+    plan = make_plan([300, 0, 200])
+    x, w = randn(g, 500, 128, dtype=torch.bfloat16), randn(g, 3, 128, 256, dtype=torch.bfloat16)
+    q, s = E.quantize_rows(x)
+    wq, ws = E.quantize_experts(w)
+    dy = randn(g, 500, 256, dtype=torch.bfloat16)
+    leaves = [x.clone().requires_grad_(), w.clone().requires_grad_()]
+    y = E.grouped_matmul(*leaves, plan)
+    want = (E.grouped_matmul(x, w, plan), E.int8_matmul(q, s, wq, ws, plan),
+            *torch.autograd.grad(y, leaves, dy, retain_graph=True))
+    torch.cuda.synchronize()
+    for i, f in enumerate((lambda: E.grouped_matmul(x, w, plan), lambda: E.int8_matmul(q, s, wq, ws, plan),
+                           lambda: torch.autograd.grad(y, leaves[:1], dy, retain_graph=True)[0],
+                           lambda: torch.autograd.grad(y, leaves[1:], dy, retain_graph=True)[0])):
+        got = []
+        f()  # its buffers are in the allocator's cache afterwards
+        thread = threading.Thread(target=lambda: got.append(f()))
+        thread.start()
+        thread.join()
+        torch.cuda.synchronize()
+        assert got and torch.equal(got[0], want[i])
+
+
 def test_same_bits_twice():
     """No result depends on the schedule."""
     plan = make_plan([40, 3, 900, 16, 0, 1], 2)
