@@ -10,10 +10,10 @@
 // rows that are left, so a group of 3 rows costs a 16-wide MMA and no padding,
 // and one kernel serves a decode step and a long prompt. For the weights'
 // gradient lanes and columns are its two dimensions and the sum runs over the
-// group's rows; of a group's last block only whole 16-row steps that hold rows
-// are multiplied, and TMA gathers that block row by row with the missing rows
-// pointing outside of the tensor, which reads zeros (so that infinities of the
-// next group stay out of it).
+// group's rows; of a group's last block only the 16-row steps that hold rows
+// are multiplied, and the last of them is gathered row by row (tile::gather4)
+// with the missing rows pointing outside of the tensor, which reads zeros (so
+// that infinities of the next group stay out of it).
 //
 // Operands are read as they lie: K-major or MN-major, through 128-byte
 // swizzled TMA boxes. Routed tokens are first copied into the rows' order: TMA
@@ -21,15 +21,17 @@
 // 2.76 ms where the copy and box loads take 1.0 ms (16384 rows, 4096 x 8192,
 // bf16). What TMA cannot read (odd addresses or strides) is copied too.
 //
-// fp32 operands are cut into three bf16 planes, x = b0 + b1 + b2 exactly, and
-// the six products b_i b_j with i + j <= 2 are added, the smallest first; what
-// is left out is at most 2^-24 of a product. The accumulator truncates each step's sum (measured: a relative
-// error of 1e-9 a unit of depth), so a sum is cut into chains of 512 that the
-// epilogue adds in fp32.
+// fp32 operands are cut into three bf16 planes, x = b0 + b1 + b2 exactly. A
+// stage holds all planes of a block of depth, and the six products b_i b_j with
+// i + j <= 2 are made from it (each operand crosses from L2 once): b0 b0 into
+// one accumulator, the other five, at most 2^-8 of it, into a second. What is
+// left out is at most 2^-24 of a product. An accumulator truncates each step's
+// sum (measured: a relative error of 1e-9 a unit of depth), so a sum is cut
+// into chains of 512 that the epilogue adds in fp32.
 //
-// Roles (8 warps): warp 0 issues the TMA loads, warp 1 the MMAs (one lane),
-// warps 2-3 clear the output rows of no expert, warps 4-7 read the
-// accumulator (TMEM lane quadrant = warp % 4) and write the output. Tiles are
+// Roles (12 warps): warp 0 issues the TMA loads, warp 1 the MMAs (an elected
+// lane), warps 2-3 clear the output rows of no expert, warps 4-11 read the
+// accumulators (TMEM lane quadrant = warp % 4) and write the output. Tiles are
 // dealt to the CTAs in turn; the accumulator is double buffered, so a tile's
 // epilogue runs under the next tile's MMAs. Every wait is bounded: when one
 // runs out the CTA sets ES_ERR_TIMEOUT, drains its copies and MMAs, frees
@@ -73,6 +75,13 @@ struct TcArgs {
   uint32_t idesc;     // instruction descriptor without N
   int pairs;          // two neighbouring lanes may be stored together
   int32_t* status;
+};
+
+// Tensor maps of the operands. The weights' gradient reads a group's last block
+// by steps of 16 rows and by gathers of single rows.
+struct TcMaps {
+  CUtensorMap a, b;
+  CUtensorMap a_steps, b_steps, a_rows, b_rows;
 };
 
 struct TcCtl {
@@ -307,29 +316,36 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 
 // ------------------------------------------------------------------- kernel
 
-// Planes of the six products of fp32 operands, in the order they are added.
+// Planes of the six products of fp32 operands: the last goes to the first
+// accumulator, the others, smallest first, to the second.
+constexpr int kTerms = 6;
 __host__ __device__ constexpr int term_a(int t) { return t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0; }
 __host__ __device__ constexpr int term_b(int t) { return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0; }
 
 template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
 struct TcShape {
-  static constexpr int MT = MT_;  // accumulators of 128 lanes (of each CTA) that share B
-  static constexpr int kTerms = PLANES_ == 3 ? 6 : 1;
-  static constexpr int kChain = PLANES_ == 3 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int CG = CG_;        // CTAs of one MMA
+  static constexpr int MT = MT_;        // accumulators of 128 lanes (of each CTA) that share B
   static constexpr int NT = NT_;        // widest MMA
   static constexpr int KIND = KIND_;
   static constexpr bool A_MN = A_MN_;   // lanes contiguous in memory
   static constexpr bool WGRAD = WGRAD_;
   static constexpr bool SPLIT = SPLIT_; // the cluster's CTAs share one tile's depth
+  static constexpr int PLANES = PLANES_;
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
+  static constexpr int kChain = PLANES > 1 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int kLanes = 128 * MT * CG;
-  static constexpr int kBufs = 2 * MT * NT <= 512 ? 2 : 1;  // tiles in TMEM
-  static constexpr bool kHeld = kBufs == 1 && PLANES_ == 1;  // tiles are held in registers, see drain_held
-  static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;
+  static constexpr int kATiles = PLANES > 1 ? PLANES : MT;  // 128-lane tiles of A in a stage
+  static constexpr int kAccs = PLANES > 1 ? 2 : MT;         // accumulators of a tile
+  static constexpr int kBufs = 2 * kAccs * NT <= 512 ? 2 : 1;  // tiles in TMEM
+  static constexpr bool kHeld = kBufs == 1;  // tiles are held in registers, see drain_held
+  static constexpr int kBBytes = NT / CG * kSwizzleRow;        // of one plane
+  static constexpr int kStageBytes = kATiles * kABytes + PLANES * kBBytes;
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
+  static_assert(PLANES == 1 || (MT == 1 && kBufs == 2), "planes take the tiles that accumulators would share B with");
+  static_assert(kStages >= 2, "stages");
 };
 
 // One output tile, and what of its depth this CTA multiplies.
@@ -597,16 +613,19 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
   for (int s0 = at.kb0; s0 < at.kb1; s0 += min(S::kChain, at.kb1 - s0)) {
     if (!wait(&ctl.acc_full[buf], acc_phase)) return false;
     tc_fence_after();
-    const uint32_t acc = tmem + buf * S::NT + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t acc = tmem + buf * S::kAccs * S::NT + (static_cast<uint32_t>(quad * 32) << 16);
 #pragma unroll 1
     for (int c0 = set * 8; c0 < at.rows; c0 += 16) {
       float v[8];
       tmem_ld8(acc + c0, v);
+      if constexpr (S::PLANES > 1) {
+        float u[8];
+        tmem_ld8(acc + S::NT + c0, u);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // columns past the tile's are written and not read
-        if (S::kTerms > 1 && s0 > at.kb0) v[i] += mine[(c0 + i) * 128];
-        mine[(c0 + i) * 128] = v[i];
+        for (int i = 0; i < 8; ++i) v[i] += u[i] + (s0 > at.kb0 ? mine[(c0 + i) * 128] : 0.0f);
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[(c0 + i) * 128] = v[i];  // columns past the tile's are not read
     }
     tc_fence_before();
     __syncwarp();
@@ -651,10 +670,8 @@ static_assert(128 * kRoleRegs + 256 * kEpiRegs == kTcThreads * kLaunchRegs, "reg
 
 template <typename S>
 __global__ void __launch_bounds__(kTcThreads, 1)
-    grouped_tc_kernel(const __grid_constant__ TcArgs p, const __grid_constant__ CUtensorMap map_a,
-                      const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap rows_a,
-                      const __grid_constant__ CUtensorMap rows_b) {
-  constexpr int CG = S::CG, MT = S::MT, NT = S::NT, BK = S::BK, STAGES = S::kStages;
+    grouped_tc_kernel(const __grid_constant__ TcArgs p, const __grid_constant__ TcMaps m) {
+  constexpr int CG = S::CG, MT = S::MT, NT = S::NT, BK = S::BK, STAGES = S::kStages, PLANES = S::PLANES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcCtl ctl;
   __shared__ alignas(16) float x_scales[S::KIND == kKindI8 ? 2 : 1][S::KIND == kKindI8 ? NT : 4];
@@ -671,8 +688,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const bool leader = pair_rank == 0;
 
   if (threadIdx.x == 0) {
-    prefetch_map(&map_a);
-    prefetch_map(&map_b);
+    prefetch_map(&m.a);
+    prefetch_map(&m.b);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ctl.full[s], 1);
       mbar_init(&ctl.empty[s], 1);
@@ -689,7 +706,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ctl.progress = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kBufs * MT * NT);
+  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kBufs * S::kAccs * NT);
   wait_for_earlier_grids();
   if (warp == 2) {  // tiles of each group
     int run = 0;
@@ -735,88 +752,96 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int half = width / CG;  // columns of this CTA's part of B
         const int lane0 = static_cast<int>(at.lane0) + static_cast<int>(pair_rank) * 128;
         const int col0 = at.row0 + static_cast<int>(pair_rank) * half;
-        for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
-          const int s1 = s0 + min(S::kChain, at.kb1 - s0);
-          for (int term = 0; term < S::kTerms && ok; ++term) {
-            const int plane_a = S::kTerms > 1 ? term_a(term) : 0, plane_b = S::kTerms > 1 ? term_b(term) : 0;
-            for (int kb = s0; kb < s1; ++kb) {
-              uint32_t bytes;
-              int src[4];            // weights' gradient, last block: four rows of a gather
-              int rows16 = BK;       // rows of the block in whole MMA steps
-              bool tail = false;
-              if constexpr (S::WGRAD) {
-                const int valid = min(at.depth - kb * BK, BK);
-                tail = valid < BK;
-                if (tail) {
-                  rows16 = (valid + 15) & ~15;
-      #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const int r = (lane & 15) * 4 + i;
-                    src[i] = r < valid ? at.first + kb * BK + r : -1;
-                  }
-                }
-                bytes = (2 * MT + (half + 63) / 64) * rows16 * 128u;
+        for (int kb = at.kb0; kb < at.kb1; ++kb) {
+          uint32_t bytes;
+          int valid = BK;  // weights' gradient: rows of the block
+          const int boxes = (half + 63) / 64;
+          if constexpr (S::WGRAD) {
+            valid = min(at.depth - kb * BK, BK);
+            bytes = (2 * S::kATiles + PLANES * boxes) * ((valid + 15) & ~15) * 128u;
+          } else {
+            bytes = S::kATiles * kABytes + PLANES * ((half + kBoxRows - 1) / kBoxRows) * (kBoxRows * 128u);
+          }
+          int go = 0;
+          if (lane == 0) {
+            go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+            if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
+            if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+          }
+          go = __shfl_sync(0xffffffffu, go, 0);
+          if (!go) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kATiles * kABytes;
+          const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
+          // tile a of A: the next lanes, or the next plane
+          constexpr int next_lanes = PLANES > 1 ? 0 : 128 * CG, next_plane = PLANES > 1 ? 1 : 0;
+          if constexpr (S::WGRAD) {
+            // operand boxes of 64 lanes (columns) by 64 rows
+            const int row = at.first + kb * BK;
+            const int operands = 2 * S::kATiles + PLANES * boxes;
+            auto place = [&](int u, uint32_t& to, int& x, int& y) {
+              if (u < 2 * S::kATiles) {
+                const int a = u >> 1;
+                to = sa + u * 8192;
+                x = lane0 + a * next_lanes + (u & 1) * 64;
+                y = a * next_plane * p.plane_rows;
               } else {
-                bytes = MT * kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
+                const int plane = (u - 2 * S::kATiles) / boxes, box = u - 2 * S::kATiles - plane * boxes;
+                to = sb + plane * S::kBBytes + box * 8192;
+                x = col0 + box * 64;
+                y = plane * p.plane_rows;
               }
-              int go = 0;
-              if (lane == 0) {
-                go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
-                if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
-                if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+            };
+            uint32_t to;
+            int x, y;
+            if (valid == BK) {
+              if (lane < operands) {
+                place(lane, to, x, y);
+                load_2d<CG>(to, lane < 2 * S::kATiles ? &m.a : &m.b, x, row + y, bar);
               }
-              go = __shfl_sync(0xffffffffu, go, 0);
-              if (!go) {
-                ok = false;
-                break;
+            } else {
+              // the last block: whole steps of 16 rows, then the rest by
+              // gathers of four rows (which cost as much as a box each)
+              const int full = valid >> 4, rest = valid & 15;
+              for (int i = lane; i < operands * full; i += 32) {
+                const int u = i / full, s = i - u * full;
+                place(u, to, x, y);
+                load_2d<CG>(to + s * 2048, u < 2 * S::kATiles ? &m.a_steps : &m.b_steps, x, row + s * 16 + y, bar);
               }
-              const uint32_t sa = base + stage * S::kStageBytes, sb = sa + MT * kABytes;
-              const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
-              if constexpr (S::WGRAD) {
-                // operand boxes of 64 lanes (columns) by 64 rows; of the last block
-                // loads of four rows, dealt to half a warp a box
-                const int row_a = at.first + kb * BK + plane_a * p.plane_rows;
-                const int row_b = at.first + kb * BK + plane_b * p.plane_rows;
-                const int boxes = (half + 63) / 64;
-                if (tail) {
-                  const int quad = lane & 15;
-                  if (quad * 4 < rows16) {
-                    int ra[4], rb[4];
-      #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                      ra[i] = src[i] < 0 ? p.src_rows : src[i] + plane_a * p.plane_rows;
-                      rb[i] = src[i] < 0 ? p.src_rows : src[i] + plane_b * p.plane_rows;
-                    }
-  #pragma unroll
-                    for (int m = 0; m < MT; ++m)
-                      load_rows<CG>(sa + m * kABytes + (lane >> 4) * 8192 + quad * 512, &rows_a,
-                                    lane0 + m * 128 * CG + (lane >> 4) * 64, ra, bar);
-                    for (int b = lane >> 4; b < boxes; b += 2)
-                      load_rows<CG>(sb + b * 8192 + quad * 512, &rows_b, col0 + b * 64, rb, bar);
-                  }
-                } else if (lane < 2 * MT) {
-                  load_2d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, row_a, bar);
-                } else if (lane - 2 * MT < boxes) {
-                  load_2d<CG>(sb + (lane - 2 * MT) * 8192, &map_b, col0 + (lane - 2 * MT) * 64, row_b, bar);
-                }
-              } else {
-                const int z = at.expert * p.expert_step + plane_a * p.plane_experts;
-                if constexpr (S::A_MN) {
-                  if (lane < 2 * MT)
-                    load_3d<CG>(sa + lane * 8192, &map_a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
-                                bar);
-                } else {
-                  if (lane < MT) load_3d<CG>(sa + lane * kABytes, &map_a, kb * BK, lane0 + lane * 128 * CG, z, bar);
-                }
-                if (lane * kBoxRows < half)
-                  load_2d<CG>(sb + lane * (kBoxRows * 128), &map_b, kb * BK,
-                              col0 + lane * kBoxRows + plane_b * p.plane_rows, bar);
-              }
-              if (++stage == STAGES) {
-                stage = 0;
-                phase ^= 1;
+              for (int i = lane; i < (rest ? operands * 4 : 0); i += 32) {
+                const int u = i >> 2, q = i & 3;
+                place(u, to, x, y);
+                int r[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  r[j] = q * 4 + j < rest ? row + full * 16 + q * 4 + j + y : p.src_rows;
+                load_rows<CG>(to + full * 2048 + q * 512, u < 2 * S::kATiles ? &m.a_rows : &m.b_rows, x, r, bar);
               }
             }
+          } else {
+            const int z = at.expert * p.expert_step;
+            if constexpr (S::A_MN) {
+              if (lane < 2 * S::kATiles) {
+                const int a = lane >> 1;
+                load_3d<CG>(sa + lane * 8192, &m.a, lane0 + a * next_lanes + (lane & 1) * 64, kb * BK,
+                            z + a * next_plane * p.plane_experts, bar);
+              }
+            } else {
+              if (lane < S::kATiles)
+                load_3d<CG>(sa + lane * kABytes, &m.a, kb * BK, lane0 + lane * next_lanes,
+                            z + lane * next_plane * p.plane_experts, bar);
+            }
+            if (lane * kBoxRows < half)
+#pragma unroll
+              for (int plane = 0; plane < PLANES; ++plane)
+                load_2d<CG>(sb + plane * S::kBBytes + lane * (kBoxRows * 128), &m.b, kb * BK,
+                            col0 + lane * kBoxRows + plane * p.plane_rows, bar);
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
           }
         }
       }
@@ -854,32 +879,36 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             ok = tc_wait_warp(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t d = tmem + buf * MT * NT;
+            const uint32_t d = tmem + buf * S::kAccs * NT;
             uint32_t more = 0;
-            for (int term = 0; term < S::kTerms && ok; ++term)
-              for (int kb = s0; kb < s1; ++kb) {
-                ok = tc_wait_warp(&ctl.full[stage], phase, &ctl, p.status);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t sa = base + stage * S::kStageBytes;
-                const uint64_t da = operand(sa, S::A_MN), db = operand(sa + MT * kABytes, S::WGRAD);
-                constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
-                int steps = 4;
-                if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+            for (int kb = s0; kb < s1; ++kb) {
+              ok = tc_wait_warp(&ctl.full[stage], phase, &ctl, p.status);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t sa = base + stage * S::kStageBytes;
+              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + S::kATiles * kABytes, S::WGRAD);
+              constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
+              int steps = 4;
+              if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+              constexpr int products = PLANES > 1 ? kTerms : MT;
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                  const uint64_t dm = da + m * (kABytes >> 4);
+              for (int m = 0; m < products; ++m) {
+                const int a = PLANES > 1 ? term_a(m) : m, b = PLANES > 1 ? term_b(m) : 0;
+                const int acc = PLANES > 1 ? (m < kTerms - 1 ? 1 : 0) : m;
+                const uint32_t old = PLANES > 1 && m > 0 && m < kTerms - 1 ? 1 : more;
 #pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    if (i < steps) mma<CG, S::KIND>(d + m * NT, dm + i * step_a, db + i * step_b, idesc, more | i);
-                }
-                more = 1;
-                commit<CG>(&ctl.empty[stage]);
-                if (++stage == STAGES) {
-                  stage = 0;
-                  phase ^= 1;
-                }
+                for (int i = 0; i < 4; ++i)
+                  if (i < steps)
+                    mma<CG, S::KIND>(d + acc * NT, da + a * (kABytes >> 4) + i * step_a,
+                                     db + b * (S::kBBytes >> 4) + i * step_b, idesc, old | i);
               }
+              more = 1;
+              commit<CG>(&ctl.empty[stage]);
+              if (++stage == STAGES) {
+                stage = 0;
+                phase ^= 1;
+              }
+            }
             if (!ok) break;
             commit<CG>(&ctl.acc_full[buf]);
             if (++buf == S::kBufs) {
@@ -947,7 +976,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if (!ok) break;
           tc_fence_after();
         }
-        const uint32_t acc = tmem + buf * MT * NT + (static_cast<uint32_t>(quad * 32) << 16);
+        const uint32_t acc = tmem + buf * S::kAccs * NT + (static_cast<uint32_t>(quad * 32) << 16);
         auto release = [&] {
           tc_fence_before();
           __syncwarp();
@@ -979,13 +1008,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           float v[32];
           if (any) {
             tmem_ld32(acc + m * NT + c0, v);
+            if constexpr (PLANES > 1) {
+              float u[32];
+              tmem_ld32(acc + NT + c0, u);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] += u[i];
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.0f;
           }
           if constexpr (S::KIND == kKindI8) scale_block(v, xs + c0, m ? ws[MT - 1] : ws[0]);
           const int64_t at0 = out0 + c0 * p.out_col + ch;
-          if constexpr (S::kTerms > 1) {
+          if constexpr (PLANES > 1) {
             float* o = static_cast<float*>(p.out) + at0;
             if (!first && live) {
               int64_t stride = p.out_col;
@@ -1019,7 +1054,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   if (csize > 1) cluster_sync();
   tc_fence_after();
-  if (warp == 1) tc_dealloc<CG>(tmem, S::kBufs * MT * NT);
+  if (warp == 1) tc_dealloc<CG>(tmem, S::kBufs * S::kAccs * NT);
 }
 
 // --------------------------------------------------------------------- host
@@ -1266,7 +1301,7 @@ bool encode_operand(const Operand& o, int dtype, int box_cols, int box_rows, int
 }
 
 template <typename S>
-int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int csize, cudaStream_t stream) {
+int launch(const TcArgs& p, const TcMaps& m, int64_t max_tiles, int csize, cudaStream_t stream) {
   const size_t smem = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kPartBytes +
                       (3 * p.g.groups() + 1) * sizeof(int);
   static std::atomic<bool> raised[kMaxAttrDevices];
@@ -1301,7 +1336,7 @@ int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int cs
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, grouped_tc_kernel<S>, p, m[0], m[1], m[2], m[3]) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, grouped_tc_kernel<S>, p, m) != cudaSuccess) {
     cudaGetLastError();
     return ES_ERR_CUDA;
   }
@@ -1312,9 +1347,10 @@ int launch(const TcArgs& p, const CUtensorMap (&m)[4], int64_t max_tiles, int cs
 constexpr int64_t kMaxTiles = 0x7fffffffLL;
 
 template <int KIND, bool A_MN, int PLANES>
-int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
-  using Wide = TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>;
-  using Middle = TcShape<1, 2, 128, KIND, A_MN, false, false, PLANES>;
+int rows_launch(TcArgs& p, const TcMaps& m, cudaStream_t stream) {
+  using Wide = std::conditional_t<PLANES == 1, TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>,
+                                  TcShape<2, 1, 128, KIND, A_MN, false, false, PLANES>>;
+  using Middle = TcShape<1, 2, 128, KIND, A_MN, false, false, 1>;
   using Narrow = TcShape<1, 1, 64, KIND, A_MN, false, false, PLANES>;
   using Split = TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>;
   const int64_t R = p.g.rows, groups = p.g.groups();
@@ -1329,13 +1365,16 @@ int rows_launch(TcArgs& p, const CUtensorMap (&m)[4], cudaStream_t stream) {
   // rows 118, 111, 119; 144 rows 339, 144, 154; 176 rows 397, 173, 160. In 8
   // bits Wide gains from 300 rows (224: 105 and 111, 300: 142 and 126).
   const int64_t wide = tiles(Wide::kLanes, Wide::NT);
-  if (mean > (KIND == kKindI8 ? 240 : 160) && wide >= kSMs / 2) {
+  const int64_t least = PLANES > 1 ? 8 : KIND == kKindI8 ? 240 : 160;
+  if (mean > least && wide >= kSMs / 2) {
     p.idesc |= 16u << 24;
     return launch<Wide>(p, m, wide, 2, stream);
   }
   p.idesc |= 8u << 24;
-  const int64_t middle = tiles(Middle::kLanes, Middle::NT);
-  if (mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
+  if constexpr (PLANES == 1) {
+    const int64_t middle = tiles(Middle::kLanes, Middle::NT);
+    if (mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
+  }
   // few rows, or few tiles: a tile's depth is shared by a cluster while the
   // tiles alone do not fill the SMs
   const int64_t narrow = tiles(Narrow::kLanes, Narrow::NT);
@@ -1415,13 +1454,11 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
   p.idesc = idesc_of(dtype, o.mn, false);
   p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(y) & 3) == 0;
   p.status = status;
-  CUtensorMap m[4];
+  TcMaps m{};
   const int bk = static_cast<int>(128 / tc_size(dtype));
-  if (!bind_context() || !encode_operand(o.w, dtype, o.mn ? 64 : bk, o.mn ? 64 : 128, 3, &m[0]) ||
-      !encode_operand(o.x, dtype, bk, kBoxRows, 2, &m[1]))
+  if (!bind_context() || !encode_operand(o.w, dtype, o.mn ? 64 : bk, o.mn ? 64 : 128, 3, &m.a) ||
+      !encode_operand(o.x, dtype, bk, kBoxRows, 2, &m.b))
     return ES_ERR_CUDA;
-  m[2] = m[0];
-  m[3] = m[1];
   if (dtype == kInt8) return rows_launch<kKindI8, false, 1>(p, m, stream);
   if (dtype == ES_F32)
     return o.mn ? rows_launch<kKindF16, true, 3>(p, m, stream) : rows_launch<kKindF16, false, 3>(p, m, stream);
@@ -1461,16 +1498,20 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
   p.pairs = p.lanes % 2 == 0 && p.out_col % 2 == 0 && p.out_expert % 2 == 0 &&
             (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
   p.status = status;
-  p.lane_tiles = static_cast<int>((p.lanes + 511) / 512);
-  p.col_tiles = static_cast<int>((p.cols + 255) / 256);
-  CUtensorMap m[4];
+  using Tile = TcShape<2, 2, 256, kKindF16, true, true, false, 1>;
+  using Tile32 = TcShape<2, 1, 128, kKindF16, true, true, false, 3>;
+  const int lanes = dtype == ES_F32 ? Tile32::kLanes : Tile::kLanes, nt = dtype == ES_F32 ? Tile32::NT : Tile::NT;
+  p.lane_tiles = static_cast<int>((p.lanes + lanes - 1) / lanes);
+  p.col_tiles = static_cast<int>((p.cols + nt - 1) / nt);
+  TcMaps m{};
   const Operand &a = n_lanes ? o.dy : o.x, &b = n_lanes ? o.x : o.dy;
-  if (!bind_context() || !encode_operand(a, dtype, 64, 64, 2, &m[0]) || !encode_operand(b, dtype, 64, 64, 2, &m[1]) ||
-      !encode_operand(a, dtype, 64, 1, 2, &m[2]) || !encode_operand(b, dtype, 64, 1, 2, &m[3]))
+  if (!bind_context() || !encode_operand(a, dtype, 64, 64, 2, &m.a) || !encode_operand(b, dtype, 64, 64, 2, &m.b) ||
+      !encode_operand(a, dtype, 64, 16, 2, &m.a_steps) || !encode_operand(b, dtype, 64, 16, 2, &m.b_steps) ||
+      !encode_operand(a, dtype, 64, 1, 2, &m.a_rows) || !encode_operand(b, dtype, 64, 1, 2, &m.b_rows))
     return ES_ERR_CUDA;
   const int64_t tiles = static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles;
-  if (dtype == ES_F32) return launch<TcShape<2, 2, 256, kKindF16, true, true, false, 3>>(p, m, tiles, 2, stream);
-  return launch<TcShape<2, 2, 256, kKindF16, true, true, false, 1>>(p, m, tiles, 2, stream);
+  if (dtype == ES_F32) return launch<Tile32>(p, m, tiles, 2, stream);
+  return launch<Tile>(p, m, tiles, 2, stream);
 }
 
 }  // namespace es
