@@ -338,13 +338,13 @@ struct TcShape {
   static constexpr int kATiles = PLANES > 1 ? PLANES : MT;  // 128-lane tiles of A in a stage
   static constexpr int kAccs = PLANES > 1 ? 2 : MT;         // accumulators of a tile
   static constexpr int kBufs = 2 * kAccs * NT <= 512 ? 2 : 1;  // tiles in TMEM
-  static constexpr bool kHeld = kBufs == 1;  // tiles are held in registers, see drain_held
+  static constexpr bool kHeld = kBufs == 1 && PLANES == 1;  // tiles are held in registers, see drain_held
   static constexpr int kBBytes = NT / CG * kSwizzleRow;        // of one plane
   static constexpr int kStageBytes = kATiles * kABytes + PLANES * kBBytes;
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
-  static_assert(PLANES == 1 || (MT == 1 && kBufs == 2), "planes take the tiles that accumulators would share B with");
+  static_assert(PLANES == 1 || MT == 1, "planes take the tiles that accumulators would share B with");
   static_assert(kStages >= 2, "stages");
 };
 
@@ -1499,7 +1499,7 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
             (reinterpret_cast<uintptr_t>(dw) & 3) == 0;
   p.status = status;
   using Tile = TcShape<2, 2, 256, kKindF16, true, true, false, 1>;
-  using Tile32 = TcShape<2, 1, 128, kKindF16, true, true, false, 3>;
+  using Tile32 = TcShape<2, 1, 256, kKindF16, true, true, false, 3>;
   const int lanes = dtype == ES_F32 ? Tile32::kLanes : Tile::kLanes, nt = dtype == ES_F32 ? Tile32::NT : Tile::NT;
   p.lane_tiles = static_cast<int>((p.lanes + lanes - 1) / lanes);
   p.col_tiles = static_cast<int>((p.cols + nt - 1) / nt);
