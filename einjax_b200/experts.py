@@ -59,19 +59,39 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
-def _call(fn: str, dev, *args):
-    """Calls the entry point on ``dev`` and its current stream (the last argument)."""
+def _status(fn: str, dev, *args) -> int:
+    """The entry point's answer on ``dev`` and its current stream (its last argument)."""
     index = dev.index
     here = _current_device()
-    if here != index:
-        torch.cuda.set_device(index)
+    if here == index:
+        return getattr(L.lib(), fn)(*args, _raw_stream(index))
+    torch.cuda.set_device(index)
     try:
-        status = getattr(L.lib(), fn)(*args, _raw_stream(index))
+        return getattr(L.lib(), fn)(*args, _raw_stream(index))
     finally:
-        if here != index:
-            torch.cuda.set_device(here)
+        torch.cuda.set_device(here)
+
+
+def _call(fn: str, dev, *args):
+    status = _status(fn, dev, *args)
     if status:
         L.check(fn, status)
+
+
+def _product(fn: str, dev, args, outs, need: bool):
+    """Calls ``fn(*args, *outs, workspace, its size, status word, stream)``. The
+    workspace's size is asked for when the call surely takes one (``need``), or
+    once the call has said so (operands that have to be laid out anew)."""
+    word = _STATUS.address(fn, dev.index)
+    if not need:
+        status = _status(fn, dev, *args, *outs, None, 0, word)
+        if status != L.ES_ERR_WORKSPACE:
+            if status:
+                L.check(fn, status)
+            return
+    nbytes = getattr(L.lib(), fn + "_workspace_size")(*args)
+    ws = _scratch(nbytes, dev)
+    _call(fn, dev, *args, *outs, _ptr(ws), nbytes, word)
 
 
 def _empty(rows: int, cols: int, dtype, dev):
@@ -228,10 +248,7 @@ def _grouped(x, w, plan, gather, out_dtype):
     y = _empty(R, N, out_dtype, dev)
     args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), plan.offsets.data_ptr(),
             plan.order.data_ptr() if gather else None, plan.top_k, R)
-    nbytes = L.lib().es_grouped_matmul_workspace_size(*args)
-    ws = _scratch(nbytes, dev)
-    _call("es_grouped_matmul", dev, *args, y.data_ptr(), _DTYPES[out_dtype], _ptr(ws), nbytes,
-          _STATUS.address("es_grouped_matmul", dev.index))
+    _product("es_grouped_matmul", dev, args, (y.data_ptr(), _DTYPES[out_dtype]), gather or code == L.ES_F32)
     return y
 
 
@@ -244,10 +261,7 @@ def _wgrad(x, dy, w, plan, gather):
     R, code = plan.num_rows, _DTYPES[x.dtype]
     args = (x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E, K, N, plan.offsets.data_ptr(),
             plan.order.data_ptr() if gather else None, plan.top_k, R, dw.data_ptr(), *dw.stride())
-    nbytes = L.lib().es_grouped_matmul_wgrad_workspace_size(*args)
-    ws = _scratch(nbytes, dev)
-    _call("es_grouped_matmul_wgrad", dev, *args, _ptr(ws), nbytes,
-          _STATUS.address("es_grouped_matmul_wgrad", dev.index))
+    _product("es_grouped_matmul_wgrad", dev, args, (), gather or code == L.ES_F32)
     return dw
 
 
@@ -427,10 +441,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     args = (q.data_ptr(), scale.data_ptr(), q.shape[0], q.stride(0), wq.data_ptr(), wscale.data_ptr(), E, K, N,
             wq.stride(0) if E else 0, wq.stride(-2), plan.offsets.data_ptr() if E else None,
             plan.order.data_ptr() if gather else None, plan.top_k if E else 1, R)
-    nbytes = L.lib().es_int8_matmul_workspace_size(*args)
-    ws = _scratch(nbytes, dev)
-    _call("es_int8_matmul", dev, *args, y.data_ptr(), code, _ptr(ws), nbytes,
-          _STATUS.address("es_int8_matmul", dev.index))
+    _product("es_int8_matmul", dev, args, (y.data_ptr(), code), gather)
     return y
 
 

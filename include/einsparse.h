@@ -418,7 +418,8 @@ int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride
                       int64_t K, int64_t N, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
                       const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, void* y,
                       int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
-/* dw[e] = sum over e's rows of x[row(r)]^T dy[r], with dw's element strides;
+/* dw[e] = sum over e's rows of x[row(r)]^T dy[r], with dw's element strides
+ * (that of K or of N is 1);
  * zero for an expert without rows. dw has the operands' type. */
 size_t es_grouped_matmul_wgrad_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride,
                                               const void* dy, int64_t dy_stride, int num_experts, int64_t K,
