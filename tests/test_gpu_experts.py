@@ -656,6 +656,19 @@ def test_expert_mlp():
     assert float((q.double() - ref.detach()).norm()) <= 0.03 * float(ref.detach().norm())
 
 
+def test_example_trains_and_serves():
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "expert_mlp.py")
+    spec = importlib.util.spec_from_file_location("expert_mlp_example", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    got = example.main(steps=60, tokens=300)
+    assert got["last"] < 0.7 * got["first"]
+    # as in test_expert_mlp: four operands in 8 bits, half a step of max / 127 each, and bf16 beside it
+    assert got["int8_off"] < 0.03
+
+
 def test_streams_and_graph():
     """Calls on another stream, and captured in a CUDA graph, give what they give on the default stream."""
     plan = make_plan([40, 0, 200, 16], 2)
