@@ -22,9 +22,10 @@
 // bf16). What TMA cannot read (odd addresses or strides) is copied too.
 //
 // fp32 operands are cut into three bf16 planes, x = b0 + b1 + b2 exactly. A
-// stage holds all planes of a block of depth, and the six products b_i b_j with
-// i + j <= 2 are made from it (each operand crosses from L2 once): b0 b0 into
-// one accumulator, the other five, at most 2^-8 of it, into a second. What is
+// block of depth takes three stages, one for each plane, and the six products
+// b_i b_j with i + j <= 2 are made from them (each operand crosses from L2
+// once): b0 b0 into one accumulator, the other five, at most 2^-8 of it, into a
+// second. What is
 // left out is at most 2^-24 of a product. An accumulator truncates each step's
 // sum (measured: a relative error of 1e-9 a unit of depth), so a sum is cut
 // into chains of 512 that the epilogue adds in fp32.
@@ -316,12 +317,6 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 
 // ------------------------------------------------------------------- kernel
 
-// Planes of the six products of fp32 operands: the last goes to the first
-// accumulator, the others, smallest first, to the second.
-constexpr int kTerms = 6;
-__host__ __device__ constexpr int term_a(int t) { return t == 0 ? 2 : t == 2 || t == 3 ? 1 : 0; }
-__host__ __device__ constexpr int term_b(int t) { return t == 1 ? 2 : t == 2 || t == 4 ? 1 : 0; }
-
 template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
 struct TcShape {
   static constexpr int CG = CG_;        // CTAs of one MMA
@@ -335,17 +330,15 @@ struct TcShape {
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
   static constexpr int kChain = PLANES > 1 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int kLanes = 128 * MT * CG;
-  static constexpr int kATiles = PLANES > 1 ? PLANES : MT;  // 128-lane tiles of A in a stage
   static constexpr int kAccs = PLANES > 1 ? 2 : MT;         // accumulators of a tile
   static constexpr int kBufs = 2 * kAccs * NT <= 512 ? 2 : 1;  // tiles in TMEM
   static constexpr bool kHeld = kBufs == 1 && PLANES == 1;  // tiles are held in registers, see drain_held
-  static constexpr int kBBytes = NT / CG * kSwizzleRow;        // of one plane
-  static constexpr int kStageBytes = kATiles * kABytes + PLANES * kBBytes;
+  static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;  // one plane of a block of depth
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
   static_assert(PLANES == 1 || MT == 1, "planes take the tiles that accumulators would share B with");
-  static_assert(kStages >= 2, "stages");
+  static_assert(kStages > PLANES, "a block's planes and the next block's first");
 };
 
 // One output tile, and what of its depth this CTA multiplies.
@@ -758,91 +751,81 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int boxes = (half + 63) / 64;
           if constexpr (S::WGRAD) {
             valid = min(at.depth - kb * BK, BK);
-            bytes = (2 * S::kATiles + PLANES * boxes) * ((valid + 15) & ~15) * 128u;
+            bytes = (2 * MT + boxes) * ((valid + 15) & ~15) * 128u;
           } else {
-            bytes = S::kATiles * kABytes + PLANES * ((half + kBoxRows - 1) / kBoxRows) * (kBoxRows * 128u);
+            bytes = MT * kABytes + (half + kBoxRows - 1) / kBoxRows * (kBoxRows * 128u);
           }
-          int go = 0;
-          if (lane == 0) {
-            go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
-            if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
-            if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
-          }
-          go = __shfl_sync(0xffffffffu, go, 0);
-          if (!go) {
-            ok = false;
-            break;
-          }
-          const uint32_t sa = base + stage * S::kStageBytes, sb = sa + S::kATiles * kABytes;
-          const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
-          // tile a of A: the next lanes, or the next plane
-          constexpr int next_lanes = PLANES > 1 ? 0 : 128 * CG, next_plane = PLANES > 1 ? 1 : 0;
-          if constexpr (S::WGRAD) {
-            // operand boxes of 64 lanes (columns) by 64 rows
-            const int row = at.first + kb * BK;
-            const int operands = 2 * S::kATiles + PLANES * boxes;
-            auto place = [&](int u, uint32_t& to, int& x, int& y) {
-              if (u < 2 * S::kATiles) {
-                const int a = u >> 1;
-                to = sa + u * 8192;
-                x = lane0 + a * next_lanes + (u & 1) * 64;
-                y = a * next_plane * p.plane_rows;
+          for (int plane = 0; plane < PLANES; ++plane) {
+            int go = 0;
+            if (lane == 0) {
+              go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+              if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], CG * bytes);
+              if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
+            }
+            go = __shfl_sync(0xffffffffu, go, 0);
+            if (!go) {
+              ok = false;
+              break;
+            }
+            const uint32_t sa = base + stage * S::kStageBytes, sb = sa + MT * kABytes;
+            const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
+            if constexpr (S::WGRAD) {
+              // operand boxes of 64 lanes (columns) by 64 rows
+              const int row = at.first + kb * BK + plane * p.plane_rows;
+              const int operands = 2 * MT + boxes;
+              auto place = [&](int u, uint32_t& to, int& x) {
+                if (u < 2 * MT) {
+                  to = sa + u * 8192;
+                  x = lane0 + (u >> 1) * 128 * CG + (u & 1) * 64;
+                } else {
+                  to = sb + (u - 2 * MT) * 8192;
+                  x = col0 + (u - 2 * MT) * 64;
+                }
+              };
+              uint32_t to;
+              int x;
+              if (valid == BK) {
+                if (lane < operands) {
+                  place(lane, to, x);
+                  load_2d<CG>(to, lane < 2 * MT ? &m.a : &m.b, x, row, bar);
+                }
               } else {
-                const int plane = (u - 2 * S::kATiles) / boxes, box = u - 2 * S::kATiles - plane * boxes;
-                to = sb + plane * S::kBBytes + box * 8192;
-                x = col0 + box * 64;
-                y = plane * p.plane_rows;
-              }
-            };
-            uint32_t to;
-            int x, y;
-            if (valid == BK) {
-              if (lane < operands) {
-                place(lane, to, x, y);
-                load_2d<CG>(to, lane < 2 * S::kATiles ? &m.a : &m.b, x, row + y, bar);
+                // the last block: whole steps of 16 rows, then the rest by
+                // gathers of four rows (which cost as much as a box each)
+                const int full = valid >> 4, rest = valid & 15;
+                for (int i = lane; i < operands * full; i += 32) {
+                  const int u = i / full, s = i - u * full;
+                  place(u, to, x);
+                  load_2d<CG>(to + s * 2048, u < 2 * MT ? &m.a_steps : &m.b_steps, x, row + s * 16, bar);
+                }
+                for (int i = lane; i < (rest ? operands * 4 : 0); i += 32) {
+                  const int u = i >> 2, q = i & 3;
+                  place(u, to, x);
+                  int r[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) r[j] = q * 4 + j < rest ? row + full * 16 + q * 4 + j : p.src_rows;
+                  load_rows<CG>(to + full * 2048 + q * 512, u < 2 * MT ? &m.a_rows : &m.b_rows, x, r, bar);
+                }
               }
             } else {
-              // the last block: whole steps of 16 rows, then the rest by
-              // gathers of four rows (which cost as much as a box each)
-              const int full = valid >> 4, rest = valid & 15;
-              for (int i = lane; i < operands * full; i += 32) {
-                const int u = i / full, s = i - u * full;
-                place(u, to, x, y);
-                load_2d<CG>(to + s * 2048, u < 2 * S::kATiles ? &m.a_steps : &m.b_steps, x, row + s * 16 + y, bar);
+              const int z = at.expert * p.expert_step + plane * p.plane_experts;
+              if constexpr (S::A_MN) {
+                if (lane < 2 * MT)
+                  load_3d<CG>(sa + lane * 8192, &m.a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
+                              bar);
+              } else {
+                if (lane < MT) load_3d<CG>(sa + lane * kABytes, &m.a, kb * BK, lane0 + lane * 128 * CG, z, bar);
               }
-              for (int i = lane; i < (rest ? operands * 4 : 0); i += 32) {
-                const int u = i >> 2, q = i & 3;
-                place(u, to, x, y);
-                int r[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  r[j] = q * 4 + j < rest ? row + full * 16 + q * 4 + j + y : p.src_rows;
-                load_rows<CG>(to + full * 2048 + q * 512, u < 2 * S::kATiles ? &m.a_rows : &m.b_rows, x, r, bar);
-              }
-            }
-          } else {
-            const int z = at.expert * p.expert_step;
-            if constexpr (S::A_MN) {
-              if (lane < 2 * S::kATiles) {
-                const int a = lane >> 1;
-                load_3d<CG>(sa + lane * 8192, &m.a, lane0 + a * next_lanes + (lane & 1) * 64, kb * BK,
-                            z + a * next_plane * p.plane_experts, bar);
-              }
-            } else {
-              if (lane < S::kATiles)
-                load_3d<CG>(sa + lane * kABytes, &m.a, kb * BK, lane0 + lane * next_lanes,
-                            z + lane * next_plane * p.plane_experts, bar);
-            }
-            if (lane * kBoxRows < half)
-#pragma unroll
-              for (int plane = 0; plane < PLANES; ++plane)
-                load_2d<CG>(sb + plane * S::kBBytes + lane * (kBoxRows * 128), &m.b, kb * BK,
+              if (lane * kBoxRows < half)
+                load_2d<CG>(sb + lane * (kBoxRows * 128), &m.b, kb * BK,
                             col0 + lane * kBoxRows + plane * p.plane_rows, bar);
+            }
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
           }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (!ok) break;
         }
       }
       if (lane == 0) {
@@ -881,29 +864,48 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             const uint32_t d = tmem + buf * S::kAccs * NT;
             uint32_t more = 0;
+            constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
             for (int kb = s0; kb < s1; ++kb) {
+              int steps = 4;
+              if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
+              auto product = [&](int sa, int sb, int acc, uint32_t old) {  // of the tiles in stages sa and sb
+                const uint64_t da = operand(base + sa * S::kStageBytes, S::A_MN);
+                const uint64_t db = operand(base + sb * S::kStageBytes + MT * kABytes, S::WGRAD);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (i < steps)
+                      mma<CG, S::KIND>(d + (acc + m) * NT, da + m * (kABytes >> 4) + i * step_a, db + i * step_b,
+                                       idesc, old | i);
+              };
+              auto next = [&](int s) { return s + 1 == STAGES ? 0 : s + 1; };
               ok = tc_wait_warp(&ctl.full[stage], phase, &ctl, p.status);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t sa = base + stage * S::kStageBytes;
-              const uint64_t da = operand(sa, S::A_MN), db = operand(sa + S::kATiles * kABytes, S::WGRAD);
-              constexpr uint64_t step_a = (S::A_MN ? 2048 : 32) >> 4, step_b = (S::WGRAD ? 2048 : 32) >> 4;
-              int steps = 4;
-              if constexpr (S::WGRAD) steps = (min(at.depth - kb * BK, BK) + 15) >> 4;
-              constexpr int products = PLANES > 1 ? kTerms : MT;
-#pragma unroll
-              for (int m = 0; m < products; ++m) {
-                const int a = PLANES > 1 ? term_a(m) : m, b = PLANES > 1 ? term_b(m) : 0;
-                const int acc = PLANES > 1 ? (m < kTerms - 1 ? 1 : 0) : m;
-                const uint32_t old = PLANES > 1 && m > 0 && m < kTerms - 1 ? 1 : more;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (i < steps)
-                    mma<CG, S::KIND>(d + acc * NT, da + a * (kABytes >> 4) + i * step_a,
-                                     db + b * (S::kBBytes >> 4) + i * step_b, idesc, old | i);
+              product(stage, stage, 0, more);
+              if constexpr (PLANES == 1) {
+                commit<CG>(&ctl.empty[stage]);
+              } else {
+                const int s1st = next(stage), s2nd = next(s1st);
+                ok = tc_wait_warp(&ctl.full[s1st], phase ^ (s1st < stage ? 1 : 0), &ctl, p.status);
+                if (!ok) break;
+                tc_fence_after();
+                product(stage, s1st, 1, more);
+                product(s1st, stage, 1, 1);
+                product(s1st, s1st, 1, 1);
+                commit<CG>(&ctl.empty[s1st]);
+                ok = tc_wait_warp(&ctl.full[s2nd], phase ^ (s2nd < stage ? 1 : 0), &ctl, p.status);
+                if (!ok) break;
+                tc_fence_after();
+                product(stage, s2nd, 1, 1);
+                product(s2nd, stage, 1, 1);
+                commit<CG>(&ctl.empty[stage]);
+                commit<CG>(&ctl.empty[s2nd]);
+                if (s2nd < stage) phase ^= 1;
+                stage = s2nd;
               }
               more = 1;
-              commit<CG>(&ctl.empty[stage]);
               if (++stage == STAGES) {
                 stage = 0;
                 phase ^= 1;
