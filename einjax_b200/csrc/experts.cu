@@ -1,6 +1,6 @@
 // Routing of tokens to experts, the row order of the routed choices, the
 // weighted sum of the experts' rows back to tokens, and the 8-bit rounding of
-// token rows. The products between routing and sum are in grouped.cu.
+// token rows. The products between routing and sum are in grouped_tc.cu.
 //
 // T tokens choose k of E experts each; choice a = t * k + j. Row r of the
 // grouped order holds choice order[r]; expert e owns rows offsets[e] to
@@ -21,13 +21,14 @@ constexpr unsigned kFull = 0xffffffffu;
 // ------------------------------------------------------------------ routing
 //
 // One warp per token, the token's logits in registers (lane l holds experts
-// l, l + 32, ...). The k largest are found one after the other: a local
-// maximum, one warp reduction of the order-preserving bits, one of the lowest
+// l, l + 32, ...). The k largest are found one after the other: each lane's
+// largest, one warp reduction of the order-preserving bits, one of the lowest
 // index among equals. With m the largest logit, w_j = exp(l_j - m) / sum,
 // where the sum runs over the chosen (renorm) or over all experts. -inf is a
 // masked expert and is never chosen. NaN is never chosen either, and makes
-// every weight of its token NaN. Bound by launch latency for decode steps and
-// by the selection's reductions (2 per choice and warp) for long prompts.
+// every weight of its token NaN. Bound by launch latency for decode steps (3 us)
+// and by the selection's instructions for long prompts: 32768 tokens, 128
+// experts, k 8 take 18 us, the 17 MB of logits alone 2.6 us.
 
 // Bits whose unsigned order is the order of the floats; 0 for -inf and NaN.
 // x + 0 makes -0 equal to +0, so that ties go by index alone.
@@ -209,7 +210,8 @@ int route_typed(const void* logits, int64_t T_, int E, int64_t stride, int k, in
 // (kPlanDirect); else a launch in between does that for all. Within a CTA each
 // warp owns a consecutive run of choices, 32 at a time; a choice's rank is the
 // warp's earlier choices of the same expert (match + popcount), so the order
-// never depends on the schedule. Bound by latency: each choice is read once.
+// never depends on the schedule. Bound by latency: each choice is read once, and
+// 262144 choices of 128 experts take three launches of 4, 3 and 8 us.
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
@@ -372,8 +374,9 @@ size_t plan_smem(int E) { return static_cast<size_t>(kPlanWarps + 2) * (E + 1) *
 //
 // out_t = sum_j w_tj y_pos(t,j), in fp32, rounded once. Backward in one pass:
 // dy_pos(t,j) = w_tj dout_t and dw_tj = <dout_t, y_pos(t,j)>. Both are bound
-// by memory: every row is read (and written) once, in 16-byte pieces, by TP
-// threads per token; all the token's rows are in flight together.
+// by memory: every row is read (and written) once, in 16-byte pieces, by tp
+// threads a token (16384 x 4 rows of 4096 bf16: 105 us and 182 us, 6.4 and 6.6
+// TB/s of their bytes).
 
 template <typename T, int VEC>
 struct alignas(VEC * sizeof(T)) Piece {
@@ -585,8 +588,8 @@ int combine_grad_typed(const void* y, int64_t rows, int64_t stride, const float*
 // scale_t = max_i |x_ti| / 127 (one division rounded to nearest), q_ti =
 // rint(x_ti / scale_t), kept within +-127. A row of zeros has scale 0 and q 0;
 // a row with an infinity or NaN has scale NaN, so that its products are NaN
-// and not a finite guess. Bound by memory: a row is read once and its 8-bit
-// copy written once.
+// and not a finite guess. A row is read once and its 8-bit copy written once:
+// 8191 x 4096 bf16 take 27 us, 3.7 TB/s, between memory and the conversions.
 
 constexpr int kQuantThreads = 256;
 

@@ -14,7 +14,9 @@ constexpr int kMaxTopK = 32;
 // Programmatic dependent launch: the next kernel of the stream, if it was
 // launched for it, may start before this one is done; it waits for the earlier
 // ones' results before it touches memory.
-__device__ __forceinline__ void let_next_grid_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void let_next_grid_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void wait_for_earlier_grids() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float to_f32(float x) { return x; }

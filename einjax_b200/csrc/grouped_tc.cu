@@ -25,16 +25,24 @@
 // block of depth takes three stages, one for each plane, and the six products
 // b_i b_j with i + j <= 2 are made from them (each operand crosses from L2
 // once): b0 b0 into one accumulator, the other five, at most 2^-8 of it, into a
-// second. What is
-// left out is at most 2^-24 of a product. An accumulator truncates each step's
-// sum (measured: a relative error of 1e-9 a unit of depth), so a sum is cut
-// into chains of 512 that the epilogue adds in fp32.
+// second. What is left out is at most 2^-24 of a product. An accumulator
+// truncates each step's sum (measured: a relative error of 1e-9 a unit of
+// depth), so a sum is cut into chains of 512 that the epilogue adds in fp32; a
+// 16-bit result, rounded at 2^-9, keeps one chain.
+//
+// Bounds (B200, measured): 16384 rows, 8 experts, 4096 x 8192, bf16 759 us
+// forward, the tensor pipe 84% active (on equal groups 88%, as cuBLAS's product
+// of that size); 60 experts of 2048 x 2816 with 69 rows each 115 us, 6.2 TB/s of
+// HBM; 16 rows over 16 experts of 2048 x 4096 30 us, 5.0 TB/s; 8 bits, 8191 x
+// 4096 x 8192 184 us, 3.0 POP/s; fp32, 3000 rows, 16 experts, 1000 x 2024 98 us
+// without the planes' 59 us. Before the 512 x 256 tile a long group's bound was
+// the L2's bandwidth to the SMs (64 bytes a clock and SM for 256 x 256).
 //
 // Roles (12 warps): warp 0 issues the TMA loads, warp 1 the MMAs (an elected
 // lane), warps 2-3 clear the output rows of no expert, warps 4-11 read the
 // accumulators (TMEM lane quadrant = warp % 4) and write the output. Tiles are
-// dealt to the CTAs in turn; the accumulator is double buffered, so a tile's
-// epilogue runs under the next tile's MMAs. Every wait is bounded: when one
+// dealt to the CTAs in turn; where two tiles fit TMEM a tile's epilogue runs
+// under the next tile's MMAs (else see drain_held). Every wait is bounded: when one
 // runs out the CTA sets ES_ERR_TIMEOUT, drains its copies and MMAs, frees
 // TMEM and returns.
 #include <cuda.h>

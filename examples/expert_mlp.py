@@ -62,4 +62,5 @@ if __name__ == "__main__":
     parser = argparse.ArgumentParser(description=__doc__)
     parser.add_argument("--steps", type=int, default=200)
     result = main(parser.parse_args().steps)
-    print(f"loss {result['first']:.4f} -> {result['last']:.4f}; 8-bit outputs differ by {100 * result['int8_off']:.2f}%")
+    print(f"loss {result['first']:.4f} -> {result['last']:.4f}; "
+          f"8-bit outputs differ by {100 * result['int8_off']:.2f}%")

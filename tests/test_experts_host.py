@@ -9,7 +9,8 @@ from einjax_b200 import _lib as L
 FAKE = 1 << 20  # an aligned address that is never read
 
 
-def rows_args(K=64, N=128, dtype=L.ES_BF16, x=FAKE, w=FAKE, x_stride=None, order=None, strides=None, experts=4, rows=100):
+def rows_args(K=64, N=128, dtype=L.ES_BF16, x=FAKE, w=FAKE, x_stride=None, order=None, strides=None, experts=4,
+              rows=100):
     x_rows = rows if order is None else 50
     se, sk, sn = strides or (K * N, N, 1)
     return (x, dtype, x_rows, x_stride or K, w, experts, K, N, se, sk, sn, FAKE, order, 2, rows)
