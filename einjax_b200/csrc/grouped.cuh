@@ -8,8 +8,8 @@
 
 namespace es {
 
-// |sum| <= 127^2 K stays inside int32
-constexpr int64_t kMaxInt8Depth = 133152;
+// |sum| <= 128^2 K stays inside int32
+constexpr int64_t kMaxInt8Depth = 131071;
 
 struct GroupedArgs {
   int num_experts;  // 0: one group of all rows

@@ -24,7 +24,7 @@ import torch
 from . import _lib as L
 from .sparse import _STATUS, _raw_stream
 
-MAX_EXPERTS, MAX_TOP_K, MAX_INT8_DEPTH = 1024, 32, 133152
+MAX_EXPERTS, MAX_TOP_K, MAX_INT8_DEPTH = 1024, 32, 131071
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -412,7 +412,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     ``plan`` the products are grouped by expert as in ``grouped_matmul``:
     ``wq`` (num_experts, N, K), ``wscale`` (num_experts, N), and with
     ``gather`` ``q`` and ``scale`` are by token. Returns (rows, N) of
-    ``out_dtype`` (float32, bfloat16, float16). K is at most 133,152."""
+    ``out_dtype`` (float32, bfloat16, float16). K is at most 131,071."""
     _on_gpu("int8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=q if plan is None else plan.offsets)
     code = _code("int8_matmul", "out_dtype", out_dtype)
     if q.dtype != torch.int8 or wq.dtype != torch.int8:

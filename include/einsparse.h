@@ -453,7 +453,7 @@ int es_quantize_rows(const void* x, int dtype, int64_t num_rows, int64_t width, 
                      float* scale, void* stream);
 
 /* y[r, n] = x_scale[row(r)] w_scale[e(r), n] sum_k q[row(r), k] wq[e(r), n, k],
- * the sum exact in 32-bit integers (K <= 133152). wq: (num_experts, N, K) int8
+ * the sum exact in 32-bit integers (K <= 131071). wq: (num_experts, N, K) int8
  * with contiguous k, w_scale (num_experts, N). num_experts == 0: one matrix
  * for all rows (offsets and order NULL). y (num_rows, N) contiguous. */
 size_t es_int8_matmul_workspace_size(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,

@@ -261,6 +261,28 @@ def test_grouped(sizes, K, N, dtype, gather):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_many_experts(dtype):
+    """As many experts as there may be, most of them without rows."""
+    sizes = [0] * 1024
+    sizes[3], sizes[500], sizes[501], sizes[1023] = 5, 40, 1, 18
+    plan = make_plan(sizes, 2)
+    g = gen(14)
+    x = randn(g, plan.num_tokens, 40, dtype=dtype).requires_grad_()
+    w = randn(g, 1024, 40, 24, dtype=dtype).requires_grad_()
+    dy = randn(g, plan.num_rows, 24, dtype=dtype)
+    y = E.grouped_matmul(x, w, plan, gather=True)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    ry, my, rx, mx, rw, mw = grouped_ref(x, w, plan, True, dy)
+    near(y.detach(), ry, my, 40, dtype)
+    near(dx, rx, mx, 24 + 2, dtype)
+    near(dw, rw, mw, 40, dtype)
+    wq, ws = E.quantize_experts(w)
+    q, s = E.quantize_rows(x)
+    check_int8(E.int8_matmul(q, s, wq, ws, plan, gather=True, out_dtype=dtype),
+               int8_ref(q, s, wq, ws, plan, True), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_long(dtype):
     """Depths where a sum's own rounding shows, and more tiles than SMs."""
     plan = make_plan([700, 33, 0, 1400, 5, 301], 1, dropped=3)
@@ -278,7 +300,8 @@ def test_grouped_long(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("layout", ["transposed", "sliced", "padded", "strided", "offset", "broadcast"])
+@pytest.mark.parametrize("layout", ["transposed", "sliced", "padded", "strided", "offset", "broadcast", "permuted",
+                                    "turned"])
 def test_grouped_layouts(dtype, layout):
     """Weights and rows that lie otherwise in memory give what their copies give."""
     plan = make_plan([5, 130, 0, 64], 1)
@@ -297,6 +320,10 @@ def test_grouped_layouts(dtype, layout):
     elif layout == "offset":  # a base address that no 16-byte load may start at
         w = randn(g, 4 * K * N + 1, dtype=dtype)[1:].reshape(4, K, N)
         x = randn(g, n * K + 1, dtype=dtype)[1:].reshape(n, K)
+    elif layout == "permuted":  # the experts' matrices interleaved row by row
+        w = randn(g, K, 4, N, dtype=dtype, scale=K ** -0.5).transpose(0, 1)
+    elif layout == "turned":  # the experts innermost
+        w = randn(g, K, N, 4, dtype=dtype, scale=K ** -0.5).permute(2, 0, 1)
     else:
         w, x = w[:1].expand(4, K, N), x[:1].expand(n, K)
     x.requires_grad_()
@@ -573,6 +600,21 @@ def test_int8_grouped(sizes, K, N, gather):
         y = E.int8_matmul(q, s * 2.0 ** -12, wq, ws, plan, gather=gather, out_dtype=dtype)
         check_int8(y, int8_ref(q, s * 2.0 ** -12, wq, ws, plan, gather), dtype)
     E.check_device_errors()
+
+
+def test_int8_deepest():
+    """The largest sums that 32-bit integers hold, and one step more, which is refused."""
+    K = 131071
+    for depth in (K, K - 15):  # odd rows are laid out anew, the others read as they lie
+        q = torch.full((3, depth), -128, dtype=torch.int8, device=DEV)
+        wq = torch.full((17, depth), -128, dtype=torch.int8, device=DEV)
+        q[1], wq[5] = 127, 127
+        one = torch.ones(17, device=DEV)
+        y = E.int8_matmul(q, one[:3], wq, one, out_dtype=torch.float32)
+        check_int8(y, int8_ref(q, one[:3], wq, one, None, False), torch.float32)
+    q = torch.zeros(1, K + 1, dtype=torch.int8, device=DEV)
+    with pytest.raises(ValueError):
+        E.int8_matmul(q, torch.ones(1, device=DEV), q, torch.ones(1, device=DEV))
 
 
 def test_int8_layouts():
