@@ -1,8 +1,9 @@
 // Entry points of the products grouped by expert: checks of arguments, and the
 // cases that have no product (no depth, no rows). The kernels are in
-// grouped_tc.cu. A first form on the CUDA cores was right for every case and is
-// gone: with operands that TMA cannot read copied first, the tensor cores were
-// faster for all but products of some 2^18 steps, and there by 2 us.
+// grouped_tc.cu, and in grouped_few.cu for fp32 groups of a few rows. A first,
+// general form on the CUDA cores is gone: with operands that TMA cannot read
+// copied first, the tensor cores were faster for all but products of some 2^18
+// steps, and there slower by 2 us.
 #include "experts.cuh"
 #include "grouped.cuh"
 
@@ -55,7 +56,8 @@ extern "C" size_t es_grouped_matmul_workspace_size(const void* x, int dtype, int
                                                    int64_t num_rows) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
                       w_k_stride, w_n_stride, nullptr, nullptr};
-  return check_args(g) == ES_OK && !empty(g) ? grouped_rows_tc_workspace(g, dtype, x, w) : 0;
+  if (check_args(g) != ES_OK || empty(g) || grouped_rows_few_ok(g, dtype, w)) return 0;
+  return grouped_rows_tc_workspace(g, dtype, x, w);
 }
 
 extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
@@ -72,6 +74,7 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
   if (!y || (K && ((x_rows && !x) || !w))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
   if (empty(g)) return clear_rows_of(g, y, out_dtype, s);
+  if (grouped_rows_few_ok(g, dtype, w)) return grouped_rows_few(g, x, w, y, s);
   if (!grouped_rows_tc_ok(g, dtype)) return ES_ERR_UNSUPPORTED;
   if (workspace_bytes < grouped_rows_tc_workspace(g, dtype, x, w)) return ES_ERR_WORKSPACE;
   return grouped_rows_tc(g, dtype, x, w, y, out_dtype, workspace, status, s);

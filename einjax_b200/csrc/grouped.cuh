@@ -51,6 +51,10 @@ struct GroupedArgs {
 
 constexpr int kInt8 = 0x100;  // operand type of the 8-bit product
 
+// The fp32 rows' product for groups of a few rows (grouped_few.cu): no workspace.
+bool grouped_rows_few_ok(const GroupedArgs& g, int dtype, const void* w);
+int grouped_rows_few(const GroupedArgs& g, const void* x, const void* w, void* y, cudaStream_t stream);
+
 // Tensor-core forms (grouped_tc.cu). The workspace holds copies of what TMA
 // cannot read as it lies.
 bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype);

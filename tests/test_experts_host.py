@@ -27,6 +27,8 @@ def test_workspace_sizes():
     assert size(*rows_args(strides=(2 * 64 * 128, 256, 2))) >= 4 * 64 * 128 * 2
     assert size(*rows_args(strides=(0, 128, 1))) == 0                 # one matrix for all experts
     assert size(*rows_args(dtype=L.ES_F32)) >= 3 * 2 * (100 * 64 + 4 * 64 * 128)
+    assert size(*rows_args(dtype=L.ES_F32, rows=20)) == 0             # few rows: read where they lie
+    assert size(*rows_args(dtype=L.ES_F32, rows=20, w=FAKE + 4)) > 0
     assert size(*rows_args(K=0)) == 0 and size(*rows_args(rows=0)) == 0
     plan = lib.es_expert_plan_workspace_size
     assert plan(100, 8) == 0 and plan(1 << 20, 8) > 0 and plan(1 << 20, 1024) > plan(1 << 20, 8)

@@ -234,6 +234,7 @@ SIZES = {
     "edges": [16, 31, 32, 33, 64, 65, 127, 1],
     "big": [300, 1, 0, 511, 129, 257, 0, 2],
     "last": [0, 0, 0, 260],
+    "uneven": [30, 0, 0, 0, 1, 2, 0, 9],
 }
 
 
@@ -258,6 +259,27 @@ def test_grouped(sizes, K, N, dtype, gather):
     kept = sum(s)
     assert not y[kept:].any()
     E.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes", [[1], [1, 4, 0, 5, 8, 9], [0, 0, 25, 0, 0, 0]])
+@pytest.mark.parametrize("K,N", [(2100, 132), (1028, 1000), (1024, 64), (4, 4), (2052, 20)])
+def test_grouped_few_rows(dtype, sizes, K, N):
+    """Groups of a few rows, depths past a chunk, both orders of the weights."""
+    plan = make_plan(sizes, 1, dropped=2)
+    g = gen(K + N)
+    x = randn(g, plan.num_tokens, K, dtype=dtype).requires_grad_()
+    w = randn(g, len(sizes), K, N, dtype=dtype, scale=K ** -0.5)
+    dy = randn(g, plan.num_rows, N, dtype=dtype)
+    for v in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        v = v.detach().requires_grad_()
+        y = E.grouped_matmul(x, v, plan, gather=True)
+        dx, dw = torch.autograd.grad(y, (x, v), dy)
+        ry, my, rx, mx, rw, mw = grouped_ref(x, v, plan, True, dy)
+        near(y.detach(), ry, my, K, dtype)
+        near(dx, rx, mx, N + 1, dtype)
+        near(dw, rw, mw, max(sizes), dtype)
+        assert not y[sum(sizes):].any()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
