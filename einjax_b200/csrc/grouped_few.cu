@@ -4,9 +4,10 @@
 // the weights' bytes: at HBM's rate an SM gets 6 fp32 weights a clock, 8 rows of
 // which are 47 of its 128 multiply-adds.
 //
-// A CTA makes the columns of one tile for one expert's rows, RT (4 or 8) at a
-// time, in chunks of kChunk of the depth, whose part of x is staged in shared
-// memory. Every lane has eight 16-byte loads of weights in flight.
+// A CTA makes a tile of columns for up to RT (4 or 8) rows of one expert, in
+// chunks of kChunk of the depth, whose part of x is staged in shared memory. Every
+// lane has eight 16-byte loads of weights in flight. A longer group is several
+// CTAs' that meet in L2, so a step whose rows all chose one expert fills the SMs.
 //
 // Columns contiguous (forward): a lane owns four columns, the half warps share
 // the depth and their sums are added in the end. Depth contiguous (the gradient
@@ -26,44 +27,51 @@ constexpr int kChunk = 1024;
 constexpr int kWarpCols = 4;  // columns of a warp, depth contiguous
 constexpr int kTileCols = 64;  // columns of a CTA, columns contiguous
 constexpr int kFewRows = 8;
-// Rows of a group up to which this is taken. 36 experts of 2520 x 1456, us here
-// and on the tensor cores (which read the weights' planes after writing them):
-// columns contiguous 69 and 241 at 1 row, 159 and 339 at 4, 213 and 340 at 8, 444
-// and 345 at 16; depth contiguous 81 and 243, 169 and 345, 259 and 346, 519 and
-// 351. The weights alone take 52 us at 1 row (23 experts in use) and 81 from 4.
-constexpr int64_t kFewMean = 8;
+// Rows of a group (the mean) up to which this is taken. 36 experts of 2520 x 1456,
+// rows spread by chance, us here and on the tensor cores (which read the weights'
+// planes after writing them): columns contiguous 70 and 241 at 1 row, 125 and 339
+// at 4, 196 and 340 at 8, 242 and 343 at 12, 292 and 345 at 16, 406 and 349 at 24;
+// depth contiguous 83 and 243, 153 and 345, 248 and 346, 327 and 350, 409 and 353
+// (121 experts of 1136 x 728: 245 and 280 at 9 rows, 306 and 286 at 12). The
+// weights alone take 52 us at 1 row (23 experts in use) and 81 from 4. Where all
+// rows chose one expert: 129 and 188 us at a mean of 8, 241 at 16 (tensor cores 147).
+constexpr int64_t kColumnsMean = 16, kDepthMean = 10;
 
-// The n-th expert that has rows; false: there is none.
-__device__ __forceinline__ bool nth_group(const GroupedArgs& g, int n, int& expert, int64_t& lo, int64_t& hi) {
+// The n-th tile of up to kFewRows rows of one expert; false: there is none.
+__device__ __forceinline__ bool nth_tile(const GroupedArgs& g, int n, int& expert, int64_t& r0, int64_t& hi) {
   __shared__ int64_t found[3];
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int at = -1, seen = 0;
-    int64_t a = 0, b = 0;
+    int64_t at = -1, a = 0, b = 0, seen = 0;
     for (int e0 = 0; e0 < g.groups() && at < 0; e0 += 32) {
       int64_t l = 0, h = 0;
       if (e0 + lane < g.groups()) g.bounds(e0 + lane, l, h);
-      const unsigned live = __ballot_sync(0xffffffffu, h > l);
-      const int here = __popc(live);
-      if (n < seen + here) {
-        const unsigned before = __popc(live & ((1u << lane) - 1));
-        const unsigned mine = __ballot_sync(0xffffffffu, h > l && static_cast<int>(before) == n - seen);
+      const int64_t tiles = h > l ? (h - l + kFewRows - 1) / kFewRows : 0;
+      int64_t past = tiles;  // tiles of the lanes up to this one
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t before = __shfl_up_sync(0xffffffffu, past, o);
+        if (lane >= o) past += before;
+      }
+      past += seen;
+      const unsigned mine = __ballot_sync(0xffffffffu, n < past && n >= past - tiles);
+      if (mine) {
         const int src = __ffs(mine) - 1;
         at = e0 + src;
-        a = __shfl_sync(0xffffffffu, l, src);
+        a = __shfl_sync(0xffffffffu, l + (n - (past - tiles)) * kFewRows, src);
         b = __shfl_sync(0xffffffffu, h, src);
       }
-      seen += here;
+      seen = __shfl_sync(0xffffffffu, past, 31);
     }
     if (lane == 0) {
       found[0] = at;
       found[1] = a;
-      found[2] = b;
+      found[2] = min(b, a + kFewRows);
     }
   }
   __syncthreads();
   expert = static_cast<int>(found[0]);
-  lo = found[1];
+  r0 = found[1];
   hi = found[2];
   return expert >= 0;
 }
@@ -85,6 +93,7 @@ template <int RT>
 __device__ __forceinline__ void columns_tile(const GroupedArgs& g, const float* x, const float* we, float* y,
                                              int64_t n0, int64_t r0, int64_t hi, float* buffer, int64_t* src) {
   constexpr int AHEAD = 8, SHARES = 2 * kFewWarps;
+  static_assert(kChunk % (AHEAD * SHARES) == 0, "reads of x past the depth stay in the chunk");
   const int share = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const bool live = n0 + lane * 4 < g.N;
   load_sources<RT>(g, r0, hi, src);
@@ -96,10 +105,11 @@ __device__ __forceinline__ void columns_tile(const GroupedArgs& g, const float* 
     __syncthreads();
     for (int i = threadIdx.x; i < RT * kChunk; i += kFewThreads) {  // x[depth][row]
       const int r = i / kChunk, k = i % kChunk;
-      if (k < depth) buffer[k * RT + r] = src[r] >= 0 ? x[src[r] * g.x_stride + k0 + k] : 0.0f;
+      buffer[k * RT + r] = k < depth && src[r] >= 0 ? x[src[r] * g.x_stride + k0 + k] : 0.0f;
     }
     __syncthreads();
-    const int per = (depth + SHARES - 1) / SHARES, k1 = min(depth, (share + 1) * per);
+    const int per = ((depth + SHARES - 1) / SHARES + AHEAD - 1) / AHEAD * AHEAD;
+    const int k1 = min(depth, (share + 1) * per);
     if (!live) continue;
     for (int k = share * per; k < k1; k += AHEAD) {
       float4 p[AHEAD];
@@ -109,7 +119,7 @@ __device__ __forceinline__ void columns_tile(const GroupedArgs& g, const float* 
                           : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const float* xr = buffer + min(k + u, k1 - 1) * RT;
+        const float* xr = buffer + (k + u) * RT;  // past the depth both factors are zeros
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           acc[r].x = fmaf(xr[r], p[u].x, acc[r].x);
@@ -143,18 +153,20 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_columns_kernel(const __gri
   const int64_t n0 = blockIdx.x * static_cast<int64_t>(kTileCols);
   clear_columns(g, y, n0, min(n0 + kTileCols, g.N));
   int e;
-  int64_t lo, hi;
-  if (!nth_group(g, blockIdx.y, e, lo, hi)) return;
+  int64_t r0, hi;
+  if (!nth_tile(g, blockIdx.y, e, r0, hi)) return;
   const float* we = w + e * g.w_e + n0;
-  int64_t r0 = lo;
-  for (; hi - r0 > 4; r0 += 8) columns_tile<8>(g, x, we, y, n0, r0, hi, buffer, src);
-  if (r0 < hi) columns_tile<4>(g, x, we, y, n0, r0, hi, buffer, src);
+  if (hi - r0 > 4)
+    columns_tile<kFewRows>(g, x, we, y, n0, r0, hi, buffer, src);
+  else
+    columns_tile<4>(g, x, we, y, n0, r0, hi, buffer, src);
 }
 
 template <int RT>
 __device__ __forceinline__ void depth_tile(const GroupedArgs& g, const float* x, const float* we, float* y, int64_t n,
                                            int64_t r0, int64_t hi, float* buffer, int64_t* src) {
   constexpr int AHEAD = 2;
+  static_assert(kChunk % (128 * AHEAD) == 0, "reads of x past the depth stay in the chunk");
   const int lane = threadIdx.x & 31;
   load_sources<RT>(g, r0, hi, src);
   float acc[RT][kWarpCols];
@@ -183,8 +195,8 @@ __device__ __forceinline__ void depth_tile(const GroupedArgs& g, const float* x,
       for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const int at = min(k + u * 128, kChunk - 4);  // past the depth the weights are zeros
-          const float4 xv = *reinterpret_cast<const float4*>(buffer + r * kChunk + at);
+          // past the depth both factors are zeros
+          const float4 xv = *reinterpret_cast<const float4*>(buffer + r * kChunk + k + u * 128);
 #pragma unroll
           for (int c = 0; c < kWarpCols; ++c) {
             acc[r][c] = fmaf(xv.x, p[u][c].x, acc[r][c]);
@@ -214,12 +226,13 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_depth_kernel(const __grid_
   const int64_t n0 = blockIdx.x * static_cast<int64_t>(COLS), n = n0 + (threadIdx.x >> 5) * kWarpCols;
   clear_columns(g, y, n0, min(n0 + COLS, g.N));
   int e;
-  int64_t lo, hi;
-  if (!nth_group(g, blockIdx.y, e, lo, hi)) return;
+  int64_t r0, hi;
+  if (!nth_tile(g, blockIdx.y, e, r0, hi)) return;
   const float* we = w + e * g.w_e + n * g.w_n;
-  int64_t r0 = lo;
-  for (; hi - r0 > 4; r0 += 8) depth_tile<8>(g, x, we, y, n, r0, hi, buffer, src);
-  if (r0 < hi) depth_tile<4>(g, x, we, y, n, r0, hi, buffer, src);
+  if (hi - r0 > 4)
+    depth_tile<kFewRows>(g, x, we, y, n, r0, hi, buffer, src);
+  else
+    depth_tile<4>(g, x, we, y, n, r0, hi, buffer, src);
 }
 
 bool by_columns(const GroupedArgs& g) { return g.w_n == 1 && g.N > 1; }
@@ -236,14 +249,16 @@ bool grouped_rows_few_ok(const GroupedArgs& g, int dtype, const void* w) {
   if ((reinterpret_cast<uintptr_t>(w) & 15) != 0 || inner % 4 != 0 || (rows > 1 && row % 4 != 0) ||
       (g.num_experts > 1 && g.w_e % 4 != 0))
     return false;
-  return g.rows / live <= kFewMean;
+  return g.rows <= live * (columns ? kColumnsMean : kDepthMean);
 }
 
 int grouped_rows_few(const GroupedArgs& g, const void* x, const void* w, void* y, cudaStream_t s) {
   const bool columns = by_columns(g);
   const int64_t cols = columns ? kTileCols : kFewWarps * kWarpCols;
+  // groups of n rows have at most this many tiles: one begun by each live group, the others full
   const int64_t live = min(static_cast<int64_t>(g.num_experts), g.rows);
-  const dim3 grid(static_cast<unsigned>((g.N + cols - 1) / cols), static_cast<unsigned>(live));
+  const int64_t tiles = live + (g.rows - live) / kFewRows;
+  const dim3 grid(static_cast<unsigned>((g.N + cols - 1) / cols), static_cast<unsigned>(tiles));
   const float *xf = static_cast<const float*>(x), *wf = static_cast<const float*>(w);
   if (columns)
     ES_LAUNCH(few_columns_kernel, grid, kFewThreads, 0, s, g, xf, wf, static_cast<float*>(y));

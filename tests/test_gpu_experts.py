@@ -282,6 +282,41 @@ def test_grouped_few_rows(dtype, sizes, K, N):
         assert not y[sum(sizes):].any()
 
 
+@pytest.mark.parametrize("experts,rows", [(40, 300), (7, 41), (64, 9)])
+def test_grouped_few_rows_of_one_expert(experts, rows):
+    """All rows at one expert (more than its share of the launch) or all but one."""
+    g = gen(rows)
+    K, N = 1032, 76
+    for other in (0, 1):
+        sizes = [0] * experts
+        sizes[experts // 2], sizes[-1] = rows - other, other
+        plan = make_plan(sizes, 1, dropped=1)
+        x = randn(g, plan.num_tokens, K, dtype=torch.float32).requires_grad_()
+        w = randn(g, experts, K, N, dtype=torch.float32, scale=K ** -0.5).requires_grad_()
+        dy = randn(g, plan.num_rows, N, dtype=torch.float32)
+        y = E.grouped_matmul(x, w, plan, gather=True)
+        dx, = torch.autograd.grad(y, x, dy)
+        ry, my, rx, mx, _, _ = grouped_ref(x, w, plan, True, dy)
+        near(y.detach(), ry, my, K, torch.float32)
+        near(dx, rx, mx, N + 1, torch.float32)
+        assert not y[rows:].any()
+
+
+@pytest.mark.parametrize("K,N", [(2100, 132), (1028, 20), (12, 64)])
+def test_grouped_few_rows_infinite(K, N):
+    """An infinity at the end of a row's depth makes infinities, and leaves the other rows alone."""
+    plan = make_plan([3, 0, 2], 1)
+    g = gen(K)
+    x = randn(g, 5, K, dtype=torch.float32)
+    w = randn(g, 3, K, N, dtype=torch.float32).abs() + 1
+    bad = x.clone()
+    bad[1, K - 1], bad[4, 0] = math.inf, -math.inf
+    for v in (w, w.transpose(1, 2).contiguous().transpose(1, 2)):
+        y, want = E.grouped_matmul(bad, v, plan), E.grouped_matmul(x, v, plan)
+        assert bool((y[1] == math.inf).all()) and bool((y[4] == -math.inf).all())
+        assert torch.equal(y[[0, 2, 3]], want[[0, 2, 3]])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_many_experts(dtype):
     """As many experts as there may be, most of them without rows."""
