@@ -1,41 +1,53 @@
-// The rows' product grouped by expert for groups of a few rows (a decode step,
-// or a short prompt over many experts), on the CUDA cores: each weight is read
-// once from HBM, as it lies, and multiplied with up to RT rows in fp32. Bound by
-// the weights' bytes: at HBM's rate an SM gets 6 fp32 weights a clock, 8 rows of
-// which are 47 of its 128 multiply-adds.
+// The rows' product grouped by expert in fp32 for groups of a few rows (a decode
+// step, or a short prompt over many experts): each weight is read once from HBM,
+// as it lies, cut into three bf16 planes in the registers that it was loaded to and
+// multiplied there. The planes that the tcgen05 kernels read from memory cost 16
+// bytes of traffic a weight for its 4.
 //
-// A CTA makes a tile of columns for up to RT (4 or 8) rows of one expert, in
-// chunks of kChunk of the depth, whose part of x is staged in shared memory. Every
-// lane has eight 16-byte loads of weights in flight. A longer group is several
-// CTAs' that meet in L2, so a step whose rows all chose one expert fills the SMs.
+// x w = sum of xi wj over the planes with i + j <= 2 (the others are below the last
+// bit of an fp32 product). The planes are rounded to nearest, so three hold all 24
+// bits. x0 w0 and the five smaller products have sums of their own; the first is
+// added in fp32 after each chunk of the depth, since the tensor cores' own
+// addition truncates. Error at 8 rows, 2520 deep: 1.4e-7 of the output.
 //
-// Columns contiguous (forward): a lane owns four columns, the half warps share
-// the depth and their sums are added in the end. Depth contiguous (the gradient
-// of the rows): the lanes share the depth of four columns a warp (so that each
-// value of x that is read serves four weights) and add up by shuffles. Both
-// orders of addition are fixed.
+// A CTA makes kTileCols channels for up to 16 rows of one expert. Its 8 warps are 2
+// groups of 32 channels x 4 shares of the depth; the shares' sums are added in the
+// end, in their order. (4 groups x 2 shares: half the staging of x for a weight,
+// but 121 us for 71 where all rows chose one of 8 experts of 4096 x 4096, and
+// 133 for 120 at 36 of 2520 x 1456, 8 rows.) The channels are the rows of the MMA
+// and the expert's rows its columns. Depth and channels are permuted within a step
+// so that every lane's part of it is four 16-byte loads, whichever of the two is
+// contiguous: (columns) depths 4t .. 4t+3 of channels 4g .. 4g+3; (depth) the same
+// depths of channels g, g+8, g+16, g+24. A longer group is several CTAs' that meet
+// in L2, so a step whose rows all chose one expert fills the SMs.
 //
-// fp32 only: in 16 bits the tensor cores read the weights as fast.
+// Bound by HBM up to 4 rows (36 experts of 2520 x 1456, 4 rows: 105 us, the weights
+// alone 78), then by the instructions issued: 8 for each weight of a lane to cut it
+// and x. A ring of asynchronous copies, 48 KB ahead, was slower (175 us for 120 at 8
+// rows): latency is not the bound.
+//
+// fp32 only: in 16 bits the grouped_tc kernels read the weights as fast.
 #include "grouped.cuh"
 
 namespace es {
 namespace {
 
 constexpr int kFewThreads = 256;
-constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kChunk = 1024;
-constexpr int kWarpCols = 4;  // columns of a warp, depth contiguous
-constexpr int kTileCols = 64;  // columns of a CTA, columns contiguous
-constexpr int kFewRows = 8;
+constexpr int kFewRows = 16;
+constexpr int kTileCols = 64;  // channels of a CTA
+constexpr int kGroups = kTileCols / 32;  // of its channels, 32 a warp
+constexpr int kShares = kFewThreads / 32 / kGroups;  // of the depth
+constexpr int kStep = 16;      // depth of an MMA
+constexpr int kPlanes = 3;
+constexpr int kPlaneBytes = 12288;  // of x in shared memory: chunk x rows
 // Rows of a group (the mean) up to which this is taken. 36 experts of 2520 x 1456,
-// rows spread by chance, us here and on the tensor cores (which read the weights'
-// planes after writing them): columns contiguous 70 and 241 at 1 row, 125 and 339
-// at 4, 196 and 340 at 8, 242 and 343 at 12, 292 and 345 at 16, 406 and 349 at 24;
-// depth contiguous 83 and 243, 153 and 345, 248 and 346, 327 and 350, 409 and 353
-// (121 experts of 1136 x 728: 245 and 280 at 9 rows, 306 and 286 at 12). The
-// weights alone take 52 us at 1 row (23 experts in use) and 81 from 4. Where all
-// rows chose one expert: 129 and 188 us at a mean of 8, 241 at 16 (tensor cores 147).
-constexpr int64_t kColumnsMean = 16, kDepthMean = 10;
+// rows spread by chance, us here and on the tcgen05 kernels: 71 and 241 at 1 row,
+// 105 and 339 at 4, 120 and 340 at 8, 178 and 345 at 16, 222 and 349 at 24, 267 and
+// 373 at 32, 375 and 372 at 48 (121 of 1136 x 728: 188 and 294 at 24, 317 and 301 at
+// 48). Both orders of the weights are within 6%. Where all rows chose one of the
+// 36: 118 and 147 at a mean of 16, 227 and 145 at 32; 24 is between the two.
+constexpr int64_t kFewMean = 24;
+constexpr int64_t kMaxDepth = 1 << 30;  // counted in 32 bits
 
 // The n-th tile of up to kFewRows rows of one expert; false: there is none.
 __device__ __forceinline__ bool nth_tile(const GroupedArgs& g, int n, int& expert, int64_t& r0, int64_t& hi) {
@@ -76,163 +88,205 @@ __device__ __forceinline__ bool nth_tile(const GroupedArgs& g, int n, int& exper
   return expert >= 0;
 }
 
-// The tokens of rows r0 .. r0 + RT, -1 past the last.
-template <int RT>
-__device__ __forceinline__ void load_sources(const GroupedArgs& g, int64_t r0, int64_t hi, int64_t* src) {
-  __syncthreads();
-  if (threadIdx.x < RT) src[threadIdx.x] = r0 + threadIdx.x < hi ? g.source(r0 + threadIdx.x) : -1;
-  __syncthreads();
+struct Planes {
+  uint32_t p[kPlanes];  // two values each
+};
+
+__device__ __forceinline__ Planes split(float a, float b) {
+  Planes s;
+#pragma unroll
+  for (int i = 0; i < kPlanes; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    s.p[i] = *reinterpret_cast<const uint32_t*>(&h);
+    a -= __uint_as_float(s.p[i] << 16);
+    b -= __uint_as_float(s.p[i] & 0xffff0000u);
+  }
+  return s;
 }
 
-__device__ __forceinline__ void clear_columns(const GroupedArgs& g, float* y, int64_t n0, int64_t n1) {
-  for (int64_t r = g.kept() + blockIdx.y; r < g.rows; r += gridDim.y)
-    for (int64_t n = n0 + threadIdx.x; n < n1; n += kFewThreads) y[r * g.N + n] = 0.0f;
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint2 b) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 
-template <int RT>
-__device__ __forceinline__ void columns_tile(const GroupedArgs& g, const float* x, const float* we, float* y,
-                                             int64_t n0, int64_t r0, int64_t hi, float* buffer, int64_t* src) {
-  constexpr int AHEAD = 8, SHARES = 2 * kFewWarps;
-  static_assert(kChunk % (AHEAD * SHARES) == 0, "reads of x past the depth stay in the chunk");
-  const int share = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const bool live = n0 + lane * 4 < g.N;
-  load_sources<RT>(g, r0, hi, src);
-  float4 acc[RT];
+// Planes of a chunk of x, [plane][step][8 rows][row][t] of depths 4t .. 4t+3 (so a
+// warp's operand is 256 bytes in a row); zeros past the depth and the rows. A
+// thread has the same row and t of every step it fills; `from` is there, `left`
+// the depth from there on (none: no row).
+template <int NT>
+__device__ __forceinline__ void stage_rows(const float* from, int left, bool wide, uint2* planes) {
+  constexpr int QUADS = kPlaneBytes / 8, EACH = QUADS / kFewThreads, DEPTH = kFewThreads / (32 * NT) * kStep;
+  static_assert(kFewThreads % (32 * NT) == 0 && QUADS % kFewThreads == 0);
+  planes += threadIdx.x;
+  float4 v[EACH];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) acc[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int64_t k0 = 0; k0 < g.K; k0 += kChunk) {
-    const int depth = static_cast<int>(min(g.K - k0, static_cast<int64_t>(kChunk)));
-    __syncthreads();
-    for (int i = threadIdx.x; i < RT * kChunk; i += kFewThreads) {  // x[depth][row]
-      const int r = i / kChunk, k = i % kChunk;
-      buffer[k * RT + r] = k < depth && src[r] >= 0 ? x[src[r] * g.x_stride + k0 + k] : 0.0f;
-    }
-    __syncthreads();
-    const int per = ((depth + SHARES - 1) / SHARES + AHEAD - 1) / AHEAD * AHEAD;
-    const int k1 = min(depth, (share + 1) * per);
-    if (!live) continue;
-    for (int k = share * per; k < k1; k += AHEAD) {
-      float4 p[AHEAD];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        p[u] = k + u < k1 ? __ldcs(reinterpret_cast<const float4*>(we + (k0 + k + u) * g.w_k + lane * 4))
-                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const float* xr = buffer + (k + u) * RT;  // past the depth both factors are zeros
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          acc[r].x = fmaf(xr[r], p[u].x, acc[r].x);
-          acc[r].y = fmaf(xr[r], p[u].y, acc[r].y);
-          acc[r].z = fmaf(xr[r], p[u].z, acc[r].z);
-          acc[r].w = fmaf(xr[r], p[u].w, acc[r].w);
-        }
-      }
+  for (int i = 0; i < EACH; ++i) {
+    const float* p = from + i * DEPTH;
+    const int n = left - i * DEPTH;
+    v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (wide && n >= 4) {
+      v[i] = *reinterpret_cast<const float4*>(p);
+    } else if (n > 0) {
+      v[i].x = p[0];
+      if (n > 1) v[i].y = p[1];
+      if (n > 2) v[i].z = p[2];
+      if (n > 3) v[i].w = p[3];
     }
   }
-  __syncthreads();
 #pragma unroll
-  for (int r = 0; r < RT; ++r)  // [share][row][column]
-    *reinterpret_cast<float4*>(buffer + (share * RT + r) * kTileCols + lane * 4) = acc[r];
+  for (int i = 0; i < EACH; ++i) {
+    const Planes a = split(v[i].x, v[i].y), b = split(v[i].z, v[i].w);
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) planes[p * QUADS + i * kFewThreads] = make_uint2(a.p[p], b.p[p]);
+  }
+}
+
+// A lane's part of a step, 4 depths x 4 channels. COLUMNS: depth j (of the `left`
+// ones) of four channels; else depths 0 .. 3 of channel 8 j.
+template <bool COLUMNS>
+__device__ __forceinline__ void load_step(float4* v, const float* from, int64_t stride, int left, int live) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j, from += stride) {
+    const bool in = COLUMNS ? j < left : left > 0 && (live >> j & 1);
+    v[j] = in ? __ldcs(reinterpret_cast<const float4*>(from)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+}
+
+__device__ __forceinline__ float lane_of(const float4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// The step's products: MMA tile i has channels (i, 0) in its rows 0 .. 7 and (i, 1) in 8 .. 15.
+template <bool COLUMNS, int NT>
+__device__ __forceinline__ void multiply(float (*main)[NT][4], float (*small)[NT][4], const float4* v,
+                                         const uint2* planes) {
+  constexpr int QUADS = kPlaneBytes / 8;
+  uint2 b[NT][kPlanes];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) b[n][p] = planes[p * QUADS + n * 32];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t a[kPlanes][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int d = 0; d < 2; ++d) {
+        const int c = 2 * i + h;
+        const Planes s = COLUMNS ? split(lane_of(v[2 * d], c), lane_of(v[2 * d + 1], c))
+                                 : split(lane_of(v[c], 2 * d), lane_of(v[c], 2 * d + 1));
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p) a[p][2 * d + h] = s.p[p];
+      }
+#pragma unroll
+    for (int m = 2; m > 0; --m)  // planes i + j = m, smallest first
+#pragma unroll
+      for (int j = 0; j <= m; ++j)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma(small[i][n], a[m - j], b[n][j]);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) mma(main[i][n], a[0], b[n][0]);
+  }
+}
+
+template <bool COLUMNS, int NT>
+__device__ __forceinline__ void few_tile(const GroupedArgs& g, const float* x, const float* we, float* y, bool wide,
+                                         int64_t n0, int64_t r0, int64_t hi, uint2* planes, int64_t* src) {
+  constexpr int CHUNK = kPlaneBytes / 2 / (8 * NT), STEPS = CHUNK / kStep / kShares;
+  static_assert(STEPS % 2 == 0 && kShares * 8 * NT * kTileCols * 4 <= kPlanes * kPlaneBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp / kGroups, t = lane & 3, q = lane >> 2;
+  const int64_t c0 = n0 + warp % kGroups * 32 + (COLUMNS ? 4 * q : q);  // the lane's first channel
+  int live = 0;  // COLUMNS: all four or none
+#pragma unroll
+  for (int j = 0; j < 4; ++j) live |= (COLUMNS ? c0 : c0 + 8 * j) < g.N ? 1 << j : 0;
+  if (threadIdx.x < 8 * NT) src[threadIdx.x] = r0 + threadIdx.x < hi ? g.source(r0 + threadIdx.x) : -1;
   __syncthreads();
-  for (int i = threadIdx.x; i < RT * kTileCols; i += kFewThreads) {
-    const int r = i / kTileCols, c = i % kTileCols;
-    if (r0 + r >= hi || n0 + c >= g.N) continue;
+  const int depth = static_cast<int>(g.K);
+  // this thread's part of x to stage, this lane's weights and what is left of their depth
+  const int x_row = (threadIdx.x >> 2) % (8 * NT), x_k = threadIdx.x / (32 * NT) * kStep + (threadIdx.x & 3) * 4;
+  const float* x_from = x + src[x_row] * g.x_stride + x_k;
+  const bool x_live = src[x_row] >= 0;
+  int k = share * kStep + 4 * t;
+  const int64_t stride = COLUMNS ? g.w_k : 8 * g.w_n;
+  const int64_t ahead = kStep * kShares * (COLUMNS ? g.w_k : 1);
+  const float* from = we + c0 * g.w_n + k * g.w_k;
+  const int end = COLUMNS && !live ? 0 : depth;
+
+  float main[2][NT][4] = {}, small[2][NT][4] = {}, total[2][NT][4] = {};
+  float4 v[2][4];
+  const auto load = [&](float4* to) {
+    load_step<COLUMNS>(to, from, stride, end - k, live);
+    k += kStep * kShares;
+    from += ahead;
+  };
+  load(v[0]);
+  for (int k0 = 0; k0 < depth; k0 += CHUNK, x_from += CHUNK) {
+    if (k0) __syncthreads();
+    stage_rows<NT>(x_from, x_live ? depth - k0 - x_k : 0, wide, planes);
+    __syncthreads();
+    const uint2* mine = planes + share * 32 * NT + lane;
+    const int steps = min(STEPS, (depth - k0 - share * kStep + kStep * kShares - 1) / (kStep * kShares));
+#pragma unroll 1
+    for (int i = 0; i < steps; i += 2, mine += 2 * kShares * 32 * NT) {
+      load(v[1]);
+      multiply<COLUMNS, NT>(main, small, v[0], mine);
+      load(v[0]);
+      multiply<COLUMNS, NT>(main, small, v[1], mine + kShares * 32 * NT);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NT * 4; ++i) {
+      (&total[0][0][0])[i] += (&main[0][0][0])[i];
+      (&main[0][0][0])[i] = 0.0f;
+    }
+  }
+
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(planes);  // [share][row][channel]
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = n * 8 + 2 * t + (j & 1), c = 2 * i + (j >> 1);
+        const int channel = warp % kGroups * 32 + (COLUMNS ? 4 * q + c : 8 * c + q);
+        sums[(share * 8 * NT + row) * kTileCols + channel] = total[i][n][j] + small[i][n][j];
+      }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 8 * NT * kTileCols; i += kFewThreads) {
+    const int row = i / kTileCols, c = i % kTileCols;
+    if (r0 + row >= hi || n0 + c >= g.N) continue;
     float s = 0.0f;
 #pragma unroll
-    for (int v = 0; v < SHARES; ++v) s += buffer[(v * RT + r) * kTileCols + c];
-    y[(r0 + r) * g.N + n0 + c] = s;
+    for (int h = 0; h < kShares; ++h) s += sums[(h * 8 * NT + row) * kTileCols + c];
+    // Infinities have no planes, nor has a value that rounds to one: from the values themselves.
+    if (!isfinite(s) && src[row] >= 0) {
+      s = 0.0f;
+      for (int64_t k = 0; k < g.K; ++k)
+        s = fmaf(x[src[row] * g.x_stride + k], we[(n0 + c) * g.w_n + k * g.w_k], s);
+    }
+    y[(r0 + row) * g.N + n0 + c] = s;
   }
 }
 
-__global__ void __launch_bounds__(kFewThreads, 2) few_columns_kernel(const __grid_constant__ GroupedArgs g,
-                                                                     const float* x, const float* w, float* y) {
-  __shared__ alignas(16) float buffer[kFewRows * kChunk];
-  static_assert(2 * kFewWarps * kFewRows * kTileCols <= kFewRows * kChunk, "the shares' sums");
+template <bool COLUMNS>
+__global__ void __launch_bounds__(kFewThreads, 2) few_kernel(const __grid_constant__ GroupedArgs g, const float* x,
+                                                             const float* w, float* y, bool wide) {
+  __shared__ alignas(16) uint2 planes[kPlanes * kPlaneBytes / 8];
   __shared__ int64_t src[kFewRows];
-  const int64_t n0 = blockIdx.x * static_cast<int64_t>(kTileCols);
-  clear_columns(g, y, n0, min(n0 + kTileCols, g.N));
+  const int64_t n0 = blockIdx.x * static_cast<int64_t>(kTileCols), n1 = min(n0 + kTileCols, g.N);
+  for (int64_t r = g.kept() + blockIdx.y; r < g.rows; r += gridDim.y)
+    for (int64_t n = n0 + threadIdx.x; n < n1; n += kFewThreads) y[r * g.N + n] = 0.0f;
   int e;
   int64_t r0, hi;
   if (!nth_tile(g, blockIdx.y, e, r0, hi)) return;
-  const float* we = w + e * g.w_e + n0;
-  if (hi - r0 > 4)
-    columns_tile<kFewRows>(g, x, we, y, n0, r0, hi, buffer, src);
+  const float* we = w + e * g.w_e;
+  if (hi - r0 > 8)
+    few_tile<COLUMNS, 2>(g, x, we, y, wide, n0, r0, hi, planes, src);
   else
-    columns_tile<4>(g, x, we, y, n0, r0, hi, buffer, src);
-}
-
-template <int RT>
-__device__ __forceinline__ void depth_tile(const GroupedArgs& g, const float* x, const float* we, float* y, int64_t n,
-                                           int64_t r0, int64_t hi, float* buffer, int64_t* src) {
-  constexpr int AHEAD = 2;
-  static_assert(kChunk % (128 * AHEAD) == 0, "reads of x past the depth stay in the chunk");
-  const int lane = threadIdx.x & 31;
-  load_sources<RT>(g, r0, hi, src);
-  float acc[RT][kWarpCols];
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < kWarpCols; ++c) acc[r][c] = 0.0f;
-  for (int64_t k0 = 0; k0 < g.K; k0 += kChunk) {
-    const int depth = static_cast<int>(min(g.K - k0, static_cast<int64_t>(kChunk)));
-    __syncthreads();
-    for (int i = threadIdx.x; i < RT * kChunk; i += kFewThreads) {  // x[row][depth]
-      const int r = i / kChunk, k = i % kChunk;
-      buffer[i] = k < depth && src[r] >= 0 ? x[src[r] * g.x_stride + k0 + k] : 0.0f;
-    }
-    __syncthreads();
-    for (int k = lane * 4; k < depth; k += 128 * AHEAD) {
-      float4 p[AHEAD][kWarpCols];
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-        for (int c = 0; c < kWarpCols; ++c)
-          p[u][c] = n + c < g.N && k + u * 128 < depth
-                        ? __ldcs(reinterpret_cast<const float4*>(we + c * g.w_n + k0 + k + u * 128))
-                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          // past the depth both factors are zeros
-          const float4 xv = *reinterpret_cast<const float4*>(buffer + r * kChunk + k + u * 128);
-#pragma unroll
-          for (int c = 0; c < kWarpCols; ++c) {
-            acc[r][c] = fmaf(xv.x, p[u][c].x, acc[r][c]);
-            acc[r][c] = fmaf(xv.y, p[u][c].y, acc[r][c]);
-            acc[r][c] = fmaf(xv.z, p[u][c].z, acc[r][c]);
-            acc[r][c] = fmaf(xv.w, p[u][c].w, acc[r][c]);
-          }
-        }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-#pragma unroll
-    for (int c = 0; c < kWarpCols; ++c) {
-      float s = acc[r][c];
-#pragma unroll
-      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (lane == 0 && r0 + r < hi && n + c < g.N) y[(r0 + r) * g.N + n + c] = s;
-    }
-}
-
-__global__ void __launch_bounds__(kFewThreads, 2) few_depth_kernel(const __grid_constant__ GroupedArgs g,
-                                                                   const float* x, const float* w, float* y) {
-  constexpr int COLS = kFewWarps * kWarpCols;
-  __shared__ alignas(16) float buffer[kFewRows * kChunk];
-  __shared__ int64_t src[kFewRows];
-  const int64_t n0 = blockIdx.x * static_cast<int64_t>(COLS), n = n0 + (threadIdx.x >> 5) * kWarpCols;
-  clear_columns(g, y, n0, min(n0 + COLS, g.N));
-  int e;
-  int64_t r0, hi;
-  if (!nth_tile(g, blockIdx.y, e, r0, hi)) return;
-  const float* we = w + e * g.w_e + n * g.w_n;
-  if (hi - r0 > 4)
-    depth_tile<kFewRows>(g, x, we, y, n, r0, hi, buffer, src);
-  else
-    depth_tile<4>(g, x, we, y, n, r0, hi, buffer, src);
+    few_tile<COLUMNS, 1>(g, x, we, y, wide, n0, r0, hi, planes, src);
 }
 
 bool by_columns(const GroupedArgs& g) { return g.w_n == 1 && g.N > 1; }
@@ -249,21 +303,19 @@ bool grouped_rows_few_ok(const GroupedArgs& g, int dtype, const void* w) {
   if ((reinterpret_cast<uintptr_t>(w) & 15) != 0 || inner % 4 != 0 || (rows > 1 && row % 4 != 0) ||
       (g.num_experts > 1 && g.w_e % 4 != 0))
     return false;
-  return g.rows <= live * (columns ? kColumnsMean : kDepthMean);
+  return g.K <= kMaxDepth && g.rows <= live * kFewMean;
 }
 
 int grouped_rows_few(const GroupedArgs& g, const void* x, const void* w, void* y, cudaStream_t s) {
   const bool columns = by_columns(g);
-  const int64_t cols = columns ? kTileCols : kFewWarps * kWarpCols;
   // groups of n rows have at most this many tiles: one begun by each live group, the others full
   const int64_t live = min(static_cast<int64_t>(g.num_experts), g.rows);
   const int64_t tiles = live + (g.rows - live) / kFewRows;
-  const dim3 grid(static_cast<unsigned>((g.N + cols - 1) / cols), static_cast<unsigned>(tiles));
+  const dim3 grid(static_cast<unsigned>((g.N + kTileCols - 1) / kTileCols), static_cast<unsigned>(tiles));
   const float *xf = static_cast<const float*>(x), *wf = static_cast<const float*>(w);
-  if (columns)
-    ES_LAUNCH(few_columns_kernel, grid, kFewThreads, 0, s, g, xf, wf, static_cast<float*>(y));
-  else
-    ES_LAUNCH(few_depth_kernel, grid, kFewThreads, 0, s, g, xf, wf, static_cast<float*>(y));
+  const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && g.x_stride % 4 == 0;
+  const auto kernel = columns ? few_kernel<true> : few_kernel<false>;
+  ES_LAUNCH(kernel, grid, kFewThreads, 0, s, g, xf, wf, static_cast<float*>(y), wide);
   return ES_OK;
 }
 

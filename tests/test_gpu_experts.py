@@ -302,6 +302,40 @@ def test_grouped_few_rows_of_one_expert(experts, rows):
         assert not y[rows:].any()
 
 
+@pytest.mark.parametrize("K,N", [(388, 72), (768, 200), (20, 4), (1500, 64)])
+@pytest.mark.parametrize("pad", [0, 1, 4])
+def test_grouped_few_rows_strides(K, N, pad):
+    """Several tiles of rows an expert, x and weights as views: offset, with a longer pitch, one of them not 16 bytes."""
+    sizes = [16, 17, 0, 31, 33, 2, 8]
+    plan = make_plan(sizes, 1, dropped=3)
+    g = gen(K + pad)
+    base = randn(g, plan.num_tokens, K + 2 * pad, dtype=torch.float32)
+    x = base[:, pad:pad + K].detach().requires_grad_()
+    wbase = randn(g, len(sizes), K + 4, N + 8, dtype=torch.float32, scale=K ** -0.5)
+    w = wbase[:, 4:, 4:4 + N].detach().requires_grad_()
+    dy = randn(g, plan.num_rows, N, dtype=torch.float32)
+    for gather in (True, False):
+        y = E.grouped_matmul(x, w, plan, gather=gather)
+        dx, = torch.autograd.grad(y, x, dy)
+        ry, my, rx, mx, _, _ = grouped_ref(x, w, plan, gather, dy)
+        near(y.detach(), ry, my, K, torch.float32)
+        near(dx, rx, mx, N + 1, torch.float32)
+        assert not y[sum(sizes):].any()
+
+
+def test_grouped_few_rows_largest():
+    """Values next to the type's largest, whose first plane would be an infinity."""
+    big = torch.finfo(torch.float32).max
+    plan = make_plan([2, 1], 1)
+    g = gen(5)
+    x = randn(g, 3, 64, dtype=torch.float32) * 2.0 ** -10
+    w = randn(g, 2, 64, 8, dtype=torch.float32)
+    w[0, 3, 2], w[1, 63, 7] = big, -big
+    y = E.grouped_matmul(x, w, plan)
+    ry, my = grouped_ref(x, w, plan, False, torch.zeros(3, 8, device=DEV))[:2]
+    near(y, ry, my, 64, torch.float32)
+
+
 @pytest.mark.parametrize("K,N", [(2100, 132), (1028, 20), (12, 64)])
 def test_grouped_few_rows_infinite(K, N):
     """An infinity at the end of a row's depth makes infinities, and leaves the other rows alone."""
