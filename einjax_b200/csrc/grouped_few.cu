@@ -21,10 +21,11 @@
 // depths of channels g, g+8, g+16, g+24. A longer group is several CTAs' that meet
 // in L2, so a step whose rows all chose one expert fills the SMs.
 //
-// Bound by HBM up to 4 rows (36 experts of 2520 x 1456, 4 rows: 105 us, the weights
-// alone 78), then by the instructions issued: 8 for each weight of a lane to cut it
-// and x. A ring of asynchronous copies, 48 KB ahead, was slower (175 us for 120 at 8
-// rows): latency is not the bound.
+// Bound by HBM up to 4 rows (36 experts of 2520 x 1456, 4 rows each: 105 us, 4.8
+// TB/s with the 2.8 rounds of CTAs taking 3; the weights alone 78), then by the
+// dependent chain load, cut, multiply of the 16 warps that an SM holds (16 rows: 130
+// us, 42% of the issue slots, 36% of the tensor pipe). A ring of asynchronous copies,
+// 48 KB ahead, did not help (107 us at 4 rows, 171 for 167 at 16).
 //
 // fp32 only: in 16 bits the grouped_tc kernels read the weights as fast.
 #include "grouped.cuh"
