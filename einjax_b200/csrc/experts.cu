@@ -632,25 +632,41 @@ __device__ __forceinline__ float piece_peak(const Piece<__half, VEC>& p) {
   }
 }
 
-// rint(x / s) as a division rounded to nearest gives it. x times the
-// reciprocal is at most a few units in the last place of 127 from that
-// quotient, so a piece is divided only where one of its values is next to a
-// tie (or the reciprocal overflows). Adding 1.5 * 2^23 rounds to the nearest
-// integer and leaves it in the low bits. (A division for every value took
-// three times as long.)
+// rint(x / s) as a division rounded to nearest gives it; inv = 1 / s, rounded.
+// Adding 1.5 * 2^23 rounds to the nearest integer and leaves it in the low bits.
+//
+// 16 bits: x * inv is corrected by its remainder x - q s, which an FMA gives
+// exactly (Markstein, IBM J. Res. Dev. 34, 1990): q + (x - q s) * inv is the
+// quotient rounded to nearest for all pairs of values and largest values of both
+// types. Scales are kept clear of underflow. Ties are common in 16 bits (half the
+// pieces of a warp have one), so no form that treats them apart is as fast.
+//
+// fp32: x * inv is within 2e-5 of the quotient (at most 127), so a piece is divided
+// where one of its values is as close to a tie, or the reciprocal overflows.
 template <typename T, int VEC>
 __device__ __forceinline__ Piece<int8_t, VEC> quantize_piece(const Piece<T, VEC>& p, float s, float inv) {
-  constexpr float kRound = 12582912.0f;
+  constexpr float kRound = 12582912.0f, kClear = 18446744073709551616.0f;  // 2^64
   Piece<int8_t, VEC> o;
-  float off = 0.0f;
+  bool divide;
+  if constexpr (sizeof(T) == 2) {
+    divide = !(s > 1.0f / kClear && s < kClear);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const float q = to_f32(p.v[i]) * inv;
-    const float r = q + kRound;
-    off = max_nan(off, fabsf(q - (r - kRound)));
-    o.v[i] = static_cast<int8_t>(__float_as_int(r));
+    for (int i = 0; i < VEC; ++i) {
+      const float v = to_f32(p.v[i]), q = v * inv;
+      o.v[i] = static_cast<int8_t>(__float_as_int(fmaf(fmaf(-q, s, v), inv, q) + kRound));
+    }
+  } else {
+    float off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float q = to_f32(p.v[i]) * inv;
+      const float r = q + kRound;
+      off = max_nan(off, fabsf(q - (r - kRound)));
+      o.v[i] = static_cast<int8_t>(__float_as_int(r));
+    }
+    divide = !(off < 0.4999f);
   }
-  if (!(off < 0.4999f)) {
+  if (divide) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float r = s > 0.0f ? rintf(__fdiv_rn(to_f32(p.v[i]), s)) : 0.0f;

@@ -630,6 +630,23 @@ def test_quantize(rows, width, dtype):
         assert torch.equal(s, rs) and torch.equal(q, rq)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantize_every_value(dtype):
+    """Every finite value of a type under largest values of every kind of mantissa, and next to the type's ends."""
+    every = torch.arange(2 ** 15, dtype=torch.int32, device=DEV).to(torch.int16).view(dtype)
+    every = every[every.isfinite()]
+    n = 128 if dtype == torch.bfloat16 else 1024
+    peaks = [(1 + m / n) * 2.0 ** e for e in (-3, 0, 9) for m in range(0, n, 1 if n == 128 else 7)]
+    peaks += every[[1, 2, 3, 77, 300, -300, -2, -1]].tolist()
+    for some in torch.tensor(peaks, dtype=torch.float64).split(32):
+        top = some.to(DEV, dtype)
+        x = torch.where(every[None, :] <= top[:, None], every[None, :], top[:, None])
+        x[:, ::2] = -x[:, ::2]
+        q, s = E.quantize_rows(x)
+        rq, rs = quant_ref(x)
+        assert torch.equal(s, rs) and torch.equal(q, rq)
+
+
 def test_quantize_special():
     x = torch.tensor([[1.0, math.inf, 0], [math.nan, 1.0, 2.0], [0, 0, 0], [2.0 ** -149, 0, 0], [-3.0, 1.5, 3.0]],
                      device=DEV)
