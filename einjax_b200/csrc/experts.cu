@@ -589,7 +589,7 @@ int combine_grad_typed(const void* y, int64_t rows, int64_t stride, const float*
 // rint(x_ti / scale_t), kept within +-127. A row of zeros has scale 0 and q 0;
 // a row with an infinity or NaN has scale NaN, so that its products are NaN
 // and not a finite guess. A row is read once and its 8-bit copy written once:
-// 8191 x 4096 bf16 take 27 us, 3.7 TB/s, between memory and the conversions.
+// 8191 x 4096 bf16 take 25 us, 4.0 TB/s, between memory and the conversions.
 
 constexpr int kQuantThreads = 256;
 
