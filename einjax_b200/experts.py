@@ -248,7 +248,9 @@ def _grouped(x, w, plan, gather, out_dtype):
     y = _empty(R, N, out_dtype, dev)
     args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), plan.offsets.data_ptr(),
             plan.order.data_ptr() if gather else None, plan.top_k, R)
-    _product("es_grouped_matmul", dev, args, (y.data_ptr(), _DTYPES[out_dtype]), gather or code == L.ES_F32)
+    # fp32 mostly needs no workspace for up to 24 rows a group (12.8 us for 14.9 a small call)
+    need = R > 24 * E if code == L.ES_F32 else gather
+    _product("es_grouped_matmul", dev, args, (y.data_ptr(), _DTYPES[out_dtype]), need)
     return y
 
 
