@@ -21,7 +21,7 @@
 // 2.76 ms where the copy and box loads take 1.0 ms (16384 rows, 4096 x 8192,
 // bf16). What TMA cannot read (odd addresses or strides) is copied too.
 //
-// fp32 operands are cut into three bf16 planes, x = b0 + b1 + b2 exactly. A
+// fp32 operands are cut into three bf16 planes, x / 2 = b0 + b1 + b2 (split3). A
 // block of depth takes three stages, one for each plane, and the six products
 // b_i b_j with i + j <= 2 are made from them (each operand crosses from L2
 // once): b0 b0 into one accumulator, the other five, at most 2^-8 of it, into a
@@ -513,6 +513,14 @@ __device__ __forceinline__ void clear_rows(const TcArgs& p, int64_t from, int64_
   for (int64_t i = head + n * 8 + t; i < halves; i += nt) reinterpret_cast<uint16_t*>(a)[i] = 0;
 }
 
+// A chain's sum from its two accumulators of halved planes: the products of the
+// first planes, and the others. An infinity's other planes are zero, so its products
+// with a value's lower planes are NaN or of either sign and belong to no sum: where
+// the first planes' sum is infinite or NaN it alone is what fp32 arithmetic gives.
+__device__ __forceinline__ float plane_sum(float first, float others) {
+  return 4.0f * (fabsf(first) < INFINITY ? first + others : first);
+}
+
 // The 8-bit product's sums times the scales of their rows (xs) and channel.
 __device__ __forceinline__ void scale_block(float (&v)[32], const float* xs, float w) {
 #pragma unroll
@@ -623,7 +631,7 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
         float u[8];
         tmem_ld8(acc + S::NT + c0, u);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += u[i] + (s0 > at.kb0 ? mine[(c0 + i) * 128] : 0.0f);
+        for (int i = 0; i < 8; ++i) v[i] = plane_sum(v[i], u[i]) + (s0 > at.kb0 ? mine[(c0 + i) * 128] : 0.0f);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) mine[(c0 + i) * 128] = v[i];  // columns past the tile's are not read
@@ -1022,7 +1030,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               float u[32];
               tmem_ld32(acc + NT + c0, u);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] += u[i];
+              for (int i = 0; i < 32; ++i) v[i] = plane_sum(v[i], u[i]);
             }
           } else {
 #pragma unroll
@@ -1136,17 +1144,17 @@ struct LayoutArgs {
   int wide;     // 16-byte loads
 };
 
-// b0 + b1 + b2 == x exactly: each plane is what is left, rounded to 8 bits
-// (to nearest: a rest is at most 2^-8 of its number, twice less than after
-// truncation, which the products left out have in their square). A value that
-// would round past the type's largest is truncated; an infinity or NaN is its
-// first plane alone, so that its products are infinite or NaN.
+// Half of x in planes, b0 + b1 + b2 == x / 2 for magnitudes from 2^-109 on (below,
+// the third plane ends at bf16's smallest value): each is what is left, rounded to
+// 8 bits (to nearest: a rest is at most 2^-8 of its number, twice less than after
+// truncation, which the products left out have in their square). Halves, since a
+// rounded plane is up to 2^-8 larger than its value: no finite value has an
+// infinite plane, and no product of planes overflows where the values' does not. An
+// infinity or NaN is its first plane alone; a value below 2^-132 may have none.
 __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
-  const uint32_t u = __float_as_uint(x);
-  const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-  __nv_bfloat16 b0 = __float2bfloat16_rn(x);
-  if (finite && __hisinf(b0)) b0 = __ushort_as_bfloat16(static_cast<uint16_t>(u >> 16));
-  const float r1 = finite ? x - __bfloat162float(b0) : 0.0f;
+  const float h = 0.5f * x;
+  const __nv_bfloat16 b0 = __float2bfloat16_rn(h);
+  const float r1 = fabsf(h) < INFINITY ? h - __bfloat162float(b0) : 0.0f;
   const __nv_bfloat16 b1 = __float2bfloat16_rn(r1);
   b[0] = __bfloat16_as_ushort(b0);
   b[1] = __bfloat16_as_ushort(b1);

@@ -409,7 +409,8 @@ int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts,
 /* y[r] = x[row(r)] w[e(r)] for the num_rows grouped rows: w[e] is (K, N) with
  * any element strides, row(r) = order[r] / top_k when order is given (x by
  * token), else r. y (num_rows, N) contiguous, of out_dtype (ES_F32 or the
- * operands' type). The workspace's size goes by the call's own arguments. */
+ * operands' type). Infinities and NaN give what fp32 arithmetic gives, except
+ * that a magnitude below 2^-132 may count as zero beside them. The workspace's size goes by the call's own arguments. */
 size_t es_grouped_matmul_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
                                         int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
                                         int64_t w_k_stride, int64_t w_n_stride, const int32_t* offsets,

@@ -1,0 +1,82 @@
+"""Expert operators on the GPU at the ends of their types, of their depths and of their tile shapes.
+
+Bounds are derived as in ``test_gpu_experts``: one rounding of the result's
+type, and for fp32 sums ``2**-23`` of the products' magnitudes a step, in the
+2-norm over many values at most ``2**-19``.
+"""
+
+import math
+
+import pytest
+import torch
+
+import einjax_b200 as E
+from test_gpu_experts import TYPES, UNIT, check_int8, gen, grouped_ref, int8_ref, int8s, make_plan, near, randn
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def same_kinds(got, ref):
+    """The infinities and NaN of got are those of ref (64 bits); where ref is finite the two are near."""
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got.isposinf(), ref.isposinf()) and torch.equal(got.isneginf(), ref.isneginf())
+    there = ref.isfinite()
+    err = (got.double() - ref)[there].norm()
+    assert float(err) <= (UNIT[got.dtype] + 2.0 ** -19) * float(ref[there].norm())
+
+
+# ----------------------------------------- infinities and the largest values, fp32
+
+@pytest.mark.parametrize("sizes", [[3, 0, 2], [130, 0, 70], [700, 500, 300]])
+@pytest.mark.parametrize("K,N", [(96, 64), (1100, 132), (72, 2060)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_grouped_infinite(sizes, K, N, transposed):
+    """An infinity in fp32 is what fp32 arithmetic makes of it, whatever the length of its group."""
+    plan = make_plan(sizes, 1, dropped=2)
+    g = gen(K + N)
+    x = randn(g, plan.num_rows, K)
+    w = randn(g, 3, K, N, scale=K ** -0.5)
+    dy = randn(g, plan.num_rows, N)
+    off = plan.offsets.tolist()
+    w[0, 5, 3] = 0.0
+    x[1, 5], x[off[2], K - 1], x[off[2] + 1, 0] = math.inf, -math.inf, math.nan
+    w[2, 7, N - 1], w[2, 8, N - 1] = math.inf, -math.inf
+    dy[2, 1], dy[off[2] + 1, N - 2] = -math.inf, math.inf
+    dy[off[2], N - 1] = 0.0
+    if transposed:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    x.requires_grad_()
+    w.requires_grad_()
+    y = E.grouped_matmul(x, w, plan)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    ry, _, rx, _, rw, _ = grouped_ref(x, w, plan, False, dy)
+    for got, ref in ((y.detach(), ry), (dx, rx), (dw, rw)):
+        assert bool(ref.isinf().any()) and bool(ref.isnan().any())
+        same_kinds(got, ref)
+
+
+@pytest.mark.parametrize("sizes", [[3, 2], [130, 70], [700, 500]])
+@pytest.mark.parametrize("N", [8, 2060])
+def test_grouped_largest(sizes, N):
+    """Values and products next to the type's largest stay finite, though their first planes are rounded up."""
+    big = torch.finfo(torch.float32).max
+    plan = make_plan(sizes, 1)
+    g = gen(N)
+    K = 72
+    x = randn(g, plan.num_rows, K) * 2.0 ** -10
+    w = randn(g, 2, K, N)
+    w[0, 3, 2], w[1, K - 1, N - 1] = big, -big
+    x[1], w[0, :, 5] = 0.0, 0.0
+    x[1, 3], w[0, 3, 5] = 3.385e38, 1.0045  # both planes round up: their product is past the largest value
+    x[1, 4], w[0, 4, 2] = 0.0, 0.0
+    w[0, 3, 2] = 0.9
+    w[0, 4, 3] = big
+    w[0, 3, torch.arange(N, device=DEV) > 5] = 0.0
+    w[0, 3, :2] = 0.5
+    w[0, 3, 3:5] = -1.0
+    y = E.grouped_matmul(x, w, plan)
+    ry, my = grouped_ref(x, w, plan, False)[:2]
+    assert bool(ry.abs().max() < big) and bool(ry.abs().max() > 0.999 * big)
+    near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
