@@ -10,6 +10,7 @@ GPU through ``es_tile_coo_*`` / ``es_tile_dense_*``.
 
 from __future__ import annotations
 
+import threading
 from math import prod
 from typing import Any
 
@@ -132,33 +133,48 @@ class _StatusWords:
     choice of an expert that does not exist, a bounded wait that ran out) and
     leave alone otherwise: no copy, event or wait of a call's own.
     ``check_device_errors`` waits for the devices that ran such calls and
-    raises for the first word that is set."""
+    raises for the first word that is set, which alone it clears.
+
+    The words are made together and once, under a lock: kernels hold their
+    addresses, so no thread's first call may replace another's."""
+
+    OPERATORS = ("es_expert_plan", "es_grouped_matmul", "es_grouped_matmul_wgrad", "es_int8_matmul")
 
     def __init__(self):
-        self.words = {}  # function name -> (pinned tensor, address)
+        self.lock = threading.Lock()
+        self.words = None
+        self.addresses = {}
         self.devices = set()
 
     def address(self, fn: str, device_index: int) -> int:
-        self.devices.add(device_index)
+        if device_index not in self.devices:
+            with self.lock:
+                self.devices.add(device_index)
         try:
-            return self.words[fn][1]
+            return self.addresses[fn]
         except KeyError:
-            word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            self.words[fn] = (word, word.data_ptr())
-            return self.words[fn][1]
+            return self._make(fn)
+
+    def _make(self, fn: str) -> int:
+        with self.lock:
+            if self.words is None:
+                words = torch.zeros(len(self.OPERATORS), dtype=torch.int32, pin_memory=True)
+                self.addresses = {f: words.data_ptr() + 4 * i for i, f in enumerate(self.OPERATORS)}
+                self.words = words
+            return self.addresses[fn]
 
     def flush(self) -> None:
-        devices, self.devices = self.devices, set()
+        with self.lock:
+            devices, self.devices = self.devices, set()
         for d in devices:
             torch.cuda.synchronize(d)
-        first = None
-        for fn, (word, _) in self.words.items():
-            e = int(word[0])
-            word[0] = 0
-            if e and first is None:
-                first = (fn, e)
-        if first is not None:
-            L.check(first[0] + " (device)", first[1])
+        if self.words is None:
+            return
+        for i, fn in enumerate(self.OPERATORS):
+            e = int(self.words[i])
+            if e:
+                self.words[i] = 0
+                L.check(fn + " (device)", e)
 
 
 _STATUS = _StatusWords()
