@@ -132,8 +132,9 @@ class _StatusWords:
     """One pinned int32 per operator that its kernels write when they fail (a
     choice of an expert that does not exist, a bounded wait that ran out) and
     leave alone otherwise: no copy, event or wait of a call's own.
-    ``check_device_errors`` waits for the devices that ran such calls and
-    raises for the first word that is set, which alone it clears.
+    ``check_device_errors`` waits for the devices that ever ran such calls
+    (a captured call runs again with no call of Python's) and raises for the
+    first word that is set, which alone it clears.
 
     The words are made together and once, under a lock: kernels hold their
     addresses, so no thread's first call may replace another's."""
@@ -165,7 +166,7 @@ class _StatusWords:
 
     def flush(self) -> None:
         with self.lock:
-            devices, self.devices = self.devices, set()
+            devices = list(self.devices)
         for d in devices:
             torch.cuda.synchronize(d)
         if self.words is None:

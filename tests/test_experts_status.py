@@ -94,3 +94,13 @@ def test_flush_while_threads_call(status):
         for t in threads:
             t.join()
     assert not errors
+
+
+def test_devices_are_waited_for_again(status):
+    """A replay of a captured call names no device."""
+    status.address("es_grouped_matmul", 1)
+    status.address("es_expert_plan", 3)
+    for _ in range(2):
+        status.waited.clear()
+        status.flush()
+        assert sorted(status.waited) == [1, 3]

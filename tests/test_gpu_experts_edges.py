@@ -80,3 +80,27 @@ def test_grouped_largest(sizes, N):
     ry, my = grouped_ref(x, w, plan, False)[:2]
     assert bool(ry.abs().max() < big) and bool(ry.abs().max() > 0.999 * big)
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
+
+
+# ------------------------------------------------------------------ captured calls
+
+def test_replayed_failure_is_raised():
+    """check_device_errors waits for the kernels of a replayed graph."""
+    e = torch.zeros(10, 1, dtype=torch.int32, device=DEV)
+    long = torch.zeros(8192, 8192, device=DEV)
+    E.plan_experts(e, 4)
+    E.check_device_errors()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(8):  # tens of milliseconds before the kernel that fails
+            long @ long
+        E.plan_experts(e, 4)
+    E.check_device_errors()
+    e[3] = 9
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(ValueError, match="es_expert_plan"):
+            E.check_device_errors()
+    E.check_device_errors()
+    del graph
