@@ -794,10 +794,20 @@ extern "C" int es_expert_plan(const int32_t* experts, int64_t num_choices, int n
   if (workspace_bytes < es_expert_plan_workspace_size(num_choices, num_experts)) return ES_ERR_WORKSPACE;
   cudaStream_t s = as_stream(stream);
   const size_t smem = plan_smem(num_experts);
-  if (smem > 48 * 1024)
-    if (cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem)) != cudaSuccess)
-      return ES_ERR_CUDA;
+  if (smem > 48 * 1024) {
+    // to the largest, once a device: a limit of this call's own size could be
+    // lowered by another thread's call before the launch
+    static std::atomic<bool> raised[kMaxAttrDevices];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return ES_ERR_CUDA;
+    const bool tracked = dev >= 0 && dev < kMaxAttrDevices;
+    if (!tracked || !raised[dev].load(std::memory_order_relaxed)) {
+      if (cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(plan_smem(kMaxExperts))) != cudaSuccess)
+        return ES_ERR_CUDA;
+      if (tracked) raised[dev].store(true, std::memory_order_relaxed);
+    }
+  }
   const int64_t chunks = num_choices > kPlanChunk ? (num_choices + kPlanChunk - 1) / kPlanChunk : 1;
   int32_t* counts = nullptr;
   if (chunks > 1) {

@@ -6,11 +6,13 @@ type, and for fp32 sums ``2**-23`` of the products' magnitudes a step, in the
 """
 
 import math
+import threading
 
 import pytest
 import torch
 
 import einjax_b200 as E
+from einjax_b200 import _lib as L
 from test_gpu_experts import TYPES, UNIT, check_int8, gen, grouped_ref, int8_ref, int8s, make_plan, near, randn
 
 pytestmark = pytest.mark.gpu
@@ -80,6 +82,36 @@ def test_grouped_largest(sizes, N):
     ry, my = grouped_ref(x, w, plan, False)[:2]
     assert bool(ry.abs().max() < big) and bool(ry.abs().max() > 0.999 * big)
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
+
+
+# --------------------------------------------------------------------- threads
+
+def test_plans_of_many_experts_from_threads():
+    """Threads that order rows of different numbers of experts, whose kernels ask for different shared memory."""
+    lib = L.lib()
+    wanted = (1024, 690, 1000, 700)
+    start = threading.Barrier(len(wanted))
+    answers = []
+
+    def calls(n):
+        torch.cuda.set_device(0)
+        e = torch.zeros(4, 1, dtype=torch.int32, device=DEV)
+        off, order, position = (torch.empty(m, dtype=torch.int32, device=DEV) for m in (n + 1, 4, 4))
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        args = (e.data_ptr(), 4, n, None, 0, off.data_ptr(), order.data_ptr(), position.data_ptr(), None,
+                stream.cuda_stream)
+        start.wait()
+        got = {lib.es_expert_plan(*args) for _ in range(5000)}
+        stream.synchronize()
+        answers.append(got)
+
+    threads = [threading.Thread(target=calls, args=(n,)) for n in wanted]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert answers == [{L.ES_OK}] * len(wanted)
 
 
 # ------------------------------------------------------------------ captured calls
