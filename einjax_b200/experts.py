@@ -12,7 +12,8 @@ so it runs beside the tile-COO path instead of on it:
   in 8-bit integers with a scale for each token and output channel;
 * ``expert_mlp``: a gated layer made of these.
 
-All of it runs on torch's current CUDA stream with no wait of the host. What
+Gradients are reverse-mode; a forward-mode tangent is refused. All of it runs
+on torch's current CUDA stream with no wait of the host. What
 only the device can see (a choice of an expert that does not exist, a bounded
 wait that ran out) is raised by ``check_device_errors``.
 """
@@ -20,6 +21,7 @@ wait that ran out) is raised by ``check_device_errors``.
 from __future__ import annotations
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib as L
 from .sparse import _STATUS, _raw_stream
@@ -50,6 +52,12 @@ def _on_gpu(fn: str, **tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError(f"{fn}: {name} is on {t.device}, the other operands on {dev}")
+
+
+def _no_tangent(fn: str, *tensors):
+    """Raises where forward-mode differentiation is on for one of ``tensors``: the kernels would drop its tangent."""
+    if _forward_ad._current_level >= 0 and any(_forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{fn}: no forward-mode derivative; gradients are reverse-mode only")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -177,6 +185,7 @@ class _Route(torch.autograd.Function):
     def backward(ctx, dweights, _):
         if dweights is None:
             return None, None, None
+        _no_tangent("route_experts", dweights)
         logits, weights, experts = ctx.saved_tensors
         dev = logits.device
         T, E = logits.shape
@@ -207,6 +216,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True):
     if not 1 <= top_k <= min(E, MAX_TOP_K) or E > MAX_EXPERTS:
         raise ValueError(f"route_experts: top_k={top_k} of {E} experts; 1 <= top_k <= min(num_experts, {MAX_TOP_K}) "
                          f"and num_experts <= {MAX_EXPERTS}")
+    _no_tangent("route_experts", logits)
     run = _Route.apply if logits.requires_grad and torch.is_grad_enabled() else _route
     return run(_rows(logits), top_k, 1 if renormalize else 0)
 
@@ -279,6 +289,7 @@ class _GroupedMatmul(torch.autograd.Function):
     def backward(ctx, dy):
         x, w = ctx.saved_tensors
         plan, gather = ctx.plan, ctx.gather
+        _no_tangent("grouped_matmul", dy)
         dy = _rows(dy)
         dx = dw = None
         if ctx.needs_input_grad[0]:
@@ -316,6 +327,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan, gather: b
     if w.dim() != 3 or w.shape[0] != plan.num_experts:
         raise ValueError(f"grouped_matmul: w has shape {tuple(w.shape)}, wanted ({plan.num_experts}, K, N)")
     _check_rows("grouped_matmul", x, "x", plan, gather, w.shape[1])
+    _no_tangent("grouped_matmul", x, w)
     x, gather = _rows(x), bool(gather)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         return _GroupedMatmul.apply(x, w, plan, gather)
@@ -344,6 +356,7 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, dout):
         y, weights = ctx.saved_tensors
         plan, dev = ctx.plan, y.device
+        _no_tangent("combine_experts", dout)
         dout = _rows(dout)
         dy = _empty(*y.shape, y.dtype, dev)
         dweights = torch.empty_like(weights)
@@ -369,6 +382,7 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) ->
     if weights.shape != plan.position.shape:
         raise ValueError(f"combine_experts: weights have shape {tuple(weights.shape)}, the plan's choices "
                          f"{tuple(plan.position.shape)}")
+    _no_tangent("combine_experts", y, weights)
     y, weights = _rows(y), weights.contiguous()
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad):
         return _Combine.apply(y, weights, plan)

@@ -84,6 +84,35 @@ def test_grouped_largest(sizes, N):
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
 
 
+# ------------------------------------------------------------- derivatives refused
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(leaf):
+    """A tangent raises instead of being dropped, in an operand and in a gradient; without one a level changes nothing."""
+    import torch.autograd.forward_ad as fw
+    plan = make_plan([3, 5], 2)
+    g = gen(1)
+    logits, x, w = randn(g, 4, 2), randn(g, 4, 16), randn(g, 2, 16, 8)
+    y, weights, router = randn(g, 8, 16), torch.rand(4, 2, generator=g, device=DEV), randn(g, 16, 2)
+    calls = ((lambda a: E.route_experts(a, 2)[0], [logits]), (lambda a, b: E.grouped_matmul(a, b, plan, True), [x, w]),
+             (lambda a, b: E.combine_experts(a, b, plan), [y, weights]),
+             (lambda a, b: E.expert_mlp(a, b, randn(gen(2), 2, 16, 32), randn(gen(2), 2, 16, 16), 2), [x, router]))
+    for call, args in calls:
+        args = [a.detach().requires_grad_(leaf) for a in args]
+        want = call(*args)
+        with fw.dual_level():
+            assert torch.equal(call(*args), want)
+            for i in range(len(args)):
+                duals = list(args)
+                duals[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(NotImplementedError):
+                    call(*duals)
+            if leaf:
+                out = call(*args)
+                with pytest.raises(NotImplementedError):
+                    torch.autograd.grad(out, args, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
 # --------------------------------------------------------------------- threads
 
 def test_plans_of_many_experts_from_threads():
