@@ -394,7 +394,8 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, plan: ExpertPlan) ->
 def quantize_rows(x: torch.Tensor):
     """``(q, scale)``: each row of ``x`` (rows, width) in 8-bit integers with
     ``scale = max |x| / 127`` (float32), ``q = rint(x / scale)``. A row of
-    zeros has scale 0; a row with an infinity or NaN has scale NaN."""
+    zeros has scale 0; a row with an infinity or NaN has scale NaN. Not
+    differentiable: the result has no history."""
     _on_gpu("quantize_rows", x=x)
     code = _code("quantize_rows", "x", x.dtype)
     if x.dim() != 2:
@@ -428,7 +429,8 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
     ``plan`` the products are grouped by expert as in ``grouped_matmul``:
     ``wq`` (num_experts, N, K), ``wscale`` (num_experts, N), and with
     ``gather`` ``q`` and ``scale`` are by token. Returns (rows, N) of
-    ``out_dtype`` (float32, bfloat16, float16). K is at most 131,071."""
+    ``out_dtype`` (float32, bfloat16, float16). K is at most 131,071. Not
+    differentiable: the result has no history."""
     _on_gpu("int8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=q if plan is None else plan.offsets)
     code = _code("int8_matmul", "out_dtype", out_dtype)
     if q.dtype != torch.int8 or wq.dtype != torch.int8:
@@ -463,20 +465,20 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: 
 
 # ----------------------------------------------------------- a layer of experts
 
-def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, renormalize: bool = True):
-    """A gated layer of experts: for each token ``x`` (num_tokens, D) the
-    weighted sum, over its ``top_k`` experts ``e``, of
-    ``(silu(x @ gate_e) * (x @ up_e)) @ w_out_e``.
+class _Served(torch.autograd.Function):
+    """The 8-bit layer's output. A gradient through it would hold the routing's share alone, so there is none."""
 
-    ``router`` (D, num_experts). ``w_in`` (num_experts, D, 2 F) holds gate and
-    up side by side, ``w_out`` (num_experts, F, D): tensors of x's type for
-    training (differentiable in everything), or both ``(wq, scale)`` pairs
-    of ``quantize_experts`` for serving in 8-bit integers."""
-    quantized = isinstance(w_in, (tuple, list))
-    if quantized != isinstance(w_out, (tuple, list)):
-        raise TypeError("expert_mlp: w_in and w_out must both be tensors or both be (wq, scale) pairs")
-    logits = x.float() @ router.float()
-    weights, experts = route_experts(logits, top_k, renormalize)
+    @staticmethod
+    def forward(ctx, out, x, router):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError("expert_mlp: the 8-bit form has no gradient; train with the weights' tensors")
+
+
+def _layer(x, router, w_in, w_out, top_k, renormalize, quantized):
+    weights, experts = route_experts(x.float() @ router.float(), top_k, renormalize)
     plan = plan_experts(experts, router.shape[1])
     if quantized:
         h = int8_matmul(*quantize_rows(x), *w_in, plan, gather=True, out_dtype=x.dtype)
@@ -487,3 +489,25 @@ def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, r
     y = int8_matmul(*quantize_rows(h), *w_out, plan, out_dtype=x.dtype) if quantized else \
         grouped_matmul(h, w_out, plan)
     return combine_experts(y, weights, plan)
+
+
+def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, renormalize: bool = True):
+    """A gated layer of experts: for each token ``x`` (num_tokens, D) the
+    weighted sum, over its ``top_k`` experts ``e``, of
+    ``(silu(x @ gate_e) * (x @ up_e)) @ w_out_e``.
+
+    ``router`` (D, num_experts). ``w_in`` (num_experts, D, 2 F) holds gate and
+    up side by side, ``w_out`` (num_experts, F, D): tensors of x's type for
+    training (differentiable in everything), or both ``(wq, scale)`` pairs
+    of ``quantize_experts`` for serving in 8-bit integers, where a gradient
+    through the result raises."""
+    quantized = isinstance(w_in, (tuple, list))
+    if quantized != isinstance(w_out, (tuple, list)):
+        raise TypeError("expert_mlp: w_in and w_out must both be tensors or both be (wq, scale) pairs")
+    if not quantized:
+        return _layer(x, router, w_in, w_out, top_k, renormalize, False)
+    with torch.no_grad():
+        out = _layer(x, router, w_in, w_out, top_k, renormalize, True)
+    if torch.is_grad_enabled() and (x.requires_grad or router.requires_grad):
+        return _Served.apply(out, x, router)
+    return out

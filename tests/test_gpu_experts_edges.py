@@ -113,6 +113,24 @@ def test_forward_mode_is_refused(leaf):
                     torch.autograd.grad(out, args, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
 
 
+@pytest.mark.parametrize("leaf", ["x", "router"])
+def test_gradient_through_8_bits_is_refused(leaf):
+    """The 8-bit layer serves operands that require a gradient, and gives none of it instead of a part."""
+    g = gen(3)
+    x, router = randn(g, 10, 16), randn(g, 16, 4)
+    w_in, w_out = E.quantize_experts(randn(g, 4, 16, 32)), E.quantize_experts(randn(g, 4, 16, 16))
+    want = E.expert_mlp(x, router, w_in, w_out, 2)
+    assert not want.requires_grad
+    (x if leaf == "x" else router).requires_grad_()
+    with torch.no_grad():
+        assert torch.equal(E.expert_mlp(x, router, w_in, w_out, 2), want)
+    out = E.expert_mlp(x, router, w_in, w_out, 2)
+    assert torch.equal(out.detach(), want)
+    for loss in (out.sum(), (x + out).sum()):
+        with pytest.raises(RuntimeError, match="8-bit"):
+            loss.backward(retain_graph=True)
+
+
 # --------------------------------------------------------------------- threads
 
 def test_plans_of_many_experts_from_threads():
