@@ -20,6 +20,8 @@ wait that ran out) is raised by ``check_device_errors``.
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.autograd.forward_ad as _forward_ad
 
@@ -415,7 +417,7 @@ def quantize_experts(w: torch.Tensor):
     if not isinstance(w, torch.Tensor) or w.dim() < 2:
         raise ValueError("quantize_experts: w must be a tensor (..., K, N)")
     wt = w.detach().transpose(-1, -2).contiguous()
-    q, scale = quantize_rows(wt.reshape(-1, wt.shape[-1]))
+    q, scale = quantize_rows(wt.reshape(math.prod(wt.shape[:-1]), wt.shape[-1]))
     return q.reshape(wt.shape), scale.reshape(wt.shape[:-1])
 
 

@@ -84,6 +84,15 @@ def test_grouped_largest(sizes, N):
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
 
 
+# ------------------------------------------------------------------- empty weights
+
+@pytest.mark.parametrize("shape", [(3, 0, 5), (0, 4, 5), (3, 4, 0), (0, 0), (7, 0), (0, 7)])
+def test_quantize_experts_empty(shape):
+    q, s = E.quantize_experts(torch.zeros(shape, device=DEV))
+    assert q.dtype == torch.int8 and q.shape == (*shape[:-2], shape[-1], shape[-2])
+    assert s.dtype == torch.float32 and s.shape == (*shape[:-2], shape[-1]) and not s.any()
+
+
 # ------------------------------------------------------------- derivatives refused
 
 @pytest.mark.parametrize("leaf", [False, True])
