@@ -521,15 +521,24 @@ __device__ __forceinline__ float plane_sum(float first, float others) {
   return 4.0f * (fabsf(first) < INFINITY ? first + others : first);
 }
 
+// A row's scale in two factors, one of them 1: what is above 1 is multiplied last.
+// A sum (at least 1, or 0) times a scale of up to 1 neither overflows nor loses
+// bits, so that no step is infinite unless the result is.
+__device__ __forceinline__ float2 scale_parts(float x) {
+  return x > 1.0f ? make_float2(1.0f, x) : make_float2(x, 1.0f);
+}
+
+__device__ __forceinline__ float scaled(int sum, float first, float w, float last) {
+  return static_cast<float>(sum) * first * w * last;
+}
+
 // The 8-bit product's sums times the scales of their rows (xs) and channel.
-__device__ __forceinline__ void scale_block(float (&v)[32], const float* xs, float w) {
+__device__ __forceinline__ void scale_block(float (&v)[32], const float2* xs, float w) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < 32; i += 2) {
     const float4 x = *reinterpret_cast<const float4*>(xs + i);
-    v[i] = static_cast<float>(__float_as_int(v[i])) * x.x * w;
-    v[i + 1] = static_cast<float>(__float_as_int(v[i + 1])) * x.y * w;
-    v[i + 2] = static_cast<float>(__float_as_int(v[i + 2])) * x.z * w;
-    v[i + 3] = static_cast<float>(__float_as_int(v[i + 3])) * x.w * w;
+    v[i] = scaled(__float_as_int(v[i]), x.x, w, x.y);
+    v[i + 1] = scaled(__float_as_int(v[i + 1]), x.z, w, x.w);
   }
 }
 
@@ -541,7 +550,7 @@ constexpr int kAtOnce = 0;   // blocks stored at once, 16-bit tiles
 constexpr int kAtOnce32 = 3; // and fp32 tiles: the rest fits the registers
 
 template <typename T, bool I8, typename Release>
-__device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, const float* xs,
+__device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, const float2* xs,
                                            float w, Release release) {
   // all of the accumulator, whatever `rows`: no branch parts the registers' lives
   if constexpr (sizeof(T) == 2) {
@@ -658,7 +667,8 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
       int sum = 0;
 #pragma unroll
       for (int r = 0; r < 8; ++r) sum += __float_as_int(f[r]);
-      v = static_cast<float>(sum) * __shfl_sync(0xffffffffu, xs, i) * ws;
+      const float2 x = scale_parts(__shfl_sync(0xffffffffu, xs, i));
+      v = scaled(sum, x.x, ws, x.y);
     } else {
 #pragma unroll
       for (int r = 0; r < 8; ++r) v += f[r];
@@ -683,7 +693,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   constexpr int CG = S::CG, MT = S::MT, NT = S::NT, BK = S::BK, STAGES = S::kStages, PLANES = S::PLANES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ TcCtl ctl;
-  __shared__ alignas(16) float x_scales[S::KIND == kKindI8 ? 2 : 1][S::KIND == kKindI8 ? NT : 4];
+  __shared__ alignas(16) float2 x_scales[S::KIND == kKindI8 ? 2 : 1][S::KIND == kKindI8 ? NT : 4];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   float* part = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + STAGES * S::kStageBytes);
   int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(part) + S::kPartBytes);
@@ -963,13 +973,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int64_t out0 = (S::WGRAD ? at.expert * p.out_expert : 0) + at.row0 * p.out_col;
       // scales of 8-bit operands, loaded under the MMAs; two tiles' worth, so
       // that one barrier a tile is enough
-      const float* xs = x_scales[nth & 1];
+      const float2* xs = x_scales[nth & 1];
       float ws[MT];
       if constexpr (S::KIND == kKindI8) {
         const int c = threadIdx.x - 128;
         if (c < NT) {
           const int64_t tok = c < at.rows ? p.g.source(at.row0 + c) : -1;
-          x_scales[nth & 1][c] = tok >= 0 ? p.g.x_scale[tok] : 0.0f;
+          x_scales[nth & 1][c] = scale_parts(tok >= 0 ? p.g.x_scale[tok] : 0.0f);
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)

@@ -84,6 +84,26 @@ def test_grouped_largest(sizes, N):
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
 
 
+# --------------------------------------------------------------- 8-bit scales
+
+@pytest.mark.parametrize("rows,N", [(3, 40), (70, 1000), (700, 5000)])
+@pytest.mark.parametrize("grouped", [False, True])
+def test_int8_scales_of_any_size(rows, N, grouped):
+    """Large scales of rows and small ones of channels, or the reverse: finite products stay finite."""
+    g = gen(rows + N)
+    K = 1040
+    plan = make_plan([rows // 3, 0, rows - rows // 3], 1) if grouped else None
+    q, wq = int8s(g, rows, K), int8s(g, *((3, N, K) if grouped else (N, K)))
+    q[0], wq[..., 0, :], wq[..., 1, :] = 127, -127, 0  # the largest sum, and sums of zero
+    for big, small in ((3e35, 1e-35), (1e-37, 3e33), (2e15, 1e14), (1e-19, 1e-18)):
+        s, ws = ((1 + torch.rand(*shape, generator=g, device=DEV)) * scale
+                 for shape, scale in (((rows,), big), (wq.shape[:-1], small)))
+        y = E.int8_matmul(q, s, wq, ws, plan, out_dtype=torch.float32)
+        ref = int8_ref(q, s, wq, ws, plan, False)
+        assert bool(((ref.abs() > 2e-38) & (ref.abs() < 3.4e38) | (ref == 0)).all())
+        check_int8(y, ref, torch.float32)
+
+
 # ------------------------------------------------------------------- empty weights
 
 @pytest.mark.parametrize("shape", [(3, 0, 5), (0, 4, 5), (3, 4, 0), (0, 0), (7, 0), (0, 7)])
