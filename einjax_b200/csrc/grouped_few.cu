@@ -50,9 +50,10 @@ constexpr int kPlaneBytes = 12288;  // of x in shared memory: chunk x rows
 constexpr int64_t kFewMean = 24;
 constexpr int64_t kMaxDepth = 1 << 30;  // counted in 32 bits
 
-// The n-th tile of up to kFewRows rows of one expert; false: there is none.
-__device__ __forceinline__ bool nth_tile(const GroupedArgs& g, int n, int& expert, int64_t& r0, int64_t& hi) {
-  __shared__ int64_t found[3];
+// The n-th tile of up to kFewRows rows of one expert, left in shared memory too (expert,
+// first row, end); false: there is none.
+__device__ __forceinline__ bool nth_tile(const GroupedArgs& g, int n, int& expert, int64_t& r0, int64_t& hi,
+                                         int64_t* found) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
     int64_t at = -1, a = 0, b = 0, seen = 0;
@@ -194,7 +195,7 @@ __device__ __forceinline__ void multiply(float (*main)[NT][4], float (*small)[NT
 
 template <bool COLUMNS, int NT>
 __device__ __forceinline__ void few_tile(const GroupedArgs& g, const float* x, const float* we, float* y, bool wide,
-                                         int64_t n0, int64_t r0, int64_t hi, uint2* planes, int64_t* src) {
+                                         int64_t n0, int64_t r0, int64_t hi, uint2* planes, int64_t* src, int* again) {
   constexpr int CHUNK = kPlaneBytes / 2 / (8 * NT), STEPS = CHUNK / kStep / kShares;
   static_assert(STEPS % 2 == 0 && kShares * 8 * NT * kTileCols * 4 <= kPlanes * kPlaneBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = warp / kGroups, t = lane & 3, q = lane >> 2;
@@ -262,13 +263,70 @@ __device__ __forceinline__ void few_tile(const GroupedArgs& g, const float* x, c
     float s = 0.0f;
 #pragma unroll
     for (int h = 0; h < kShares; ++h) s += sums[(h * 8 * NT + row) * kTileCols + c];
-    // Infinities have no planes, nor has a value that rounds to one: from the values themselves.
-    if (!isfinite(s) && src[row] >= 0) {
-      s = 0.0f;
-      for (int64_t k = 0; k < g.K; ++k)
-        s = fmaf(x[src[row] * g.x_stride + k], we[(n0 + c) * g.w_n + k * g.w_k], s);
-    }
+    if (!isfinite(s) && src[row] >= 0) atomicOr(again, 1 << row);
     y[(r0 + row) * g.N + n0 + c] = s;
+  }
+}
+
+// Sums of the CTA's channels that are not finite, in the rows of `left`: made again from the
+// values, in fp32, since infinities have no planes, nor has a value that rounds to one. A NaN
+// in a row of x (a poisoned token) has made all its sums NaN already. Four threads share
+// a channel's depth; four rows are made from one reading of the weights. 36 experts of 2520
+// x 1456, 8 rows each, 104 us: 130 with an infinity in one row, 683 with one in every row,
+// 124 with a NaN in every row.
+__device__ __forceinline__ void sums_again(const GroupedArgs& g, const float* x, const int64_t* src, const float* we,
+                                           float* y, int64_t n0, int left, float* part) {
+  constexpr int kParts = kFewThreads / kTileCols, kAtOnce = 4;
+  static_assert(kAtOnce == kParts, "one thread for each row and channel in the end");
+  for (int rows = left; rows; rows &= rows - 1) {
+    const int row = __ffs(rows) - 1;
+    const float* xr = x + src[row] * g.x_stride;
+    bool nan = false;
+    for (int64_t k = threadIdx.x; k < g.K; k += kFewThreads) nan |= isnan(xr[k]);
+    if (__syncthreads_or(nan)) left &= ~(1 << row);
+  }
+  const int c = threadIdx.x % kTileCols, p = threadIdx.x / kTileCols;
+  while (left) {
+    int row[kAtOnce];  // the last of them again where there are fewer
+    bool any = false;
+    float s[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      row[i] = left ? __ffs(left) - 1 : row[i > 0 ? i - 1 : 0];
+      left &= left - 1;
+      any |= n0 + c < g.N && !isfinite(y[row[i] * g.N + n0 + c]);
+      s[i] = 0.0f;
+    }
+    if (any) {
+      const float* w = we + (n0 + c) * g.w_n;
+#pragma unroll 4
+      for (int64_t k = p; k < g.K; k += kParts) {
+        const float v = w[k * g.w_k];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) s[i] = fmaf(x[src[row[i]] * g.x_stride + k], v, s[i]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) part[i * kFewThreads + threadIdx.x] = s[i];
+    __syncthreads();
+    // thread (p, c) has the p-th of the rows
+    int mine = row[0];
+    bool there = n0 + c < g.N;
+#pragma unroll
+    for (int i = 1; i < kAtOnce; ++i)
+      if (p == i) {
+        mine = row[i];
+        there &= row[i] != row[i - 1];
+      }
+    float* to = y + mine * g.N + n0 + c;
+    if (there && !isfinite(*to)) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) sum += part[p * kFewThreads + i * kTileCols + c];
+      *to = sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -277,17 +335,25 @@ __global__ void __launch_bounds__(kFewThreads, 2) few_kernel(const __grid_consta
                                                              const float* w, float* y, bool wide) {
   __shared__ alignas(16) uint2 planes[kPlanes * kPlaneBytes / 8];
   __shared__ int64_t src[kFewRows];
+  __shared__ int64_t found[3];
+  __shared__ int again;  // rows with a sum that is not finite
+  if (threadIdx.x == 0) again = 0;
   const int64_t n0 = blockIdx.x * static_cast<int64_t>(kTileCols), n1 = min(n0 + kTileCols, g.N);
   for (int64_t r = g.kept() + blockIdx.y; r < g.rows; r += gridDim.y)
     for (int64_t n = n0 + threadIdx.x; n < n1; n += kFewThreads) y[r * g.N + n] = 0.0f;
   int e;
   int64_t r0, hi;
-  if (!nth_tile(g, blockIdx.y, e, r0, hi)) return;
+  if (!nth_tile(g, blockIdx.y, e, r0, hi, found)) return;
   const float* we = w + e * g.w_e;
   if (hi - r0 > 8)
-    few_tile<COLUMNS, 2>(g, x, we, y, wide, n0, r0, hi, planes, src);
+    few_tile<COLUMNS, 2>(g, x, we, y, wide, n0, r0, hi, planes, src, &again);
   else
-    few_tile<COLUMNS, 1>(g, x, we, y, wide, n0, r0, hi, planes, src);
+    few_tile<COLUMNS, 1>(g, x, we, y, wide, n0, r0, hi, planes, src, &again);
+  __syncthreads();
+  // from shared memory: nothing of this is held in registers through the product
+  if (again)
+    sums_again(g, x, src, w + found[0] * g.w_e, y + found[1] * g.N, blockIdx.x * static_cast<int64_t>(kTileCols), again,
+               reinterpret_cast<float*>(planes));
 }
 
 bool by_columns(const GroupedArgs& g) { return g.w_n == 1 && g.N > 1; }

@@ -84,6 +84,49 @@ def test_grouped_largest(sizes, N):
     near(y / 2.0 ** 64, ry / 2.0 ** 64, my / 2.0 ** 64, K, torch.float32)
 
 
+@pytest.mark.parametrize("K,N", [(260, 132), (2520, 68), (8, 200)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_grouped_few_rows_all_infinite(K, N, transposed):
+    """Every row of several tiles holds an infinity, or a NaN beside it, or the weights do."""
+    sizes = [19, 0, 7, 16, 1]
+    plan = make_plan(sizes, 1)
+    g = gen(K)
+    x, w = randn(g, plan.num_rows, K), randn(g, 5, K, N, scale=K ** -0.5)
+    rows = torch.arange(plan.num_rows, device=DEV)
+    x[rows, rows % K] = math.inf * (1 - 2 * (rows % 2).float())
+    x[rows[::5], (rows[::5] + 3) % K] = math.nan
+    x[4] = 0.0
+    w[0, :, 7], w[2, 1, N - 1], w[3, K - 1, ::3] = 0.0, math.nan, math.inf
+    if transposed:
+        w = w.transpose(1, 2).contiguous().transpose(1, 2)
+    y = E.grouped_matmul(x, w, plan)
+    same_kinds(y, grouped_ref(x, w, plan, False)[0])
+
+
+def test_grouped_few_rows_poisoned_time():
+    """Rows that are NaN take about the time of rows that are not."""
+    plan = make_plan([8] * 12, 1)
+    g = gen(1)
+    w = randn(g, 12, 2048, 1024)
+    clean = randn(g, 96, 2048)
+    bad = torch.full_like(clean, math.nan)
+
+    def microseconds(x):
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                E.grouped_matmul(x, w, plan)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 100)
+        return best
+
+    microseconds(clean)
+    assert microseconds(bad) <= 2 * microseconds(clean)
+
+
 # --------------------------------------------------------------- 8-bit scales
 
 @pytest.mark.parametrize("rows,N", [(3, 40), (70, 1000), (700, 5000)])
