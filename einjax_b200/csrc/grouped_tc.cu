@@ -25,10 +25,15 @@
 // block of depth takes three stages, one for each plane, and the six products
 // b_i b_j with i + j <= 2 are made from them (each operand crosses from L2
 // once): b0 b0 into one accumulator, the other five, at most 2^-8 of it, into a
-// second. What is left out is at most 2^-24 of a product. An accumulator
-// truncates each step's sum (measured: a relative error of 1e-9 a unit of
-// depth), so a sum is cut into chains of 512 that the epilogue adds in fp32; a
-// 16-bit result, rounded at 2^-9, keeps one chain.
+// second. What is left out is at most 2^-24 of a product.
+//
+// Long sums. An accumulator truncates what it adds, so sums of one sign come out
+// low (measured, relative, bf16 / f16 operands: 7e-7 / 2.5e-6 at a depth of 512, 1.1e-5 /
+// 2.3e-5 at 4096, 1.4e-4 / 1.2e-4 at 16384, 1.1e-3 / 8e-4 at 131072). fp32 sums are
+// therefore cut into chains of 448, which the epilogue adds in fp32 (6e-7 at any depth).
+// 16-bit results keep one chain while its error is a quarter of their rounding
+// (one_chain); longer sums (DEEP) are chains of 4096 whose fp32 total stands beside the
+// accumulator in TMEM.
 //
 // Bounds (B200, measured): 16384 rows, 8 experts, 4096 x 8192, bf16 759 us
 // forward, the tensor pipe 84% active (on equal groups 88%, as cuBLAS's product
@@ -83,6 +88,7 @@ struct TcArgs {
   int src_rows;       // rows of the weights' gradient's operands: this row index reads zeros
   uint32_t idesc;     // instruction descriptor without N
   int pairs;          // two neighbouring lanes may be stored together
+  int most;           // weights' gradient: groups of more rows than this are the DEEP kernel's
   int32_t* status;
 };
 
@@ -325,7 +331,7 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 
 // ------------------------------------------------------------------- kernel
 
-template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_>
+template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_, bool DEEP_ = false>
 struct TcShape {
   static constexpr int CG = CG_;        // CTAs of one MMA
   static constexpr int MT = MT_;        // accumulators of 128 lanes (of each CTA) that share B
@@ -336,17 +342,26 @@ struct TcShape {
   static constexpr bool SPLIT = SPLIT_; // the cluster's CTAs share one tile's depth
   static constexpr int PLANES = PLANES_;
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
-  static constexpr int kChain = PLANES > 1 ? 8 : 1 << 30;  // blocks of depth between fp32 additions
+  static constexpr bool DEEP = DEEP_;   // an fp32 total in TMEM
+  static constexpr int kChain = PLANES > 1 ? 7 : DEEP ? 64 : 1 << 30;  // blocks of depth between fp32 additions
   static constexpr int kLanes = 128 * MT * CG;
   static constexpr int kAccs = PLANES > 1 ? 2 : MT;         // accumulators of a tile
-  static constexpr int kBufs = 2 * kAccs * NT <= 512 ? 2 : 1;  // tiles in TMEM
-  static constexpr bool kHeld = kBufs == 1 && PLANES == 1;  // tiles are held in registers, see drain_held
+  static constexpr int kTotal = DEEP ? NT : 0;              // columns of the total
+  static constexpr int kBufs = 2 * kAccs * NT + kTotal <= 512 ? 2 : 1;  // tiles in TMEM
+  static constexpr int kUsed = kBufs * kAccs * NT + kTotal;
+  static constexpr int kColumns = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;  // allocated
+  static constexpr bool kHeld = kBufs == 1 && PLANES == 1 && !DEEP;  // tiles are held in registers, see drain_held
+  static constexpr bool kSums = PLANES > 1 && !WGRAD && !SPLIT;  // the epilogue adds chains in registers
   static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;  // one plane of a block of depth
   static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
   static_assert(PLANES == 1 || MT == 1, "planes take the tiles that accumulators would share B with");
   static_assert(kStages > PLANES, "a block's planes and the next block's first");
+  static_assert(kUsed <= 512 && !(DEEP && (MT > 1 || PLANES > 1 || SPLIT)), "one accumulator and its total");
+
+  // Tiles that the other kernel of the same call makes.
+  __device__ static __forceinline__ bool skips(int depth, int most) { return WGRAD && (depth > most) != DEEP; }
 };
 
 // One output tile, and what of its depth this CTA multiplies.
@@ -725,7 +740,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ctl.progress = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kBufs * S::kAccs * NT);
+  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kColumns);
   wait_for_earlier_grids();
   if (warp == 2) {  // tiles of each group
     int run = 0;
@@ -767,6 +782,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool ok = true;
       for (int t = t0; t < tiles.total && ok; t += step) {
         const TileAt at = tiles.at(t, rank, csize);
+        if (S::skips(at.depth, p.most)) continue;
         const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
         const int half = width / CG;  // columns of this CTA's part of B
         const int lane0 = static_cast<int>(at.lane0) + static_cast<int>(pair_rank) * 128;
@@ -880,7 +896,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         bool ok = true;
         for (int t = t0; t < tiles.total && ok; t += step) {
           const TileAt at = tiles.at(t, rank, csize);
-          if (at.kb0 == at.kb1) continue;
+          if (at.kb0 == at.kb1 || S::skips(at.depth, p.most)) continue;
           const int width = (at.rows + 16 * CG - 1) / (16 * CG) * (16 * CG);
           const uint32_t idesc = p.idesc | (static_cast<uint32_t>(width >> 3) << 17);
           for (int s0 = at.kb0; s0 < at.kb1 && ok; s0 += min(S::kChain, at.kb1 - s0)) {
@@ -964,6 +980,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint32_t acc_phase = 0, red_phase = 0, nth = 0;
     for (int t = t0; t < tiles.total; t += step) {
       const TileAt at = tiles.at(t, rank, csize);
+      if (S::skips(at.depth, p.most)) continue;
       const int64_t ch0 = at.lane0 + pair_rank * 128 + quad * 32 + lane;
       const int blocks = (at.rows + 31) / 32;
       if constexpr (S::SPLIT) {
@@ -995,6 +1012,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       bool ok = true;
       int s0 = at.kb0;
+      float total[S::kSums ? NT / 64 : 1][32];
       do {  // the chains of the sum; one pass over zeros where there is no depth
         const bool any = s0 < at.kb1, first = s0 == at.kb0;
         if (any) {
@@ -1029,6 +1047,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             released = true;
           }
         }
+        if constexpr (S::kSums) {  // the chains' sum stays in registers
+#pragma unroll
+          for (int i = 0; i < NT / 64; ++i) {
+            const int c0 = (set + 2 * i) * 32;
+            if (c0 < at.rows) {
+              float v[32], u[32];
+              tmem_ld32(acc + c0, v);
+              tmem_ld32(acc + NT + c0, u);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float s = plane_sum(v[j], u[j]);
+                total[i][j] = first ? s : total[i][j] + s;
+              }
+            }
+          }
+          release();
+          released = true;
+          if (s0 + S::kChain >= at.kb1) {
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) {
+              const int c0 = (set + 2 * i) * 32;
+              if (c0 < at.rows)
+                store_cols(static_cast<float*>(p.out) + out0 + c0 * p.out_col + ch0, p.out_col, total[i], at.rows - c0,
+                           ch0 < p.lanes, false);
+            }
+          }
+        }
         for (int b = set; b < MT * blocks && (!released || !any); b += 2) {
           const int m = b / blocks, c0 = (b - m * blocks) * 32, n = at.rows - c0;
           const int64_t ch = ch0 + m * 128 * CG;
@@ -1041,6 +1086,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               tmem_ld32(acc + NT + c0, u);
 #pragma unroll
               for (int i = 0; i < 32; ++i) v[i] = plane_sum(v[i], u[i]);
+            }
+            if constexpr (S::DEEP) {  // each warp has its own part of the total
+              const uint32_t total = acc + (S::kBufs - buf) * S::kAccs * NT + c0;
+              if (!first) {
+                float u[32];
+                tmem_ld32(total, u);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] += u[i];
+              }
+              if (s0 + S::kChain < at.kb1) {
+                tmem_st32(total, v);
+                continue;
+              }
             }
           } else {
 #pragma unroll
@@ -1082,7 +1140,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   if (csize > 1) cluster_sync();
   tc_fence_after();
-  if (warp == 1) tc_dealloc<CG>(tmem, S::kBufs * S::kAccs * NT);
+  if (warp == 1) tc_dealloc<CG>(tmem, S::kColumns);
 }
 
 // --------------------------------------------------------------------- host
@@ -1374,8 +1432,15 @@ int launch(const TcArgs& p, const TcMaps& m, int64_t max_tiles, int csize, cudaS
 
 constexpr int64_t kMaxTiles = 0x7fffffffLL;
 
+// The depth up to which a sum with a 16-bit result is one chain: its truncation (1.2e-4 at
+// 16384 in f16, 7e-4 at 65536 in bf16, relative, of sums of one sign) is then a quarter of
+// half a unit in the result's last place (4.9e-4, 3.9e-3). Longer ones take a half to two
+// thirds longer: f16, 4096 rows x 20480 x 4096 780 us (one chain 500), the weights' gradient
+// of 4 groups of 65536 rows, 2048 x 2048, 2300 (1570).
+int64_t one_chain(int dtype) { return dtype == ES_F16 ? 16384 : 65536; }
+
 template <int KIND, bool A_MN, int PLANES>
-int rows_launch(TcArgs& p, const TcMaps& m, cudaStream_t stream) {
+int rows_launch(TcArgs& p, const TcMaps& m, int dtype, cudaStream_t stream) {
   using Wide = std::conditional_t<PLANES == 1, TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>,
                                   TcShape<2, 1, 128, KIND, A_MN, false, false, PLANES>>;
   using Middle = TcShape<1, 2, 128, KIND, A_MN, false, false, 1>;
@@ -1394,14 +1459,19 @@ int rows_launch(TcArgs& p, const TcMaps& m, cudaStream_t stream) {
   // bits Wide gains from 300 rows (224: 105 and 111, 300: 142 and 126).
   const int64_t wide = tiles(Wide::kLanes, Wide::NT);
   const int64_t least = PLANES > 1 ? 8 : KIND == kKindI8 ? 240 : 160;
+  const bool one = PLANES > 1 || KIND == kKindI8 || p.g.K <= one_chain(dtype);
   if (mean > least && wide >= kSMs / 2) {
     p.idesc |= 16u << 24;
+    if constexpr (PLANES == 1 && KIND == kKindF16) {
+      using Deep = TcShape<2, 1, 256, KIND, A_MN, false, false, 1, true>;
+      if (!one) return launch<Deep>(p, m, tiles(Deep::kLanes, Deep::NT), 2, stream);
+    }
     return launch<Wide>(p, m, wide, 2, stream);
   }
   p.idesc |= 8u << 24;
   if constexpr (PLANES == 1) {
     const int64_t middle = tiles(Middle::kLanes, Middle::NT);
-    if (mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
+    if (one && mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
   }
   // few rows, or few tiles: a tile's depth is shared by a cluster while the
   // tiles alone do not fill the SMs
@@ -1409,7 +1479,11 @@ int rows_launch(TcArgs& p, const TcMaps& m, cudaStream_t stream) {
   const int64_t nkb = (p.g.K + Split::BK - 1) / Split::BK;
   int split = 1;
   while (split < 8 && narrow * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
-  if (split > 1) return launch<Split>(p, m, narrow, split, stream);
+  if (split > 1 && (one || p.g.K <= split * one_chain(dtype))) return launch<Split>(p, m, narrow, split, stream);
+  if constexpr (PLANES == 1 && KIND == kKindF16) {
+    using Deep = TcShape<1, 1, 64, KIND, A_MN, false, false, 1, true>;
+    if (!one) return launch<Deep>(p, m, narrow, 1, stream);
+  }
   return launch<Narrow>(p, m, narrow, 1, stream);
 }
 
@@ -1487,10 +1561,10 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
   if (!bind_context() || !encode_operand(o.w, dtype, o.mn ? 64 : bk, o.mn ? 64 : 128, 3, &m.a) ||
       !encode_operand(o.x, dtype, bk, kBoxRows, 2, &m.b))
     return ES_ERR_CUDA;
-  if (dtype == kInt8) return rows_launch<kKindI8, false, 1>(p, m, stream);
+  if (dtype == kInt8) return rows_launch<kKindI8, false, 1>(p, m, dtype, stream);
   if (dtype == ES_F32)
-    return o.mn ? rows_launch<kKindF16, true, 3>(p, m, stream) : rows_launch<kKindF16, false, 3>(p, m, stream);
-  return o.mn ? rows_launch<kKindF16, true, 1>(p, m, stream) : rows_launch<kKindF16, false, 1>(p, m, stream);
+    return o.mn ? rows_launch<kKindF16, true, 3>(p, m, dtype, stream) : rows_launch<kKindF16, false, 3>(p, m, dtype, stream);
+  return o.mn ? rows_launch<kKindF16, true, 1>(p, m, dtype, stream) : rows_launch<kKindF16, false, 1>(p, m, dtype, stream);
 }
 
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype) {
@@ -1538,8 +1612,16 @@ int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void*
       !encode_operand(a, dtype, 64, 1, 2, &m.a_rows) || !encode_operand(b, dtype, 64, 1, 2, &m.b_rows))
     return ES_ERR_CUDA;
   const int64_t tiles = static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles;
+  p.most = static_cast<int>(kMaxTiles);
   if (dtype == ES_F32) return launch<Tile32>(p, m, tiles, 2, stream);
-  return launch<Tile>(p, m, tiles, 2, stream);
+  if (g.rows <= one_chain(dtype)) return launch<Tile>(p, m, tiles, 2, stream);
+  // groups may be longer than one chain: those have a kernel of their own
+  p.most = static_cast<int>(one_chain(dtype));
+  ES_TRY(launch<Tile>(p, m, tiles, 2, stream));
+  using Deep = TcShape<2, 1, 256, kKindF16, true, true, false, 1, true>;
+  p.lane_tiles = static_cast<int>((p.lanes + Deep::kLanes - 1) / Deep::kLanes);
+  p.col_tiles = static_cast<int>((p.cols + Deep::NT - 1) / Deep::NT);
+  return launch<Deep>(p, m, static_cast<int64_t>(g.groups()) * p.lane_tiles * p.col_tiles, 2, stream);
 }
 
 }  // namespace es

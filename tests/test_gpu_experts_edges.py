@@ -127,6 +127,62 @@ def test_grouped_few_rows_poisoned_time():
     assert microseconds(bad) <= 2 * microseconds(clean)
 
 
+# ----------------------------------------------------------- long sums of one sign
+
+def positive(g, *shape, dtype, scale=1.0):
+    return (torch.rand(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def unbiased(got, ref, n):
+    """Positive sums of n products. Where they are rounded once, to nearest, the mean error over many is a small part
+    of the rounding's unit; a third leaves room for an accumulator that truncates."""
+    near(got, ref, ref, n, got.dtype)
+    unit = max(UNIT[got.dtype], 2.0 ** -19)
+    assert abs(float(((got.double() - ref) / ref).mean())) <= unit / 3
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes", [[131072, 300], [16384, 0, 16385, 70000], [7, 20000, 65536, 3]])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_long_groups_weights_gradient(dtype, sizes, transposed):
+    plan = make_plan(sizes, 1, dropped=5)
+    g = gen(len(sizes))
+    K, N = 40, 23 if transposed else 136
+    x = positive(g, plan.num_rows, K, dtype=dtype)
+    w = torch.zeros(len(sizes), *((N, K) if transposed else (K, N)), dtype=dtype, device=DEV)
+    w = (w.transpose(1, 2) if transposed else w).requires_grad_()
+    dy = positive(g, plan.num_rows, N, dtype=dtype, scale=2.0 ** -6)
+    dw, = torch.autograd.grad(E.grouped_matmul(x, w, plan), w, dy)
+    off = plan.offsets.tolist()
+    for e, n in enumerate(sizes):
+        r = slice(off[e], off[e + 1])
+        if n:
+            unbiased(dw[e], x[r].double().t() @ dy[r].double(), n)
+        else:
+            assert not dw[e].any()
+
+
+@pytest.mark.parametrize("dtype,K", [(torch.float16, 20000), (torch.float16, 16384), (torch.bfloat16, 66000),
+                                     (torch.float32, 20000)])
+@pytest.mark.parametrize("sizes,N", [([30], 9608), ([5, 0, 2], 136), ([700], 12301)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_deep_rows(dtype, K, sizes, N, transposed):
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    plan = make_plan(sizes, 1, dropped=1)
+    g = gen(N)
+    x = positive(g, plan.num_rows, K, dtype=dtype)
+    w = positive(g, len(sizes), *((N, K) if transposed else (K, N)), dtype=dtype, scale=2.0 ** -6)
+    w = w.transpose(1, 2) if transposed else w
+    y = E.grouped_matmul(x, w, plan)
+    off = plan.offsets.tolist()
+    for e in range(len(sizes)):
+        if sizes[e]:
+            r = slice(off[e], off[e + 1])
+            unbiased(y[r], x[r].double() @ w[e].double(), K)
+    assert not y[off[-1]:].any()
+
+
 # --------------------------------------------------------------- 8-bit scales
 
 @pytest.mark.parametrize("rows,N", [(3, 40), (70, 1000), (700, 5000)])
