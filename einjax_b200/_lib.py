@@ -19,6 +19,8 @@ ES_OK, ES_ERR_INVALID, ES_ERR_INDEX, ES_ERR_WORKSPACE, ES_ERR_CUDA, ES_ERR_UNSUP
 ES_F32, ES_BF16, ES_F64, ES_I32, ES_I64, ES_F16 = range(6)
 ES_PREC_AUTO, ES_PREC_EXACT, ES_PREC_TC = range(3)
 ES_DUP_LAST, ES_DUP_SUM = range(2)
+(ES_GROUPED_FEW, ES_GROUPED_NARROW, ES_GROUPED_SPLIT, ES_GROUPED_MIDDLE, ES_GROUPED_WIDE, ES_GROUPED_DEEP_NARROW,
+ ES_GROUPED_DEEP_WIDE) = range(7)
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
@@ -86,6 +88,8 @@ SIGNATURES = {
                                                  c_i64, c_vp, c_vp, c_int, c_i64]),
     "es_grouped_matmul": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
                                   c_vp, c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
+    "es_grouped_matmul_path": (c_int, [c_int, c_int, c_i64, c_i64, c_i64]),
+    "es_int8_matmul_path": (c_int, [c_int, c_i64, c_i64, c_i64]),
     "es_grouped_matmul_wgrad_workspace_size": (c_sz, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_i64, c_i64,
                                                        c_vp, c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_i64]),
     "es_grouped_matmul_wgrad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp,

@@ -80,6 +80,19 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
   return grouped_rows_tc(g, dtype, x, w, y, out_dtype, workspace, status, s);
 }
 
+extern "C" int es_grouped_matmul_path(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows) {
+  const GroupedArgs g{num_experts, K, N, num_rows, num_rows, K, 1, nullptr, nullptr, K * N, N, 1, nullptr, nullptr};
+  if (num_experts < 1 || num_experts > kMaxExperts || !value_type(dtype) || empty(g)) return -1;
+  if (grouped_rows_few_ok(g, dtype, nullptr)) return ES_GROUPED_FEW;
+  return grouped_rows_tc_ok(g, dtype) ? grouped_rows_tc_path(g, dtype) : -1;
+}
+
+extern "C" int es_int8_matmul_path(int num_experts, int64_t K, int64_t N, int64_t num_rows) {
+  const GroupedArgs g{num_experts, K, N, num_rows, num_rows, K, 1, nullptr, nullptr, K * N, 1, K, nullptr, nullptr};
+  if (num_experts < 0 || num_experts > kMaxExperts || K > kMaxInt8Depth || empty(g)) return -1;
+  return grouped_rows_tc_ok(g, kInt8) ? grouped_rows_tc_path(g, kInt8) : -1;
+}
+
 extern "C" size_t es_grouped_matmul_wgrad_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride,
                                                          const void* dy, int64_t dy_stride, int num_experts, int64_t K,
                                                          int64_t N, const int32_t* offsets, const int32_t* order,

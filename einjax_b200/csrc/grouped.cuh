@@ -58,6 +58,7 @@ int grouped_rows_few(const GroupedArgs& g, const void* x, const void* w, void* y
 // Tensor-core forms (grouped_tc.cu). The workspace holds copies of what TMA
 // cannot read as it lies.
 bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype);
+int grouped_rows_tc_path(const GroupedArgs& g, int dtype);  // an es_grouped_path
 size_t grouped_rows_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w);
 int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
                     void* workspace, int32_t* status, cudaStream_t stream);

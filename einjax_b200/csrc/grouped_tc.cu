@@ -1439,6 +1439,47 @@ constexpr int64_t kMaxTiles = 0x7fffffffLL;
 // of 4 groups of 65536 rows, 2048 x 2048, 2300 (1570).
 int64_t one_chain(int dtype) { return dtype == ES_F16 ? 16384 : 65536; }
 
+// The kernel shape of a rows' product, and its tiles of lanes x cols.
+struct RowsForm {
+  int path;
+  int lanes, cols;
+  int split;  // CTAs that share a tile's depth
+  int64_t tiles;
+};
+
+RowsForm rows_form(const GroupedArgs& g, int dtype) {
+  const int64_t R = g.rows, groups = g.groups();
+  const int64_t live = groups < R ? groups : R;  // groups that can have rows
+  const int64_t mean = R / live;
+  auto form = [&](int path, int lanes, int cols) {
+    return RowsForm{path, lanes, cols, 1, (R / cols + live) * ((g.N + lanes - 1) / lanes)};
+  };
+  // By the rows of a group, where the tiles then fill the SMs. 60 experts,
+  // 2048 x 2816, bf16, us for Narrow, Middle, Wide: 8 rows 104, 107, 118; 24
+  // rows 118, 111, 119; 144 rows 339, 144, 154; 176 rows 397, 173, 160. In 8
+  // bits Wide gains from 300 rows (224: 105 and 111, 300: 142 and 126).
+  const bool f32 = dtype == ES_F32, i8 = dtype == kInt8;
+  const RowsForm wide = form(ES_GROUPED_WIDE, f32 ? 256 : 512, f32 ? 128 : 256);
+  const int64_t least = f32 ? 8 : i8 ? 240 : 160;
+  const bool one = f32 || i8 || g.K <= one_chain(dtype);
+  if (mean > least && wide.tiles >= kSMs / 2) return one ? wide : form(ES_GROUPED_DEEP_WIDE, 256, 256);
+  const RowsForm middle = form(ES_GROUPED_MIDDLE, 256, 128);
+  if (!f32 && one && mean > 8 && middle.tiles >= kSMs) return middle;
+  // few rows, or few tiles: a tile's depth is shared by a cluster while the
+  // tiles alone do not fill the SMs
+  RowsForm narrow = form(ES_GROUPED_NARROW, 128, 64);
+  const int64_t bk = i8 ? 128 : 64, nkb = (g.K + bk - 1) / bk;
+  int split = 1;
+  while (split < 8 && narrow.tiles * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
+  if (split > 1 && (one || g.K <= split * one_chain(dtype))) {
+    narrow.path = ES_GROUPED_SPLIT;
+    narrow.split = split;
+  } else if (!one) {
+    narrow.path = ES_GROUPED_DEEP_NARROW;
+  }
+  return narrow;
+}
+
 template <int KIND, bool A_MN, int PLANES>
 int rows_launch(TcArgs& p, const TcMaps& m, int dtype, cudaStream_t stream) {
   using Wide = std::conditional_t<PLANES == 1, TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>,
@@ -1446,45 +1487,26 @@ int rows_launch(TcArgs& p, const TcMaps& m, int dtype, cudaStream_t stream) {
   using Middle = TcShape<1, 2, 128, KIND, A_MN, false, false, 1>;
   using Narrow = TcShape<1, 1, 64, KIND, A_MN, false, false, PLANES>;
   using Split = TcShape<1, 1, 64, KIND, A_MN, false, true, PLANES>;
-  const int64_t R = p.g.rows, groups = p.g.groups();
-  const int64_t live = groups < R ? groups : R;  // groups that can have rows
-  const int64_t mean = R / live;
-  auto tiles = [&](int lanes, int nt) {
-    p.lane_tiles = static_cast<int>((p.lanes + lanes - 1) / lanes);
-    return (R / nt + live) * p.lane_tiles;
+  using DeepWide = TcShape<2, 1, 256, kKindF16, A_MN, false, false, 1, true>;
+  using DeepNarrow = TcShape<1, 1, 64, kKindF16, A_MN, false, false, 1, true>;
+  const RowsForm f = rows_form(p.g, dtype);
+  p.lane_tiles = static_cast<int>((p.lanes + f.lanes - 1) / f.lanes);
+  auto go = [&](auto shape, int csize) {
+    using S = decltype(shape);
+    if (f.lanes != S::kLanes || f.cols != S::NT) return static_cast<int>(ES_ERR_INVALID);
+    p.idesc |= S::CG == 2 ? 16u << 24 : 8u << 24;
+    return launch<S>(p, m, f.tiles, csize, stream);
   };
-  // By the rows of a group, where the tiles then fill the SMs. 60 experts,
-  // 2048 x 2816, bf16, us for Narrow, Middle, Wide: 8 rows 104, 107, 118; 24
-  // rows 118, 111, 119; 144 rows 339, 144, 154; 176 rows 397, 173, 160. In 8
-  // bits Wide gains from 300 rows (224: 105 and 111, 300: 142 and 126).
-  const int64_t wide = tiles(Wide::kLanes, Wide::NT);
-  const int64_t least = PLANES > 1 ? 8 : KIND == kKindI8 ? 240 : 160;
-  const bool one = PLANES > 1 || KIND == kKindI8 || p.g.K <= one_chain(dtype);
-  if (mean > least && wide >= kSMs / 2) {
-    p.idesc |= 16u << 24;
-    if constexpr (PLANES == 1 && KIND == kKindF16) {
-      using Deep = TcShape<2, 1, 256, KIND, A_MN, false, false, 1, true>;
-      if (!one) return launch<Deep>(p, m, tiles(Deep::kLanes, Deep::NT), 2, stream);
-    }
-    return launch<Wide>(p, m, wide, 2, stream);
-  }
-  p.idesc |= 8u << 24;
-  if constexpr (PLANES == 1) {
-    const int64_t middle = tiles(Middle::kLanes, Middle::NT);
-    if (one && mean > 8 && middle >= kSMs) return launch<Middle>(p, m, middle, 1, stream);
-  }
-  // few rows, or few tiles: a tile's depth is shared by a cluster while the
-  // tiles alone do not fill the SMs
-  const int64_t narrow = tiles(Narrow::kLanes, Narrow::NT);
-  const int64_t nkb = (p.g.K + Split::BK - 1) / Split::BK;
-  int split = 1;
-  while (split < 8 && narrow * split * 2 <= kSMs && nkb >= split * 4) split *= 2;
-  if (split > 1 && (one || p.g.K <= split * one_chain(dtype))) return launch<Split>(p, m, narrow, split, stream);
+  if (f.path == ES_GROUPED_WIDE) return go(Wide{}, 2);
+  if (f.path == ES_GROUPED_SPLIT) return go(Split{}, f.split);
+  if (f.path == ES_GROUPED_NARROW) return go(Narrow{}, 1);
+  if constexpr (PLANES == 1)
+    if (f.path == ES_GROUPED_MIDDLE) return go(Middle{}, 1);
   if constexpr (PLANES == 1 && KIND == kKindF16) {
-    using Deep = TcShape<1, 1, 64, KIND, A_MN, false, false, 1, true>;
-    if (!one) return launch<Deep>(p, m, narrow, 1, stream);
+    if (f.path == ES_GROUPED_DEEP_WIDE) return go(DeepWide{}, 2);
+    if (f.path == ES_GROUPED_DEEP_NARROW) return go(DeepNarrow{}, 1);
   }
-  return launch<Narrow>(p, m, narrow, 1, stream);
+  return ES_ERR_INVALID;
 }
 
 uint32_t idesc_of(int dtype, bool a_mn, bool b_mn) {
@@ -1533,6 +1555,8 @@ bool sizes_ok(const GroupedArgs& g, int dtype) {
 bool grouped_rows_tc_ok(const GroupedArgs& g, int dtype) {
   return sizes_ok(g, dtype) && (g.rows / 64 + g.groups()) * ((g.N + 127) / 128) < kMaxTiles;
 }
+
+int grouped_rows_tc_path(const GroupedArgs& g, int dtype) { return rows_form(g, dtype).path; }
 
 size_t grouped_rows_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w) {
   const RowsOperands o = rows_operands(g, dtype, x, w);

@@ -422,6 +422,20 @@ int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride
                       int64_t K, int64_t N, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
                       const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, void* y,
                       int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The kernel that a rows' product of these sizes runs on (weights contiguous
+ * and 16-byte aligned; the rows' gradient is the product with K and N
+ * exchanged), -1 for sizes that have none. */
+typedef enum es_grouped_path {
+  ES_GROUPED_FEW = 0,         /* fp32, few rows a group: weights cut in registers */
+  ES_GROUPED_NARROW = 1,      /* 128 channels x 64 rows */
+  ES_GROUPED_SPLIT = 2,       /* the same, the depth shared by a cluster */
+  ES_GROUPED_MIDDLE = 3,      /* 256 x 128 */
+  ES_GROUPED_WIDE = 4,        /* 512 x 256 of a pair of CTAs (fp32: 256 x 128) */
+  ES_GROUPED_DEEP_NARROW = 5, /* 16 bits, long sums: chains with an fp32 total, 128 x 64 */
+  ES_GROUPED_DEEP_WIDE = 6    /* 256 x 256 */
+} es_grouped_path;
+int es_grouped_matmul_path(int dtype, int num_experts, int64_t K, int64_t N, int64_t num_rows);
+int es_int8_matmul_path(int num_experts, int64_t K, int64_t N, int64_t num_rows);
 /* dw[e] = sum over e's rows of x[row(r)]^T dy[r], with dw's element strides
  * (that of K or of N is 1);
  * zero for an expert without rows. dw has the operands' type. */
