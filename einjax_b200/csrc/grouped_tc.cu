@@ -558,36 +558,29 @@ __device__ __forceinline__ void scale_block(float (&v)[32], const float2* xs, fl
 }
 
 // Reads one accumulator of an output tile. TMEM holds a single tile of this
-// size, so the next tile's MMAs wait for this: the last blocks of 32 columns
-// are held in registers (16-bit ones packed) and stored after the accumulator has been
-// handed back (`release`). xs, w: scales of 8-bit operands (I8).
-constexpr int kAtOnce = 0;   // blocks stored at once, 16-bit tiles
-constexpr int kAtOnce32 = 3; // and fp32 tiles: the rest fits the registers
+// size, so the next tile's MMAs wait for this: a 16-bit tile (packed) and the last
+// blocks of 32 columns of an fp32 one are held in registers, a few of them spilled (45 in
+// 16 bits, 92 in 8), and stored after the accumulator has been handed back (`release`).
+// xs, w: scales of 8-bit operands (I8).
+constexpr int kAtOnce32 = 3; // blocks of fp32 tiles that are stored at once: the rest fits the registers
 
 template <typename T, bool I8, typename Release>
 __device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride, int rows, bool live, const float2* xs,
                                            float w, Release release) {
   // all of the accumulator, whatever `rows`: no branch parts the registers' lives
   if constexpr (sizeof(T) == 2) {
-    uint32_t held[8 - kAtOnce][16];
+    uint32_t held[8][16];
 #pragma unroll
     for (int b = 0; b < 8; ++b) {
       float v[32];
       tmem_ld32(acc + b * 32, v);
       if constexpr (I8) scale_block(v, xs + b * 32, w);
-      if (b < kAtOnce) {
-        uint32_t two[16];
-        pack_cols<T>(v, two);
-        store_packed(out, stride, two, rows - b * 32, live);
-        out += 32 * stride;
-      } else {
-        pack_cols<T>(v, held[b - kAtOnce]);
-      }
+      pack_cols<T>(v, held[b]);
     }
     release();
 #pragma unroll
-    for (int b = kAtOnce; b < 8; ++b) {
-      store_packed(out, stride, held[b - kAtOnce], rows - b * 32, live);
+    for (int b = 0; b < 8; ++b) {
+      store_packed(out, stride, held[b], rows - b * 32, live);
       out += 32 * stride;
     }
   } else {
@@ -1074,7 +1067,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
           }
         }
-        for (int b = set; b < MT * blocks && (!released || !any); b += 2) {
+        for (int b = set; !S::kSums && b < MT * blocks && (!released || !any); b += 2) {
           const int m = b / blocks, c0 = (b - m * blocks) * 32, n = at.rows - c0;
           const int64_t ch = ch0 + m * 128 * CG;
           const bool live = ch < p.lanes;
