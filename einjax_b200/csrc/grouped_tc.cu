@@ -39,9 +39,11 @@
 // forward, the tensor pipe 84% active (on equal groups 88%, as cuBLAS's product
 // of that size); 60 experts of 2048 x 2816 with 69 rows each 115 us, 6.2 TB/s of
 // HBM; 16 rows over 16 experts of 2048 x 4096 30 us, 5.0 TB/s; 8 bits, 8191 x
-// 4096 x 8192 184 us, 3.0 POP/s; fp32, 3000 rows, 16 experts, 1000 x 2024 98 us
-// without the planes' 59 us. Before the 512 x 256 tile a long group's bound was
-// the L2's bandwidth to the SMs (64 bytes a clock and SM for 256 x 256).
+// 4096 x 8192 179 to 184 us, 3.0 POP/s, but 16400 rows of 64 experts, 2048 x 1408, 72 us
+// with the tensor pipe 33% active: a tile's hand-over takes 11k cycles whatever its
+// depth; fp32, 3000 rows, 16 experts, 1000 x 2024 92 us without the planes' 59 us.
+// Before the 512 x 256 tile a long group's bound was the L2's bandwidth to the SMs (64
+// bytes a clock and SM for 256 x 256).
 //
 // Roles (12 warps): warp 0 issues the TMA loads, warp 1 the MMAs (an elected
 // lane), warps 2-3 clear the output rows of no expert, warps 4-11 read the
@@ -1580,8 +1582,10 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
     return ES_ERR_CUDA;
   if (dtype == kInt8) return rows_launch<kKindI8, false, 1>(p, m, dtype, stream);
   if (dtype == ES_F32)
-    return o.mn ? rows_launch<kKindF16, true, 3>(p, m, dtype, stream) : rows_launch<kKindF16, false, 3>(p, m, dtype, stream);
-  return o.mn ? rows_launch<kKindF16, true, 1>(p, m, dtype, stream) : rows_launch<kKindF16, false, 1>(p, m, dtype, stream);
+    return o.mn ? rows_launch<kKindF16, true, 3>(p, m, dtype, stream)
+                : rows_launch<kKindF16, false, 3>(p, m, dtype, stream);
+  return o.mn ? rows_launch<kKindF16, true, 1>(p, m, dtype, stream)
+              : rows_launch<kKindF16, false, 1>(p, m, dtype, stream);
 }
 
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype) {

@@ -216,7 +216,7 @@ def test_quantize_experts_empty(shape):
 
 @pytest.mark.parametrize("leaf", [False, True])
 def test_forward_mode_is_refused(leaf):
-    """A tangent raises instead of being dropped, in an operand and in a gradient; without one a level changes nothing."""
+    """A tangent raises instead of being dropped, in an operand and in a gradient; a level without one changes nothing."""
     import torch.autograd.forward_ad as fw
     plan = make_plan([3, 5], 2)
     g = gen(1)
