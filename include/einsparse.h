@@ -410,7 +410,8 @@ int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts,
  * any element strides, row(r) = order[r] / top_k when order is given (x by
  * token), else r. y (num_rows, N) contiguous, of out_dtype (ES_F32 or the
  * operands' type). Infinities and NaN give what fp32 arithmetic gives, except
- * that a magnitude below 2^-132 may count as zero beside them. The tensor
+ * that a magnitude below 2^-132 may count as zero beside them. fp32 operands
+ * keep all their bits from 2^-109 on, sums from 2^-120 on. The tensor
  * cores' sums truncate: of one sign they come out low by up to 8e-7 (fp32
  * operands, any depth), or a quarter of the rounding to the operands' 16-bit
  * type (also where y is ES_F32). The workspace's size goes by the call's own arguments. */
