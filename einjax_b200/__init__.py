@@ -13,6 +13,7 @@ from .experts import (ExpertPlan, combine_experts, expert_mlp, grouped_matmul, i
                       plan_experts, quantize_experts, quantize_rows, route_experts)
 from .kernels import (block_sparse_matmul, block_sparse_matmul_generic, coordinate_join_hash,  # noqa: F401
                       coordinate_join_sorted)
+from .norms import residual_norm, rms_norm  # noqa: F401
 from .partition import tile_shape_to_partition_spec  # noqa: F401
 from .plan import PlanStep, execute_sparse_plan, plan_from_path, reduction_keys  # noqa: F401
 from .registry import register_b200_kernels  # noqa: F401

@@ -21,9 +21,11 @@ ES_PREC_AUTO, ES_PREC_EXACT, ES_PREC_TC = range(3)
 ES_DUP_LAST, ES_DUP_SUM = range(2)
 (ES_GROUPED_FEW, ES_GROUPED_NARROW, ES_GROUPED_SPLIT, ES_GROUPED_MIDDLE, ES_GROUPED_WIDE, ES_GROUPED_DEEP_NARROW,
  ES_GROUPED_DEEP_WIDE) = range(7)
+ES_GATE_NONE, ES_GATE_CHANNEL, ES_GATE_TOKEN, ES_GATE_FULL = range(4)
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
+c_f32 = ctypes.c_float
 c_vp = ctypes.c_void_p
 c_sz = ctypes.c_size_t
 c_i64p = ctypes.POINTER(ctypes.c_int64)
@@ -102,6 +104,12 @@ SIGNATURES = {
                                               c_vp, c_vp, c_int, c_i64]),
     "es_int8_matmul": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
+    "es_residual_norm": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_i64,
+                                 c_f32, c_f32, c_vp, c_vp, c_vp, c_vp]),
+    "es_residual_norm_grad_workspace_size": (c_sz, [c_int, c_i64, c_i64, c_int]),
+    "es_residual_norm_grad": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int,
+                                      c_i64, c_f32, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                      c_vp, c_sz, c_vp]),
     "es_scatter_add_workspace_size": (c_sz, [c_i64]),
     "es_scatter_add_rows": (c_int, [c_vp, c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_sz, c_vp, c_vp, c_vp]),
 }

@@ -1,0 +1,617 @@
+// Norms before and after a block, with its gate and residual scale.
+//
+//   z = h w_out / rms(h)   (or h)          rms(v) = sqrt(mean(v^2) + eps)
+//   out = x + s g z
+//   y = out w_in / rms(out)
+//
+// and backwards, with r1 = 1 / rms(h), r2 = 1 / rms(out), hat = h r1, unit =
+// out r2, b = dy w_in, c2 = mean(b unit):
+//   d = dout + r2 (b - unit c2)                       the gradient of out, and dx
+//   dz = s g d,  dh = r1 (dz w_out - hat mean(dz w_out hat))   (or dz)
+//   dg = s z d,  dw_out = sum_rows dz hat,  dw_in = sum_rows dy unit
+//
+// d is linear in c2, so the backward pass needs one reduction a row: the sums of
+// b unit, s g z d0 and s g z d1 with d0 = dout + r2 b and d1 = r2 unit. r1 and r2
+// are kept from the forward pass, `out` is made again in fp32.
+//
+// Everything is fp32 between a value's load and its one rounding. Bound by
+// memory: a row is read once into registers (a group of threads a row, NP
+// pieces of 16 bytes each) and every output written once. Column sums stay in
+// registers over the rows of a group; each group writes its part, and a second
+// kernel adds the parts in their order, so that results repeat to the bit.
+#include <type_traits>
+
+#include "experts.cuh"
+
+namespace es {
+namespace {
+
+constexpr int kNormThreads = 256;  // of a CTA whose rows take fewer
+constexpr int kMostThreads = 512;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct NormArgs {
+  const void* x;
+  const void* h;
+  const void* w_in;
+  const void* w_out;
+  const void* gate;
+  int64_t x_stride, h_stride, gate_stride, dout_stride, dy_stride;
+  int64_t rows, width;
+  int gate_kind;
+  float scale, eps;
+  void* out;
+  void* y;
+  float* stats;  // (rows, 2): r1, r2
+  // backward
+  const void* dout;
+  const void* dy;
+  void* dx;
+  void* dh;
+  void* dgate;
+  float* part;     // (groups, columns, width)
+  int in_col, out_col, gate_col;  // which of a group's parts, -1: none
+  int columns;
+  int tp;          // threads of a row
+};
+
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T) >= 16 ? 16 : VEC * sizeof(T)) Vec {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Vec<T, VEC> load(const T* p, int64_t piece) {
+  return reinterpret_cast<const Vec<T, VEC>*>(p)[piece];
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, int64_t piece, const float (&v)[VEC]) {
+  Vec<T, VEC> o;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(v[i]);
+  reinterpret_cast<Vec<T, VEC>*>(p)[piece] = o;
+}
+
+// Sums of N values over the tp threads of a group, for all of them. `part` is not
+// written again before every thread of the CTA has passed another barrier.
+template <int N>
+__device__ __forceinline__ void group_sum(float (&v)[N], float (*part)[32], int tp) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(kAll, v[i], o);
+  if (tp <= 32) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tp >> 5;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i][warp] = v[i];
+  }
+  __syncthreads();
+  const int first = warp / nw * nw;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    v[i] = lane < nw ? part[i][first + lane] : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(kAll, v[i], o);
+  }
+}
+
+constexpr float kDown = 2.6469779601696886e-23f;  // 2^-75: squares of the largest values, 2^16 of them and more, are finite
+
+__device__ __forceinline__ float inv_rms(float sum, float width, float eps) {
+  return 1.0f / sqrtf(sum / width + eps);
+}
+
+template <typename T, typename W, int VEC, int NP>
+__global__ void __launch_bounds__(kMostThreads) norm_kernel(const __grid_constant__ NormArgs p) {
+  constexpr bool LONG = NP == 0;  // rows that no group of threads holds are read again for each step
+  constexpr int HELD = LONG ? 1 : NP;
+  __shared__ float part[4][1][32];
+  const int tp = p.tp, c0 = threadIdx.x % tp;
+  const int64_t t = blockIdx.x * static_cast<int64_t>(blockDim.x / tp) + threadIdx.x / tp;
+  const bool live = t < p.rows;
+  const int64_t row = live ? t : 0, pieces = p.width / VEC;
+  const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+  const T* h = static_cast<const T*>(p.h) + row * p.h_stride;
+  const T* gate = static_cast<const T*>(p.gate) + (p.gate_kind == ES_GATE_CHANNEL ? 0 : row * p.gate_stride);
+  const W* w_out = static_cast<const W*>(p.w_out);
+  const W* w_in = static_cast<const W*>(p.w_in);
+  const float width = static_cast<float>(p.width);
+  Vec<T, VEC> xv[HELD], hv[HELD];
+  float o[HELD][VEC];
+
+  // fn(slot, piece) for this thread's pieces of the row
+  auto each = [&](auto fn) {
+    if constexpr (LONG) {
+      if (live)
+        for (int64_t c = c0; c < pieces; c += tp) fn(0, c);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        if (live && c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
+    }
+  };
+  if constexpr (!LONG) {
+    each([&](int n, int64_t c) {
+      xv[n] = load<T, VEC>(x, c);
+      if (p.h) hv[n] = load<T, VEC>(h, c);
+    });
+  }
+  float r1 = 1.0f, r2 = 1.0f;
+  auto rms = [&](auto value, float (*buf)[32], float (*again)[32]) {
+    float sum[1] = {0.0f};
+    each([&](int n, int64_t c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float v = value(n, c, i);
+        sum[0] = fmaf(v, v, sum[0]);
+      }
+    });
+    group_sum(sum, buf, tp);
+    // squares past the largest value: the same sum of smaller ones. All threads of the
+    // CTA decide alike, for the barrier in it.
+    if (tp > 32 ? __syncthreads_or(!(sum[0] < INFINITY)) : __any_sync(kAll, !(sum[0] < INFINITY))) {
+      float small[1] = {0.0f};
+      each([&](int n, int64_t c) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float v = value(n, c, i) * kDown;
+          small[0] = fmaf(v, v, small[0]);
+        }
+      });
+      group_sum(small, again, tp);
+      if (!(sum[0] < INFINITY)) return inv_rms(small[0], width, p.eps * kDown * kDown) * kDown;
+    }
+    return inv_rms(sum[0], width, p.eps);
+  };
+  if (p.w_out)
+    r1 = rms(
+        [&](int n, int64_t c, int i) {
+          if constexpr (LONG) return to_f32(load<T, VEC>(h, c).v[i]);
+          return to_f32(hv[n].v[i]);
+        },
+        part[0], part[1]);
+  const float token = p.gate_kind == ES_GATE_TOKEN && live ? to_f32(gate[0]) : 1.0f;
+  auto residual = [&](int n, int64_t c, float (&v)[VEC]) {  // out, in fp32
+    const Vec<T, VEC> xs = LONG ? load<T, VEC>(x, c) : xv[n];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(xs.v[i]);
+    if (!p.h) return;
+    const Vec<T, VEC> hs = LONG ? load<T, VEC>(h, c) : hv[n];
+    float z[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) z[i] = to_f32(hs.v[i]) * r1;
+    if (p.w_out) {
+      const Vec<W, VEC> w = load<W, VEC>(w_out, c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] *= to_f32(w.v[i]);
+    }
+    if (p.gate_kind == ES_GATE_CHANNEL || p.gate_kind == ES_GATE_FULL) {
+      const Vec<T, VEC> g = load<T, VEC>(gate, c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf(p.scale * to_f32(g.v[i]), z[i], v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = fmaf(p.scale * token, z[i], v[i]);
+    }
+  };
+  each([&](int n, int64_t c) {
+    residual(n, c, o[n]);
+    if (p.out) store<T, VEC>(static_cast<T*>(p.out) + t * p.width, c, o[n]);
+  });
+  if (p.w_in) {
+    r2 = rms(
+        [&](int n, int64_t c, int i) {
+          if constexpr (LONG) {
+            if (i == 0) residual(n, c, o[0]);
+            return o[0][i];
+          }
+          return o[n][i];
+        },
+        part[2], part[3]);
+    each([&](int n, int64_t c) {
+      if constexpr (LONG) residual(n, c, o[0]);
+      const Vec<W, VEC> w = load<W, VEC>(w_in, c);
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = o[n][i] * r2 * to_f32(w.v[i]);
+      store<T, VEC>(static_cast<T*>(p.y) + t * p.width, c, v);
+    });
+  }
+  if (p.stats && live && c0 == 0) {
+    p.stats[2 * t] = r1;
+    p.stats[2 * t + 1] = r2;
+  }
+}
+
+template <typename T, typename W, int VEC, int NP>
+__global__ void __launch_bounds__(kMostThreads) norm_grad_kernel(const __grid_constant__ NormArgs p) {
+  constexpr bool LONG = NP == 0;  // column sums of long rows stay in memory, each thread's its own
+  constexpr int HELD = LONG ? 1 : NP;
+  __shared__ float part[2][3][32];
+  const int tp = p.tp, c0 = threadIdx.x % tp, per = blockDim.x / tp;
+  const int64_t pieces = p.width / VEC;
+  const int64_t group = blockIdx.x * static_cast<int64_t>(per) + threadIdx.x / tp;
+  const W* w_out = static_cast<const W*>(p.w_out);
+  const W* w_in = static_cast<const W*>(p.w_in);
+  const float width = static_cast<float>(p.width);
+  float* parts = p.part + group * p.columns * p.width;
+  float sums[3][HELD][VEC];
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int n = 0; n < HELD; ++n)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sums[k][n][i] = 0.0f;
+  if constexpr (LONG)
+    for (int k = 0; k < p.columns; ++k)
+      for (int64_t c = c0; c < pieces; c += tp)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) parts[k * p.width + c * VEC + i] = 0.0f;
+
+  int turn = 0;
+  for (int64_t t0 = blockIdx.x * static_cast<int64_t>(per); t0 < p.rows;
+       t0 += gridDim.x * static_cast<int64_t>(per), turn ^= 1) {
+    const int64_t t = t0 + threadIdx.x / tp;
+    const bool live = t < p.rows;
+    const int64_t row = live ? t : 0;
+    const T* x = static_cast<const T*>(p.x) + row * p.x_stride;
+    const T* h = static_cast<const T*>(p.h) + row * p.h_stride;
+    const T* gate = static_cast<const T*>(p.gate) + (p.gate_kind == ES_GATE_CHANNEL ? 0 : row * p.gate_stride);
+    const T* dout = static_cast<const T*>(p.dout) + row * p.dout_stride;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.dy_stride;
+    const float r1 = p.w_out ? p.stats[2 * row] : 1.0f, r2 = p.dy ? p.stats[2 * row + 1] : 0.0f;
+    const float token = p.gate_kind == ES_GATE_TOKEN ? to_f32(gate[0]) : 1.0f;
+    Vec<T, VEC> xv[HELD], hv[HELD], ov[HELD], yv[HELD], gv[HELD];
+    auto fetch = [&](int n, int64_t c) {
+      xv[n] = load<T, VEC>(x, c);
+      if (p.h) hv[n] = load<T, VEC>(h, c);
+      if (p.dout) ov[n] = load<T, VEC>(dout, c);
+      if (p.dy) yv[n] = load<T, VEC>(dy, c);
+      if (p.gate_kind == ES_GATE_CHANNEL || p.gate_kind == ES_GATE_FULL) gv[n] = load<T, VEC>(gate, c);
+    };
+    auto each = [&](auto fn) {
+      if constexpr (LONG) {
+        if (live)
+          for (int64_t c = c0; c < pieces; c += tp) {
+            fetch(0, c);
+            fn(0, c);
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+          if (live && c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
+      }
+    };
+    if constexpr (!LONG) each(fetch);
+    struct Terms {
+      float hat, z, g, unit, b, d0, d1;
+    };
+    auto terms = [&](int n, int64_t c, auto use) {  // use(i, the terms of value i)
+      Vec<W, VEC> wo, wi;
+      if (p.w_out) wo = load<W, VEC>(w_out, c);
+      if (p.dy) wi = load<W, VEC>(w_in, c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        Terms e;
+        e.g = p.scale * token;
+        if (p.gate_kind == ES_GATE_CHANNEL || p.gate_kind == ES_GATE_FULL) e.g = p.scale * to_f32(gv[n].v[i]);
+        e.hat = p.h ? to_f32(hv[n].v[i]) * r1 : 0.0f;
+        e.z = p.w_out ? e.hat * to_f32(wo.v[i]) : e.hat;
+        e.unit = fmaf(e.g, e.z, to_f32(xv[n].v[i])) * r2;
+        e.b = p.dy ? to_f32(yv[n].v[i]) * to_f32(wi.v[i]) : 0.0f;
+        e.d0 = fmaf(r2, e.b, p.dout ? to_f32(ov[n].v[i]) : 0.0f);
+        e.d1 = r2 * e.unit;
+        use(i, e);
+      }
+    };
+    float v[3] = {0.0f, 0.0f, 0.0f};
+    const bool by_token = p.gate_kind == ES_GATE_TOKEN;
+    each([&](int n, int64_t c) {
+      terms(n, c, [&](int, const Terms& e) {
+        v[0] = fmaf(e.b, e.unit, v[0]);
+        const float z = by_token ? e.z : e.g * e.z;
+        v[1] = fmaf(z, e.d0, v[1]);
+        v[2] = fmaf(z, e.d1, v[2]);
+      });
+    });
+    group_sum(v, part[turn], tp);
+    const float c2 = v[0] / width, zd = v[1] - c2 * v[2];
+    const float c1 = (by_token ? p.scale * token * zd : zd) / width;
+    if (by_token && p.dgate && live && c0 == 0) static_cast<T*>(p.dgate)[t] = from_f32<T>(p.scale * zd);
+    each([&](int n, int64_t c) {
+      float dx[VEC], dh[VEC], dg[VEC];
+      float add[3][VEC];
+      terms(n, c, [&](int i, const Terms& e) {
+        const float d = e.d0 - c2 * e.d1, dz = e.g * d;
+        dx[i] = d;
+        dg[i] = p.scale * e.z * d;
+        add[0][i] = p.dy ? to_f32(yv[n].v[i]) * e.unit : 0.0f;
+        add[1][i] = dz * e.hat;
+        dh[i] = dz;
+      });
+      if (p.w_out) {
+        const Vec<W, VEC> wo = load<W, VEC>(w_out, c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          dh[i] = r1 * (dh[i] * to_f32(wo.v[i]) - to_f32(hv[n].v[i]) * r1 * c1);
+      }
+      if (p.dx) store<T, VEC>(static_cast<T*>(p.dx) + t * p.width, c, dx);
+      if (p.dh) store<T, VEC>(static_cast<T*>(p.dh) + t * p.width, c, dh);
+      if (p.dgate && p.gate_kind == ES_GATE_FULL) store<T, VEC>(static_cast<T*>(p.dgate) + t * p.width, c, dg);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) add[2][i] = dg[i];
+      if constexpr (LONG) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (p.in_col >= 0) parts[p.in_col * p.width + c * VEC + i] += add[0][i];
+          if (p.out_col >= 0) parts[p.out_col * p.width + c * VEC + i] += add[1][i];
+          if (p.gate_col >= 0) parts[p.gate_col * p.width + c * VEC + i] += add[2][i];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sums[k][n][i] += add[k][i];
+      }
+    });
+  }
+  if constexpr (!LONG) {
+    const int at[3] = {p.in_col, p.out_col, p.gate_col};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (at[k] < 0) continue;
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        if (c0 + n * tp < pieces) store<float, VEC>(parts + at[k] * p.width, c0 + n * tp, sums[k][n]);
+    }
+  }
+}
+
+// Adds the groups' parts of each column in their order: 32 columns by 8 slices
+// of the groups a CTA, the slices' sums added in their order.
+struct SumArgs {
+  const float* part;
+  int64_t groups, width;
+  int columns;
+  void* out[3];
+  int dtype[3];
+};
+
+__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ SumArgs p) {
+  __shared__ float slices[8][32];
+  const int64_t n = p.columns * p.width, at = blockIdx.x * 32LL + (threadIdx.x & 31);
+  const int slice = threadIdx.x >> 5;
+  float sum = 0.0f;
+  if (at < n) {
+    const int64_t from = p.groups * slice / 8, to = p.groups * (slice + 1) / 8;
+#pragma unroll 8
+    for (int64_t g = from; g < to; ++g) sum += p.part[g * n + at];
+  }
+  slices[slice][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (slice || at >= n) return;
+  for (int s = 1; s < 8; ++s) sum += slices[s][threadIdx.x];
+  const int k = static_cast<int>(at / p.width);
+  const int64_t c = at - k * p.width;
+  if (p.dtype[k] == ES_BF16)
+    static_cast<__nv_bfloat16*>(p.out[k])[c] = __float2bfloat16(sum);
+  else if (p.dtype[k] == ES_F16)
+    static_cast<__half*>(p.out[k])[c] = __float2half(sum);
+  else
+    static_cast<float*>(p.out[k])[c] = sum;
+}
+
+// Threads of a row (a multiple of 32) and pieces that each holds, a power of two up
+// to `most`; 0 pieces: a row that no 512 threads hold.
+struct RowForm {
+  int tp, np;
+  int groups() const { return tp < kNormThreads ? kNormThreads / tp : 1; }  // of a CTA
+  int threads() const { return tp * groups(); }
+};
+
+RowForm row_form(int64_t pieces, int most) {
+  for (int threads = kNormThreads; threads <= kMostThreads; threads *= 2)
+    for (int np = 1; np <= most; np *= 2) {
+      const int64_t tp = (pieces + 32 * np - 1) / (32 * np) * 32;
+      if (tp <= threads) return RowForm{static_cast<int>(tp), np};
+    }
+  return RowForm{kMostThreads, 0};
+}
+
+// Groups of threads that walk the rows of a backward pass.
+int64_t grad_groups(int64_t rows, const RowForm& f) {
+  const int64_t per = f.groups(), ctas = (rows + per - 1) / per, most = kSMs * (kMostThreads / f.threads());
+  return (ctas < most ? ctas : most) * per;
+}
+
+// Pieces that a thread holds, at most: registers for three fp32 sums of a value in
+// the backward pass, for the residual in fp32 in the forward one.
+constexpr int held(int vec) { return vec == 1 ? 16 : 4; }
+constexpr int held_grad(int vec) { return vec == 1 ? 16 : 16 / vec; }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int64_t piece_size(const NormArgs& p, int esz) {
+  const int64_t vec = 16 / esz;
+  const bool ok = p.width % vec == 0 && p.x_stride % vec == 0 && p.h_stride % vec == 0 &&
+                  (p.gate_kind != ES_GATE_FULL || p.gate_stride % vec == 0) && p.dout_stride % vec == 0 &&
+                  p.dy_stride % vec == 0 && aligned16(p.x) && aligned16(p.h) && aligned16(p.w_in) &&
+                  aligned16(p.w_out) && (p.gate_kind == ES_GATE_TOKEN || aligned16(p.gate)) && aligned16(p.out) &&
+                  aligned16(p.y) && aligned16(p.dout) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh) &&
+                  (p.gate_kind != ES_GATE_FULL || aligned16(p.dgate)) && aligned16(p.part);
+  return ok ? vec : 1;
+}
+
+// fn(integral_constant<pieces>)
+template <int MOST, typename Fn>
+int by_pieces(int np, Fn fn) {
+  if (np == 0) return fn(std::integral_constant<int, 0>{});
+  if constexpr (MOST > 1)
+    if (np < MOST) return by_pieces<MOST / 2>(np, fn);
+  return fn(std::integral_constant<int, MOST>{});
+}
+
+template <typename T, typename W, int VEC>
+int forward(NormArgs& p, cudaStream_t s) {
+  const RowForm f = row_form(p.width / VEC, held(VEC));
+  p.tp = f.tp;
+  const int64_t per = f.groups();
+  const unsigned blocks = static_cast<unsigned>((p.rows + per - 1) / per);
+  return by_pieces<held(VEC)>(f.np, [&](auto np) {
+    ES_LAUNCH((norm_kernel<T, W, VEC, decltype(np)::value>), blocks, f.threads(), 0, s, p);
+    return static_cast<int>(ES_OK);
+  });
+}
+
+template <typename T, typename W, int VEC>
+int backward(NormArgs& p, const SumArgs& sums, cudaStream_t s) {
+  const RowForm f = row_form(p.width / VEC, held_grad(VEC));
+  p.tp = f.tp;
+  const int64_t groups = grad_groups(p.rows, f);
+  const unsigned blocks = static_cast<unsigned>(groups / f.groups());
+  ES_TRY(by_pieces<held_grad(VEC)>(f.np, [&](auto np) {
+    ES_LAUNCH((norm_grad_kernel<T, W, VEC, decltype(np)::value>), blocks, f.threads(), 0, s, p);
+    return static_cast<int>(ES_OK);
+  }));
+  if (!p.columns) return ES_OK;
+  SumArgs a = sums;
+  a.groups = groups;
+  ES_LAUNCH(column_sum_kernel, static_cast<unsigned>((p.columns * p.width + 31) / 32), 256, 0, s, a);
+  return ES_OK;
+}
+
+int check_norm(const NormArgs& p, int dtype, int weight_dtype) {
+  if (p.rows < 0 || p.width < 0 || p.gate_kind < ES_GATE_NONE || p.gate_kind > ES_GATE_FULL) return ES_ERR_INVALID;
+  if ((p.gate_kind != ES_GATE_NONE) != (p.gate != nullptr) || (!p.h && (p.gate || p.w_out || !p.w_in)))
+    return ES_ERR_INVALID;
+  if (p.rows > 0x7fffff00LL || p.width > 0x7fffff00LL / 4) return ES_ERR_UNSUPPORTED;
+  if (dtype != ES_F32 && dtype != ES_BF16 && dtype != ES_F16) return ES_ERR_UNSUPPORTED;
+  if (weight_dtype != dtype && weight_dtype != ES_F32) return ES_ERR_UNSUPPORTED;
+  return ES_OK;
+}
+
+// fn<T, W, VEC>() by types and alignment
+#define ES_NORM_CALL(fn, ...)                                                             \
+  ES_BY_TYPE(dtype, {                                                                     \
+    constexpr int VEC = 16 / sizeof(T);                                                   \
+    const bool wide = piece_size(p, sizeof(T)) == VEC;                                    \
+    if (weight_dtype == dtype) return wide ? fn<T, T, VEC>(__VA_ARGS__) : fn<T, T, 1>(__VA_ARGS__); \
+    return wide ? fn<T, float, VEC>(__VA_ARGS__) : fn<T, float, 1>(__VA_ARGS__);          \
+  })
+
+}  // namespace
+}  // namespace es
+
+using namespace es;
+
+extern "C" int es_residual_norm(const void* x, int64_t x_stride, const void* h, int64_t h_stride, int dtype,
+                                int64_t num_rows, int64_t width, const void* norm_in, const void* norm_out,
+                                int weight_dtype, const void* gate, int gate_kind, int64_t gate_stride, float scale,
+                                float eps, void* out, void* y, float* stats, void* stream) {
+  NormArgs p{};
+  p.x = x;
+  p.h = h;
+  p.x_stride = x_stride;
+  p.h_stride = h_stride;
+  p.w_in = norm_in;
+  p.w_out = norm_out;
+  p.gate = gate;
+  p.gate_kind = gate_kind;
+  p.gate_stride = gate_stride;
+  p.rows = num_rows;
+  p.width = width;
+  p.scale = scale;
+  p.eps = eps;
+  p.out = out;
+  p.y = y;
+  p.stats = stats;
+  if (num_rows < 0 || width < 0) return ES_ERR_INVALID;
+  if (num_rows == 0 || width == 0) return ES_OK;
+  ES_TRY(check_norm(p, dtype, weight_dtype));
+  if (!x || (h && !out) || (norm_in && !y)) return ES_ERR_INVALID;
+  cudaStream_t s = as_stream(stream);
+  ES_NORM_CALL(forward, p, s);
+  return ES_ERR_UNSUPPORTED;
+}
+
+// Column sums that the gradients given need.
+static int norm_columns(const void* dnorm_in, const void* dnorm_out, const void* dgate, int gate_kind) {
+  return (dnorm_in ? 1 : 0) + (dnorm_out ? 1 : 0) + (dgate && gate_kind == ES_GATE_CHANNEL ? 1 : 0);
+}
+
+extern "C" size_t es_residual_norm_grad_workspace_size(int dtype, int64_t num_rows, int64_t width, int num_columns) {
+  if (num_rows <= 0 || width <= 0 || num_columns <= 0) return 0;
+  // the pieces may be single values, by addresses that are not known here
+  const int vec = dtype == ES_F32 ? 4 : 8;
+  const int64_t one = grad_groups(num_rows, row_form(width, held_grad(1)));
+  const int64_t wide = grad_groups(num_rows, row_form((width + vec - 1) / vec, held_grad(vec)));
+  const int64_t groups = one > wide ? one : wide;
+  return static_cast<size_t>(groups) * num_columns * width * sizeof(float);
+}
+
+extern "C" int es_residual_norm_grad(const void* x, int64_t x_stride, const void* h, int64_t h_stride, int dtype,
+                                     int64_t num_rows, int64_t width, const void* norm_in, const void* norm_out,
+                                     int weight_dtype, const void* gate, int gate_kind, int64_t gate_stride,
+                                     float scale, const float* stats, const void* dout, int64_t dout_stride,
+                                     const void* dy, int64_t dy_stride, void* dx, void* dh, void* dgate,
+                                     void* dnorm_in, void* dnorm_out, void* workspace, size_t workspace_bytes,
+                                     void* stream) {
+  NormArgs p{};
+  p.x = x;
+  p.h = h;
+  p.x_stride = x_stride;
+  p.h_stride = h_stride;
+  p.w_in = norm_in;
+  p.w_out = norm_out;
+  p.gate = gate;
+  p.gate_kind = gate_kind;
+  p.gate_stride = gate_stride;
+  p.rows = num_rows;
+  p.width = width;
+  p.scale = scale;
+  p.stats = const_cast<float*>(stats);
+  p.dout = dout;
+  p.dout_stride = dout ? dout_stride : 0;
+  p.dy = dy;
+  p.dy_stride = dy ? dy_stride : 0;
+  p.dx = dx;
+  p.dh = dh;
+  p.dgate = dgate;
+  if (num_rows < 0 || width < 0) return ES_ERR_INVALID;
+  if (width == 0) return ES_OK;
+  if (num_rows > 0) {  // tensors without values have no addresses
+    ES_TRY(check_norm(p, dtype, weight_dtype));
+    if ((dy && !norm_in) || (dh && !h) || (dgate && !gate) || (dnorm_in && !norm_in) || (dnorm_out && !norm_out) ||
+        !x || ((norm_out || dy) && !stats))
+      return ES_ERR_INVALID;
+  }
+  cudaStream_t s = as_stream(stream);
+  SumArgs sums{};
+  sums.width = width;
+  p.in_col = p.out_col = p.gate_col = -1;
+  auto column = [&](int& col, void* out, int type) {
+    col = sums.columns;
+    sums.out[sums.columns] = out;
+    sums.dtype[sums.columns++] = type;
+  };
+  if (dnorm_in) column(p.in_col, dnorm_in, weight_dtype);
+  if (dnorm_out) column(p.out_col, dnorm_out, weight_dtype);
+  if (dgate && gate_kind == ES_GATE_CHANNEL) column(p.gate_col, dgate, dtype);
+  p.columns = sums.columns;
+  if (num_rows == 0) {  // sums of nothing
+    for (int k = 0; k < sums.columns; ++k)
+      if (cudaMemsetAsync(sums.out[k], 0, width * (sums.dtype[k] == ES_F32 ? 4 : 2), s) != cudaSuccess)
+        return ES_ERR_CUDA;
+    return ES_OK;
+  }
+  if (workspace_bytes < es_residual_norm_grad_workspace_size(
+                            dtype, num_rows, width, norm_columns(dnorm_in, dnorm_out, dgate, gate_kind)))
+    return ES_ERR_WORKSPACE;
+  if (p.columns && !workspace) return ES_ERR_WORKSPACE;
+  p.part = static_cast<float*>(workspace);
+  sums.part = p.part;
+  ES_NORM_CALL(backward, p, sums, s);
+  return ES_ERR_UNSUPPORTED;
+}

@@ -484,6 +484,39 @@ int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_
                    int64_t w_n_stride, const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows,
                    void* y, int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Norms before and after a block, with its gate and residual scale. Rows of
+ * `width` contiguous values (row strides in elements), rms(v) = sqrt(mean(v^2)
+ * + eps), all in fp32 and rounded once:
+ *   z = h norm_out / rms(h)  (norm_out NULL: z = h),
+ *   out = x + scale gate z,   y = out norm_in / rms(out)
+ * norm_in NULL: no y. h NULL: out = x is not written, and there is no gate and
+ * no norm_out. x, h, gate, out and y have one type (ES_F32, ES_BF16, ES_F16),
+ * the norms' weights (width) have it or are ES_F32. out and y (num_rows, width)
+ * are contiguous. stats (may be NULL): float32 (num_rows, 2) for the gradient.
+ * ------------------------------------------------------------------------- */
+typedef enum es_gate {
+  ES_GATE_NONE = 0,
+  ES_GATE_CHANNEL = 1, /* gate (width) */
+  ES_GATE_TOKEN = 2,   /* one value a row, gate_stride elements apart */
+  ES_GATE_FULL = 3     /* (num_rows, width), rows gate_stride elements apart */
+} es_gate;
+int es_residual_norm(const void* x, int64_t x_stride, const void* h, int64_t h_stride, int dtype, int64_t num_rows,
+                     int64_t width, const void* norm_in, const void* norm_out, int weight_dtype, const void* gate,
+                     int gate_kind, int64_t gate_stride, float scale, float eps, void* out, void* y, float* stats,
+                     void* stream);
+/* Gradients from dout and dy (NULL: zero) and the forward pass's stats. dx, dh,
+ * dgate, dnorm_in, dnorm_out: NULL for what is not wanted; contiguous, of the
+ * types and shapes of x, h, gate and the norms. num_columns of the workspace:
+ * how many of dnorm_in, dnorm_out and a dgate by channel are wanted. */
+size_t es_residual_norm_grad_workspace_size(int dtype, int64_t num_rows, int64_t width, int num_columns);
+int es_residual_norm_grad(const void* x, int64_t x_stride, const void* h, int64_t h_stride, int dtype,
+                          int64_t num_rows, int64_t width, const void* norm_in, const void* norm_out,
+                          int weight_dtype, const void* gate, int gate_kind, int64_t gate_stride, float scale,
+                          const float* stats, const void* dout, int64_t dout_stride, const void* dy,
+                          int64_t dy_stride, void* dx, void* dh, void* dgate, void* dnorm_in, void* dnorm_out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
