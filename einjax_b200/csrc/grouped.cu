@@ -15,7 +15,7 @@ constexpr int kClearThreads = 256;
 // Zeros in an (experts, K, N) tensor of any strides.
 template <typename T>
 __global__ void __launch_bounds__(kClearThreads) clear_kernel(GroupedArgs g, T* out) {
-  const int64_t n = g.num_experts * g.K * g.N, step = gridDim.x * static_cast<int64_t>(kClearThreads);
+  const int64_t n = g.groups() * g.K * g.N, step = gridDim.x * static_cast<int64_t>(kClearThreads);
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kClearThreads) + threadIdx.x; i < n; i += step) {
     const int64_t col = i % g.N, row = i / g.N % g.K, e = i / g.N / g.K;
     out[e * g.w_e + row * g.w_k + col * g.w_n] = T(0);
@@ -67,7 +67,6 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
                                  int32_t* status, void* stream) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
                       w_k_stride, w_n_stride, nullptr, nullptr};
-  if (num_experts < 1) return ES_ERR_INVALID;
   ES_TRY(check_args(g));
   if (!value_type(dtype) || (out_dtype != dtype && out_dtype != ES_F32)) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
@@ -111,14 +110,13 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
                                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride,
                       dw_k_stride, dw_n_stride, nullptr, nullptr};
-  if (num_experts < 1) return ES_ERR_INVALID;
   ES_TRY(check_args(g));
   if (!value_type(dtype)) return ES_ERR_UNSUPPORTED;
   if (K == 0 || N == 0) return ES_OK;
   if (!dw || (num_rows && (!dy || (x_rows && !x)))) return ES_ERR_INVALID;
   cudaStream_t s = as_stream(stream);
   if (empty(g)) {
-    const int blocks = grid_for(static_cast<int64_t>(num_experts) * K * N, kClearThreads);
+    const int blocks = grid_for(g.groups() * K * N, kClearThreads);
     ES_BY_TYPE(dtype, {
       ES_LAUNCH((clear_kernel<T>), blocks, kClearThreads, 0, s, g, static_cast<T*>(dw));
       return ES_OK;

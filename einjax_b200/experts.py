@@ -252,14 +252,22 @@ def plan_experts(experts: torch.Tensor, num_experts: int) -> ExpertPlan:
 
 # ---------------------------------------------------------- grouped products
 
+def _groups(x, plan, gather):
+    """(experts, offsets, order, top_k, rows) as the products take them; no plan: one matrix for all rows of x."""
+    if plan is None:
+        return 0, None, None, 1, x.shape[0]
+    return (plan.num_experts, plan.offsets.data_ptr(), plan.order.data_ptr() if gather else None, plan.top_k,
+            plan.num_rows)
+
+
 def _grouped(x, w, plan, gather, out_dtype):
-    """``w`` (num_experts, K, N), any strides."""
+    """``w`` (num_experts, K, N), any strides; (1, K, N) without a plan."""
     dev = x.device
-    E, K, N = w.shape
-    R, code = plan.num_rows, _DTYPES[x.dtype]
+    K, N = w.shape[1:]
+    E, offsets, order, top_k, R = _groups(x, plan, gather)
+    code = _DTYPES[x.dtype]
     y = _empty(R, N, out_dtype, dev)
-    args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), plan.offsets.data_ptr(),
-            plan.order.data_ptr() if gather else None, plan.top_k, R)
+    args = (x.data_ptr(), code, x.shape[0], x.stride(0), w.data_ptr(), E, K, N, *w.stride(), offsets, order, top_k, R)
     # fp32 mostly needs no workspace for up to 24 rows a group (12.8 us for 14.9 a small call)
     need = R > 24 * E if code == L.ES_F32 else gather
     _product("es_grouped_matmul", dev, args, (y.data_ptr(), _DTYPES[out_dtype]), need)
@@ -272,9 +280,10 @@ def _wgrad(x, dy, w, plan, gather):
     # the gradient takes w's layout when it is a transposed view
     dw = torch.empty((E, N, K), dtype=w.dtype, device=dev).transpose(1, 2) if w.stride(1) == 1 and w.stride(2) != 1 \
         else torch.empty((E, K, N), dtype=w.dtype, device=dev)
-    R, code = plan.num_rows, _DTYPES[x.dtype]
-    args = (x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), E, K, N, plan.offsets.data_ptr(),
-            plan.order.data_ptr() if gather else None, plan.top_k, R, dw.data_ptr(), *dw.stride())
+    groups, offsets, order, top_k, R = _groups(x, plan, gather)
+    code = _DTYPES[x.dtype]
+    args = (x.data_ptr(), code, x.shape[0], x.stride(0), dy.data_ptr(), dy.stride(0), groups, K, N, offsets, order,
+            top_k, R, dw.data_ptr(), *dw.stride())
     _product("es_grouped_matmul_wgrad", dev, args, (), gather or code == L.ES_F32)
     return dw
 

@@ -139,7 +139,8 @@ class _StatusWords:
     The words are made together and once, under a lock: kernels hold their
     addresses, so no thread's first call may replace another's."""
 
-    OPERATORS = ("es_expert_plan", "es_grouped_matmul", "es_grouped_matmul_wgrad", "es_int8_matmul")
+    OPERATORS = ("es_expert_plan", "es_grouped_matmul", "es_grouped_matmul_wgrad", "es_int8_matmul",
+                 "es_gated_matmul")
 
     def __init__(self):
         self.lock = threading.Lock()

@@ -407,7 +407,7 @@ int es_expert_plan(const int32_t* experts, int64_t num_choices, int num_experts,
                    void* stream);
 
 /* y[r] = x[row(r)] w[e(r)] for the num_rows grouped rows: w[e] is (K, N) with
- * any element strides, row(r) = order[r] / top_k when order is given (x by
+ * any element strides (num_experts == 0: one matrix for all rows, offsets and order NULL), row(r) = order[r] / top_k when order is given (x by
  * token), else r. y (num_rows, N) contiguous, of out_dtype (ES_F32 or the
  * operands' type). Infinities and NaN give what fp32 arithmetic gives, except
  * that a magnitude below 2^-132 may count as zero beside them. fp32 operands
@@ -450,6 +450,31 @@ int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_
                             const int32_t* order, int top_k, int64_t num_rows, void* dw, int64_t dw_expert_stride,
                             int64_t dw_k_stride, int64_t dw_n_stride, void* workspace, size_t workspace_bytes,
                             int32_t* status, void* stream);
+
+/* h[r] = act(x[row(r)] gate[e(r)]) * (x[row(r)] up[e(r)]) for the num_rows grouped
+ * rows, w[e] = [gate | up] (K, 2F) with any element strides; num_experts == 0: one
+ * matrix for all rows (offsets and order NULL). h (num_rows, F) contiguous, of the
+ * operands' type; slopes (num_rows, 2F), the same type or NULL: [act'(x gate) * (x up)
+ * | act(x gate)], the rows of no expert left alone. */
+typedef enum es_activation {
+  ES_ACT_SILU = 0,      /* g / (1 + exp(-g)) */
+  ES_ACT_GELU = 1,      /* g (1 + erf(g / sqrt(2))) / 2 */
+  ES_ACT_GELU_TANH = 2, /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+  ES_ACT_RELU = 3
+} es_activation;
+size_t es_gated_matmul_workspace_size(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w,
+                                      int num_experts, int64_t K, int64_t F, int64_t w_expert_stride,
+                                      int64_t w_k_stride, int64_t w_n_stride, const int32_t* offsets,
+                                      const int32_t* order, int top_k, int64_t num_rows);
+int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w, int num_experts,
+                    int64_t K, int64_t F, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
+                    const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, int activation,
+                    void* h, void* slopes, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* dy = dh times the slopes (num_rows, 2F), contiguous: the gradient of [x gate | x up],
+ * from which es_grouped_matmul and es_grouped_matmul_wgrad make those of x and w.
+ * kept_rows (device int32, or NULL for all): the rows from there on are zero. */
+int es_gated_matmul_grad(const void* dh, int dtype, int64_t dh_stride, const void* slopes, int64_t num_rows,
+                         int64_t F, const int32_t* kept_rows, void* dy, void* stream);
 
 /* out[t] = sum_j weights[t, j] y[position[t, j]] (weights NULL: 1), y
  * (num_rows, width). out (num_tokens, width) contiguous, of out_dtype: y's
