@@ -22,6 +22,7 @@ ES_DUP_LAST, ES_DUP_SUM = range(2)
 (ES_GROUPED_FEW, ES_GROUPED_NARROW, ES_GROUPED_SPLIT, ES_GROUPED_MIDDLE, ES_GROUPED_WIDE, ES_GROUPED_DEEP_NARROW,
  ES_GROUPED_DEEP_WIDE) = range(7)
 ES_ACT_SILU, ES_ACT_GELU, ES_ACT_GELU_TANH, ES_ACT_RELU = range(4)
+ES_GATED_TWO = 7
 ES_GATE_NONE, ES_GATE_CHANNEL, ES_GATE_TOKEN, ES_GATE_FULL = range(4)
 
 c_i64 = ctypes.c_int64
@@ -101,6 +102,7 @@ SIGNATURES = {
                                                c_vp, c_vp, c_int, c_i64]),
     "es_gated_matmul": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                 c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_sz, c_vp, c_vp]),
+    "es_gated_matmul_path": (c_int, [c_int, c_int, c_i64, c_i64, c_i64]),
     "es_gated_matmul_grad": (c_int, [c_vp, c_int, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "es_combine_experts": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_i64, c_int, c_i64, c_vp, c_int, c_vp]),
     "es_combine_experts_grad": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_int, c_i64, c_vp,

@@ -103,6 +103,13 @@ int grad_launch(const void* dh, int64_t stride, const void* slopes, int64_t rows
   return ES_OK;
 }
 
+// 16 bits up to a depth that is summed in one chain: the activation is the product's
+// epilogue. Else (fp32, whose planes take the accumulators; deep sums; empty products)
+// the product is made in fp32 and read again.
+bool one_kernel(const GroupedArgs& g, int dtype) {
+  return check_grouped(g) == ES_OK && grouped_gated_tc_ok(g, dtype);
+}
+
 size_t product_bytes(int64_t rows, int64_t F) {
   return (static_cast<size_t>(rows) * 2 * F * sizeof(float) + 255) / 256 * 256;
 }
@@ -118,6 +125,9 @@ extern "C" size_t es_gated_matmul_workspace_size(const void* x, int dtype, int64
                                                  const int32_t* offsets, const int32_t* order, int top_k,
                                                  int64_t num_rows) {
   if (num_rows <= 0 || F <= 0) return 0;
+  const GroupedArgs g{num_experts, K, F, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
+                      w_k_stride, w_n_stride, nullptr, nullptr};
+  if (one_kernel(g, dtype)) return grouped_gated_tc_workspace(g, dtype, x, w);
   return product_bytes(num_rows, F) +
          es_grouped_matmul_workspace_size(x, dtype, x_rows, x_stride, w, num_experts, K, 2 * F, w_expert_stride,
                                           w_k_stride, w_n_stride, offsets, order, top_k, num_rows);
@@ -131,6 +141,13 @@ extern "C" int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t
   if (activation < ES_ACT_SILU || activation > ES_ACT_RELU || F < 0 || num_rows < 0) return ES_ERR_INVALID;
   if (F > 0x3fffff00LL) return ES_ERR_UNSUPPORTED;
   if (F > 0 && num_rows > 0 && !h) return ES_ERR_INVALID;
+  const GroupedArgs g{num_experts, K, F, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
+                      w_k_stride, w_n_stride, nullptr, nullptr};
+  if (one_kernel(g, dtype)) {
+    if (!h || !x || !w) return ES_ERR_INVALID;
+    if (workspace_bytes < grouped_gated_tc_workspace(g, dtype, x, w)) return ES_ERR_WORKSPACE;
+    return grouped_gated_tc(g, dtype, x, w, activation, h, slopes, workspace, status, as_stream(stream));
+  }
   const size_t own = num_rows > 0 && F > 0 ? product_bytes(num_rows, F) : 0;
   if (workspace_bytes < own) return ES_ERR_WORKSPACE;
   float* y = static_cast<float*>(workspace);
@@ -140,6 +157,14 @@ extern "C" int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t
   if (num_rows == 0 || F == 0) return ES_OK;
   ES_BY_TYPE(dtype, ES_BY_ACT(activation, return (act_launch<T, ACT>(y, num_rows, F, h, slopes, as_stream(stream)))));
   return ES_ERR_UNSUPPORTED;
+}
+
+extern "C" int es_gated_matmul_path(int dtype, int num_experts, int64_t K, int64_t F, int64_t num_rows) {
+  const GroupedArgs g{num_experts, K, F, num_rows, num_rows, K, 1, nullptr, nullptr, 2 * K * F, 2 * F, 1, nullptr,
+                      nullptr};
+  if (num_experts < 0 || num_experts > kMaxExperts || num_rows <= 0 || K <= 0 || F <= 0) return -1;
+  if (dtype != ES_F32 && dtype != ES_BF16 && dtype != ES_F16) return -1;
+  return grouped_gated_tc_ok(g, dtype) ? grouped_gated_tc_path(g) : ES_GATED_TWO;
 }
 
 extern "C" int es_gated_matmul_grad(const void* dh, int dtype, int64_t dh_stride, const void* slopes,

@@ -28,7 +28,13 @@ int clear_rows_of(const GroupedArgs& g, void* y, int out_dtype, cudaStream_t s) 
   return cudaMemsetAsync(y, 0, bytes, s) == cudaSuccess ? ES_OK : ES_ERR_CUDA;
 }
 
-int check_args(const GroupedArgs& g) {
+bool value_type(int dtype) { return dtype == ES_F32 || dtype == ES_BF16 || dtype == ES_F16; }
+
+bool empty(const GroupedArgs& g) { return g.K == 0 || g.N == 0 || g.rows == 0 || g.x_rows == 0; }
+
+}  // namespace
+
+int check_grouped(const GroupedArgs& g) {
   if (g.num_experts < 0 || g.K < 0 || g.N < 0 || g.rows < 0 || g.x_rows < 0) return ES_ERR_INVALID;
   if (g.num_experts > 0 && !g.offsets) return ES_ERR_INVALID;
   if (g.num_experts == 0 && (g.order || g.offsets || g.x_rows != g.rows)) return ES_ERR_INVALID;
@@ -40,11 +46,6 @@ int check_args(const GroupedArgs& g) {
   return ES_OK;
 }
 
-bool value_type(int dtype) { return dtype == ES_F32 || dtype == ES_BF16 || dtype == ES_F16; }
-
-bool empty(const GroupedArgs& g) { return g.K == 0 || g.N == 0 || g.rows == 0 || g.x_rows == 0; }
-
-}  // namespace
 }  // namespace es
 
 using namespace es;
@@ -56,7 +57,7 @@ extern "C" size_t es_grouped_matmul_workspace_size(const void* x, int dtype, int
                                                    int64_t num_rows) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
                       w_k_stride, w_n_stride, nullptr, nullptr};
-  if (check_args(g) != ES_OK || empty(g) || grouped_rows_few_ok(g, dtype, w)) return 0;
+  if (check_grouped(g) != ES_OK || empty(g) || grouped_rows_few_ok(g, dtype, w)) return 0;
   return grouped_rows_tc_workspace(g, dtype, x, w);
 }
 
@@ -67,7 +68,7 @@ extern "C" int es_grouped_matmul(const void* x, int dtype, int64_t x_rows, int64
                                  int32_t* status, void* stream) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
                       w_k_stride, w_n_stride, nullptr, nullptr};
-  ES_TRY(check_args(g));
+  ES_TRY(check_grouped(g));
   if (!value_type(dtype) || (out_dtype != dtype && out_dtype != ES_F32)) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
   if (!y || (K && ((x_rows && !x) || !w))) return ES_ERR_INVALID;
@@ -100,7 +101,7 @@ extern "C" size_t es_grouped_matmul_wgrad_workspace_size(const void* x, int dtyp
                                                          int64_t dw_n_stride) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride,
                       dw_k_stride, dw_n_stride, nullptr, nullptr};
-  return check_args(g) == ES_OK && !empty(g) ? grouped_wgrad_tc_workspace(g, dtype, x, dy, dy_stride) : 0;
+  return check_grouped(g) == ES_OK && !empty(g) ? grouped_wgrad_tc_workspace(g, dtype, x, dy, dy_stride) : 0;
 }
 
 extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* dy,
@@ -110,7 +111,7 @@ extern "C" int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows,
                                        void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, dw_expert_stride,
                       dw_k_stride, dw_n_stride, nullptr, nullptr};
-  ES_TRY(check_args(g));
+  ES_TRY(check_grouped(g));
   if (!value_type(dtype)) return ES_ERR_UNSUPPORTED;
   if (K == 0 || N == 0) return ES_OK;
   if (!dw || (num_rows && (!dy || (x_rows && !x)))) return ES_ERR_INVALID;
@@ -134,7 +135,7 @@ extern "C" size_t es_int8_matmul_workspace_size(const int8_t* q, const float* x_
                                                 int top_k, int64_t num_rows) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, 1,
                       w_n_stride, x_scale, w_scale};
-  return check_args(g) == ES_OK && !empty(g) ? grouped_rows_tc_workspace(g, kInt8, q, wq) : 0;
+  return check_grouped(g) == ES_OK && !empty(g) ? grouped_rows_tc_workspace(g, kInt8, q, wq) : 0;
 }
 
 extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,
@@ -144,7 +145,7 @@ extern "C" int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_r
                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   const GroupedArgs g{num_experts, K, N, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride, 1,
                       w_n_stride, x_scale, w_scale};
-  ES_TRY(check_args(g));
+  ES_TRY(check_grouped(g));
   if (K > kMaxInt8Depth || !value_type(out_dtype)) return ES_ERR_UNSUPPORTED;
   if (num_rows == 0 || N == 0) return ES_OK;
   if (!y || !w_scale || (x_rows && !x_scale) || (K && ((x_rows && !q) || !wq))) return ES_ERR_INVALID;

@@ -49,6 +49,8 @@ struct GroupedArgs {
   }
 };
 
+int check_grouped(const GroupedArgs& g);  // an es_status for sizes and orders that do not belong together
+
 constexpr int kInt8 = 0x100;  // operand type of the 8-bit product
 
 // The fp32 rows' product for groups of a few rows (grouped_few.cu): no workspace.
@@ -62,6 +64,13 @@ int grouped_rows_tc_path(const GroupedArgs& g, int dtype);  // an es_grouped_pat
 size_t grouped_rows_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w);
 int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, void* y, int out_dtype,
                     void* workspace, int32_t* status, cudaStream_t stream);
+// Gated products of 16-bit operands in one kernel: N is the channels of h, up lies N
+// columns behind gate.
+bool grouped_gated_tc_ok(const GroupedArgs& g, int dtype);
+int grouped_gated_tc_path(const GroupedArgs& g);
+size_t grouped_gated_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w);
+int grouped_gated_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, int activation, void* h,
+                     void* slopes, void* workspace, int32_t* status, cudaStream_t stream);
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype);
 size_t grouped_wgrad_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride);
 int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,

@@ -57,6 +57,7 @@
 
 #include <cstring>
 
+#include "activation.cuh"
 #include "grouped.cuh"
 #include "tc_ptx.cuh"
 
@@ -91,6 +92,8 @@ struct TcArgs {
   uint32_t idesc;     // instruction descriptor without N
   int pairs;          // two neighbouring lanes may be stored together
   int most;           // weights' gradient: groups of more rows than this are the DEEP kernel's
+  int activation;     // gated products
+  void* slopes;       // (rows, 2 lanes) or NULL
   int32_t* status;
 };
 
@@ -98,6 +101,7 @@ struct TcArgs {
 // by steps of 16 rows and by gathers of single rows.
 struct TcMaps {
   CUtensorMap a, b;
+  CUtensorMap up;  // gated products: the second accumulator's lanes
   CUtensorMap a_steps, b_steps, a_rows, b_rows;
 };
 
@@ -333,7 +337,8 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
 
 // ------------------------------------------------------------------- kernel
 
-template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_, bool DEEP_ = false>
+template <int CG_, int MT_, int NT_, int KIND_, bool A_MN_, bool WGRAD_, bool SPLIT_, int PLANES_, bool DEEP_ = false,
+          bool GATED_ = false>
 struct TcShape {
   static constexpr int CG = CG_;        // CTAs of one MMA
   static constexpr int MT = MT_;        // accumulators of 128 lanes (of each CTA) that share B
@@ -346,7 +351,8 @@ struct TcShape {
   static constexpr int BK = KIND == kKindI8 ? 128 : 64;  // depth of a stage
   static constexpr bool DEEP = DEEP_;   // an fp32 total in TMEM
   static constexpr int kChain = PLANES > 1 ? 7 : DEEP ? 64 : 1 << 30;  // blocks of depth between fp32 additions
-  static constexpr int kLanes = 128 * MT * CG;
+  static constexpr bool GATED = GATED_;  // the two accumulators are gate and up of the same lanes
+  static constexpr int kLanes = 128 * (GATED ? 1 : MT) * CG;
   static constexpr int kAccs = PLANES > 1 ? 2 : MT;         // accumulators of a tile
   static constexpr int kTotal = DEEP ? NT : 0;              // columns of the total
   static constexpr int kBufs = 2 * kAccs * NT + kTotal <= 512 ? 2 : 1;  // tiles in TMEM
@@ -355,11 +361,13 @@ struct TcShape {
   static constexpr bool kHeld = kBufs == 1 && PLANES == 1 && !DEEP;  // tiles are held in registers, see drain_held
   static constexpr bool kSums = PLANES > 1 && !WGRAD && !SPLIT;  // the epilogue adds chains in registers
   static constexpr int kStageBytes = MT * kABytes + NT / CG * kSwizzleRow;  // one plane of a block of depth
-  static constexpr int kPartBytes = SPLIT ? NT * 128 * 4 : 0;
+  static constexpr int kPartBytes = SPLIT ? MT * NT * 128 * 4 : 0;
   static constexpr int kStages =
       (200 * 1024 - kPartBytes) / kStageBytes > kMaxTcStages ? kMaxTcStages : (200 * 1024 - kPartBytes) / kStageBytes;
   static_assert(PLANES == 1 || MT == 1, "planes take the tiles that accumulators would share B with");
   static_assert(kStages > PLANES, "a block's planes and the next block's first");
+  static_assert(!GATED || (MT == 2 && KIND == kKindF16 && !WGRAD && !DEEP), "gate and up in 16 bits");
+  static_assert(!SPLIT || MT == 1 || GATED, "parts of one accumulator");
   static_assert(kUsed <= 512 && !(DEEP && (MT > 1 || PLANES > 1 || SPLIT)), "one accumulator and its total");
 
   // Tiles that the other kernel of the same call makes.
@@ -609,6 +617,96 @@ __device__ __forceinline__ void drain_held(uint32_t acc, T* out, int64_t stride,
   }
 }
 
+__device__ __forceinline__ void store_16(void* out, int dtype, int64_t at, int64_t stride, const float (&v)[32], int n,
+                                         bool live, bool pairs) {
+  if (dtype == ES_BF16)
+    store_cols(static_cast<__nv_bfloat16*>(out) + at, stride, v, n, live, pairs);
+  else
+    store_cols(static_cast<__half*>(out) + at, stride, v, n, live, pairs);
+}
+
+// Activation, product and (for a training step) slopes of 32 columns, rounded and stored.
+__device__ __forceinline__ void gated_block(const TcArgs& p, float (&g)[32], const float (&u)[32], int64_t row, int n,
+                                            int64_t ch, bool live) {
+  float s[32];
+  if (p.activation == ES_ACT_GELU) {
+    // rolled, through local memory: 32 times erfc's code keeps the compiler from holding
+    // the other activations' values in registers
+    float a[32], d[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a[i] = g[i];
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i) activate<ES_ACT_GELU, false>(a[i], a[i], d[i]);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      g[i] = a[i];
+      s[i] = d[i];
+    }
+  } else {
+    ES_BY_ACT(p.activation, {
+      if constexpr (ACT != ES_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) activate<ACT, false>(g[i], g[i], s[i]);
+      }
+    });
+  }
+  const bool pairs = p.pairs != 0;
+  if (p.slopes) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s[i] *= u[i];
+    store_16(p.slopes, p.out_dtype, row * 2 * p.out_col + ch, 2 * p.out_col, s, n, live, pairs);
+    store_16(p.slopes, p.out_dtype, (row * 2 + 1) * p.out_col + ch, 2 * p.out_col, g, n, live, pairs);
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) g[i] *= u[i];
+  store_16(p.out, p.out_dtype, row * p.out_col + ch, p.out_col, g, n, live, pairs);
+}
+
+// The epilogue of a gated tile. A warp has every other block of 32 columns of both
+// accumulators; where TMEM holds a single tile the last of them is taken into registers
+// as it is, so that TMEM is handed back before the last two are worked on. False: given up.
+template <typename S>
+__device__ __forceinline__ bool gated_tile(const TcArgs& p, TcCtl& ctl, const TileAt& at, uint32_t tmem, int64_t ch,
+                                           uint32_t rank, int set, int quad, int& buf, uint32_t& acc_phase) {
+  constexpr int PER = S::NT / 64, TAKEN = S::kHeld ? 1 : 0;
+  const int lane = threadIdx.x & 31;
+  int go = 0;
+  if (lane == 0) go = tc_wait(&ctl.acc_full[buf], acc_phase, &ctl, p.status, true) ? 1 : 0;
+  if (!__shfl_sync(0xffffffffu, go, 0)) return false;
+  tc_fence_after();
+  const uint32_t acc = tmem + buf * S::kAccs * S::NT + (static_cast<uint32_t>(quad * 32) << 16) + set * 32;
+  float g[32], u[32], last_g[32], last_u[32];
+#pragma unroll 1
+  for (int i = 0; i < PER; ++i) {
+    if (i < PER - TAKEN) {
+      tmem_ld32(acc + i * 64, g);
+      tmem_ld32(acc + S::NT + i * 64, u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        g[j] = last_g[j];
+        u[j] = last_u[j];
+      }
+    }
+    if (i == PER - 1 - TAKEN) {
+      if constexpr (TAKEN) {
+        tmem_ld32(acc + (PER - 1) * 64, last_g);
+        tmem_ld32(acc + S::NT + (PER - 1) * 64, last_u);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), S::CG == 2 ? 0 : rank));
+    }
+    const int c0 = set * 32 + i * 64;
+    if (c0 < at.rows) gated_block(p, g, u, at.row0 + c0, at.rows - c0, ch, ch < p.lanes);
+  }
+  if (++buf == S::kBufs) {
+    buf = 0;
+    acc_phase ^= 1;
+  }
+  return true;
+}
+
 // The epilogue of a tile whose depth the cluster's CTAs share: each CTA puts
 // its part of the sum into shared memory, [column][lane], and every CTA adds
 // up every csize-th column, the parts in the CTAs' order. 8-bit products stay
@@ -652,6 +750,12 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = plane_sum(v[i], u[i]) + (s0 > at.kb0 ? mine[(c0 + i) * 128] : 0.0f);
       }
+      if constexpr (S::GATED) {
+        float u[8];
+        tmem_ld8(acc + S::NT + c0, u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[(S::NT + c0 + i) * 128] = u[i];
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) mine[(c0 + i) * 128] = v[i];  // columns past the tile's are not read
     }
@@ -682,6 +786,18 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
     } else {
 #pragma unroll
       for (int r = 0; r < 8; ++r) v += f[r];
+    }
+    if constexpr (S::GATED) {
+      float u = 0.0f, a = 0.0f, s = 0.0f;
+      const uint32_t up = smem_u32(mine + (S::NT + c) * 128);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) u += r < static_cast<int>(csize) ? load_at(at_rank(up, r)) : 0.0f;
+      ES_BY_ACT(p.activation, (activate<ACT, false>(v, a, s)));
+      if (live && p.slopes) {
+        store_one(p.slopes, p.out_dtype, (at.row0 + c) * 2 * p.out_col + ch, s * u);
+        store_one(p.slopes, p.out_dtype, ((at.row0 + c) * 2 + 1) * p.out_col + ch, a);
+      }
+      v = a * u;
     }
     if (live) store_one(p.out, p.out_dtype, (at.row0 + c) * p.out_col + ch, v);
   }
@@ -846,7 +962,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               }
             } else {
               const int z = at.expert * p.expert_step + plane * p.plane_experts;
-              if constexpr (S::A_MN) {
+              if constexpr (S::GATED) {
+                if constexpr (S::A_MN) {
+                  if (lane < 4)
+                    load_3d<CG>(sa + lane * 8192, lane < 2 ? &m.a : &m.up, lane0 + (lane & 1) * 64, kb * BK, z, bar);
+                } else {
+                  if (lane < 2) load_3d<CG>(sa + lane * kABytes, lane ? &m.up : &m.a, kb * BK, lane0, z, bar);
+                }
+              } else if constexpr (S::A_MN) {
                 if (lane < 2 * MT)
                   load_3d<CG>(sa + lane * 8192, &m.a, lane0 + (lane >> 1) * 128 * CG + (lane & 1) * 64, kb * BK, z,
                               bar);
@@ -978,6 +1101,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       if (S::skips(at.depth, p.most)) continue;
       const int64_t ch0 = at.lane0 + pair_rank * 128 + quad * 32 + lane;
       const int blocks = (at.rows + 31) / 32;
+      if constexpr (S::GATED && !S::SPLIT) {
+        if (!gated_tile<S>(p, ctl, at, tmem, ch0, rank, set, quad, buf, acc_phase)) break;
+        continue;
+      }
       if constexpr (S::SPLIT) {
         if (!split_tile<S>(p, ctl, at, part, tmem, ch0, rank, csize, set, quad, buf, acc_phase, red_phase)) break;
         continue;
@@ -1475,6 +1602,45 @@ RowsForm rows_form(const GroupedArgs& g, int dtype) {
   return narrow;
 }
 
+// The same for a gated product, whose lanes are gate's and up's of one output channel.
+RowsForm gated_form(const GroupedArgs& g) {
+  const int64_t R = g.rows, groups = g.groups();
+  const int64_t live = groups < R ? groups : R;
+  const int64_t mean = R / live;
+  auto form = [&](int path, int lanes, int cols) {
+    return RowsForm{path, lanes, cols, 1, (R / cols + live) * ((g.N + lanes - 1) / lanes)};
+  };
+  const RowsForm wide = form(ES_GROUPED_WIDE, 256, 256);
+  if (mean > 160 && wide.tiles >= kSMs / 2) return wide;
+  const RowsForm middle = form(ES_GROUPED_MIDDLE, 128, 128);
+  if (mean > 8 && middle.tiles >= kSMs) return middle;
+  RowsForm narrow = form(ES_GROUPED_NARROW, 128, 64);
+  const int64_t nkb = (g.K + 63) / 64;
+  while (narrow.split < 8 && narrow.tiles * narrow.split * 2 <= kSMs && nkb >= narrow.split * 4) narrow.split *= 2;
+  if (narrow.split > 1) narrow.path = ES_GROUPED_SPLIT;
+  return narrow;
+}
+
+template <bool A_MN>
+int gated_launch(TcArgs& p, const TcMaps& m, cudaStream_t stream) {
+  using Wide = TcShape<2, 2, 256, kKindF16, A_MN, false, false, 1, false, true>;
+  using Middle = TcShape<1, 2, 128, kKindF16, A_MN, false, false, 1, false, true>;
+  using Narrow = TcShape<1, 2, 64, kKindF16, A_MN, false, false, 1, false, true>;
+  using Split = TcShape<1, 2, 64, kKindF16, A_MN, false, true, 1, false, true>;
+  const RowsForm f = gated_form(p.g);
+  p.lane_tiles = static_cast<int>((p.lanes + f.lanes - 1) / f.lanes);
+  auto go = [&](auto shape, int csize) {
+    using S = decltype(shape);
+    if (f.lanes != S::kLanes || f.cols != S::NT) return static_cast<int>(ES_ERR_INVALID);
+    p.idesc |= S::CG == 2 ? 16u << 24 : 8u << 24;
+    return launch<S>(p, m, f.tiles, csize, stream);
+  };
+  if (f.path == ES_GROUPED_WIDE) return go(Wide{}, 2);
+  if (f.path == ES_GROUPED_MIDDLE) return go(Middle{}, 1);
+  if (f.path == ES_GROUPED_NARROW) return go(Narrow{}, 1);
+  return go(Split{}, f.split);
+}
+
 template <int KIND, bool A_MN, int PLANES>
 int rows_launch(TcArgs& p, const TcMaps& m, int dtype, cudaStream_t stream) {
   using Wide = std::conditional_t<PLANES == 1, TcShape<2, 2, 256, KIND, A_MN, false, false, PLANES>,
@@ -1586,6 +1752,63 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
                 : rows_launch<kKindF16, false, 3>(p, m, dtype, stream);
   return o.mn ? rows_launch<kKindF16, true, 1>(p, m, dtype, stream)
               : rows_launch<kKindF16, false, 1>(p, m, dtype, stream);
+}
+
+namespace {
+
+// Operands of a gated product: those of the rows' product with the gate, and up.
+struct GatedOperands {
+  RowsOperands gate;
+  Operand up;
+};
+
+GatedOperands gated_operands(const GroupedArgs& g, int dtype, const void* x, const void* w) {
+  const void* up = static_cast<const char*>(w) + g.N * g.w_n * tc_size(dtype);
+  return GatedOperands{rows_operands(g, dtype, x, w), rows_operands(g, dtype, x, up).w};
+}
+
+}  // namespace
+
+bool grouped_gated_tc_ok(const GroupedArgs& g, int dtype) {
+  return (dtype == ES_BF16 || dtype == ES_F16) && grouped_rows_tc_ok(g, dtype) && g.K <= one_chain(dtype);
+}
+
+int grouped_gated_tc_path(const GroupedArgs& g) { return gated_form(g).path; }
+
+size_t grouped_gated_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w) {
+  const GatedOperands o = gated_operands(g, dtype, x, w);
+  return o.gate.x.bytes + o.gate.w.bytes + o.up.bytes;
+}
+
+int grouped_gated_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, int activation, void* h,
+                     void* slopes, void* workspace, int32_t* status, cudaStream_t stream) {
+  GatedOperands o = gated_operands(g, dtype, x, w);
+  char* ws = static_cast<char*>(workspace);
+  ES_TRY(lay_out(g, o.gate.x, dtype, true, false, ws, stream));
+  ws += o.gate.x.bytes;
+  ES_TRY(lay_out(g, o.gate.w, dtype, false, o.gate.w.depth > 1, ws, stream));
+  ES_TRY(lay_out(g, o.up, dtype, false, o.up.depth > 1, ws + o.gate.w.bytes, stream));
+  TcArgs p{};
+  p.g = g;
+  p.out = h;
+  p.out_dtype = dtype;
+  p.lanes = g.N;
+  p.out_col = g.N;
+  p.expert_step = o.up.depth > 1 ? 1 : 0;
+  p.plane_experts = static_cast<int>(o.up.depth);
+  p.plane_rows = static_cast<int>(o.gate.x.rows);
+  p.idesc = idesc_of(dtype, o.gate.mn, false);
+  p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(h) & 3) == 0 && (reinterpret_cast<uintptr_t>(slopes) & 3) == 0;
+  p.activation = activation;
+  p.slopes = slopes;
+  p.status = status;
+  TcMaps m{};
+  const int cols = 64, rows = o.gate.mn ? 64 : 128;
+  if (!bind_context() || !encode_operand(o.gate.w, dtype, cols, rows, 3, &m.a) ||
+      !encode_operand(o.up, dtype, cols, rows, 3, &m.up) ||
+      !encode_operand(o.gate.x, dtype, cols, kBoxRows, 2, &m.b))
+    return ES_ERR_CUDA;
+  return o.gate.mn ? gated_launch<true>(p, m, stream) : gated_launch<false>(p, m, stream);
 }
 
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype) {

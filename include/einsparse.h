@@ -470,6 +470,10 @@ int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, 
                     int64_t K, int64_t F, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
                     const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, int activation,
                     void* h, void* slopes, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The kernel of a gated product of these sizes, an es_grouped_path (lanes are those of
+ * h) or ES_GATED_TWO: the product in fp32, then a pass for the activation. -1: none. */
+#define ES_GATED_TWO 7
+int es_gated_matmul_path(int dtype, int num_experts, int64_t K, int64_t F, int64_t num_rows);
 /* dy = dh times the slopes (num_rows, 2F), contiguous: the gradient of [x gate | x up],
  * from which es_grouped_matmul and es_grouped_matmul_wgrad make those of x and w.
  * kept_rows (device int32, or NULL for all): the rows from there on are zero. */

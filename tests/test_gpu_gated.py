@@ -15,6 +15,7 @@ import pytest
 import torch
 
 import einjax_b200 as E
+from einjax_b200 import _lib as L
 from test_gpu_experts import SIZES, TINY, TYPES, UNIT, gen, make_plan, randn
 
 pytestmark = pytest.mark.gpu
@@ -289,3 +290,51 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         d, = torch.autograd.grad(E.gated_matmul(x.requires_grad_(), w).sum(), x, create_graph=True)
         d.sum().backward()
+
+
+CODE = {torch.float32: L.ES_F32, torch.bfloat16: L.ES_BF16, torch.float16: L.ES_F16}
+LONG = [200, 701, 256, 0, 513, 390, 640, 511, 257]         # a mean past 160 rows
+SHORT = [10 + 37 * i % 91 for i in range(58)] + [0, 129]   # 10 to 100 rows, none, and a tile and one
+FEW = [i % 9 for i in range(80)] + [65]                    # up to 8 rows, and a tile and one
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("sizes,F,path", [(LONG, 2056, L.ES_GROUPED_WIDE), (LONG, 2049, L.ES_GROUPED_WIDE),
+                                          (SHORT, 520, L.ES_GROUPED_MIDDLE), (SHORT, 517, L.ES_GROUPED_MIDDLE),
+                                          (FEW, 520, L.ES_GROUPED_NARROW), (FEW, 517, L.ES_GROUPED_NARROW)])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+def test_shapes(dtype, sizes, F, path, transposed, gather):
+    """Every tile shape with ragged groups, several tiles a CTA, even and odd channels."""
+    k = 2 if gather and sum(sizes) % 2 == 0 else 1
+    plan = make_plan(sizes, k, dropped=4 * k)
+    K = 136
+    assert L.lib().es_gated_matmul_path(CODE[dtype], plan.num_experts, K, F, plan.num_rows) == path
+    g = gen(F + len(sizes))
+    x = randn(g, plan.num_tokens if gather else plan.num_rows, K, dtype=dtype)
+    w = randn(g, len(sizes), *((2 * F, K) if transposed else (K, 2 * F)), dtype=dtype, scale=1.5 * K ** -0.5)
+    w = w.transpose(1, 2) if transposed else w
+    check(x, w, plan, gather, ACTS[(F + gather + 2 * transposed) % 4], randn(g, plan.num_rows, F, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("R,K,F", [(1, 2048, 512), (16, 4096, 130), (64, 1030, 257), (65, 520, 1024), (3, 16384, 40)])
+@pytest.mark.parametrize("transposed", [False, True])
+def test_split(dtype, R, K, F, transposed):
+    """A decode step's few rows: a tile's depth shared by a cluster."""
+    assert L.lib().es_gated_matmul_path(CODE[dtype], 0, K, F, R) == L.ES_GROUPED_SPLIT
+    g = gen(R + F)
+    x, w = randn(g, R, K, dtype=dtype), randn(g, K, 2 * F, dtype=dtype, scale=1.5 * K ** -0.5)
+    if transposed:
+        w = w.t().contiguous().t()
+    check(x, w, None, False, ACTS[F % 4], randn(g, R, F, dtype=dtype))
+
+
+@pytest.mark.parametrize("K", [16384, 16385])
+def test_depth(K):
+    """Up to one chain of sums the activation is in the product's kernel, deeper sums are made in fp32 first."""
+    R, F = 300, 2000
+    assert (L.lib().es_gated_matmul_path(L.ES_F16, 0, K, F, R) == L.ES_GATED_TWO) == (K > 16384)
+    g = gen(K)
+    x, w = randn(g, R, K, dtype=torch.float16), randn(g, K, 2 * F, dtype=torch.float16, scale=1.5 * K ** -0.5)
+    check(x, w, None, False, "silu", None)
