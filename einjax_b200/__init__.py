@@ -11,6 +11,7 @@ from .autodiff import _reverse_einsum_string, sparse_einsum, sparse_einsum_raw  
 from .cost_model import B200_PROFILE, calibrate, detect_device_type, install_b200_profile  # noqa: F401
 from .experts import (ExpertPlan, combine_experts, expert_mlp, grouped_matmul, int8_matmul,  # noqa: F401
                       plan_experts, quantize_experts, quantize_rows, route_experts)
+from .fp8 import fp8_matmul, quantize_block_weights, quantize_blocks  # noqa: F401
 from .gated import gated_matmul  # noqa: F401
 from .kernels import (block_sparse_matmul, block_sparse_matmul_generic, coordinate_join_hash,  # noqa: F401
                       coordinate_join_sorted)

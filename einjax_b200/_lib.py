@@ -112,6 +112,13 @@ SIGNATURES = {
                                               c_vp, c_vp, c_int, c_i64]),
     "es_int8_matmul": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
                                c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
+    "es_quantize_blocks": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]),
+    "es_quantize_block_weights": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "es_fp8_matmul_workspace_size": (c_sz, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64,
+                                             c_vp, c_vp, c_int, c_i64]),
+    "es_fp8_matmul": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp,
+                              c_int, c_i64, c_vp, c_int, c_vp, c_sz, c_vp, c_vp]),
+    "es_fp8_matmul_path": (c_int, [c_int, c_i64, c_i64, c_i64]),
     "es_residual_norm": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_i64,
                                  c_f32, c_f32, c_vp, c_vp, c_vp, c_vp]),
     "es_residual_norm_grad_workspace_size": (c_sz, [c_int, c_i64, c_i64, c_int]),

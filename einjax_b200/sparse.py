@@ -140,7 +140,7 @@ class _StatusWords:
     addresses, so no thread's first call may replace another's."""
 
     OPERATORS = ("es_expert_plan", "es_grouped_matmul", "es_grouped_matmul_wgrad", "es_int8_matmul",
-                 "es_gated_matmul")
+                 "es_gated_matmul", "es_fp8_matmul")
 
     def __init__(self):
         self.lock = threading.Lock()

@@ -514,6 +514,41 @@ int es_int8_matmul(const int8_t* q, const float* x_scale, int64_t x_rows, int64_
                    void* y, int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * 8-bit floating point (e4m3: 4 exponent and 3 mantissa bits, largest 448, no
+ * infinity) with a float32 scale for each block of 128: the serving form beside
+ * the 8-bit integers above, with the same groups, orders and status.
+ * ------------------------------------------------------------------------- */
+
+/* q[r, i] = e4m3(x[r, i] / s), to nearest, ties to even, s = scale[r, i / 128]
+ * the smallest power of two (at least 2^-126) with max |x| <= 448 s over the
+ * block. A block with an infinity or NaN has scale and values NaN. activation
+ * (es_activation, -1: none): x is (num_rows, 2 width), and act(x[r, i]) *
+ * x[r, width + i] is rounded, made in fp32. q (num_rows, width) and scale
+ * (num_rows, ceil(width / 128)) contiguous. */
+int es_quantize_blocks(const void* x, int dtype, int64_t num_rows, int64_t width, int64_t row_stride, int activation,
+                       uint8_t* q, float* scale, void* stream);
+/* The same for blocks of 128 x 128 of contiguous matrices (matrices, N, K);
+ * scale (matrices, ceil(N / 128), ceil(K / 128)). */
+int es_quantize_block_weights(const void* w, int dtype, int64_t matrices, int64_t N, int64_t K, uint8_t* q,
+                              float* scale, void* stream);
+/* y[r, n] = sum_b x_scale[row(r), b] w_scale[e(r), n / 128, b] sum_{k in b} q[row(r), k] wq[e(r), n, k]
+ * over the blocks b of the depth, in fp32, rounded once; any fp32 scales. wq:
+ * (num_experts, N, K) with contiguous k, the scales contiguous. num_experts ==
+ * 0: one matrix for all rows (offsets and order NULL). y (num_rows, N)
+ * contiguous. */
+size_t es_fp8_matmul_workspace_size(const uint8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride,
+                                    const uint8_t* wq, const float* w_scale, int num_experts, int64_t K, int64_t N,
+                                    int64_t w_expert_stride, int64_t w_n_stride, const int32_t* offsets,
+                                    const int32_t* order, int top_k, int64_t num_rows);
+int es_fp8_matmul(const uint8_t* q, const float* x_scale, int64_t x_rows, int64_t x_stride, const uint8_t* wq,
+                  const float* w_scale, int num_experts, int64_t K, int64_t N, int64_t w_expert_stride,
+                  int64_t w_n_stride, const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows,
+                  void* y, int out_dtype, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+/* The kernel of a product of these sizes (ES_GROUPED_SPLIT, _NARROW: 128 rows x
+ * 128 channels, _WIDE: 256 x 256 of a pair of CTAs), -1 for sizes that have none. */
+int es_fp8_matmul_path(int num_experts, int64_t K, int64_t N, int64_t num_rows);
+
+/* ---------------------------------------------------------------------------
  * Norms before and after a block, with its gate and residual scale. Rows of
  * `width` contiguous values (row strides in elements), rms(v) = sqrt(mean(v^2)
  * + eps), all in fp32 and rounded once:
