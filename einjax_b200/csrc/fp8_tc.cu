@@ -10,15 +10,16 @@
 //
 // Orientation. The 128 lanes of an accumulator (256 for a pair of CTAs) are rows, the
 // columns channels: a thread has one row, so both scales of its columns are one number
-// a block, held in a register. (With channels in the lanes, as in grouped_tc.cu, each
+// a block. (With channels in the lanes, as in grouped_tc.cu, each
 // column would need its own, read from shared memory, whose bandwidth the MMAs need.)
 // The price is that a group's last tile multiplies empty lanes, which costs nothing where
 // few rows leave the product bound by reading W. Results go through shared memory, a
-// warp's own 4 KB, so that 128 bytes of a row are stored together.
+// warp's part of a tile as one or two TMA stores.
 //
 // Roles and waits as in grouped_tc.cu: warp 0 issues the TMA loads, warp 1 the MMAs,
-// warps 2-3 clear the rows of no expert, warps 4-11 read the accumulators. Every wait is
-// bounded.
+// warps 2-3 make the products of the scales, eight blocks ahead (loaded by the epilogue's
+// threads they cost a quarter of the time), and clear the rows of no expert, warps 4-11
+// read the accumulators. Every wait is bounded.
 #include <cfloat>
 
 #include "experts.cuh"
@@ -32,11 +33,14 @@ namespace {
 constexpr int kEpiWarps = 8;
 constexpr int kTcThreads = 128 + 32 * kEpiWarps;
 constexpr int kABytes = 16384;  // 128 rows x 128 bytes of depth
-constexpr int kBoxRows = 32;    // rows of one TMA box
-constexpr int kBoxBytes = kBoxRows * 128;
+constexpr int kFewRows = 32;    // rows of the smaller TMA box
+constexpr int kScalesAhead = 8; // blocks of depth whose scales are made together
+constexpr int kScaleSlots = 2;  // of so many blocks
+constexpr int kScalePitch = 132;  // scales of 128 rows, and no bank met twice
 constexpr int kTileBlock = 8;   // row tiles that share a channel tile's weights in L2
+constexpr int kWarpOut = 8192;  // an epilogue warp's staging of the output
 constexpr int kMaxStages = 8;
-constexpr int kMaxBufs = 4;
+constexpr int kMaxBufs = 4;     // accumulators
 
 struct Fp8Args {
   GroupedArgs g;
@@ -45,12 +49,14 @@ struct Fp8Args {
   int col_tiles;
   int expert_step;         // 0: every expert has the same matrix
   int k_blocks, n_blocks;  // scales of a row, rows of scales of a matrix
-  int wide;                // 16-byte stores
+  int wide;                // 16-byte stores, and TMA's
   int32_t* status;
 };
 
+// Boxes of 128 rows of X and W: a box costs the TMA unit some 130 cycles, so boxes of
+// 32 rows fed the MMAs at two thirds of the rate. Tiles of up to 32 rows read one of 32.
 struct Fp8Maps {
-  CUtensorMap x, w;
+  CUtensorMap x, x_few, w, out;
 };
 
 struct Fp8Ctl {
@@ -58,8 +64,12 @@ struct Fp8Ctl {
   uint64_t empty[kMaxStages];
   uint64_t acc_full[kMaxBufs];
   uint64_t acc_empty[kMaxBufs];
+  uint64_t scale_full[kScaleSlots];
+  uint64_t scale_empty[kScaleSlots];
   uint64_t red_full, red_empty;
   uint64_t drain;
+  int ends[kScaleSlots][2];  // whether a slot's rows (of either warp) have frames
+  int8_t frame[kScaleSlots][2][128];
   uint32_t tmem;
   int abort;
   uint32_t progress;
@@ -72,22 +82,24 @@ struct Fp8Shape {
   static constexpr bool SPLIT = SPLIT_;  // the cluster's CTAs share one tile's depth
   static constexpr int kRows = 128 * CG;
   static constexpr int kCols = NT / 2;  // of an epilogue warp
-  static constexpr int kBufs = 512 / NT < kMaxBufs ? 512 / NT : kMaxBufs;
-  static constexpr int kColumns = kBufs * NT;
+  static constexpr int kBlocks = NT / 128;  // blocks of channels
+  static constexpr int kBufs = 512 / NT;    // accumulators
   static constexpr int kStageBytes = kABytes + NT / CG * 128;
   static constexpr int kPitch = NT + 4;  // floats of a row of a split tile's part: no bank is met twice
-  static constexpr int kOutBytes = SPLIT ? 128 * kPitch * 4 : kEpiWarps * 4096;
-  static constexpr int kFit = (200 * 1024 - kOutBytes) / kStageBytes;
+  static constexpr int kOutBytes = SPLIT ? 128 * kPitch * 4 : kEpiWarps * kWarpOut;
+  static constexpr int kScaleBytes = kScaleSlots * kScalesAhead * kBlocks * kScalePitch * 4;
+  static constexpr int kFit = (213 * 1024 - kOutBytes - kScaleBytes) / kStageBytes;
   static constexpr int kStages = kFit < kMaxStages ? kFit : kMaxStages;
-  static constexpr bool kSplitRegs = kCols == 128;  // the epilogue takes registers of the other roles
+  static constexpr bool kSplitRegs = kCols == 128;  // 128 totals and 64 sums a thread
   static_assert(!SPLIT || CG == 1, "a cluster shares the depth or the rows");
+  static_assert(NT / CG == 128, "one box of W a stage");
 };
 
 // One output tile, and which blocks of its depth this CTA multiplies.
 struct Fp8Tile {
   int expert;
   int row0, rows;
-  int col0, width;  // width: channels of the MMA, from the tile's own rounded up
+  int col0;
   int kb0, kb1;
 };
 
@@ -116,8 +128,6 @@ struct Fp8Tiles {
     r.row0 = lo[a] + row_tile * S::kRows;
     r.rows = min(cnt[a] - row_tile * S::kRows, S::kRows);
     r.col0 = col_tile * S::NT;
-    r.width = static_cast<int>(min(p.g.N - r.col0, static_cast<int64_t>(S::NT)));
-    r.width = (r.width + 16 * S::CG - 1) / (16 * S::CG) * (16 * S::CG);
     r.kb0 = 0;
     r.kb1 = p.k_blocks;
     if constexpr (S::SPLIT) {
@@ -140,22 +150,71 @@ __device__ __forceinline__ void clear_rows(const Fp8Args& p, int64_t from, int64
   for (int64_t i = head + body * 8 + t; i < n; i += nt) a[i] = 0;
 }
 
-// A block's sums times the scales of its row and channels, added to the totals: by the
-// scales' product, or where that is past the type's ends by one after the other, the
-// smaller first where it is infinite, the larger first where it is subnormal, so that a
-// result that fp32 holds is met.
-__device__ __forceinline__ void add_block(float* total, const uint32_t (&v)[32], float xs, float ws) {
-  const float s = xs * ws;
-  const bool ends = (fabsf(s) < FLT_MIN && xs != 0.0f && ws != 0.0f) || fabsf(s) == INFINITY;
-  if (!ends) {
+// Frames. The product of two scales may be past fp32's ends where the result is not. A
+// row's products of one slot of blocks are then made in a frame of their own, times
+// 2^-128 where one of them is infinite or 2^128 where all are tiny (below 2^-64, and one
+// below the normal numbers), and the row's totals follow it: a rare step between the slots
+// that costs the sums themselves nothing (two factors a value cost them a tenth).
+constexpr float kHalfFrame = 18446744073709551616.0f;  // 2^64
+
+__device__ __forceinline__ bool past_ends(float x, float w) {
+  const float s = fabsf(x * w);
+  return (s < FLT_MIN && x != 0.0f && w != 0.0f) || s == INFINITY;
+}
+
+// Totals from one frame to another.
+template <int COLS>
+__device__ __forceinline__ void change_frame(float (&total)[COLS], int from, int to) {
+  const float f = from > to ? kHalfFrame : from < to ? 1.0f / kHalfFrame : 1.0f;
+  for (int steps = 2 * abs(from - to); __any_sync(0xffffffffu, steps > 0); --steps) {
+    const float now = steps > 0 ? f : 1.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) total[i] = fmaf(__uint_as_float(v[i]), s, total[i]);
-  } else {
-    const bool swap = (fabsf(xs) < fabsf(ws)) != (fabsf(s) == INFINITY);
-    const float first = swap ? ws : xs, last = swap ? xs : ws;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) total[i] = fmaf(__uint_as_float(v[i]) * first, last, total[i]);
+    for (int i = 0; i < COLS; ++i) total[i] *= now;
   }
+}
+
+// The scale of block kb of the channels from col on (their block of 128; col may lie
+// behind the last).
+__device__ __forceinline__ const float* channel_scales(const Fp8Args& p, int expert, int64_t col, int kb) {
+  const int64_t block = min(col >> 7, static_cast<int64_t>(p.n_blocks) - 1);
+  return p.g.w_scale + (static_cast<int64_t>(expert) * p.n_blocks + block) * p.k_blocks + kb;
+}
+
+// A block of depth: its four MMAs and the arrivals of their end, by one elected lane of a
+// converged warp (one statement: with an election for each, issuing took as long as the
+// tensor cores' work).
+template <int CG>
+__device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint64_t* acc_full,
+                                          uint64_t* empty) {
+#define ES_BLOCK(group, commit_form, mask)                                                                       \
+  asm volatile(                                                                                                  \
+      "{\n\t.reg .pred e, z, o;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\telect.sync _|e, 0xffffffff;\n\t"               \
+      "setp.ne.b32 z, 0, 0;\n\tsetp.eq.b32 o, 0, 0;\n\t"                                                         \
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"                                       \
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"                                       \
+      "@e tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], %1, %2, %3, z;\n\t"                               \
+      "@e tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], a1, b1, %3, o;\n\t"                               \
+      "@e tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], a2, b2, %3, o;\n\t"                               \
+      "@e tcgen05.mma.cta_group::" group ".kind::f8f6f4 [%0], a3, b3, %3, o;\n\t"                               \
+      "@e tcgen05.commit.cta_group::" group ".mbarrier::arrive::one.shared::cluster" commit_form ".b64 [%4]" mask  \
+      ";\n\t"                                                                                                    \
+      "@e tcgen05.commit.cta_group::" group ".mbarrier::arrive::one.shared::cluster" commit_form ".b64 [%5]" mask  \
+      ";\n\t}" ::"r"(d),                                                                                         \
+      "l"(a), "l"(b), "r"(idesc), "r"(smem_u32(acc_full)), "r"(smem_u32(empty)), "h"(static_cast<uint16_t>(3))   \
+      : "memory")
+  if constexpr (CG == 2)
+    ES_BLOCK("2", ".multicast::cluster", ", %6");
+  else
+    ES_BLOCK("1", "", "");
+#undef ES_BLOCK
+}
+
+// Two totals at once.
+__device__ __forceinline__ void fma2(float& t0, float& t1, float a, float b, float s) {
+  asm("{\n\t.reg .b64 v, t, f;\n\tmov.b64 v, {%2, %3};\n\tmov.b64 t, {%0, %1};\n\tmov.b64 f, {%4, %4};\n\t"
+      "fma.rn.f32x2 t, v, f, t;\n\tmov.b64 {%0, %1}, t;\n\t}"
+      : "+f"(t0), "+f"(t1)
+      : "f"(a), "f"(b), "f"(s));
 }
 
 template <typename T>
@@ -166,37 +225,51 @@ __device__ __forceinline__ uint4 pack16(const float* v) {
   return *reinterpret_cast<uint4*>(o);
 }
 
-// Rounds and stores a warp's 32 rows (a lane's each) of COLS channels, 128 bytes of a
-// row at a time through the warp's 4 KB: 16-byte pieces, swapped by the row so that
-// neither side meets a bank twice.
+// Rounds and stores a warp's 32 rows (a lane's each) of COLS channels through the warp's
+// 8 KB of shared memory, in blocks of 32 rows x 128 bytes whose 16-byte pieces are swapped
+// by the row, as TMA reads them: a whole block is one TMA store, which runs under the next
+// tile; a row at a time, or by the warps themselves, the stores of a tile took 5000 cycles.
+// What no TMA store may write (rows behind the group's, odd addresses) the warp stores.
 template <typename T, int COLS>
-__device__ __forceinline__ void store_rows(const Fp8Args& p, uint8_t* stage, const float (&total)[COLS], int row0,
-                                           int rows, int64_t col0) {
-  constexpr int VEC = 16 / sizeof(T), PASS = 8 * VEC;
+__device__ __forceinline__ void store_rows(const Fp8Args& p, const CUtensorMap* map, uint8_t* stage,
+                                           const float (&total)[COLS], int row0, int rows, int64_t col0) {
+  constexpr int VEC = 16 / sizeof(T), BLOCK = 8 * VEC, PASS = COLS < 2 * BLOCK ? COLS : 2 * BLOCK;
   const int lane = threadIdx.x & 31, j = lane & 7;
+  const bool whole = p.wide && rows >= 32;
 #pragma unroll
   for (int c = 0; c < COLS; c += PASS) {
-    uint4* mine = reinterpret_cast<uint4*>(stage + lane * 128);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mine[i ^ j] = pack16<T>(total + c + i * VEC);
+    if (lane == 0) bulk_wait_read();
     __syncwarp();
-    const int64_t col = col0 + c + j * VEC;
-    T* out = static_cast<T*>(p.out) + (row0 + (lane >> 3)) * p.g.N + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = i * 4 + (lane >> 3);
-      const uint4 v = reinterpret_cast<const uint4*>(stage + row * 128)[j ^ (row & 7)];
-      if (row < rows) {
-        if (p.wide && col + VEC <= p.g.N) {
-          *reinterpret_cast<uint4*>(out) = v;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&v);
+    for (int i = 0; i < PASS / VEC; ++i)
+      reinterpret_cast<uint4*>(stage + i / 8 * 4096 + lane * 128)[(i & 7) ^ j] = pack16<T>(total + c + i * VEC);
+    if (whole) fence_proxy_async();
+    __syncwarp();
+    if (whole) {
+      if (lane == 0) {
 #pragma unroll
-          for (int q = 0; q < VEC; ++q)
-            if (col + q < p.g.N) out[q] = e[q];
+        for (int i = 0; i < PASS / BLOCK; ++i)
+          if (col0 + c + i * BLOCK < p.g.N)
+            tma_store_2d(map, stage + i * 4096, static_cast<int>((col0 + c + i * BLOCK) * sizeof(T)), row0);
+        bulk_commit();
+      }
+    } else {
+      for (int r = lane >> 3; r < min(rows, 32); r += 4) {
+#pragma unroll
+        for (int i = 0; i < PASS / BLOCK; ++i) {
+          const uint4 v = reinterpret_cast<const uint4*>(stage + i * 4096 + r * 128)[j ^ (r & 7)];
+          const int64_t col = col0 + c + i * BLOCK + j * VEC;
+          T* out = static_cast<T*>(p.out) + static_cast<int64_t>(row0 + r) * p.g.N + col;
+          if (p.wide && col + VEC <= p.g.N) {
+            *reinterpret_cast<uint4*>(out) = v;
+          } else {
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q)
+              if (col + q < p.g.N) out[q] = e[q];
+          }
         }
       }
-      out += 4 * p.g.N;
     }
     __syncwarp();
   }
@@ -236,12 +309,13 @@ static_assert(128 * kRoleRegs + 256 * kEpiRegs == kTcThreads * kLaunchRegs, "reg
 template <typename S>
 __global__ void __launch_bounds__(kTcThreads, 1)
     fp8_tc_kernel(const __grid_constant__ Fp8Args p, const __grid_constant__ Fp8Maps m) {
-  constexpr int CG = S::CG, NT = S::NT, STAGES = S::kStages, BUFS = S::kBufs, COLS = S::kCols;
+  constexpr int CG = S::CG, NT = S::NT, STAGES = S::kStages, BUFS = S::kBufs, COLS = S::kCols, BLOCKS = S::kBlocks;
   extern __shared__ uint8_t smem_raw[];
   __shared__ Fp8Ctl ctl;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* out_smem = smem_raw + (base - smem_u32(smem_raw)) + STAGES * S::kStageBytes;
-  int* pre = reinterpret_cast<int*>(out_smem + S::kOutBytes);
+  float* scale_smem = reinterpret_cast<float*>(out_smem + S::kOutBytes);
+  int* pre = reinterpret_cast<int*>(out_smem + S::kOutBytes + S::kScaleBytes);
   const int groups = p.g.groups();
   int* lo = pre + groups + 1;
   int* cnt = lo + groups;
@@ -253,6 +327,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (threadIdx.x == 0) {
     prefetch_map(&m.x);
+    prefetch_map(&m.x_few);
+    if (p.wide) prefetch_map(&m.out);
     prefetch_map(&m.w);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&ctl.full[s], 1);
@@ -262,6 +338,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       mbar_init(&ctl.acc_full[b], 1);
       mbar_init(&ctl.acc_empty[b], CG * kEpiWarps);
     }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(&ctl.scale_full[s], 2);
+      mbar_init(&ctl.scale_empty[s], kEpiWarps);
+    }
     mbar_init(&ctl.red_full, csize * kEpiWarps);
     mbar_init(&ctl.red_empty, csize * kEpiWarps);
     mbar_init(&ctl.drain, 1);
@@ -269,7 +349,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     ctl.progress = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc_alloc<CG>(&ctl.tmem, S::kColumns);
+  if (warp == 1) tc_alloc<CG>(&ctl.tmem, BUFS * NT);
   wait_for_earlier_grids();
   if (warp == 2) {  // tiles of each group
     int run = 0;
@@ -312,18 +392,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       bool ok = true;
       for (int t = t0; t < total_tiles && ok; t += step) {
         const Fp8Tile at = tiles.at(t, rank, csize);
-        const int half = at.width / CG;
-        // boxes of 32 rows: those of X that hold rows, lanes past them are not stored
-        auto x_boxes = [&](int r) { return (min(max(at.rows - r * 128, 0), 128) + kBoxRows - 1) / kBoxRows; };
-        const int xb = x_boxes(static_cast<int>(pair_rank)), wb = (half + kBoxRows - 1) / kBoxRows;
-        const uint32_t bytes = (CG * wb + x_boxes(0) + (CG == 2 ? x_boxes(1) : 0)) * kBoxBytes;
-        const int x_row = at.row0 + static_cast<int>(pair_rank) * 128 + lane * kBoxRows;
-        const int w_row = at.col0 + static_cast<int>(pair_rank) * half + (lane - 4) * kBoxRows;
+        // X's rows past the tile's are read where its box holds them: their lanes are not stored
+        auto x_rows = [&](int r) { return at.rows <= r * 128 ? 0 : at.rows <= r * 128 + kFewRows ? kFewRows : 128; };
+        const int mine = x_rows(static_cast<int>(pair_rank));
+        const uint32_t bytes = (CG * 128 + x_rows(0) + (CG == 2 ? x_rows(1) : 0)) * 128;
+        const int x_row = at.row0 + static_cast<int>(pair_rank) * 128;
+        const int w_row = at.col0 + static_cast<int>(pair_rank) * 128;
         const int z = at.expert * p.expert_step;
         for (int kb = at.kb0; kb < at.kb1; ++kb) {
           int go = 0;
           if (lane == 0) {
-            go = tc_wait(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
+            go = tc_wait<true>(&ctl.empty[stage], phase ^ 1, &ctl, p.status) ? 1 : 0;
             if (go && leader) mbar_arrive_expect_tx(&ctl.full[stage], bytes);
             if (go) *reinterpret_cast<volatile uint32_t*>(&ctl.progress) = ++used;
           }
@@ -334,8 +413,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           const uint32_t sa = base + stage * S::kStageBytes, sb = sa + kABytes;
           const uint32_t bar = CG == 2 ? at_rank(smem_u32(&ctl.full[stage]), 0) : smem_u32(&ctl.full[stage]);
-          if (lane < xb) load_2d<CG>(sa + lane * kBoxBytes, &m.x, kb * 128, x_row, bar);
-          if (lane >= 4 && lane - 4 < wb) load_3d<CG>(sb + (lane - 4) * kBoxBytes, &m.w, kb * 128, w_row, z, bar);
+          if (lane == 0) {
+            if (mine) load_2d<CG>(sa, mine == 128 ? &m.x : &m.x_few, kb * 128, x_row, bar);
+            load_3d<CG>(sb, &m.w, kb * 128, w_row, z, bar);
+          }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -360,25 +441,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
       if (leader) {
+        const uint64_t first = operand(base, false);  // of a stage's A; its B lies kABytes behind
         int stage = 0, buf = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
         for (int t = t0; t < total_tiles && ok; t += step) {
           const Fp8Tile at = tiles.at(t, rank, csize);
           // D f32, A and B e4m3 (0) and K-major
-          const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(at.width >> 3) << 17) | ((8u * CG) << 24);
+          constexpr uint32_t idesc = (1u << 4) | ((static_cast<uint32_t>(NT) >> 3) << 17) | ((8u * CG) << 24);
           for (int kb = at.kb0; kb < at.kb1; ++kb) {
-            ok = tc_wait_warp(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status) &&
-                 tc_wait_warp(&ctl.full[stage], phase, &ctl, p.status);
+            ok = tc_wait_warp<true>(&ctl.full[stage], phase, &ctl, p.status) &&
+                 tc_wait_warp<true>(&ctl.acc_empty[buf], acc_phase ^ 1, &ctl, p.status);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t da = operand(base + stage * S::kStageBytes, false);
-            const uint64_t db = operand(base + stage * S::kStageBytes + kABytes, false);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              mma<CG, kKindF8>(tmem + buf * NT, da + i * 2, db + i * 2, idesc, static_cast<uint32_t>(i));
-            commit<CG>(&ctl.empty[stage]);
-            commit<CG>(&ctl.acc_full[buf]);
+            const uint64_t da = first + stage * (S::kStageBytes >> 4);
+            mma_block<CG>(tmem + buf * NT, da, da + (kABytes >> 4), idesc, &ctl.acc_full[buf], &ctl.empty[stage]);
             if (++stage == STAGES) {
               stage = 0;
               phase ^= 1;
@@ -396,13 +473,85 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       __syncwarp();
     } else {
+      // -------------------------------------------------------------- scales
+      // the two scales' products of kScalesAhead blocks, for 64 rows a warp and each 128
+      // channels; eight lanes a row, so that a sector is read once
+      const int row0 = (warp - 2) * 64, b = lane & 7;
+      int slot = 0;
+      uint32_t slot_phase = 0;
+      bool ok = true;
+      for (int t = t0; t < total_tiles && ok; t += step) {
+        const Fp8Tile at = tiles.at(t, rank, csize);
+        int source[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = static_cast<int>(pair_rank) * 128 + row0 + i * 32 + lane;
+          source[i] = r < at.rows ? static_cast<int>(p.g.source(at.row0 + r)) : -1;
+        }
+        for (int kb = at.kb0; kb < at.kb1; kb += kScalesAhead) {
+          ok = tc_wait_warp<true>(&ctl.scale_empty[slot], slot_phase ^ 1, &ctl, p.status, true);
+          if (!ok) break;
+          const bool there = kb + b < at.kb1;
+          float w[BLOCKS];
+#pragma unroll
+          for (int s = 0; s < BLOCKS; ++s) w[s] = there ? *channel_scales(p, at.expert, at.col0 + s * 128, kb + b) : 0.0f;
+          bool ends = false;
+          float* to = scale_smem + (slot * kScalesAhead + b) * BLOCKS * kScalePitch + row0 + (lane >> 3);
+          const float* from = p.g.x_scale + kb + b;
+          auto row_scale = [&](int i) {
+            const int r = __shfl_sync(0xffffffffu, i < 8 ? source[0] : source[1], (i & 7) * 4 + (lane >> 3));
+            return there && r >= 0 ? from[static_cast<int64_t>(r) * p.k_blocks] : 0.0f;
+          };
+#pragma unroll 1
+          for (int i0 = 0; i0 < 16; i0 += 8) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = row_scale(i0 + i);
+#pragma unroll
+            for (int s = 0; s < BLOCKS; ++s)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                to[s * kScalePitch + (i0 + i) * 4] = x[i] * w[s];
+                ends |= past_ends(x[i], w[s]);
+              }
+          }
+          ends = __any_sync(0xffffffffu, ends);
+          if (ends) {
+            const uint32_t row = 0xffu << (lane & 24);
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+              const float x = row_scale(i);
+#pragma unroll
+              for (int s = 0; s < BLOCKS; ++s) {
+                const float v = fabsf(x * w[s]);
+                const bool over = __ballot_sync(0xffffffffu, v == INFINITY) & row;
+                const bool under = __ballot_sync(0xffffffffu, past_ends(x, w[s])) & row;
+                const bool large = __ballot_sync(0xffffffffu, !(v < 1.0f / kHalfFrame)) & row;
+                const int frame = over ? 1 : under && !large ? -1 : 0;
+                const float f = frame > 0 ? 1.0f / kHalfFrame : kHalfFrame;
+                if (frame) to[s * kScalePitch + i * 4] = (x * f) * (w[s] * f);
+                if (b == 0) ctl.frame[slot][s][row0 + (lane >> 3) + i * 4] = static_cast<int8_t>(frame);
+              }
+            }
+          }
+          __syncwarp();
+          if (lane == 0) {
+            ctl.ends[slot][warp - 2] = ends;
+            mbar_arrive(&ctl.scale_full[slot]);
+          }
+          if (++slot == kScaleSlots) {
+            slot = 0;
+            slot_phase ^= 1;
+          }
+        }
+      }
       // rows of no expert
       clear_rows(p, p.g.kept(), p.g.rows, blockIdx.x * 64LL + (threadIdx.x - 64), gridDim.x * 64LL);
     }
   } else {
     if constexpr (S::kSplitRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kEpiRegs));
     // ------------------------------------------------------------- epilogue
-    const int quad = warp & 3, set = (warp - 4) >> 2;
+    const int quad = warp & 3, set = (warp - 4) >> 2, column = set * COLS;
     int buf = 0;
     uint32_t acc_phase = 0, red_phase = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -411,55 +560,72 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       return __shfl_sync(0xffffffffu, go, 0) != 0;
     };
     bool ok = true;
-    for (int t = t0; t < total_tiles && ok; t += step) {
+    const int first = static_cast<int>(pair_rank) * 128 + quad * 32;  // this warp's rows of a tile
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    for (int t = t0; t < total_tiles; t += step) {
       const Fp8Tile at = tiles.at(t, rank, csize);
-      const int first = static_cast<int>(pair_rank) * 128 + quad * 32;  // this warp's rows of the tile
-      const int rows = at.rows - first, col0 = at.col0 + set * COLS;
+      const int rows = at.rows - first, col0 = at.col0 + column;
       const bool any = rows > 0 && col0 < p.g.N;
-      const int64_t source = lane < rows ? p.g.source(at.row0 + first + lane) : -1;
-      const float* xs = p.g.x_scale + source * p.k_blocks;
-      const float* ws = p.g.w_scale +
-                        (static_cast<int64_t>(at.expert) * p.n_blocks + min(col0 >> 7, p.n_blocks - 1)) * p.k_blocks;
+      int frame = 0;
       float total[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) total[i] = 0.0f;
-      float next_x = 0.0f, next_w = 0.0f;
-      auto fetch = [&](int kb) {
-        next_x = source >= 0 ? xs[kb] : 0.0f;
-        next_w = ws[kb];
-      };
-      fetch(at.kb0);
-      for (int kb = at.kb0; kb < at.kb1; ++kb) {
-        const float x = next_x, w = next_w;
-        if (kb + 1 < at.kb1) fetch(kb + 1);
-        ok = wait(&ctl.acc_full[buf], acc_phase);
+      for (int kb0 = at.kb0; kb0 < at.kb1; kb0 += kScalesAhead) {
+        ok = tc_wait_warp<true>(&ctl.scale_full[slot], slot_phase, &ctl, p.status, true);
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16) + set * COLS;
-        auto release = [&] {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
-        };
-        if (any) {
-          uint32_t v[2][32];
-          tmem_ld32_async(acc, v[0]);
-#pragma unroll
-          for (int c = 0; c < COLS / 32; ++c) {
-            tmem_wait32(v[c & 1]);
-            if (c + 1 < COLS / 32) tmem_ld32_async(acc + (c + 1) * 32, v[(c + 1) & 1]);
-            else release();
-            add_block(total + c * 32, v[c & 1], x, w);
-          }
-        } else {
-          release();
+        const float* scales = scale_smem + (slot * kScalesAhead * BLOCKS + (column >> 7)) * kScalePitch + quad * 32 + lane;
+        int next = 0;
+        if (ctl.ends[slot][quad >> 1]) next = ctl.frame[slot][column >> 7][quad * 32 + lane];
+        if (__any_sync(0xffffffffu, next != frame)) {
+          change_frame(total, frame, next);
+          frame = next;
         }
-        if (++buf == BUFS) {
-          buf = 0;
-          acc_phase ^= 1;
+        const int n = min(at.kb1 - kb0, kScalesAhead);
+        for (int i = 0; i < n; ++i) {
+          const float s = scales[i * BLOCKS * kScalePitch];
+          ok = tc_wait_warp<true>(&ctl.acc_full[buf], acc_phase, &ctl, p.status, true);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t acc = tmem + buf * NT + (static_cast<uint32_t>(quad * 32) << 16) + column;
+          auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_done_at(at_rank(smem_u32(&ctl.acc_empty[buf]), CG == 2 ? 0 : rank));
+          };
+          if (any) {
+            // 64 columns at a time: smaller reads wait longer for TMEM (32: 252 us where this takes 242)
+#pragma unroll
+            for (int c = 0; c < COLS; c += 64) {
+              uint32_t v[2][32];
+              tmem_ld32_async(acc + c, v[0]);
+              tmem_ld32_async(acc + c + 32, v[1]);
+              tmem_wait32(v[0]);
+              tmem_wait32(v[1]);
+              if (c + 64 == COLS) release();
+#pragma unroll
+              for (int j = 0; j < 64; j += 2)
+                fma2(total[c + j], total[c + j + 1], __uint_as_float(v[j >> 5][j & 31]),
+                     __uint_as_float(v[j >> 5][(j & 31) + 1]), s);
+            }
+          } else {
+            release();
+          }
+          if (++buf == BUFS) {
+            buf = 0;
+            acc_phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.scale_empty[slot]);
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          slot_phase ^= 1;
         }
       }
       if (!ok) break;
+      if (__any_sync(0xffffffffu, frame != 0)) change_frame(total, frame, 0);
       if constexpr (S::SPLIT) {
         // every CTA puts its part into shared memory, [row][channel], and adds up every
         // csize-th piece of four channels, the parts in the CTAs' order
@@ -467,7 +633,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ok) break;
         float* part = reinterpret_cast<float*>(out_smem);
         if (lane < rows) {
-          float4* mine = reinterpret_cast<float4*>(part + (first + lane) * S::kPitch + set * COLS);
+          float4* mine = reinterpret_cast<float4*>(part + (first + lane) * S::kPitch + column);
 #pragma unroll
           for (int i = 0; i < COLS / 4; ++i)
             mine[i] = make_float4(total[4 * i], total[4 * i + 1], total[4 * i + 2], total[4 * i + 3]);
@@ -502,27 +668,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (lane < static_cast<int>(csize)) arrive_at(at_rank(smem_u32(&ctl.red_empty), lane));
         red_phase ^= 1;
       } else if (any) {
-        uint8_t* stage = out_smem + (warp - 4) * 4096;
-        const int row0 = at.row0 + first;
-        if (p.out_dtype == ES_BF16) store_rows<__nv_bfloat16, COLS>(p, stage, total, row0, rows, col0);
-        else if (p.out_dtype == ES_F16) store_rows<__half, COLS>(p, stage, total, row0, rows, col0);
-        else store_rows<float, COLS>(p, stage, total, row0, rows, col0);
+        uint8_t* stage = out_smem + (warp - 4) * kWarpOut;
+        if (p.out_dtype == ES_BF16) store_rows<__nv_bfloat16, COLS>(p, &m.out, stage, total, at.row0 + first, rows, col0);
+        else if (p.out_dtype == ES_F16) store_rows<__half, COLS>(p, &m.out, stage, total, at.row0 + first, rows, col0);
+        else store_rows<float, COLS>(p, &m.out, stage, total, at.row0 + first, rows, col0);
       }
     }
   }
+  bulk_wait();
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (csize > 1) cluster_sync();
   tc_fence_after();
-  if (warp == 1) tc_dealloc<CG>(tmem, S::kColumns);
+  if (warp == 1) tc_dealloc<CG>(tmem, BUFS * NT);
 }
 
 template <typename S>
 int launch(const Fp8Args& p, const Fp8Maps& m, int64_t max_tiles, int csize, cudaStream_t stream) {
-  constexpr size_t fixed = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kOutBytes;
+  constexpr size_t fixed = 1024 + static_cast<size_t>(S::kStages) * S::kStageBytes + S::kOutBytes + S::kScaleBytes;
   constexpr size_t most = fixed + (3 * kMaxExperts + 1) * sizeof(int);
-  static_assert(most <= 227 * 1024 - sizeof(Fp8Ctl) - 1024, "shared memory of an SM");
+  static_assert(most + sizeof(Fp8Ctl) <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<bool> raised[kMaxAttrDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return ES_ERR_CUDA;
@@ -625,9 +791,10 @@ int fp8_tc(const GroupedArgs& g, const void* x, const void* w, void* y, int out_
   p.wide = g.N * esz % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
   p.status = status;
   Fp8Maps m{};
-  if (!bind_context() || !encode_operand(o.x, kInt8, 128, kBoxRows, 2, &m.x) ||
-      !encode_operand(o.w, kInt8, 128, kBoxRows, 3, &m.w))
+  if (!bind_context() || !encode_operand(o.x, kInt8, 128, 128, 2, &m.x) ||
+      !encode_operand(o.x, kInt8, 128, kFewRows, 2, &m.x_few) || !encode_operand(o.w, kInt8, 128, 128, 3, &m.w))
     return ES_ERR_CUDA;
+  if (p.wide && !encode_bytes(y, g.N * esz, g.rows, 128, 32, &m.out)) return ES_ERR_CUDA;
   if (f.path == ES_GROUPED_WIDE) return launch<Fp8Shape<2, 256, false>>(p, m, f.tiles, 2, stream);
   if (f.path == ES_GROUPED_NARROW) return launch<Fp8Shape<1, 128, false>>(p, m, f.tiles, 1, stream);
   return launch<Fp8Shape<1, 128, true>>(p, m, f.tiles, f.split, stream);

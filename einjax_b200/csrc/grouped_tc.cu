@@ -470,7 +470,7 @@ __device__ __forceinline__ bool gated_tile(const TcArgs& p, TcCtl& ctl, const Ti
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_at(at_rank(smem_u32(&ctl.acc_empty[buf]), S::CG == 2 ? 0 : rank));
+      if (lane == 0) arrive_done_at(at_rank(smem_u32(&ctl.acc_empty[buf]), S::CG == 2 ? 0 : rank));
     }
     const int c0 = set * 32 + i * 64;
     if (c0 < at.rows) gated_block(p, g, u, at.row0 + c0, at.rows - c0, ch, ch < p.lanes);

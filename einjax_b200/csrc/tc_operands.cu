@@ -219,6 +219,10 @@ bool bind_context() {
   return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
 }
 
+bool encode_bytes(const void* p, int64_t row_bytes, int64_t rows, int box_bytes, int box_rows, CUtensorMap* map) {
+  return encode_map(MapSpec{p, kInt8, row_bytes, rows, 1, row_bytes, rows * row_bytes, box_bytes, box_rows}, 2, map);
+}
+
 bool encode_operand(const Operand& o, int dtype, int box_cols, int box_rows, int rank, CUtensorMap* map) {
   const int64_t esz = tc_size(dtype), planes = planes_of(dtype);
   const int64_t rows = rank == 2 ? planes * o.rows : o.rows, depth = rank == 3 ? planes * o.depth : 1;

@@ -40,6 +40,8 @@ Operand operand_of(const void* p, int dtype, int64_t depth, int64_t rows, int64_
 // Copies an operand that has to be copied to `to` (Operand::bytes). by_row: its rows are the
 // grouped rows of g; by_expert: a matrix an expert, those without rows left out.
 int lay_out(const GroupedArgs& g, Operand& o, int dtype, bool by_row, bool by_expert, void* to, cudaStream_t stream);
+// Map of contiguous rows of bytes (16-byte address and pitch) in swizzled boxes of box_bytes x box_rows.
+bool encode_bytes(const void* p, int64_t row_bytes, int64_t rows, int box_bytes, int box_rows, CUtensorMap* map);
 bool bind_context();
 bool encode_operand(const Operand& o, int dtype, int box_cols, int box_rows, int rank, CUtensorMap* map);
 

@@ -39,6 +39,13 @@ __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// Arrives where this thread publishes no memory (TMEM handed back, its loads done): a
+// release of the whole cluster's scope would wait for the thread's global stores and
+// loads, which cost the scaled 8-bit product 2000 cycles a block.
+__device__ __forceinline__ void arrive_done_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -73,16 +80,23 @@ __device__ __forceinline__ float load_at(uint32_t cluster_addr) {
   return v;
 }
 
+// The same within the CTA's scope: for what TMA or the tensor cores signal, and TMEM
+// handed back (no memory of another CTA is read behind it).
+__device__ __forceinline__ bool try_wait_cta(uint64_t* bar, uint32_t parity) { return mbar_try_wait(bar, parity); }
+
 // Bounded wait; false when this CTA has given up. Ctl: a struct in shared memory
 // with `abort`, set when a wait runs out, and `progress`, a counter whose movement
 // shows (where `progress` asks for it) that the wait is long and not stuck.
-template <typename Ctl>
+template <bool CTA = false, typename Ctl>
 __device__ bool tc_wait(uint64_t* bar, uint32_t parity, Ctl* ctl, int32_t* status, bool progress = false) {
-  if (try_wait_cluster(bar, parity)) return true;
+  auto try_wait = [&] { return CTA ? try_wait_cta(bar, parity) : try_wait_cluster(bar, parity); };
+  // most waits are short: the timer's own latency stays out of them
+  for (int i = 0; i < 64; ++i)
+    if (try_wait()) return true;
   uint64_t t0 = global_ns();
   uint32_t seen = *reinterpret_cast<volatile uint32_t*>(&ctl->progress);
   for (uint32_t i = 1;; ++i) {
-    if (try_wait_cluster(bar, parity)) return true;
+    if (try_wait()) return true;
     if ((i & 31) == 0) {
       if (*reinterpret_cast<volatile int*>(&ctl->abort)) return false;
       const uint64_t now = global_ns();
@@ -100,12 +114,12 @@ __device__ bool tc_wait(uint64_t* bar, uint32_t parity, Ctl* ctl, int32_t* statu
 }
 
 // The wait of a whole warp: one look by all, then lane 0 waits for them.
-template <typename Ctl>
+template <bool CTA = false, typename Ctl>
 __device__ __forceinline__ bool tc_wait_warp(uint64_t* bar, uint32_t parity, Ctl* ctl, int32_t* status,
                                              bool progress = false) {
-  if (__all_sync(0xffffffffu, try_wait_cluster(bar, parity))) return true;
+  if (__all_sync(0xffffffffu, CTA ? try_wait_cta(bar, parity) : try_wait_cluster(bar, parity))) return true;
   int go = 0;
-  if ((threadIdx.x & 31) == 0) go = tc_wait(bar, parity, ctl, status, progress) ? 1 : 0;
+  if ((threadIdx.x & 31) == 0) go = tc_wait<CTA>(bar, parity, ctl, status, progress) ? 1 : 0;
   return __shfl_sync(0xffffffffu, go, 0) != 0;
 }
 
