@@ -65,11 +65,45 @@ __device__ __forceinline__ Vec<T, VEC> load(const T* p, int64_t piece) {
   return reinterpret_cast<const Vec<T, VEC>*>(p)[piece];
 }
 
+// All values of a piece in fp32 and back: two 16-bit values an instruction.
+template <typename T, int VEC>
+__device__ __forceinline__ void widen(const Vec<T, VEC>& p, float (&v)[VEC]) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC % 2 == 0) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p.v);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {  // a bf16 is the high half of its fp32
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else if constexpr (std::is_same<T, __half>::value && VEC % 2 == 0) {
+    const __half2* w = reinterpret_cast<const __half2*>(p.v);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      const float2 f = __half22float2(w[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(p.v[i]);
+  }
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ void store(T* p, int64_t piece, const float (&v)[VEC]) {
   Vec<T, VEC> o;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value && VEC % 2 == 0) {
+    __nv_bfloat162* w = reinterpret_cast<__nv_bfloat162*>(o.v);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < VEC / 2; ++i) w[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  } else if constexpr (std::is_same<T, __half>::value && VEC % 2 == 0) {
+    __half2* w = reinterpret_cast<__half2*>(o.v);
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) w[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(v[i]);
+  }
   reinterpret_cast<Vec<T, VEC>*>(p)[piece] = o;
 }
 
@@ -81,7 +115,10 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*part)[32], int 
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(kAll, v[i], o);
-  if (tp <= 32) return;
+  if (tp <= 32) {
+    __syncwarp();
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tp >> 5;
   if (lane == 0) {
 #pragma unroll
@@ -99,8 +136,8 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*part)[32], int 
 
 constexpr float kDown = 2.6469779601696886e-23f;  // 2^-75: squares of the largest values, 2^16 of them and more, are finite
 
-__device__ __forceinline__ float inv_rms(float sum, float width, float eps) {
-  return 1.0f / sqrtf(sum / width + eps);
+__device__ __forceinline__ float inv_rms(float sum, float inv_width, float eps) {
+  return rsqrtf(fmaf(sum, inv_width, eps));
 }
 
 template <typename T, typename W, int VEC, int NP>
@@ -117,7 +154,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_kernel(const __grid_constan
   const T* gate = static_cast<const T*>(p.gate) + (p.gate_kind == ES_GATE_CHANNEL ? 0 : row * p.gate_stride);
   const W* w_out = static_cast<const W*>(p.w_out);
   const W* w_in = static_cast<const W*>(p.w_in);
-  const float width = static_cast<float>(p.width);
+  const float width = 1.0f / static_cast<float>(p.width);
   Vec<T, VEC> xv[HELD], hv[HELD];
   float o[HELD][VEC];
 
@@ -369,6 +406,370 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_kernel(const __grid_co
   }
 }
 
+// ------------------------------------------- rows that a group holds, walked
+//
+// The form for rows of up to 1024 pieces of 16 bytes: a group of threads walks every
+// so-many-th row, NP pieces a thread.
+//
+// SHIFT: rows whose length is no multiple of a piece. Contiguous rows of one length start
+// at one phase within their 16 bytes in all tensors, so the pieces are cut at the
+// addresses' borders instead, value e of the row being value (e + phase) % VEC of its piece,
+// and only a row's first and last piece are read value by value. Weights and column sums
+// lie in shared memory with value e at [e % VEC][e / VEC], where no bank is met twice
+// whatever the phase (4099 x 5001 f16: 78 us value by value, see the launch below).
+
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// Place of value c * VEC + i - phase of a column array in shared memory; one piece of room
+// on either side.
+template <int VEC>
+__device__ __forceinline__ int column_at(int64_t c, int i, int phase, int pitch) {
+  const int j = i - phase;
+  return (j & (VEC - 1)) * pitch + static_cast<int>(c) + (j < 0 ? 0 : 1);
+}
+
+template <typename T, bool SHIFT>
+__device__ __forceinline__ Vec<T, kVec<T>> load_piece(const T* row, int64_t c, int phase, int64_t width) {
+  constexpr int VEC = kVec<T>;
+  if constexpr (!SHIFT) {
+    return load<T, VEC>(row, c);
+  } else {
+    const int64_t e = c * VEC - phase;
+    if (e >= 0 && e + VEC <= width) return *reinterpret_cast<const Vec<T, VEC>*>(row + e);
+    Vec<T, VEC> v;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v.v[i] = e + i >= 0 && e + i < width ? row[e + i] : T(0.0f);
+    return v;
+  }
+}
+
+template <typename T, bool SHIFT>
+__device__ __forceinline__ void store_piece(T* row, int64_t c, int phase, int64_t width, const float (&v)[kVec<T>]) {
+  constexpr int VEC = kVec<T>;
+  if constexpr (!SHIFT) {
+    store<T, VEC>(row, c, v);
+  } else {
+    const int64_t e = c * VEC - phase;
+    if (e >= 0 && e + VEC <= width) {
+      store<T, VEC>(row + e, 0, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (e + i >= 0 && e + i < width) row[e + i] = from_f32<T>(v[i]);
+    }
+  }
+}
+
+// The columns' arrays (norm_out, norm_in, a gate by channel): read where they lie (they
+// stay in the L1), or of shifted rows from shared memory. `at` has the first value of the
+// piece's place; values are found from it by `get`.
+template <typename T, typename W, bool SHIFT>
+struct Columns {
+  const W* w_out;
+  const W* w_in;
+  const T* gate;
+  int pitch;
+
+  // Copies what there is to `shared` and points there; the CTA's threads together.
+  __device__ __forceinline__ void read(const NormArgs& p, uint8_t* shared) {
+    w_out = static_cast<const W*>(p.w_out);
+    w_in = static_cast<const W*>(p.w_in);
+    gate = p.gate_kind == ES_GATE_CHANNEL ? static_cast<const T*>(p.gate) : nullptr;
+    pitch = static_cast<int>(p.width / kVec<T>) + 3;
+    if constexpr (SHIFT) {
+      if (w_out) w_out = copy(w_out, shared, p.width);
+      if (w_in) w_in = copy(w_in, shared, p.width);
+      if (gate) gate = copy(gate, shared, p.width);
+      __syncthreads();
+    }
+  }
+  template <typename V>
+  __device__ __forceinline__ const V* copy(const V* from, uint8_t*& shared, int64_t width) {
+    constexpr int VEC = kVec<T>;
+    V* to = reinterpret_cast<V*>(shared);
+    shared += VEC * pitch * sizeof(V);
+    for (int i = threadIdx.x; i < VEC * pitch; i += blockDim.x) {
+      const int64_t e = static_cast<int64_t>(i % pitch - 1) * VEC + i / pitch;
+      to[i] = e >= 0 && e < width ? from[e] : V(0.0f);
+    }
+    return to;
+  }
+  template <typename V>
+  __device__ __forceinline__ void get(const V* from, int64_t c, int phase, float (&v)[kVec<T>]) const {
+    constexpr int VEC = kVec<T>;
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = to_f32(from[column_at<VEC>(c, i, phase, pitch)]);
+    } else {
+      widen(load<V, VEC>(from, c), v);
+    }
+  }
+};
+
+template <typename T, typename W, int NP, bool SHIFT>
+__global__ void __launch_bounds__(kMostThreads, 2) norm_rows_kernel(const __grid_constant__ NormArgs p) {
+  constexpr int VEC = kVec<T>;
+  extern __shared__ __align__(16) uint8_t shared_columns[];
+  __shared__ float part[2][4][1][32];
+  const int tp = p.tp, c0 = threadIdx.x % tp, per = blockDim.x / tp;
+  const float inv_width = 1.0f / static_cast<float>(p.width);
+  Columns<T, W, SHIFT> cols;
+  cols.read(p, shared_columns);
+  const int64_t step = gridDim.x * static_cast<int64_t>(per);
+  int64_t t = blockIdx.x * static_cast<int64_t>(per) + threadIdx.x / tp;
+  int turn = 0;
+  for (int64_t t0 = blockIdx.x * static_cast<int64_t>(per); t0 < p.rows; t0 += step, t += step, turn ^= 1) {
+    const bool live = t < p.rows;
+    const int phase = SHIFT ? static_cast<int>(t * p.width % VEC) : 0;
+    const int64_t pieces = !live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC;
+    const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
+    const T* h = static_cast<const T*>(p.h) + t * p.h_stride;
+    const T* gate = static_cast<const T*>(p.gate) + t * p.gate_stride;
+    // fn(slot, piece); the values past a shifted row's ends are zero
+    auto each = [&](auto fn) {
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        if (c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
+    };
+    Vec<T, VEC> xv[NP], hv[NP], gv[NP];
+    each([&](int n, int64_t c) {
+      if (p.h) hv[n] = load_piece<T, SHIFT>(h, c, phase, p.width);
+      xv[n] = load_piece<T, SHIFT>(x, c, phase, p.width);
+      if (p.gate_kind == ES_GATE_FULL) gv[n] = load_piece<T, SHIFT>(gate, c, phase, p.width);
+    });
+    const float token = p.gate_kind == ES_GATE_TOKEN && live ? to_f32(gate[0]) : 1.0f;
+    auto rms = [&](auto value, float (*buf)[32], float (*again)[32]) {  // value(slot, fp32 values)
+      float sum[1] = {0.0f};
+      each([&](int n, int64_t) {
+        float v[VEC];
+        value(n, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
+      });
+      group_sum(sum, buf, tp);
+      const bool big = live && !(sum[0] < INFINITY);
+      // squares past the largest value: the same sum of smaller ones. All threads of the
+      // CTA decide alike, for the barrier in it.
+      if (per == 1 ? big : tp > 32 ? __syncthreads_or(big) : __any_sync(kAll, big)) {
+        float small[1] = {0.0f};
+        each([&](int n, int64_t) {
+          float v[VEC];
+          value(n, v);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) small[0] = fmaf(v[i] * kDown, v[i] * kDown, small[0]);
+        });
+        group_sum(small, again, tp);
+        if (big) return inv_rms(small[0], inv_width, p.eps * kDown * kDown) * kDown;
+      }
+      return inv_rms(sum[0], inv_width, p.eps);
+    };
+    float r1 = 1.0f, r2 = 1.0f, o[NP][VEC];
+    if (p.w_out) r1 = rms([&](int n, float (&v)[VEC]) { widen(hv[n], v); }, part[turn][0], part[turn][1]);
+    each([&](int n, int64_t c) {
+      widen(xv[n], o[n]);
+      if (p.h) {
+        float z[VEC], g[VEC];
+        widen(hv[n], z);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          z[i] *= r1;
+          g[i] = token;
+        }
+        if (p.w_out) {
+          float w[VEC];
+          cols.get(cols.w_out, c, phase, w);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) z[i] *= w[i];
+        }
+        if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, phase, g);
+        if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[n][i] = fmaf(p.scale * g[i], z[i], o[n][i]);
+      }
+      if (p.out) store_piece<T, SHIFT>(static_cast<T*>(p.out) + t * p.width, c, phase, p.width, o[n]);
+    });
+    if (p.w_in) {
+      r2 = rms(
+          [&](int n, float (&v)[VEC]) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = o[n][i];
+          },
+          part[turn][2], part[turn][3]);
+      each([&](int n, int64_t c) {
+        float w[VEC];
+        cols.get(cols.w_in, c, phase, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[i] *= o[n][i] * r2;
+        store_piece<T, SHIFT>(static_cast<T*>(p.y) + t * p.width, c, phase, p.width, w);
+      });
+    }
+    if (p.stats && live && c0 == 0) {
+      p.stats[2 * t] = r1;
+      p.stats[2 * t + 1] = r2;
+    }
+  }
+}
+
+// The gradients. Column sums lie in shared memory, a group's own: of shifted rows a value's
+// owner changes from row to row, and the row's reduction is a barrier between them.
+template <typename T, typename W, int NP, bool SHIFT>
+__global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __grid_constant__ NormArgs p) {
+  constexpr int VEC = kVec<T>;
+  extern __shared__ __align__(16) uint8_t shared_columns[];
+  __shared__ float part[2][3][32];
+  const int tp = p.tp, c0 = threadIdx.x % tp, per = blockDim.x / tp, pitch = static_cast<int>(p.width / VEC) + 3;
+  const float inv_width = 1.0f / static_cast<float>(p.width);
+  const int column = VEC * pitch;  // floats of a column sum
+  float* const all = reinterpret_cast<float*>(shared_columns);
+  float* const sums = all + threadIdx.x / tp * p.columns * column;
+  Columns<T, W, SHIFT> cols;
+  cols.read(p, shared_columns + static_cast<size_t>(per) * p.columns * column * sizeof(float));
+  for (int i = threadIdx.x; i < per * p.columns * column; i += blockDim.x) all[i] = 0.0f;
+  __syncthreads();
+  auto add = [&](int k, int64_t c, int phase, const float (&v)[VEC]) {
+    float* to = sums + k * column;
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) to[column_at<VEC>(c, i, phase, pitch)] += v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; i += 4) {
+        float4* at = reinterpret_cast<float4*>(to + c * VEC + i);
+        float4 s = *at;
+        s.x += v[i];
+        s.y += v[i + 1];
+        s.z += v[i + 2];
+        s.w += v[i + 3];
+        *at = s;
+      }
+    }
+  };
+  const int64_t step = gridDim.x * static_cast<int64_t>(per);
+  int64_t t = blockIdx.x * static_cast<int64_t>(per) + threadIdx.x / tp;
+  int turn = 0;
+  const bool by_token = p.gate_kind == ES_GATE_TOKEN;
+  for (int64_t t0 = blockIdx.x * static_cast<int64_t>(per); t0 < p.rows; t0 += step, t += step, turn ^= 1) {
+    const bool live = t < p.rows;
+    const int64_t row = live ? t : 0;
+    const int phase = SHIFT ? static_cast<int>(t * p.width % VEC) : 0;
+    const int64_t pieces = !live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC;
+    const T* gate = static_cast<const T*>(p.gate) + row * p.gate_stride;
+    auto each = [&](auto fn) {
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+        if (c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
+    };
+    Vec<T, VEC> xv[NP], hv[NP], ov[NP], yv[NP], gv[NP];
+    each([&](int n, int64_t c) {
+      xv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.x) + t * p.x_stride, c, phase, p.width);
+      if (p.h) hv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.h) + t * p.h_stride, c, phase, p.width);
+      if (p.dout) ov[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.dout) + t * p.dout_stride, c, phase, p.width);
+      if (p.dy) yv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.dy) + t * p.dy_stride, c, phase, p.width);
+      if (p.gate_kind == ES_GATE_FULL) gv[n] = load_piece<T, SHIFT>(gate, c, phase, p.width);
+    });
+    const float r1 = p.w_out ? p.stats[2 * row] : 1.0f, r2 = p.dy ? p.stats[2 * row + 1] : 0.0f;
+    const float token = by_token ? to_f32(gate[0]) : 1.0f;
+    // scale times the gate, and z, of a piece
+    auto branch = [&](int n, int64_t c, float (&g)[VEC], float (&z)[VEC]) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        g[i] = token;
+        z[i] = 0.0f;
+      }
+      if (p.h) widen(hv[n], z);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) z[i] *= r1;
+      if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, phase, g);
+      if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] *= p.scale;
+      if (p.w_out) {
+        float w[VEC];
+        cols.get(cols.w_out, c, phase, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[i] *= w[i];
+      }
+    };
+    float unit[NP][VEC], d0[NP][VEC], v[3] = {0.0f, 0.0f, 0.0f};
+    each([&](int n, int64_t c) {
+      float g[VEC], z[VEC], b[VEC];
+      branch(n, c, g, z);
+      widen(xv[n], unit[n]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        unit[n][i] = fmaf(g[i], z[i], unit[n][i]) * r2;
+        d0[n][i] = 0.0f;
+      }
+      if (p.dout) widen(ov[n], d0[n]);
+      if (p.dy) {
+        float y[VEC];
+        widen(yv[n], y);
+        cols.get(cols.w_in, c, phase, b);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          b[i] *= y[i];
+          d0[n][i] = fmaf(r2, b[i], d0[n][i]);
+          v[0] = fmaf(b[i], unit[n][i], v[0]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (!by_token) z[i] *= g[i];
+        v[1] = fmaf(z[i], d0[n][i], v[1]);
+        v[2] = fmaf(z[i], unit[n][i], v[2]);
+      }
+    });
+    group_sum(v, part[turn], tp);
+    const float c2 = v[0] * inv_width * r2, zd = v[1] - c2 * v[2];
+    const float c1 = (by_token ? p.scale * token * zd : zd) * inv_width;
+    if (by_token && p.dgate && live && c0 == 0) static_cast<T*>(p.dgate)[t] = from_f32<T>(p.scale * zd);
+    each([&](int n, int64_t c) {
+      float g[VEC], z[VEC], d[VEC];
+      branch(n, c, g, z);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) d[i] = fmaf(-c2, unit[n][i], d0[n][i]);
+      if (p.dx) store_piece<T, SHIFT>(static_cast<T*>(p.dx) + t * p.width, c, phase, p.width, d);
+      if (p.in_col >= 0) {
+        float a[VEC];
+        widen(yv[n], a);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a[i] *= unit[n][i];
+        add(p.in_col, c, phase, a);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        z[i] *= p.scale * d[i];  // the gate's gradient
+        d[i] *= g[i];            // z's
+      }
+      if (p.gate_col >= 0) add(p.gate_col, c, phase, z);
+      if (p.dgate && p.gate_kind == ES_GATE_FULL)
+        store_piece<T, SHIFT>(static_cast<T*>(p.dgate) + t * p.width, c, phase, p.width, z);
+      if (p.w_out) {
+        float w[VEC], hat[VEC];
+        cols.get(cols.w_out, c, phase, w);
+        widen(hv[n], hat);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) hat[i] *= r1;
+        if (p.out_col >= 0) {
+          float a[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) a[i] = d[i] * hat[i];
+          add(p.out_col, c, phase, a);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d[i] = r1 * fmaf(-hat[i], c1, d[i] * w[i]);
+      }
+      if (p.dh) store_piece<T, SHIFT>(static_cast<T*>(p.dh) + t * p.width, c, phase, p.width, d);
+    });
+  }
+  __syncthreads();
+  float* parts = p.part + (blockIdx.x * static_cast<int64_t>(per) + threadIdx.x / tp) * p.columns * p.width;
+  for (int k = 0; k < p.columns; ++k)
+    for (int64_t e = c0; e < p.width; e += tp)
+      parts[k * p.width + e] = sums[k * column + (SHIFT ? (e % VEC) * pitch + e / VEC + 1 : e)];
+}
+
 // Adds the groups' parts of each column in their order: 32 columns by 8 slices
 // of the groups a CTA, the slices' sums added in their order.
 struct SumArgs {
@@ -414,34 +815,77 @@ struct RowForm {
 RowForm row_form(int64_t pieces, int most) {
   for (int threads = kNormThreads; threads <= kMostThreads; threads *= 2)
     for (int np = 1; np <= most; np *= 2) {
-      const int64_t tp = (pieces + 32 * np - 1) / (32 * np) * 32;
+      const int64_t tp = pieces > 0 ? (pieces + 32 * np - 1) / (32 * np) * 32 : 32;
       if (tp <= threads) return RowForm{static_cast<int>(tp), np};
     }
   return RowForm{kMostThreads, 0};
 }
 
-// Groups of threads that walk the rows of a backward pass.
-int64_t grad_groups(int64_t rows, const RowForm& f) {
-  const int64_t per = f.groups(), ctas = (rows + per - 1) / per, most = kSMs * (kMostThreads / f.threads());
+// Groups of threads that walk the rows, `resident` threads an SM.
+int64_t walking_groups(int64_t rows, const RowForm& f, int resident) {
+  const int64_t per = f.groups(), ctas = (rows + per - 1) / per, most = kSMs * (resident / f.threads());
   return (ctas < most ? ctas : most) * per;
 }
 
-// Pieces that a thread holds, at most: registers for three fp32 sums of a value in
-// the backward pass, for the residual in fp32 in the forward one.
-constexpr int held(int vec) { return vec == 1 ? 16 : 4; }
-constexpr int held_grad(int vec) { return vec == 1 ? 16 : 16 / vec; }
+// The general backward form's.
+int64_t grad_groups(int64_t rows, const RowForm& f) { return walking_groups(rows, f, kMostThreads); }
+
+// The walked form's: with few rows a piece a thread while 512 threads hold the row; with
+// many two, since what a warp does for a row (its reductions) costs as much as a piece.
+RowForm walked_form(int64_t pieces, int64_t rows) {
+  for (int np = rows < 4 * kSMs ? 1 : 2; np <= 2; np *= 2) {
+    const int64_t tp = pieces > 0 ? (pieces + 32 * np - 1) / (32 * np) * 32 : 32;
+    if (tp <= kMostThreads) {
+      while (np > 1 && np * 16 >= pieces) np /= 2;  // rows that fewer pieces a lane hold
+      return RowForm{static_cast<int>(tp), np};
+    }
+  }
+  return RowForm{kMostThreads, 0};
+}
+
+constexpr size_t kMostColumnsSmem = 200 * 1024;
+
+size_t columns_bytes(int64_t width, int vec, size_t bytes) {
+  return static_cast<size_t>(vec) * (width / vec + 3) * bytes;
+}
+
+// Bytes of one channel of the arrays that shifted rows keep in shared memory.
+size_t array_bytes(const NormArgs& p, size_t weight, size_t value) {
+  return ((p.w_in != nullptr) + (p.w_out != nullptr)) * weight + (p.gate_kind == ES_GATE_CHANNEL ? value : 0);
+}
+
+// Raises a kernel's limit of shared memory, once a device.
+template <typename K>
+int raise_smem(K kernel, std::atomic<bool> (&raised)[kMaxAttrDevices]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return ES_ERR_CUDA;
+  const bool tracked = dev >= 0 && dev < kMaxAttrDevices;
+  if (tracked && raised[dev].load(std::memory_order_relaxed)) return ES_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMostColumnsSmem)) !=
+      cudaSuccess)
+    return ES_ERR_CUDA;
+  if (tracked) raised[dev].store(true, std::memory_order_relaxed);
+  return ES_OK;
+}
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int64_t piece_size(const NormArgs& p, int esz) {
+// How the rows lie: in whole pieces of 16 bytes, all at one phase within them, or neither.
+enum Lie { kWhole, kPhase, kAny };
+
+Lie lie_of(const NormArgs& p, int esz) {
   const int64_t vec = 16 / esz;
-  const bool ok = p.width % vec == 0 && p.x_stride % vec == 0 && p.h_stride % vec == 0 &&
-                  (p.gate_kind != ES_GATE_FULL || p.gate_stride % vec == 0) && p.dout_stride % vec == 0 &&
-                  p.dy_stride % vec == 0 && aligned16(p.x) && aligned16(p.h) && aligned16(p.w_in) &&
-                  aligned16(p.w_out) && (p.gate_kind == ES_GATE_TOKEN || aligned16(p.gate)) && aligned16(p.out) &&
-                  aligned16(p.y) && aligned16(p.dout) && aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh) &&
-                  (p.gate_kind != ES_GATE_FULL || aligned16(p.dgate)) && aligned16(p.part);
-  return ok ? vec : 1;
+  const bool full = p.gate_kind == ES_GATE_FULL;
+  if (!(aligned16(p.x) && aligned16(p.h) && aligned16(p.out) && aligned16(p.y) && aligned16(p.dout) &&
+        aligned16(p.dy) && aligned16(p.dx) && aligned16(p.dh) && (!full || (aligned16(p.gate) && aligned16(p.dgate)))))
+    return kAny;
+  if (p.width % vec == 0 && p.x_stride % vec == 0 && p.h_stride % vec == 0 && (!full || p.gate_stride % vec == 0) &&
+      p.dout_stride % vec == 0 && p.dy_stride % vec == 0 && aligned16(p.w_in) && aligned16(p.w_out) &&
+      (p.gate_kind != ES_GATE_CHANNEL || aligned16(p.gate)) && aligned16(p.part))
+    return kWhole;
+  const bool one = p.x_stride == p.width && (!p.h || p.h_stride == p.width) && (!full || p.gate_stride == p.width) &&
+                   (!p.dout || p.dout_stride == p.width) && (!p.dy || p.dy_stride == p.width);
+  return one ? kPhase : kAny;
 }
 
 // fn(integral_constant<pieces>)
@@ -453,28 +897,83 @@ int by_pieces(int np, Fn fn) {
   return fn(std::integral_constant<int, MOST>{});
 }
 
-template <typename T, typename W, int VEC>
-int forward(NormArgs& p, cudaStream_t s) {
-  const RowForm f = row_form(p.width / VEC, held(VEC));
+template <typename T, typename W, bool SHIFT>
+int forward_rows(NormArgs& p, const RowForm& f, size_t smem, cudaStream_t s) {
   p.tp = f.tp;
-  const int64_t per = f.groups();
-  const unsigned blocks = static_cast<unsigned>((p.rows + per - 1) / per);
-  return by_pieces<held(VEC)>(f.np, [&](auto np) {
-    ES_LAUNCH((norm_kernel<T, W, VEC, decltype(np)::value>), blocks, f.threads(), 0, s, p);
+  const unsigned blocks = static_cast<unsigned>(walking_groups(p.rows, f, 2 * kMostThreads) / f.groups());
+  return by_pieces<2>(f.np, [&](auto np) {
+    constexpr int NP = decltype(np)::value;
+    if constexpr (NP > 0) {
+      static std::atomic<bool> raised[kMaxAttrDevices];
+      if (smem > 48 * 1024) ES_TRY(raise_smem(norm_rows_kernel<T, W, NP, SHIFT>, raised));
+      ES_LAUNCH((norm_rows_kernel<T, W, NP, SHIFT>), blocks, f.threads(), smem, s, p);
+    }
     return static_cast<int>(ES_OK);
   });
 }
 
-template <typename T, typename W, int VEC>
-int backward(NormArgs& p, const SumArgs& sums, cudaStream_t s) {
-  const RowForm f = row_form(p.width / VEC, held_grad(VEC));
-  p.tp = f.tp;
-  const int64_t groups = grad_groups(p.rows, f);
-  const unsigned blocks = static_cast<unsigned>(groups / f.groups());
-  ES_TRY(by_pieces<held_grad(VEC)>(f.np, [&](auto np) {
-    ES_LAUNCH((norm_grad_kernel<T, W, VEC, decltype(np)::value>), blocks, f.threads(), 0, s, p);
+template <typename T, typename W>
+int forward(NormArgs& p, cudaStream_t s) {
+  constexpr int VEC = kVec<T>;
+  const Lie lie = lie_of(p, sizeof(T));
+  const RowForm f = walked_form(lie == kPhase ? (p.width + 2 * VEC - 2) / VEC : p.width / VEC, p.rows);
+  const size_t smem = lie == kPhase ? columns_bytes(p.width, VEC, array_bytes(p, sizeof(W), sizeof(T))) : 0;
+  if (f.np && lie != kAny && smem <= kMostColumnsSmem)
+    return lie == kWhole ? forward_rows<T, W, false>(p, f, smem, s) : forward_rows<T, W, true>(p, f, smem, s);
+  const RowForm r = lie == kWhole ? RowForm{kMostThreads, 0} : row_form(p.width, 16);
+  p.tp = r.tp;
+  const int64_t per = r.groups();
+  const unsigned blocks = static_cast<unsigned>((p.rows + per - 1) / per);
+  if (lie == kWhole) {
+    ES_LAUNCH((norm_kernel<T, W, VEC, 0>), blocks, r.threads(), 0, s, p);
+    return ES_OK;
+  }
+  return by_pieces<16>(r.np, [&](auto np) {
+    ES_LAUNCH((norm_kernel<T, W, 1, decltype(np)::value>), blocks, r.threads(), 0, s, p);
     return static_cast<int>(ES_OK);
-  }));
+  });
+}
+
+template <typename T, typename W, bool SHIFT>
+int backward_rows(NormArgs& p, const RowForm& f, int64_t groups, size_t smem, cudaStream_t s) {
+  p.tp = f.tp;
+  return by_pieces<2>(f.np, [&](auto np) {
+    constexpr int NP = decltype(np)::value;
+    if constexpr (NP > 0) {
+      static std::atomic<bool> raised[kMaxAttrDevices];
+      if (smem > 48 * 1024) ES_TRY(raise_smem(norm_grad_rows_kernel<T, W, NP, SHIFT>, raised));
+      ES_LAUNCH((norm_grad_rows_kernel<T, W, NP, SHIFT>), static_cast<unsigned>(groups / f.groups()), f.threads(),
+                smem, s, p);
+    }
+    return static_cast<int>(ES_OK);
+  });
+}
+
+template <typename T, typename W>
+int backward(NormArgs& p, const SumArgs& sums, cudaStream_t s) {
+  constexpr int VEC = kVec<T>;
+  const Lie lie = lie_of(p, sizeof(T));
+  const RowForm f = walked_form(lie == kPhase ? (p.width + 2 * VEC - 2) / VEC : p.width / VEC, p.rows);
+  const size_t smem = columns_bytes(p.width, VEC, p.columns * f.groups() * sizeof(float) +
+                                                      (lie == kPhase ? array_bytes(p, sizeof(W), sizeof(T)) : 0));
+  int64_t groups;
+  if (f.np && lie != kAny && smem <= kMostColumnsSmem) {
+    groups = walking_groups(p.rows, f, kMostThreads);
+    ES_TRY((lie == kWhole ? backward_rows<T, W, false>(p, f, groups, smem, s)
+                          : backward_rows<T, W, true>(p, f, groups, smem, s)));
+  } else {
+    const RowForm r = lie == kWhole ? RowForm{kMostThreads, 0} : row_form(p.width, 16);
+    p.tp = r.tp;
+    groups = grad_groups(p.rows, r);
+    const unsigned blocks = static_cast<unsigned>(groups / r.groups());
+    if (lie == kWhole)
+      ES_LAUNCH((norm_grad_kernel<T, W, VEC, 0>), blocks, r.threads(), 0, s, p);
+    else
+      ES_TRY(by_pieces<16>(r.np, [&](auto np) {
+        ES_LAUNCH((norm_grad_kernel<T, W, 1, decltype(np)::value>), blocks, r.threads(), 0, s, p);
+        return static_cast<int>(ES_OK);
+      }));
+  }
   if (!p.columns) return ES_OK;
   SumArgs a = sums;
   a.groups = groups;
@@ -492,14 +991,9 @@ int check_norm(const NormArgs& p, int dtype, int weight_dtype) {
   return ES_OK;
 }
 
-// fn<T, W, VEC>() by types and alignment
-#define ES_NORM_CALL(fn, ...)                                                             \
-  ES_BY_TYPE(dtype, {                                                                     \
-    constexpr int VEC = 16 / sizeof(T);                                                   \
-    const bool wide = piece_size(p, sizeof(T)) == VEC;                                    \
-    if (weight_dtype == dtype) return wide ? fn<T, T, VEC>(__VA_ARGS__) : fn<T, T, 1>(__VA_ARGS__); \
-    return wide ? fn<T, float, VEC>(__VA_ARGS__) : fn<T, float, 1>(__VA_ARGS__);          \
-  })
+// fn<T, W>() by types
+#define ES_NORM_CALL(fn, ...)                                                                     \
+  ES_BY_TYPE(dtype, return weight_dtype == dtype ? fn<T, T>(__VA_ARGS__) : fn<T, float>(__VA_ARGS__))
 
 }  // namespace
 }  // namespace es
@@ -543,11 +1037,14 @@ static int norm_columns(const void* dnorm_in, const void* dnorm_out, const void*
 
 extern "C" size_t es_residual_norm_grad_workspace_size(int dtype, int64_t num_rows, int64_t width, int num_columns) {
   if (num_rows <= 0 || width <= 0 || num_columns <= 0) return 0;
-  // the pieces may be single values, by addresses that are not known here
+  // as many groups as the form has that takes most, by addresses that are not known here
   const int vec = dtype == ES_F32 ? 4 : 8;
-  const int64_t one = grad_groups(num_rows, row_form(width, held_grad(1)));
-  const int64_t wide = grad_groups(num_rows, row_form((width + vec - 1) / vec, held_grad(vec)));
-  const int64_t groups = one > wide ? one : wide;
+  int64_t groups = grad_groups(num_rows, row_form(width, 16));
+  for (const RowForm f : {RowForm{kMostThreads, 0}, walked_form(width / vec, num_rows),
+                          walked_form((width + 2 * vec - 2) / vec, num_rows)}) {
+    const int64_t n = walking_groups(num_rows, f, kMostThreads);
+    if (n > groups) groups = n;
+  }
   return static_cast<size_t>(groups) * num_columns * width * sizeof(float);
 }
 
