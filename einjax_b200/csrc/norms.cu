@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_kernel(const __grid_co
 
 // ------------------------------------------- rows that a group holds, walked
 //
-// The form for rows of up to 1024 pieces of 16 bytes: a group of threads walks every
+// The form for rows of up to 2048 pieces of 16 bytes: a group of threads walks every
 // so-many-th row, NP pieces a thread.
 //
 // SHIFT: rows whose length is no multiple of a piece. Contiguous rows of one length start
@@ -421,13 +421,21 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_kernel(const __grid_co
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 
-// Place of value c * VEC + i - phase of a column array in shared memory; one piece of room
-// on either side.
-template <int VEC>
-__device__ __forceinline__ int column_at(int64_t c, int i, int phase, int pitch) {
-  const int j = i - phase;
-  return (j & (VEC - 1)) * pitch + static_cast<int>(c) + (j < 0 ? 0 : 1);
-}
+// Places of the values of a row's first piece in a column array in shared memory (one piece
+// of room on either side); piece c's lie c further on.
+template <int VEC, bool SHIFT>
+struct Places {
+  int at[SHIFT ? VEC : 1];
+  __device__ __forceinline__ Places(int phase, int pitch) {
+    if constexpr (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int j = i - phase;
+        at[i] = (j & (VEC - 1)) * pitch + (j < 0 ? 0 : 1);
+      }
+    }
+  }
+};
 
 template <typename T, bool SHIFT>
 __device__ __forceinline__ Vec<T, kVec<T>> load_piece(const T* row, int64_t c, int phase, int64_t width) {
@@ -496,11 +504,12 @@ struct Columns {
     return to;
   }
   template <typename V>
-  __device__ __forceinline__ void get(const V* from, int64_t c, int phase, float (&v)[kVec<T>]) const {
+  __device__ __forceinline__ void get(const V* from, int64_t c, const Places<kVec<T>, SHIFT>& places,
+                                      float (&v)[kVec<T>]) const {
     constexpr int VEC = kVec<T>;
     if constexpr (SHIFT) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = to_f32(from[column_at<VEC>(c, i, phase, pitch)]);
+      for (int i = 0; i < VEC; ++i) v[i] = to_f32(from[places.at[i] + static_cast<int>(c)]);
     } else {
       widen(load<V, VEC>(from, c), v);
     }
@@ -508,7 +517,7 @@ struct Columns {
 };
 
 template <typename T, typename W, int NP, bool SHIFT>
-__global__ void __launch_bounds__(kMostThreads, 2) norm_rows_kernel(const __grid_constant__ NormArgs p) {
+__global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel(const __grid_constant__ NormArgs p) {
   constexpr int VEC = kVec<T>;
   extern __shared__ __align__(16) uint8_t shared_columns[];
   __shared__ float part[2][4][1][32];
@@ -523,6 +532,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) norm_rows_kernel(const __grid
     const bool live = t < p.rows;
     const int phase = SHIFT ? static_cast<int>(t * p.width % VEC) : 0;
     const int64_t pieces = !live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC;
+    const Places<VEC, SHIFT> places(phase, cols.pitch);
     const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
     const T* h = static_cast<const T*>(p.h) + t * p.h_stride;
     const T* gate = static_cast<const T*>(p.gate) + t * p.gate_stride;
@@ -578,11 +588,11 @@ __global__ void __launch_bounds__(kMostThreads, 2) norm_rows_kernel(const __grid
         }
         if (p.w_out) {
           float w[VEC];
-          cols.get(cols.w_out, c, phase, w);
+          cols.get(cols.w_out, c, places, w);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) z[i] *= w[i];
         }
-        if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, phase, g);
+        if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
         if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[n][i] = fmaf(p.scale * g[i], z[i], o[n][i]);
@@ -598,7 +608,7 @@ __global__ void __launch_bounds__(kMostThreads, 2) norm_rows_kernel(const __grid
           part[turn][2], part[turn][3]);
       each([&](int n, int64_t c) {
         float w[VEC];
-        cols.get(cols.w_in, c, phase, w);
+        cols.get(cols.w_in, c, places, w);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) w[i] *= o[n][i] * r2;
         store_piece<T, SHIFT>(static_cast<T*>(p.y) + t * p.width, c, phase, p.width, w);
@@ -627,11 +637,11 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
   cols.read(p, shared_columns + static_cast<size_t>(per) * p.columns * column * sizeof(float));
   for (int i = threadIdx.x; i < per * p.columns * column; i += blockDim.x) all[i] = 0.0f;
   __syncthreads();
-  auto add = [&](int k, int64_t c, int phase, const float (&v)[VEC]) {
+  auto add = [&](int k, int64_t c, const Places<VEC, SHIFT>& places, const float (&v)[VEC]) {
     float* to = sums + k * column;
     if constexpr (SHIFT) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) to[column_at<VEC>(c, i, phase, pitch)] += v[i];
+      for (int i = 0; i < VEC; ++i) to[places.at[i] + static_cast<int>(c)] += v[i];
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; i += 4) {
@@ -654,6 +664,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
     const int64_t row = live ? t : 0;
     const int phase = SHIFT ? static_cast<int>(t * p.width % VEC) : 0;
     const int64_t pieces = !live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC;
+    const Places<VEC, SHIFT> places(phase, pitch);
     const T* gate = static_cast<const T*>(p.gate) + row * p.gate_stride;
     auto each = [&](auto fn) {
 #pragma unroll
@@ -680,44 +691,53 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
       if (p.h) widen(hv[n], z);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) z[i] *= r1;
-      if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, phase, g);
+      if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
       if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) g[i] *= p.scale;
       if (p.w_out) {
         float w[VEC];
-        cols.get(cols.w_out, c, phase, w);
+        cols.get(cols.w_out, c, places, w);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) z[i] *= w[i];
       }
     };
-    float unit[NP][VEC], d0[NP][VEC], v[3] = {0.0f, 0.0f, 0.0f};
-    each([&](int n, int64_t c) {
-      float g[VEC], z[VEC], b[VEC];
-      branch(n, c, g, z);
-      widen(xv[n], unit[n]);
+    // unit, b and d0 of a piece; of more than two pieces they are made twice instead of held
+    constexpr bool HOLD = NP <= 2;
+    float unit[HOLD ? NP : 1][VEC], d0[HOLD ? NP : 1][VEC], v[3] = {0.0f, 0.0f, 0.0f};
+    auto terms = [&](int n, int64_t c, const float (&g)[VEC], const float (&z)[VEC], float (&u)[VEC], float (&d)[VEC],
+                     float (&b)[VEC]) {
+      widen(xv[n], u);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        unit[n][i] = fmaf(g[i], z[i], unit[n][i]) * r2;
-        d0[n][i] = 0.0f;
+        u[i] = fmaf(g[i], z[i], u[i]) * r2;
+        d[i] = 0.0f;
+        b[i] = 0.0f;
       }
-      if (p.dout) widen(ov[n], d0[n]);
+      if (p.dout) widen(ov[n], d);
       if (p.dy) {
         float y[VEC];
         widen(yv[n], y);
-        cols.get(cols.w_in, c, phase, b);
+        cols.get(cols.w_in, c, places, b);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           b[i] *= y[i];
-          d0[n][i] = fmaf(r2, b[i], d0[n][i]);
-          v[0] = fmaf(b[i], unit[n][i], v[0]);
+          d[i] = fmaf(r2, b[i], d[i]);
         }
       }
+    };
+    each([&](int n, int64_t c) {
+      float g[VEC], z[VEC], b[VEC];
+      branch(n, c, g, z);
+      float(&u)[VEC] = unit[HOLD ? n : 0];
+      float(&d)[VEC] = d0[HOLD ? n : 0];
+      terms(n, c, g, z, u, d, b);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         if (!by_token) z[i] *= g[i];
-        v[1] = fmaf(z[i], d0[n][i], v[1]);
-        v[2] = fmaf(z[i], unit[n][i], v[2]);
+        v[0] = fmaf(b[i], u[i], v[0]);
+        v[1] = fmaf(z[i], d[i], v[1]);
+        v[2] = fmaf(z[i], u[i], v[2]);
       }
     });
     group_sum(v, part[turn], tp);
@@ -727,27 +747,32 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
     each([&](int n, int64_t c) {
       float g[VEC], z[VEC], d[VEC];
       branch(n, c, g, z);
+      float(&u)[VEC] = unit[HOLD ? n : 0];
+      if constexpr (!HOLD) {
+        float b[VEC];
+        terms(n, c, g, z, u, d0[0], b);
+      }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) d[i] = fmaf(-c2, unit[n][i], d0[n][i]);
+      for (int i = 0; i < VEC; ++i) d[i] = fmaf(-c2, u[i], d0[HOLD ? n : 0][i]);
       if (p.dx) store_piece<T, SHIFT>(static_cast<T*>(p.dx) + t * p.width, c, phase, p.width, d);
       if (p.in_col >= 0) {
         float a[VEC];
         widen(yv[n], a);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) a[i] *= unit[n][i];
-        add(p.in_col, c, phase, a);
+        for (int i = 0; i < VEC; ++i) a[i] *= u[i];
+        add(p.in_col, c, places, a);
       }
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         z[i] *= p.scale * d[i];  // the gate's gradient
         d[i] *= g[i];            // z's
       }
-      if (p.gate_col >= 0) add(p.gate_col, c, phase, z);
+      if (p.gate_col >= 0) add(p.gate_col, c, places, z);
       if (p.dgate && p.gate_kind == ES_GATE_FULL)
         store_piece<T, SHIFT>(static_cast<T*>(p.dgate) + t * p.width, c, phase, p.width, z);
       if (p.w_out) {
         float w[VEC], hat[VEC];
-        cols.get(cols.w_out, c, phase, w);
+        cols.get(cols.w_out, c, places, w);
         widen(hv[n], hat);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) hat[i] *= r1;
@@ -755,7 +780,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
           float a[VEC];
 #pragma unroll
           for (int i = 0; i < VEC; ++i) a[i] = d[i] * hat[i];
-          add(p.out_col, c, phase, a);
+          add(p.out_col, c, places, a);
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) d[i] = r1 * fmaf(-hat[i], c1, d[i] * w[i]);
@@ -833,7 +858,7 @@ int64_t grad_groups(int64_t rows, const RowForm& f) { return walking_groups(rows
 // The walked form's: with few rows a piece a thread while 512 threads hold the row; with
 // many two, since what a warp does for a row (its reductions) costs as much as a piece.
 RowForm walked_form(int64_t pieces, int64_t rows) {
-  for (int np = rows < 4 * kSMs ? 1 : 2; np <= 2; np *= 2) {
+  for (int np = rows < 4 * kSMs ? 1 : 2; np <= 4; np *= 2) {
     const int64_t tp = pieces > 0 ? (pieces + 32 * np - 1) / (32 * np) * 32 : 32;
     if (tp <= kMostThreads) {
       while (np > 1 && np * 16 >= pieces) np /= 2;  // rows that fewer pieces a lane hold
@@ -901,7 +926,7 @@ template <typename T, typename W, bool SHIFT>
 int forward_rows(NormArgs& p, const RowForm& f, size_t smem, cudaStream_t s) {
   p.tp = f.tp;
   const unsigned blocks = static_cast<unsigned>(walking_groups(p.rows, f, 2 * kMostThreads) / f.groups());
-  return by_pieces<2>(f.np, [&](auto np) {
+  return by_pieces<4>(f.np, [&](auto np) {
     constexpr int NP = decltype(np)::value;
     if constexpr (NP > 0) {
       static std::atomic<bool> raised[kMaxAttrDevices];
@@ -937,7 +962,7 @@ int forward(NormArgs& p, cudaStream_t s) {
 template <typename T, typename W, bool SHIFT>
 int backward_rows(NormArgs& p, const RowForm& f, int64_t groups, size_t smem, cudaStream_t s) {
   p.tp = f.tp;
-  return by_pieces<2>(f.np, [&](auto np) {
+  return by_pieces<4>(f.np, [&](auto np) {
     constexpr int NP = decltype(np)::value;
     if constexpr (NP > 0) {
       static std::atomic<bool> raised[kMaxAttrDevices];
