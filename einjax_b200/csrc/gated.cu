@@ -143,6 +143,7 @@ extern "C" int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t
   if (F > 0 && num_rows > 0 && !h) return ES_ERR_INVALID;
   const GroupedArgs g{num_experts, K, F, num_rows, x_rows, x_stride, top_k, offsets, order, w_expert_stride,
                       w_k_stride, w_n_stride, nullptr, nullptr};
+  ES_TRY(check_grouped(g));
   if (one_kernel(g, dtype)) {
     if (!h || !x || !w) return ES_ERR_INVALID;
     if (workspace_bytes < grouped_gated_tc_workspace(g, dtype, x, w)) return ES_ERR_WORKSPACE;

@@ -10,7 +10,8 @@ so it runs beside the tile-COO path instead of on it:
 * ``combine_experts``: the weighted sum of a token's rows;
 * ``quantize_rows``, ``quantize_experts``, ``int8_matmul``: the serving form
   in 8-bit integers with a scale for each token and output channel;
-* ``expert_mlp``: a gated layer made of these.
+* ``expert_mlp``: a gated layer made of these, and of ``gated_matmul``,
+  ``fp8_matmul``, ``rms_norm`` and ``residual_norm``.
 
 Gradients are reverse-mode; a forward-mode tangent is refused. All of it runs
 on torch's current CUDA stream with no wait of the host. What
@@ -54,6 +55,18 @@ def _on_gpu(fn: str, **tensors):
             dev = t.device
         elif t.device != dev:
             raise ValueError(f"{fn}: {name} is on {t.device}, the other operands on {dev}")
+
+
+def _together(*tensors) -> bool:
+    """Whether all are CUDA tensors of one device: the quick look before ``_on_gpu``, which says what is wrong."""
+    try:
+        index = tensors[0].get_device()
+        for t in tensors:
+            if t.get_device() != index:
+                return False
+        return index >= 0
+    except AttributeError:
+        return False
 
 
 def _no_tangent(fn: str, *tensors):
@@ -480,7 +493,7 @@ class _Served(torch.autograd.Function):
     """The 8-bit layer's output. A gradient through it would hold the routing's share alone, so there is none."""
 
     @staticmethod
-    def forward(ctx, out, x, router):
+    def forward(ctx, out, *inputs):
         return out.view_as(out)
 
     @staticmethod
@@ -488,37 +501,77 @@ class _Served(torch.autograd.Function):
         raise RuntimeError("expert_mlp: the 8-bit form has no gradient; train with the weights' tensors")
 
 
-def _layer(x, router, w_in, w_out, top_k, renormalize, quantized):
+def _layer(x, router, w_in, w_out, top_k, renormalize, kind, activation):
+    """kind: the weights' 8-bit type, or None."""
     weights, experts = route_experts(x.float() @ router.float(), top_k, renormalize)
     plan = plan_experts(experts, router.shape[1])
-    if quantized:
+    if kind == torch.float8_e4m3fn:
+        from .fp8 import fp8_matmul, quantize_blocks
+        h = fp8_matmul(*quantize_blocks(x), *w_in, plan, gather=True, out_dtype=x.dtype)
+        y = fp8_matmul(*quantize_blocks(h, activation=activation or "silu"), *w_out, plan, out_dtype=x.dtype)
+        return combine_experts(y, weights, plan)
+    if kind is None and activation is not None:
+        from .gated import gated_matmul
+        h = gated_matmul(x, w_in, plan, gather=True, activation=activation)
+        return combine_experts(grouped_matmul(h, w_out, plan), weights, plan)
+    if kind is not None:
         h = int8_matmul(*quantize_rows(x), *w_in, plan, gather=True, out_dtype=x.dtype)
     else:
         h = grouped_matmul(x, w_in, plan, gather=True)
     gate, up = h.chunk(2, dim=1)
     h = torch.nn.functional.silu(gate) * up
-    y = int8_matmul(*quantize_rows(h), *w_out, plan, out_dtype=x.dtype) if quantized else \
+    y = int8_matmul(*quantize_rows(h), *w_out, plan, out_dtype=x.dtype) if kind is not None else \
         grouped_matmul(h, w_out, plan)
     return combine_experts(y, weights, plan)
 
 
-def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, renormalize: bool = True):
+def _block(x, router, w_in, w_out, top_k, renormalize, kind, activation, norm_in, norm_out, gate, scale, eps):
+    if norm_in is None and norm_out is None and gate is None and scale is None:
+        return _layer(x, router, w_in, w_out, top_k, renormalize, kind, activation)
+    from .norms import residual_norm, rms_norm
+    h = _layer(x if norm_in is None else rms_norm(x, norm_in, eps), router, w_in, w_out, top_k, renormalize, kind,
+               activation)
+    if norm_out is None and gate is None and scale is None:
+        return h
+    return residual_norm(x, h, norm_out=norm_out, gate=gate, scale=1.0 if scale is None else scale, eps=eps)[0]
+
+
+def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, renormalize: bool = True, *,
+               activation: str | None = None, norm_in: torch.Tensor | None = None,
+               norm_out: torch.Tensor | None = None, gate: torch.Tensor | None = None, scale: float | None = None,
+               eps: float = 1e-6):
     """A gated layer of experts: for each token ``x`` (num_tokens, D) the
     weighted sum, over its ``top_k`` experts ``e``, of
     ``(silu(x @ gate_e) * (x @ up_e)) @ w_out_e``.
 
     ``router`` (D, num_experts). ``w_in`` (num_experts, D, 2 F) holds gate and
     up side by side, ``w_out`` (num_experts, F, D): tensors of x's type for
-    training (differentiable in everything), or both ``(wq, scale)`` pairs
-    of ``quantize_experts`` for serving in 8-bit integers, where a gradient
-    through the result raises."""
+    training (differentiable in everything), or both ``(wq, scale)`` pairs for
+    serving in 8 bits, integers by ``quantize_experts`` or floating point by
+    ``quantize_block_weights``, where a gradient through the result raises.
+
+    ``activation`` names one of ``gated_matmul``'s. With tensors the gate, its
+    activation and up are then one kernel, rounded once; without it the two
+    products are rounded to x's type before silu. 8-bit integers have silu alone.
+
+    The layer as a block of a network: ``norm_in`` (D,) normalises its input
+    (``rms_norm``). With any of ``norm_out`` (D,), ``gate`` and ``scale`` the
+    result is ``x + scale * gate * (norm_out * y / rms(y))`` for the layer's
+    ``y`` (``residual_norm``)."""
     quantized = isinstance(w_in, (tuple, list))
     if quantized != isinstance(w_out, (tuple, list)):
         raise TypeError("expert_mlp: w_in and w_out must both be tensors or both be (wq, scale) pairs")
+    kind = w_in[0].dtype if quantized else None
+    if quantized and w_out[0].dtype != kind:
+        raise TypeError(f"expert_mlp: w_in is {kind}, w_out is {w_out[0].dtype}")
+    if activation is not None and kind == torch.int8:
+        raise ValueError("expert_mlp: the layer in 8-bit integers has silu alone, activation must be None")
+    args = (x, router, w_in, w_out, top_k, renormalize, kind, activation, norm_in, norm_out, gate, scale, eps)
     if not quantized:
-        return _layer(x, router, w_in, w_out, top_k, renormalize, False)
+        return _block(*args)
     with torch.no_grad():
-        out = _layer(x, router, w_in, w_out, top_k, renormalize, True)
-    if torch.is_grad_enabled() and (x.requires_grad or router.requires_grad):
-        return _Served.apply(out, x, router)
+        out = _block(*args)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                       for t in (x, router, norm_in, norm_out, gate)):
+        return _Served.apply(out, x, router, norm_in, norm_out, gate)
     return out

@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _lib as L
-from .experts import (ExpertPlan, _call, _check_rows, _code, _empty, _groups, _on_gpu, _product, _rows)
+from .experts import (ExpertPlan, _call, _check_rows, _code, _empty, _groups, _on_gpu, _product, _rows, _together)
 from .gated import _activation
 
 BLOCK = 128
@@ -33,13 +33,16 @@ def quantize_blocks(x: torch.Tensor, activation: str | None = None):
     With an ``activation`` (as in ``gated_matmul``) ``x`` is (rows, 2 width),
     gate and up side by side, and what is rounded is ``act(gate) * up``, made
     in fp32. Not differentiable: the result has no history."""
-    _on_gpu("quantize_blocks", x=x)
+    if not _together(x):
+        _on_gpu("quantize_blocks", x=x)
     code = _code("quantize_blocks", "x", x.dtype)
     act = -1 if activation is None else _activation("quantize_blocks", activation)
     if x.dim() != 2 or (act >= 0 and x.shape[1] % 2):
         raise ValueError(f"quantize_blocks: x must be (rows, {'width' if act < 0 else '2 width'}), got {tuple(x.shape)}")
-    dev, x = x.device, _rows(x.detach())
-    R, K = x.shape[0], x.shape[1] // (1 if act < 0 else 2)
+    dev, x = x.device, _rows(x)
+    R, K = x.shape
+    if act >= 0:
+        K //= 2
     q = _empty(R, K, _E4M3, dev)
     scale = _empty(R, _blocks(K), torch.float32, dev)
     _call("es_quantize_blocks", dev, x.data_ptr(), code, R, K, x.stride(0), act, q.data_ptr(), scale.data_ptr())
@@ -80,7 +83,8 @@ def fp8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: t
     result has no history."""
     if plan is not None and not isinstance(plan, ExpertPlan):
         raise TypeError(f"fp8_matmul: plan must be an ExpertPlan or None, got {type(plan).__name__}")
-    _on_gpu("fp8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=q if plan is None else plan.offsets)
+    if not _together(q, scale, wq, wscale, q if plan is None else plan.offsets):
+        _on_gpu("fp8_matmul", q=q, scale=scale, wq=wq, wscale=wscale, plan=q if plan is None else plan.offsets)
     code = _code("fp8_matmul", "out_dtype", out_dtype)
     if q.dtype != _E4M3 or wq.dtype != _E4M3:
         raise TypeError(f"fp8_matmul: q and wq must be float8_e4m3fn, got {q.dtype} and {wq.dtype}")
@@ -100,7 +104,7 @@ def fp8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: t
         raise ValueError(f"fp8_matmul: q has shape {tuple(q.shape)}, wanted (rows, {K}); gather needs a plan")
     if scale.shape != (q.shape[0], _blocks(K)):
         raise ValueError(f"fp8_matmul: scale has shape {tuple(scale.shape)}, wanted {(q.shape[0], _blocks(K))}")
-    q, scale, wscale = _rows(q.detach()), scale.detach().contiguous(), wscale.detach().contiguous()
+    q, scale, wscale = _rows(q), scale.contiguous(), wscale.contiguous()
     if wq.stride(-1) != 1 or wq.stride(-2) < K:
         wq = wq.contiguous()
     dev = q.device

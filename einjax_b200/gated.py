@@ -6,7 +6,7 @@ import torch
 
 from . import _lib as L
 from .experts import (_DTYPES, ExpertPlan, _call, _check_rows, _code, _combine, _empty, _grouped, _no_tangent, _on_gpu,
-                      _product, _rows, _wgrad)
+                      _product, _rows, _together, _wgrad)
 
 ACTIVATIONS = {"silu": L.ES_ACT_SILU, "gelu": L.ES_ACT_GELU, "gelu_tanh": L.ES_ACT_GELU_TANH, "relu": L.ES_ACT_RELU}
 
@@ -77,7 +77,8 @@ def gated_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan | None = Non
     products, (rows, 2 F) of x's type."""
     if plan is not None and not isinstance(plan, ExpertPlan):
         raise TypeError(f"gated_matmul: plan must be an ExpertPlan or None, got {type(plan).__name__}")
-    _on_gpu("gated_matmul", x=x, w=w, **({"plan": plan.offsets} if plan is not None else {}))
+    if not _together(x, w, x if plan is None else plan.offsets):
+        _on_gpu("gated_matmul", x=x, w=w, plan=x if plan is None else plan.offsets)
     _code("gated_matmul", "x", x.dtype)
     act = _activation("gated_matmul", activation)
     if w.dtype != x.dtype:

@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib as L
-from .experts import _DTYPES, _call, _code, _empty, _no_tangent, _on_gpu, _ptr, _rows, _scratch
+from .experts import _DTYPES, _call, _code, _empty, _no_tangent, _on_gpu, _ptr, _rows, _scratch, _together
 
 MIN_EPS = 1e-30
 
@@ -93,9 +93,10 @@ def _weight(fn, name, w, x):
 
 
 def _run(fn, x, h, norm_in, norm_out, gate, scale, eps):
-    tensors = {n: t for n, t in (("x", x), ("h", h), ("norm_in", norm_in), ("norm_out", norm_out), ("gate", gate))
-               if t is not None}
-    _on_gpu(fn, **tensors)
+    tensors = [t for t in (x, h, norm_in, norm_out, gate) if t is not None]
+    if not _together(*tensors):
+        _on_gpu(fn, **{n: t for n, t in zip(("x", "h", "norm_in", "norm_out", "gate"), (x, h, norm_in, norm_out, gate))
+                       if t is not None})
     _code(fn, "x", x.dtype)
     if x.dim() != 2:
         raise ValueError(f"{fn}: x must be (num_tokens, width), got {tuple(x.shape)}")
@@ -121,9 +122,9 @@ def _run(fn, x, h, norm_in, norm_out, gate, scale, eps):
         else:
             raise ValueError(f"{fn}: gate has shape {tuple(gate.shape)}, wanted ({D},), (1, {D}), ({T}, 1) or "
                              f"({T}, {D})")
-    _no_tangent(fn, *tensors.values())
+    _no_tangent(fn, *tensors)
     x, h = _rows(x), None if h is None else _rows(h)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors.values()):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         return _ResidualNorm.apply(x, h, norm_in, norm_out, gate, kind, scale, eps)
     return _forward(x, h, norm_in, norm_out, gate, kind, scale, eps, False)[:2]
 
