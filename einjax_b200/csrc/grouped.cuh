@@ -70,7 +70,7 @@ bool grouped_gated_tc_ok(const GroupedArgs& g, int dtype);
 int grouped_gated_tc_path(const GroupedArgs& g);
 size_t grouped_gated_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* w);
 int grouped_gated_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, int activation, void* h,
-                     void* slopes, void* workspace, int32_t* status, cudaStream_t stream);
+                     float* slopes, void* workspace, int32_t* status, cudaStream_t stream);
 bool grouped_wgrad_tc_ok(const GroupedArgs& g, int dtype);
 size_t grouped_wgrad_tc_workspace(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride);
 int grouped_wgrad_tc(const GroupedArgs& g, int dtype, const void* x, const void* dy, int64_t dy_stride, void* dw,

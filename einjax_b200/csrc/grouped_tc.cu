@@ -85,7 +85,7 @@ struct TcArgs {
   int pairs;          // two neighbouring lanes may be stored together
   int most;           // weights' gradient: groups of more rows than this are the DEEP kernel's
   int activation;     // gated products
-  void* slopes;       // (rows, 2 lanes) or NULL
+  float* slopes;      // (rows, 2 lanes) or NULL
   int32_t* status;
 };
 
@@ -400,7 +400,7 @@ __device__ __forceinline__ void store_16(void* out, int dtype, int64_t at, int64
     store_cols(static_cast<__half*>(out) + at, stride, v, n, live, pairs);
 }
 
-// Activation, product and (for a training step) slopes of 32 columns, rounded and stored.
+// Activation, product and (for a training step) fp32 slopes of 32 columns, stored.
 __device__ __forceinline__ void gated_block(const TcArgs& p, float (&g)[32], const float (&u)[32], int64_t row, int n,
                                             int64_t ch, bool live) {
   float s[32];
@@ -429,8 +429,8 @@ __device__ __forceinline__ void gated_block(const TcArgs& p, float (&g)[32], con
   if (p.slopes) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) s[i] *= u[i];
-    store_16(p.slopes, p.out_dtype, row * 2 * p.out_col + ch, 2 * p.out_col, s, n, live, pairs);
-    store_16(p.slopes, p.out_dtype, (row * 2 + 1) * p.out_col + ch, 2 * p.out_col, g, n, live, pairs);
+    store_cols(p.slopes + row * 2 * p.out_col + ch, 2 * p.out_col, s, n, live, false);
+    store_cols(p.slopes + (row * 2 + 1) * p.out_col + ch, 2 * p.out_col, g, n, live, false);
   }
 #pragma unroll
   for (int i = 0; i < 32; ++i) g[i] *= u[i];
@@ -569,8 +569,8 @@ __device__ __forceinline__ bool split_tile(const TcArgs& p, TcCtl& ctl, const Ti
       for (int r = 0; r < 8; ++r) u += r < static_cast<int>(csize) ? load_at(at_rank(up, r)) : 0.0f;
       ES_BY_ACT(p.activation, (activate<ACT, false>(v, a, s)));
       if (live && p.slopes) {
-        store_one(p.slopes, p.out_dtype, (at.row0 + c) * 2 * p.out_col + ch, s * u);
-        store_one(p.slopes, p.out_dtype, ((at.row0 + c) * 2 + 1) * p.out_col + ch, a);
+        p.slopes[(at.row0 + c) * 2 * p.out_col + ch] = s * u;
+        p.slopes[((at.row0 + c) * 2 + 1) * p.out_col + ch] = a;
       }
       v = a * u;
     }
@@ -1315,7 +1315,7 @@ size_t grouped_gated_tc_workspace(const GroupedArgs& g, int dtype, const void* x
 }
 
 int grouped_gated_tc(const GroupedArgs& g, int dtype, const void* x, const void* w, int activation, void* h,
-                     void* slopes, void* workspace, int32_t* status, cudaStream_t stream) {
+                     float* slopes, void* workspace, int32_t* status, cudaStream_t stream) {
   GatedOperands o = gated_operands(g, dtype, x, w);
   char* ws = static_cast<char*>(workspace);
   ES_TRY(lay_out(g, o.gate.x, dtype, true, false, ws, stream));
@@ -1332,7 +1332,7 @@ int grouped_gated_tc(const GroupedArgs& g, int dtype, const void* x, const void*
   p.plane_experts = static_cast<int>(o.up.depth);
   p.plane_rows = static_cast<int>(o.gate.x.rows);
   p.idesc = idesc_of(dtype, o.gate.mn, false);
-  p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(h) & 3) == 0 && (reinterpret_cast<uintptr_t>(slopes) & 3) == 0;
+  p.pairs = g.N % 2 == 0 && (reinterpret_cast<uintptr_t>(h) & 3) == 0;
   p.activation = activation;
   p.slopes = slopes;
   p.status = status;

@@ -24,11 +24,12 @@ def _gated(x, w, plan, gather, act, keep):
     K, F = w.shape[1], w.shape[2] // 2
     E, R = (plan.num_experts, plan.num_rows) if plan is not None else (0, x.shape[0])
     h = _empty(R, F, x.dtype, dev)
-    slopes = _empty(R, 2 * F, x.dtype, dev) if keep else None
+    slopes = _empty(R, 2 * F, torch.float32, dev) if keep else None
     args = (x.data_ptr(), _DTYPES[x.dtype], x.shape[0], x.stride(0), w.data_ptr(), E, K, F, *w.stride(),
             plan.offsets.data_ptr() if E else None, plan.order.data_ptr() if gather else None, plan.top_k if E else 1,
             R)
-    _product("es_gated_matmul", dev, args, (act, h.data_ptr(), slopes.data_ptr() if keep else None), True)
+    _product("es_gated_matmul", dev, args, (act, h.data_ptr(), slopes.data_ptr() if keep else None),
+             gather or x.dtype == torch.float32)
     return h, slopes
 
 
@@ -48,7 +49,7 @@ class _GatedMatmul(torch.autograd.Function):
         _no_tangent("gated_matmul", dh)
         dh = _rows(dh)
         R, F = dh.shape
-        dy = torch.empty_like(slopes)
+        dy = _empty(R, 2 * F, dh.dtype, dev)
         _call("es_gated_matmul_grad", dev, dh.data_ptr(), _DTYPES[dh.dtype], dh.stride(0), slopes.data_ptr(), R, F,
               plan.offsets.data_ptr() + 4 * plan.num_experts if plan is not None else None, dy.data_ptr())
         dx = dw = None
@@ -74,7 +75,7 @@ def gated_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan | None = Non
     (by erf), ``"gelu_tanh"`` or ``"relu"``. Returns (rows, F) of x's type
     (float32, bfloat16, float16); rows of no expert are zero. Differentiable
     in ``x`` and ``w``; a training step keeps the output's slopes in both
-    products, (rows, 2 F) of x's type."""
+    products, (rows, 2 F) float32."""
     if plan is not None and not isinstance(plan, ExpertPlan):
         raise TypeError(f"gated_matmul: plan must be an ExpertPlan or None, got {type(plan).__name__}")
     if not _together(x, w, x if plan is None else plan.offsets):

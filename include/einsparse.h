@@ -454,7 +454,7 @@ int es_grouped_matmul_wgrad(const void* x, int dtype, int64_t x_rows, int64_t x_
 /* h[r] = act(x[row(r)] gate[e(r)]) * (x[row(r)] up[e(r)]) for the num_rows grouped
  * rows, w[e] = [gate | up] (K, 2F) with any element strides; num_experts == 0: one
  * matrix for all rows (offsets and order NULL). h (num_rows, F) contiguous, of the
- * operands' type; slopes (num_rows, 2F), the same type or NULL: [act'(x gate) * (x up)
+ * operands' type; slopes (num_rows, 2F) float32, or NULL: [act'(x gate) * (x up)
  * | act(x gate)], the rows of no expert left alone. */
 typedef enum es_activation {
   ES_ACT_SILU = 0,      /* g / (1 + exp(-g)) */
@@ -469,7 +469,7 @@ size_t es_gated_matmul_workspace_size(const void* x, int dtype, int64_t x_rows, 
 int es_gated_matmul(const void* x, int dtype, int64_t x_rows, int64_t x_stride, const void* w, int num_experts,
                     int64_t K, int64_t F, int64_t w_expert_stride, int64_t w_k_stride, int64_t w_n_stride,
                     const int32_t* offsets, const int32_t* order, int top_k, int64_t num_rows, int activation,
-                    void* h, void* slopes, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+                    void* h, float* slopes, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 /* The kernel of a gated product of these sizes, an es_grouped_path (lanes are those of
  * h) or ES_GATED_TWO: the product in fp32, then a pass for the activation. -1: none. */
 #define ES_GATED_TWO 7
@@ -477,7 +477,7 @@ int es_gated_matmul_path(int dtype, int num_experts, int64_t K, int64_t F, int64
 /* dy = dh times the slopes (num_rows, 2F), contiguous: the gradient of [x gate | x up],
  * from which es_grouped_matmul and es_grouped_matmul_wgrad make those of x and w.
  * kept_rows (device int32, or NULL for all): the rows from there on are zero. */
-int es_gated_matmul_grad(const void* dh, int dtype, int64_t dh_stride, const void* slopes, int64_t num_rows,
+int es_gated_matmul_grad(const void* dh, int dtype, int64_t dh_stride, const float* slopes, int64_t num_rows,
                          int64_t F, const int32_t* kept_rows, void* dy, void* stream);
 
 /* out[t] = sum_j weights[t, j] y[position[t, j]] (weights NULL: 1), y
