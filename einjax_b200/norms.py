@@ -41,6 +41,10 @@ def _forward(x, h, norm_in, norm_out, gate, kind, scale, eps, keep):
     return out, y, stats
 
 
+def _column(n, dtype, dev):
+    return torch.empty_strided((n,), (1,), dtype=dtype, device=dev)
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, h, norm_in, norm_out, gate, kind, scale, eps):
@@ -53,32 +57,39 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dy):
-        none = (None,) * 8
         if dout is None and dy is None:
-            return none
+            return (None,) * 8
         x, h, norm_in, norm_out, gate, stats = ctx.saved_tensors
         _no_tangent("residual_norm", *(d for d in (dout, dy) if d is not None))
-        dev, (T, D), kind = x.device, x.shape, ctx.kind
-        dout, dy = (_rows(d) if d is not None else None for d in (dout, dy))
+        dev, dtype, (T, D), kind = x.device, x.dtype, x.shape, ctx.kind
+        if dout is not None:
+            dout = _rows(dout)
+        if dy is not None:
+            dy = _rows(dy)
         need = ctx.needs_input_grad
-
-        def like(i, t):
-            return torch.empty(t.shape, dtype=t.dtype, device=dev) if need[i] and t is not None else None
-
-        dx, dh, dnorm_in, dnorm_out, dgate = (like(i, t) for i, t in enumerate((x, h, norm_in, norm_out, gate)))
-        if dy is None and dnorm_in is not None:
-            dnorm_in.zero_()
-        din = dnorm_in if dy is not None else None
-        columns = sum(t is not None for t in (din, dnorm_out, dgate if kind == L.ES_GATE_CHANNEL else None))
-        code = _DTYPES[x.dtype]
-        nbytes = L.lib().es_residual_norm_grad_workspace_size(code, T, D, columns)
-        ws = _scratch(nbytes, dev)
+        dx = _empty(T, D, dtype, dev) if need[0] else None
+        dh = _empty(T, D, dtype, dev) if need[1] else None
         weight = norm_in if norm_in is not None else norm_out
+        dnorm_in = _column(D, weight.dtype, dev) if need[2] else None
+        dnorm_out = _column(D, weight.dtype, dev) if need[3] else None
+        columns = (dnorm_out is not None) + (dnorm_in is not None and dy is not None)
+        dgate = None
+        if need[4]:
+            if kind == L.ES_GATE_CHANNEL:
+                dgate = _column(D, dtype, dev)
+                columns += 1
+            else:
+                dgate = _empty(T, gate.shape[1], dtype, dev)
+        if dnorm_in is not None and dy is None:
+            dnorm_in.zero_()
+        code = _DTYPES[dtype]
+        nbytes = L.lib().es_residual_norm_grad_workspace_size(code, T, D, columns) if columns else 0
+        ws = _scratch(nbytes, dev)
         _call("es_residual_norm_grad", dev, x.data_ptr(), x.stride(0), _ptr(h), _stride(h), code, T, D, _ptr(norm_in),
               _ptr(norm_out), code if weight is None else _DTYPES[weight.dtype], _ptr(gate), kind,
               _stride(gate) if kind != L.ES_GATE_CHANNEL else 0, ctx.scale, stats.data_ptr(), _ptr(dout),
-              _stride(dout), _ptr(dy), _stride(dy), _ptr(dx), _ptr(dh), _ptr(dgate), _ptr(din), _ptr(dnorm_out),
-              _ptr(ws), nbytes)
+              _stride(dout), _ptr(dy), _stride(dy), _ptr(dx), _ptr(dh), _ptr(dgate),
+              _ptr(dnorm_in) if dy is not None else None, _ptr(dnorm_out), _ptr(ws), nbytes)
         return dx, dh, dnorm_in, dnorm_out, dgate, None, None, None
 
 
