@@ -52,63 +52,56 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] = to_f32(t[i]);
 }
 
-// Sixteen threads a block, eight consecutive values each, MANY blocks of a thread in
-// flight. WIDE: whole pieces at 16-byte addresses. ACT: the value is act(x[i]) * x[K + i],
-// in fp32 (-1: x[i]); the fast exp's error is far below 8 bits' rounding.
-template <typename T, int ACT, bool WIDE, int MANY>
-__global__ void __launch_bounds__(kFp8Threads) quantize_blocks_kernel(const T* x, int64_t rows, int64_t K,
+// Sixteen threads a block, eight consecutive values each. WIDE: whole pieces at 16-byte
+// addresses. ACT: the value is act(x[i]) * x[K + i], in fp32 (-1: x[i]); the fast exp's
+// error is far below 8 bits' rounding. I: the type that holds every block's number (64-bit
+// divisions are a fifth of the time).
+template <typename T, int ACT, bool WIDE, typename I>
+__global__ void __launch_bounds__(kFp8Threads) quantize_blocks_kernel(const T* x, I n, I blocks, int64_t K,
                                                                       int64_t stride, uint8_t* q, float* scale) {
   let_next_grid_start();
-  constexpr int PER = kFp8Threads / 16;
-  const int64_t blocks = (K + kScaleBlock - 1) / kScaleBlock, n = rows * blocks;
-  const int64_t first = blockIdx.x * static_cast<int64_t>(PER * MANY) + (threadIdx.x >> 4);
-  const int part = (threadIdx.x & 15) * 8;
-  float v[MANY][8];
-#pragma unroll
-  for (int m = 0; m < MANY; ++m) {
-    const int64_t at = first + m * PER, r = at / blocks, c = (at - r * blocks) * kScaleBlock + part;
-    const T* from = x + r * stride + c;
-    auto load = [&](const T* p, float (&t)[8]) {
-      if (WIDE && at < n && c < K) {
-        load8(p, t);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) t[i] = !WIDE && at < n && c + i < K ? to_f32(p[i]) : 0.0f;
-      }
-    };
-    load(from, v[m]);
-    if constexpr (ACT >= 0) {
-      float u[8];
-      load(from + K, u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float a, s;
-        activate<ACT, false>(v[m][i], a, s);
-        v[m][i] = a * u[i];
-      }
-    }
-  }
-#pragma unroll
-  for (int m = 0; m < MANY; ++m) {
-    const int64_t at = first + m * PER, r = at / blocks, c = (at - r * blocks) * kScaleBlock + part;
-    float peak = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) peak = max_nan(peak, fabsf(v[m][i]));
-#pragma unroll
-    for (int o = 8; o; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-    if (at >= n) continue;
-    float inverse;
-    const float s = block_scale(peak, inverse);
-    if (part == 0) scale[at] = s;
-    const uint2 o = make_uint2(round4(v[m], inverse), round4(v[m] + 4, inverse));
-    uint8_t* to = q + r * K + c;
-    if constexpr (WIDE) {
-      if (c < K) *reinterpret_cast<uint2*>(to) = o;
+  const I at = static_cast<I>(blockIdx.x) * (kFp8Threads / 16) + (threadIdx.x >> 4);
+  const bool live = at < n;
+  const I row = at / blocks;
+  const int64_t r = row, c = static_cast<int64_t>(at - row * blocks) * kScaleBlock + (threadIdx.x & 15) * 8;
+  const T* from = x + r * stride + c;
+  float v[8];
+  auto load = [&](const T* p, float (&t)[8]) {
+    if (WIDE && live && c < K) {
+      load8(p, t);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i < K) to[i] = static_cast<uint8_t>((i < 4 ? o.x : o.y) >> (i & 3) * 8);
+      for (int i = 0; i < 8; ++i) t[i] = !WIDE && live && c + i < K ? to_f32(p[i]) : 0.0f;
     }
+  };
+  load(from, v);
+  if constexpr (ACT >= 0) {
+    float u[8];
+    load(from + K, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float a, s;
+      activate<ACT, false>(v[i], a, s);
+      v[i] = a * u[i];
+    }
+  }
+  float peak = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) peak = max_nan(peak, fabsf(v[i]));
+#pragma unroll
+  for (int o = 8; o; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+  if (!live) return;
+  float inverse;
+  const float s = block_scale(peak, inverse);
+  if ((threadIdx.x & 15) == 0) scale[at] = s;
+  const uint2 o = make_uint2(round4(v, inverse), round4(v + 4, inverse));
+  uint8_t* to = q + r * K + c;
+  if constexpr (WIDE) {
+    if (c < K) *reinterpret_cast<uint2*>(to) = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < K) to[i] = static_cast<uint8_t>((i < 4 ? o.x : o.y) >> (i & 3) * 8);
   }
 }
 
@@ -143,27 +136,26 @@ __global__ void __launch_bounds__(kFp8Threads) quantize_weights_kernel(const T* 
 
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-template <typename T, int ACT, int MANY>
-int quantize_many(const void* x, int64_t rows, int64_t K, int64_t stride, uint8_t* q, float* scale, cudaStream_t s) {
-  const int64_t blocks = rows * ((K + kScaleBlock - 1) / kScaleBlock), per = kFp8Threads / 16 * MANY;
-  if ((blocks + per - 1) / per > 0x7fffffffLL) return ES_ERR_UNSUPPORTED;
-  const unsigned grid = static_cast<unsigned>((blocks + per - 1) / per);
+template <typename T, int ACT, typename I>
+int quantize_indexed(const void* x, int64_t rows, int64_t K, int64_t stride, uint8_t* q, float* scale,
+                     cudaStream_t s) {
+  const int64_t blocks = (K + kScaleBlock - 1) / kScaleBlock, n = rows * blocks, per = kFp8Threads / 16;
+  if ((n + per - 1) / per > 0x7fffffffLL) return ES_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>((n + per - 1) / per);
   if (K % 8 == 0 && stride * sizeof(T) % 16 == 0 && aligned(x, 16) && aligned(q, 8))
-    ES_LAUNCH((quantize_blocks_kernel<T, ACT, true, MANY>), grid, kFp8Threads, 0, s, static_cast<const T*>(x), rows, K,
-              stride, q, scale);
+    ES_LAUNCH((quantize_blocks_kernel<T, ACT, true, I>), grid, kFp8Threads, 0, s, static_cast<const T*>(x),
+              static_cast<I>(n), static_cast<I>(blocks), K, stride, q, scale);
   else
-    ES_LAUNCH((quantize_blocks_kernel<T, ACT, false, MANY>), grid, kFp8Threads, 0, s, static_cast<const T*>(x), rows,
-              K, stride, q, scale);
+    ES_LAUNCH((quantize_blocks_kernel<T, ACT, false, I>), grid, kFp8Threads, 0, s, static_cast<const T*>(x),
+              static_cast<I>(n), static_cast<I>(blocks), K, stride, q, scale);
   return ES_OK;
 }
 
 template <typename T, int ACT>
 int quantize_launch(const void* x, int64_t rows, int64_t K, int64_t stride, uint8_t* q, float* scale, cudaStream_t s) {
-  // a few rows: every block its threads at once; else enough loads in flight
-  constexpr int MANY = ACT >= 0 ? 2 : 4;
-  if (rows * ((K + kScaleBlock - 1) / kScaleBlock) < 16 * 8 * kSMs * MANY)
-    return quantize_many<T, ACT, 1>(x, rows, K, stride, q, scale, s);
-  return quantize_many<T, ACT, MANY>(x, rows, K, stride, q, scale, s);
+  if (rows * ((K + kScaleBlock - 1) / kScaleBlock) < 0x7fffff00LL)
+    return quantize_indexed<T, ACT, uint32_t>(x, rows, K, stride, q, scale, s);
+  return quantize_indexed<T, ACT, int64_t>(x, rows, K, stride, q, scale, s);
 }
 
 GroupedArgs args_of(const float* x_scale, int64_t x_rows, int64_t x_stride, const float* w_scale, int num_experts,

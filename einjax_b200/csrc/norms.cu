@@ -542,11 +542,10 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
       for (int n = 0; n < NP; ++n)
         if (c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
     };
-    Vec<T, VEC> xv[NP], hv[NP], gv[NP];
+    Vec<T, VEC> xv[NP], hv[NP];
     each([&](int n, int64_t c) {
       if (p.h) hv[n] = load_piece<T, SHIFT>(h, c, phase, p.width);
       xv[n] = load_piece<T, SHIFT>(x, c, phase, p.width);
-      if (p.gate_kind == ES_GATE_FULL) gv[n] = load_piece<T, SHIFT>(gate, c, phase, p.width);
     });
     const float token = p.gate_kind == ES_GATE_TOKEN && live ? to_f32(gate[0]) : 1.0f;
     auto rms = [&](auto value, float (*buf)[32], float (*again)[32]) {  // value(slot, fp32 values)
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
           for (int i = 0; i < VEC; ++i) z[i] *= w[i];
         }
         if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
-        if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
+        if (p.gate_kind == ES_GATE_FULL) widen(load_piece<T, SHIFT>(gate, c, phase, p.width), g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[n][i] = fmaf(p.scale * g[i], z[i], o[n][i]);
       }
@@ -671,14 +670,30 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
       for (int n = 0; n < NP; ++n)
         if (c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
     };
-    Vec<T, VEC> xv[NP], hv[NP], ov[NP], yv[NP], gv[NP];
+    Vec<T, VEC> xv[NP], hv[NP], ov[NP], yv[NP];
     each([&](int n, int64_t c) {
       xv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.x) + t * p.x_stride, c, phase, p.width);
       if (p.h) hv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.h) + t * p.h_stride, c, phase, p.width);
       if (p.dout) ov[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.dout) + t * p.dout_stride, c, phase, p.width);
       if (p.dy) yv[n] = load_piece<T, SHIFT>(static_cast<const T*>(p.dy) + t * p.dy_stride, c, phase, p.width);
-      if (p.gate_kind == ES_GATE_FULL) gv[n] = load_piece<T, SHIFT>(gate, c, phase, p.width);
     });
+    if (tp > 64 && (c0 & 7) == 0 && t + step < p.rows) {
+      // the next row towards L2, a lane a line of 128 bytes: few rows are in flight (16384 x
+      // 4096 fp32: 400 -> 329 us; rows of a warp or two have enough, and lose 4%)
+      auto ahead = [&](const void* base, int64_t stride) {
+        const T* from = static_cast<const T*>(base) + (t + step) * stride;
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+          const int64_t e = static_cast<int64_t>(c0 + n * tp) * VEC;
+          if (e < p.width) asm volatile("prefetch.global.L2 [%0];" ::"l"(from + e));
+        }
+      };
+      ahead(p.x, p.x_stride);
+      if (p.h) ahead(p.h, p.h_stride);
+      if (p.gate_kind == ES_GATE_FULL) ahead(p.gate, p.gate_stride);
+      if (p.dout) ahead(p.dout, p.dout_stride);
+      if (p.dy) ahead(p.dy, p.dy_stride);
+    }
     const float r1 = p.w_out ? p.stats[2 * row] : 1.0f, r2 = p.dy ? p.stats[2 * row + 1] : 0.0f;
     const float token = by_token ? to_f32(gate[0]) : 1.0f;
     // scale times the gate, and z, of a piece
@@ -692,7 +707,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
 #pragma unroll
       for (int i = 0; i < VEC; ++i) z[i] *= r1;
       if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
-      if (p.gate_kind == ES_GATE_FULL) widen(gv[n], g);
+      if (p.gate_kind == ES_GATE_FULL) widen(load_piece<T, SHIFT>(gate, c, phase, p.width), g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) g[i] *= p.scale;
       if (p.w_out) {
@@ -795,8 +810,8 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
       parts[k * p.width + e] = sums[k * column + (SHIFT ? (e % VEC) * pitch + e / VEC + 1 : e)];
 }
 
-// Adds the groups' parts of each column in their order: 32 columns by 8 slices
-// of the groups a CTA, the slices' sums added in their order.
+// Adds the groups' parts of each column in their order: 32 columns by 32 slices of the
+// groups a CTA, the slices' sums added in their order (296 groups of 3 x 4096: 16 us with 8).
 struct SumArgs {
   const float* part;
   int64_t groups, width;
@@ -805,20 +820,23 @@ struct SumArgs {
   int dtype[3];
 };
 
-__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ SumArgs p) {
-  __shared__ float slices[8][32];
+constexpr int kSlices = 32;
+
+__global__ void __launch_bounds__(32 * kSlices) column_sum_kernel(const __grid_constant__ SumArgs p) {
+  __shared__ float slices[kSlices][32];
   const int64_t n = p.columns * p.width, at = blockIdx.x * 32LL + (threadIdx.x & 31);
   const int slice = threadIdx.x >> 5;
   float sum = 0.0f;
   if (at < n) {
-    const int64_t from = p.groups * slice / 8, to = p.groups * (slice + 1) / 8;
-#pragma unroll 8
+    const int64_t from = p.groups * slice / kSlices, to = p.groups * (slice + 1) / kSlices;
+#pragma unroll 4
     for (int64_t g = from; g < to; ++g) sum += p.part[g * n + at];
   }
   slices[slice][threadIdx.x & 31] = sum;
   __syncthreads();
   if (slice || at >= n) return;
-  for (int s = 1; s < 8; ++s) sum += slices[s][threadIdx.x];
+#pragma unroll
+  for (int s = 1; s < kSlices; ++s) sum += slices[s][threadIdx.x];
   const int k = static_cast<int>(at / p.width);
   const int64_t c = at - k * p.width;
   if (p.dtype[k] == ES_BF16)
@@ -1002,7 +1020,7 @@ int backward(NormArgs& p, const SumArgs& sums, cudaStream_t s) {
   if (!p.columns) return ES_OK;
   SumArgs a = sums;
   a.groups = groups;
-  ES_LAUNCH(column_sum_kernel, static_cast<unsigned>((p.columns * p.width + 31) / 32), 256, 0, s, a);
+  ES_LAUNCH(column_sum_kernel, static_cast<unsigned>((p.columns * p.width + 31) / 32), 32 * kSlices, 0, s, a);
   return ES_OK;
 }
 

@@ -362,3 +362,26 @@ def test_refusals():
             call()
     x.requires_grad_()
     assert not E.quantize_blocks(x)[1].requires_grad
+
+
+def test_quantize_past_32_bits():
+    """More values than 32 bits number."""
+    R, K = 70001, 32768
+    x = torch.zeros(R, K, dtype=torch.bfloat16, device=DEV)
+    x[-2:] = randn(gen(4), 2, K, dtype=torch.bfloat16)
+    q, s = E.quantize_blocks(x)
+    rq, rs = quantize_ref(x[-2:])
+    assert torch.equal(q[-2:].double(), rq) and torch.equal(s[-2:].double(), rs)
+    assert not q[:-2].view(torch.uint8).any()
+
+
+def test_output_past_32_bits():
+    """An output of more than 2^31 values, and rows of a group behind that border."""
+    R, K, N = 300000, 64, 8192
+    g = gen(6)
+    plan = make_plan([R - 200, 200], 1)
+    q, s, wq, ws = operands(g, R, N, K, (2,))
+    y = E.fp8_matmul(q, s, wq, ws, plan)
+    ref = (q[-200:].double() * s[-200:].double()) @ (wq[1].double() * spread(ws[1], N, K)).t()
+    mag = (q[-200:].double() * s[-200:].double()).abs() @ (wq[1].double() * spread(ws[1], N, K)).abs().t()
+    check(y[-200:], ref, mag, K, torch.bfloat16)
