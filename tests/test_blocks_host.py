@@ -50,8 +50,8 @@ def test_gated_refuses():
 
 @pytest.mark.parametrize("dtype,experts,K,F,rows,path", [
     # by the mean of the rows a group, where the tiles then fill the SMs (lanes are h's channels)
-    (BF16, 60, 2048, 1408, 60 * 8, L.ES_GROUPED_NARROW), (BF16, 60, 2048, 1408, 60 * 9, L.ES_GROUPED_MIDDLE),
-    (BF16, 60, 2048, 1408, 60 * 160, L.ES_GROUPED_MIDDLE), (BF16, 60, 2048, 1408, 60 * 161, L.ES_GROUPED_WIDE),
+    (BF16, 60, 2048, 1408, 60, L.ES_GROUPED_MIDDLE), (BF16, 60, 2048, 1408, 60 * 112, L.ES_GROUPED_MIDDLE),
+    (BF16, 60, 2048, 1408, 60 * 113, L.ES_GROUPED_WIDE), (BF16, 80, 136, 128, 400, L.ES_GROUPED_NARROW),
     (F16, 0, 4096, 8192, 8192, L.ES_GROUPED_WIDE), (BF16, 0, 4096, 2048, 16, L.ES_GROUPED_SPLIT),
     (BF16, 0, 128, 2048, 16, L.ES_GROUPED_NARROW),
     # one chain of sums in one kernel; fp32 and longer sums in two

@@ -293,7 +293,7 @@ def test_refusals():
 
 
 CODE = {torch.float32: L.ES_F32, torch.bfloat16: L.ES_BF16, torch.float16: L.ES_F16}
-LONG = [200, 701, 256, 0, 513, 390, 640, 511, 257]         # a mean past 160 rows
+LONG = [200, 701, 256, 0, 513, 390, 640, 511, 257]         # a mean past 112 rows
 SHORT = [10 + 37 * i % 91 for i in range(58)] + [0, 129]   # 10 to 100 rows, none, and a tile and one
 FEW = [i % 9 for i in range(80)] + [65]                    # up to 8 rows, and a tile and one
 
@@ -301,7 +301,8 @@ FEW = [i % 9 for i in range(80)] + [65]                    # up to 8 rows, and a
 @pytest.mark.parametrize("dtype", TYPES[1:])
 @pytest.mark.parametrize("sizes,F,path", [(LONG, 2056, L.ES_GROUPED_WIDE), (LONG, 2049, L.ES_GROUPED_WIDE),
                                           (SHORT, 520, L.ES_GROUPED_MIDDLE), (SHORT, 517, L.ES_GROUPED_MIDDLE),
-                                          (FEW, 520, L.ES_GROUPED_NARROW), (FEW, 517, L.ES_GROUPED_NARROW)])
+                                          (FEW, 520, L.ES_GROUPED_MIDDLE), (FEW, 517, L.ES_GROUPED_MIDDLE),
+                                          (FEW, 100, L.ES_GROUPED_NARROW), (FEW, 97, L.ES_GROUPED_NARROW)])
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("gather", [False, True])
 def test_shapes(dtype, sizes, F, path, transposed, gather):
