@@ -14,11 +14,16 @@
 // b unit, s g z d0 and s g z d1 with d0 = dout + r2 b and d1 = r2 unit. r1 and r2
 // are kept from the forward pass, `out` is made again in fp32.
 //
-// Everything is fp32 between a value's load and its one rounding. Bound by
-// memory: a row is read once into registers (a group of threads a row, NP
-// pieces of 16 bytes each) and every output written once. Column sums stay in
-// registers over the rows of a group; each group writes its part, and a second
-// kernel adds the parts in their order, so that results repeat to the bit.
+// Everything is fp32 between a value's load and its one rounding. A row is read once into
+// registers (a group of threads a row, NP pieces of 16 bytes each) and every output written
+// once. Column sums stay in shared memory over the rows of a group; each group writes its
+// part, and a second kernel adds the parts in their order, so that results repeat to the
+// bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 117 us
+// forward (537 MB, 4.6 TB/s) and 245 us backward (805 MB, 3.3 TB/s; all of its gradients
+// with the column sums 267). The forward pass is near memory's rate; the backward pass is
+// bound by its instructions, some 80 a value, with half of the issue slots used: 16 warps an
+// SM is what its registers allow. Rows of odd length pay for values that lie at no fixed
+// place: 4099 x 5001 f16 85 us for 164 MB.
 #include <type_traits>
 
 #include "experts.cuh"
