@@ -18,12 +18,11 @@
 // registers (a group of threads a row, NP pieces of 16 bytes each) and every output written
 // once. Column sums stay in shared memory over the rows of a group; each group writes its
 // part, and a second kernel adds the parts in their order, so that results repeat to the
-// bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 117 us
-// forward (537 MB, 4.6 TB/s) and 245 us backward (805 MB, 3.3 TB/s; all of its gradients
-// with the column sums 267). The forward pass is near memory's rate; the backward pass is
-// bound by its instructions, some 80 a value, with half of the issue slots used: 16 warps an
+// bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 120 us
+// forward (537 MB, 4.5 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The forward pass is near memory's rate; the backward pass is
+// bound by its instructions, with half of the issue slots used: 16 warps an
 // SM is what its registers allow. Rows of odd length pay for values that lie at no fixed
-// place: 4099 x 5001 f16 85 us for 164 MB.
+// place: 4099 x 5001 f16 81 us for 164 MB.
 #include <type_traits>
 
 #include "experts.cuh"
@@ -92,6 +91,54 @@ __device__ __forceinline__ void widen(const Vec<T, VEC>& p, float (&v)[VEC]) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = to_f32(p.v[i]);
   }
+}
+
+// A piece's arithmetic, two values an instruction. Gradients of 16384 x 4096 bf16: 267 to 243 us, of
+// 65536 x 512: 121 to 110.
+#define ES_PAIR(op, ...)                                                                             \
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t" op         \
+      "mov.b64 {%0, %1}, c;\n\t}"                                                                   \
+      : "=f"(o0), "=f"(o1)                                                                           \
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1) __VA_ARGS__)
+
+__device__ __forceinline__ void mul_pair(float& o0, float& o1, float a0, float a1, float b0, float b1) {
+  ES_PAIR("mul.rn.f32x2 c, a, b;\n\t", );
+}
+
+__device__ __forceinline__ void fma_pair(float& o0, float& o1, float a0, float a1, float b0, float b1, float c0,
+                                         float c1) {
+  ES_PAIR("mov.b64 c, {%6, %7};\n\tfma.rn.f32x2 c, a, b, c;\n\t", , "f"(c0), "f"(c1));
+}
+#undef ES_PAIR
+
+template <int VEC>
+__device__ __forceinline__ void mul(float (&a)[VEC], const float (&b)[VEC]) {
+  static_assert(VEC % 2 == 0, "pieces hold whole pairs");
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) mul_pair(a[i], a[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+}
+template <int VEC>
+__device__ __forceinline__ void mul(float (&a)[VEC], float s) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) mul_pair(a[i], a[i + 1], a[i], a[i + 1], s, s);
+}
+// o = a b + c
+template <int VEC>
+__device__ __forceinline__ void fma(float (&o)[VEC], const float (&a)[VEC], const float (&b)[VEC],
+                                    const float (&c)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) fma_pair(o[i], o[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+}
+template <int VEC>
+__device__ __forceinline__ void fma(float (&o)[VEC], float s, const float (&b)[VEC], const float (&c)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) fma_pair(o[i], o[i + 1], s, s, b[i], b[i + 1], c[i], c[i + 1]);
+}
+// The even and the odd values' part of a sum of products.
+template <int VEC>
+__device__ __forceinline__ void dot(float2& sum, const float (&a)[VEC], const float (&b)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; i += 2) fma_pair(sum.x, sum.y, a[i], a[i + 1], b[i], b[i + 1], sum.x, sum.y);
 }
 
 template <typename T, int VEC>
@@ -554,13 +601,13 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
     });
     const float token = p.gate_kind == ES_GATE_TOKEN && live ? to_f32(gate[0]) : 1.0f;
     auto rms = [&](auto value, float (*buf)[32], float (*again)[32]) {  // value(slot, fp32 values)
-      float sum[1] = {0.0f};
+      float2 pair = make_float2(0.0f, 0.0f);
       each([&](int n, int64_t) {
         float v[VEC];
         value(n, v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
+        dot(pair, v, v);
       });
+      float sum[1] = {pair.x + pair.y};
       group_sum(sum, buf, tp);
       const bool big = live && !(sum[0] < INFINITY);
       // squares past the largest value: the same sum of smaller ones. All threads of the
@@ -585,19 +632,17 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
       if (p.h) {
         float z[VEC], g[VEC];
         widen(hv[n], z);
+        mul(z, r1);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          z[i] *= r1;
-          g[i] = token;
-        }
+        for (int i = 0; i < VEC; ++i) g[i] = token;
         if (p.w_out) {
           float w[VEC];
           cols.get(cols.w_out, c, places, w);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) z[i] *= w[i];
+          mul(z, w);
         }
         if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
         if (p.gate_kind == ES_GATE_FULL) widen(load_piece<T, SHIFT>(gate, c, phase, p.width), g);
+        // One by one: in pairs the 64 registers spilled (16384 x 4096 bf16: 123 us for 120).
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[n][i] = fmaf(p.scale * g[i], z[i], o[n][i]);
       }
@@ -613,8 +658,8 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
       each([&](int n, int64_t c) {
         float w[VEC];
         cols.get(cols.w_in, c, places, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) w[i] *= o[n][i] * r2;
+        mul(o[n], r2);
+        mul(w, o[n]);
         store_piece<T, SHIFT>(static_cast<T*>(p.y) + t * p.width, c, phase, p.width, w);
       });
     }
@@ -709,28 +754,27 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
         z[i] = 0.0f;
       }
       if (p.h) widen(hv[n], z);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) z[i] *= r1;
+      mul(z, r1);
       if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
       if (p.gate_kind == ES_GATE_FULL) widen(load_piece<T, SHIFT>(gate, c, phase, p.width), g);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] *= p.scale;
+      mul(g, p.scale);
       if (p.w_out) {
         float w[VEC];
         cols.get(cols.w_out, c, places, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) z[i] *= w[i];
+        mul(z, w);
       }
     };
     // unit, b and d0 of a piece; of more than two pieces they are made twice instead of held
     constexpr bool HOLD = NP <= 2;
-    float unit[HOLD ? NP : 1][VEC], d0[HOLD ? NP : 1][VEC], v[3] = {0.0f, 0.0f, 0.0f};
+    float unit[HOLD ? NP : 1][VEC], d0[HOLD ? NP : 1][VEC];
+    float2 pair[3] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
     auto terms = [&](int n, int64_t c, const float (&g)[VEC], const float (&z)[VEC], float (&u)[VEC], float (&d)[VEC],
                      float (&b)[VEC]) {
       widen(xv[n], u);
+      fma(u, g, z, u);
+      mul(u, r2);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        u[i] = fmaf(g[i], z[i], u[i]) * r2;
         d[i] = 0.0f;
         b[i] = 0.0f;
       }
@@ -739,11 +783,8 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
         float y[VEC];
         widen(yv[n], y);
         cols.get(cols.w_in, c, places, b);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          b[i] *= y[i];
-          d[i] = fmaf(r2, b[i], d[i]);
-        }
+        mul(b, y);
+        fma(d, r2, b, d);
       }
     };
     each([&](int n, int64_t c) {
@@ -752,14 +793,12 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
       float(&u)[VEC] = unit[HOLD ? n : 0];
       float(&d)[VEC] = d0[HOLD ? n : 0];
       terms(n, c, g, z, u, d, b);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (!by_token) z[i] *= g[i];
-        v[0] = fmaf(b[i], u[i], v[0]);
-        v[1] = fmaf(z[i], d[i], v[1]);
-        v[2] = fmaf(z[i], u[i], v[2]);
-      }
+      if (!by_token) mul(z, g);
+      dot(pair[0], b, u);
+      dot(pair[1], z, d);
+      dot(pair[2], z, u);
     });
+    float v[3] = {pair[0].x + pair[0].y, pair[1].x + pair[1].y, pair[2].x + pair[2].y};
     group_sum(v, part[turn], tp);
     const float c2 = v[0] * inv_width * r2, zd = v[1] - c2 * v[2];
     const float c1 = (by_token ? p.scale * token * zd : zd) * inv_width;
@@ -772,21 +811,17 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
         float b[VEC];
         terms(n, c, g, z, u, d0[0], b);
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) d[i] = fmaf(-c2, u[i], d0[HOLD ? n : 0][i]);
+      fma(d, -c2, u, d0[HOLD ? n : 0]);
       if (p.dx) store_piece<T, SHIFT>(static_cast<T*>(p.dx) + t * p.width, c, phase, p.width, d);
       if (p.in_col >= 0) {
         float a[VEC];
         widen(yv[n], a);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) a[i] *= u[i];
+        mul(a, u);
         add(p.in_col, c, places, a);
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        z[i] *= p.scale * d[i];  // the gate's gradient
-        d[i] *= g[i];            // z's
-      }
+      mul(z, d);
+      mul(z, p.scale);  // the gate's gradient
+      mul(d, g);        // z's
       if (p.gate_col >= 0) add(p.gate_col, c, places, z);
       if (p.dgate && p.gate_kind == ES_GATE_FULL)
         store_piece<T, SHIFT>(static_cast<T*>(p.dgate) + t * p.width, c, phase, p.width, z);
@@ -794,16 +829,17 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_rows_kernel(const __gr
         float w[VEC], hat[VEC];
         cols.get(cols.w_out, c, places, w);
         widen(hv[n], hat);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) hat[i] *= r1;
+        mul(hat, r1);
         if (p.out_col >= 0) {
           float a[VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) a[i] = d[i] * hat[i];
+          for (int i = 0; i < VEC; ++i) a[i] = d[i];
+          mul(a, hat);
           add(p.out_col, c, places, a);
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) d[i] = r1 * fmaf(-hat[i], c1, d[i] * w[i]);
+        mul(d, w);
+        fma(d, -c1, hat, d);
+        mul(d, r1);
       }
       if (p.dh) store_piece<T, SHIFT>(static_cast<T*>(p.dh) + t * p.width, c, phase, p.width, d);
     });
