@@ -19,10 +19,10 @@
 // once. Column sums stay in shared memory over the rows of a group; each group writes its
 // part, and a second kernel adds the parts in their order, so that results repeat to the
 // bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 120 us
-// forward (537 MB, 4.5 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The forward pass is near memory's rate; the backward pass is
-// bound by its instructions, with half of the issue slots used: 16 warps an
-// SM is what its registers allow. Rows of odd length pay for values that lie at no fixed
-// place: 4099 x 5001 f16 81 us for 164 MB.
+// forward (537 MB, 4.5 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The
+// forward pass is near memory's rate; the backward pass is bound by its instructions, with
+// 58% of the issue slots used: 16 warps an SM is what its registers allow. Rows of odd
+// length pay for values that lie at no fixed place: 4099 x 5001 f16 81 us for 164 MB.
 #include <type_traits>
 
 #include "experts.cuh"
@@ -93,8 +93,8 @@ __device__ __forceinline__ void widen(const Vec<T, VEC>& p, float (&v)[VEC]) {
   }
 }
 
-// A piece's arithmetic, two values an instruction. Gradients of 16384 x 4096 bf16: 267 to 243 us, of
-// 65536 x 512: 121 to 110.
+// A piece's arithmetic, two values an instruction. Gradients of 16384 x 4096
+// bf16: 267 to 243 us, of 65536 x 512: 121 to 110.
 #define ES_PAIR(op, ...)                                                                             \
   asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t" op         \
       "mov.b64 {%0, %1}, c;\n\t}"                                                                   \

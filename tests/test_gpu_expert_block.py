@@ -183,3 +183,71 @@ def test_refusals():
         E.expert_mlp(p["x"], p["router"], i8[0], f8[1], 2)
     with pytest.raises(ValueError, match="activation"):
         E.expert_mlp(p["x"], p["router"], p["w_in"], p["w_out"], 2, activation="swish")
+
+
+def test_two_threads_and_streams():
+    """Two programs at once, each on a stream of its own: what each gets alone."""
+    import threading
+    g = gen(21)
+    sets = [params(g, T, 192, 160, 6, torch.bfloat16, True) for T in (700, 37)]
+    weights = [(E.quantize_block_weights(p["w_in"]), E.quantize_block_weights(p["w_out"])) for p in sets]
+    douts = [torch.ones_like(p["x"]) for p in sets]
+    for p in sets:
+        for t in p.values():
+            t.requires_grad_()
+
+    def step(i):
+        p = sets[i]
+        out = call(p, 2, "silu", 0.5)
+        grads = torch.autograd.grad(out, list(p.values()), douts[i])
+        with torch.no_grad():
+            served = E.expert_mlp(p["x"], p["router"], *weights[i], 3, norm_in=p["norm_in"], gate=p["gate"])
+        return (out.detach(), served, *grads)
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def program(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[i].append(step(i))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=program, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for i in (0, 1):
+        assert len(got[i]) == 8
+        for one in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(one, want[i]))
+    E.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_tensor_in_two_places(dtype):
+    """The stream itself as a block's output, one weight for both norms, and the gate: the gradients add up as those
+    of tensors of their own do."""
+    g = gen(23)
+    x, w = randn(g, 90, 136, dtype=dtype), (1 + randn(g, 136, scale=0.2)).to(dtype)
+    dout, dy = randn(g, 90, 136, dtype=dtype), randn(g, 90, 136, dtype=dtype)
+    apart = [t.clone().requires_grad_() for t in (x, x, w, w, x)]
+    out, y = E.residual_norm(*apart, scale=0.25)
+    d = torch.autograd.grad((out, y), apart, (dout, dy))
+    x.requires_grad_()
+    w.requires_grad_()
+    out2, y2 = E.residual_norm(x, x, w, w, x, scale=0.25)
+    dx, dw = torch.autograd.grad((out2, y2), (x, w), (dout, dy))
+    assert torch.equal(out, out2) and torch.equal(y, y2)
+    # two sums in the tensors' type, in whatever order: each is off by half a step of its result at most
+    size = d[0].double().abs() + d[1].double().abs() + d[4].double().abs()
+    unit = torch.finfo(dtype).eps / 2
+    assert bool(((dx.double() - (d[0].double() + d[1].double() + d[4].double())).abs() <= 2.01 * unit * size).all())
+    both = d[2].double() + d[3].double()
+    assert bool(((dw.double() - both).abs() <= 1.01 * unit * both.abs()).all())
