@@ -7,6 +7,8 @@
 // the type's 15 powers of two and round twice. A block with an infinity or NaN has scale
 // and values NaN. Rows: 128 consecutive values of a row (the last block may be
 // shorter). Weights: 128 x 128 of a matrix.
+// Bound by memory's latency and the conversions alike (B200: 8191 x 4096 bf16 22 us, 4.6 TB/s
+// with 72% of the issue slots; 16400 x 1408 with silu 27 us, 4.4 TB/s, 75%).
 #include <cuda_fp8.h>
 
 #include "activation.cuh"

@@ -18,11 +18,11 @@
 // registers (a group of threads a row, NP pieces of 16 bytes each) and every output written
 // once. Column sums stay in shared memory over the rows of a group; each group writes its
 // part, and a second kernel adds the parts in their order, so that results repeat to the
-// bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 120 us
-// forward (537 MB, 4.5 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The
+// bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 114 us
+// forward (537 MB, 4.7 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The
 // forward pass is near memory's rate; the backward pass is bound by its instructions, with
 // 58% of the issue slots used: 16 warps an SM is what its registers allow. Rows of odd
-// length pay for values that lie at no fixed place: 4099 x 5001 f16 81 us for 164 MB.
+// length pay for values that lie at no fixed place: 4099 x 5001 f16 72 us for 164 MB.
 #include <type_traits>
 
 #include "experts.cuh"
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(kMostThreads) norm_grad_kernel(const __grid_co
 // addresses' borders instead, value e of the row being value (e + phase) % VEC of its piece,
 // and only a row's first and last piece are read value by value. Weights and column sums
 // lie in shared memory with value e at [e % VEC][e / VEC], where no bank is met twice
-// whatever the phase (4099 x 5001 f16: 78 us value by value, see the launch below).
+// whatever the phase.
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -571,6 +571,8 @@ struct Columns {
 template <typename T, typename W, int NP, bool SHIFT>
 __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel(const __grid_constant__ NormArgs p) {
   constexpr int VEC = kVec<T>;
+  // a piece's number: 32 bits spare whole rows registers (16384 x 4096 bf16: 120 -> 114 us)
+  using Place = typename std::conditional<SHIFT, int64_t, int>::type;
   extern __shared__ __align__(16) uint8_t shared_columns[];
   __shared__ float part[2][4][1][32];
   const int tp = p.tp, c0 = threadIdx.x % tp, per = blockDim.x / tp;
@@ -583,7 +585,8 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
   for (int64_t t0 = blockIdx.x * static_cast<int64_t>(per); t0 < p.rows; t0 += step, t += step, turn ^= 1) {
     const bool live = t < p.rows;
     const int phase = SHIFT ? static_cast<int>(t * p.width % VEC) : 0;
-    const int64_t pieces = !live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC;
+    const int pieces =
+        static_cast<int>(!live ? 0 : SHIFT ? (p.width + phase + VEC - 1) / VEC : p.width / VEC);
     const Places<VEC, SHIFT> places(phase, cols.pitch);
     const T* x = static_cast<const T*>(p.x) + t * p.x_stride;
     const T* h = static_cast<const T*>(p.h) + t * p.h_stride;
@@ -592,17 +595,17 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
     auto each = [&](auto fn) {
 #pragma unroll
       for (int n = 0; n < NP; ++n)
-        if (c0 + n * tp < pieces) fn(n, static_cast<int64_t>(c0 + n * tp));
+        if (c0 + n * tp < pieces) fn(n, Place(c0 + n * tp));
     };
     Vec<T, VEC> xv[NP], hv[NP];
-    each([&](int n, int64_t c) {
+    each([&](int n, Place c) {
       if (p.h) hv[n] = load_piece<T, SHIFT>(h, c, phase, p.width);
       xv[n] = load_piece<T, SHIFT>(x, c, phase, p.width);
     });
     const float token = p.gate_kind == ES_GATE_TOKEN && live ? to_f32(gate[0]) : 1.0f;
     auto rms = [&](auto value, float (*buf)[32], float (*again)[32]) {  // value(slot, fp32 values)
       float2 pair = make_float2(0.0f, 0.0f);
-      each([&](int n, int64_t) {
+      each([&](int n, Place) {
         float v[VEC];
         value(n, v);
         dot(pair, v, v);
@@ -614,7 +617,7 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
       // CTA decide alike, for the barrier in it.
       if (per == 1 ? big : tp > 32 ? __syncthreads_or(big) : __any_sync(kAll, big)) {
         float small[1] = {0.0f};
-        each([&](int n, int64_t) {
+        each([&](int n, Place) {
           float v[VEC];
           value(n, v);
 #pragma unroll
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
     };
     float r1 = 1.0f, r2 = 1.0f, o[NP][VEC];
     if (p.w_out) r1 = rms([&](int n, float (&v)[VEC]) { widen(hv[n], v); }, part[turn][0], part[turn][1]);
-    each([&](int n, int64_t c) {
+    each([&](int n, Place c) {
       widen(xv[n], o[n]);
       if (p.h) {
         float z[VEC], g[VEC];
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
         }
         if (p.gate_kind == ES_GATE_CHANNEL) cols.get(cols.gate, c, places, g);
         if (p.gate_kind == ES_GATE_FULL) widen(load_piece<T, SHIFT>(gate, c, phase, p.width), g);
-        // One by one: in pairs the 64 registers spilled (16384 x 4096 bf16: 123 us for 120).
+        // One by one: in pairs the 64 registers spilled, and took 3% longer.
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[n][i] = fmaf(p.scale * g[i], z[i], o[n][i]);
       }
@@ -655,7 +658,7 @@ __global__ void __launch_bounds__(kMostThreads, NP > 2 ? 1 : 2) norm_rows_kernel
             for (int i = 0; i < VEC; ++i) v[i] = o[n][i];
           },
           part[turn][2], part[turn][3]);
-      each([&](int n, int64_t c) {
+      each([&](int n, Place c) {
         float w[VEC];
         cols.get(cols.w_in, c, places, w);
         mul(o[n], r2);
@@ -1002,7 +1005,14 @@ int forward(NormArgs& p, cudaStream_t s) {
   const Lie lie = lie_of(p, sizeof(T));
   const RowForm f = walked_form(lie == kPhase ? (p.width + 2 * VEC - 2) / VEC : p.width / VEC, p.rows);
   const size_t smem = lie == kPhase ? columns_bytes(p.width, VEC, array_bytes(p, sizeof(W), sizeof(T))) : 0;
-  if (f.np && lie != kAny && smem <= kMostColumnsSmem)
+  // Odd rows of 16 bits, two pieces a thread, that are added and normalised once after it:
+  // value by value 4099 x 5001 f16 is 72 us for 81 in shifted pieces, 13324 x 1501 68 for 80,
+  // 38387 x 521 87 for 126. With norm_out, or without h, neither is faster throughout (19980
+  // x 1001 95 for 83, 3332 x 6001 81 for 94); with a gate by channel (4099 x 5001 104 for 96),
+  // one of each value's (152 for 112) or fp32 (94 for 76) shifted pieces are.
+  const bool by_value = lie == kPhase && sizeof(T) == 2 && f.np == 2 && p.h && p.w_in && !p.w_out &&
+                        (p.gate_kind == ES_GATE_NONE || p.gate_kind == ES_GATE_TOKEN);
+  if (f.np && lie != kAny && !by_value && smem <= kMostColumnsSmem)
     return lie == kWhole ? forward_rows<T, W, false>(p, f, smem, s) : forward_rows<T, W, true>(p, f, smem, s);
   const RowForm r = lie == kWhole ? RowForm{kMostThreads, 0} : row_form(p.width, 16);
   p.tp = r.tp;
