@@ -350,3 +350,14 @@ def test_refusals():
         y = E.rms_norm(x.requires_grad_(), w)
         d, = torch.autograd.grad(y.sum(), x, create_graph=True)
         d.sum().backward()
+
+
+@pytest.mark.parametrize("D", [269, 521, 1501, 5001])
+@pytest.mark.parametrize("dtype", [t for t in TYPES if t != torch.float32])
+@pytest.mark.parametrize("gate", ["", "token", "channel"])
+def test_odd_rows_of_many(D, dtype, gate):
+    """Enough odd rows for two pieces a thread: without a gate by channel, the
+    forward pass walks them value by value, the backward pass by pieces."""
+    g = gen(D)
+    check(make(g, 601, D, dtype, gate, False, True), g=g)
+    check(make(g, 601, D, dtype, gate, False, True), grads=False)
