@@ -77,8 +77,8 @@ struct Fp8Ctl {
   uint64_t scale_empty[kScaleSlots];
   uint64_t red_full, red_empty;
   uint64_t drain;
-  int ends[kScaleSlots][2];  // whether a slot's rows (of either warp) have frames
-  int8_t frame[kScaleSlots][2][128];
+  int any_coarse[kScaleSlots][4];  // of 32 rows, whether one of them is coarse from this slot on
+  int8_t coarse[kScaleSlots][2][128];
   uint32_t tmem;
   int abort;
   uint32_t progress;
@@ -159,27 +159,32 @@ __device__ __forceinline__ void clear_rows(const Fp8Args& p, int64_t from, int64
   for (int64_t i = head + body * 8 + t; i < n; i += nt) a[i] = 0;
 }
 
-// Frames. The product of two scales may be past fp32's ends where the result is not. A
-// row's products of one slot of blocks are then made in a frame of their own, times
-// 2^-128 where one of them is infinite or 2^128 where all are tiny (below 2^-64, and one
-// below the normal numbers), and the row's totals follow it: a rare step between the slots
-// that costs the sums themselves nothing (two factors a value cost them a tenth).
-constexpr float kHalfFrame = 18446744073709551616.0f;  // 2^64
+// The product of two scales may be past fp32's ends where the result is not. Products and
+// totals are therefore held times 2^40: below the normal numbers they then lose at most
+// 2^-190 of the product and 2^-165 of a term, less than any result holds. A row that meets a
+// product of 2^36 or more (whose totals could overflow) goes on in coarse products and
+// totals, times 2^-40: its total is multiplied by 2^-80 once, between two slots, and terms
+// below 2^-85 may be lost beside such a product. No total is ever multiplied by more than
+// one, so what a row has summed stays what it is, whatever blocks come next (blocks of
+// zeros, which have the least scale, among them), and the sums themselves cost nothing more
+// (a second factor for every value cost them a tenth, a second loop for such slots 2.5%).
+constexpr float kHalfFine = 0x1p20f, kFine = 0x1p40f, kCoarse = 0x1p-40f, kLargest = 0x1p76f;
 
-__device__ __forceinline__ bool past_ends(float x, float w) {
-  const float s = fabsf(x * w);
-  return (s < FLT_MIN && x != 0.0f && w != 0.0f) || s == INFINITY;
+__device__ __forceinline__ float fine_product(float x, float w) {
+  return fabsf(x) < 1.0f ? (x * kFine) * w : x * (w * kFine);
 }
 
-// Totals from one frame to another.
+// Where even the coarse product is past the largest number every sum but zero has an
+// infinite term, as it has with the largest number; infinite scales stay infinite.
+__device__ __forceinline__ float coarse_product(float x, float w) {
+  const float s = fabsf(x) < 1.0f ? x * (w * kCoarse) : (x * kCoarse) * w;
+  return fabsf(s) == INFINITY && fabsf(x) < INFINITY && fabsf(w) < INFINITY ? copysignf(FLT_MAX, s) : s;
+}
+
 template <int COLS>
-__device__ __forceinline__ void change_frame(float (&total)[COLS], int from, int to) {
-  const float f = from > to ? kHalfFrame : from < to ? 1.0f / kHalfFrame : 1.0f;
-  for (int steps = 2 * abs(from - to); __any_sync(0xffffffffu, steps > 0); --steps) {
-    const float now = steps > 0 ? f : 1.0f;
+__device__ __forceinline__ void scale_totals(float (&total)[COLS], float f) {
 #pragma unroll
-    for (int i = 0; i < COLS; ++i) total[i] *= now;
-  }
+  for (int i = 0; i < COLS; ++i) total[i] *= f;
 }
 
 // The scale of block kb of the channels from col on (their block of 128; col may lie
@@ -497,57 +502,55 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           const int r = static_cast<int>(pair_rank) * 128 + row0 + i * 32 + lane;
           source[i] = r < at.rows ? static_cast<int>(p.g.source(at.row0 + r)) : -1;
         }
+        uint32_t coarse = 0;  // bit (s * 2 + half) * 8 + i: this lane's row is coarse
         for (int kb = at.kb0; kb < at.kb1; kb += kScalesAhead) {
           ok = tc_wait_warp<true>(&ctl.scale_empty[slot], slot_phase ^ 1, &ctl, p.status, true);
           if (!ok) break;
           const bool there = kb + b < at.kb1;
+          // either scale times 2^20: where that is past the largest number, the product is looked at again
           float w[BLOCKS];
 #pragma unroll
-          for (int s = 0; s < BLOCKS; ++s) w[s] = there ? *channel_scales(p, at.expert, at.col0 + s * 128, kb + b) : 0.0f;
-          bool ends = false;
+          for (int s = 0; s < BLOCKS; ++s)
+            w[s] = there ? *channel_scales(p, at.expert, at.col0 + s * 128, kb + b) * kHalfFine : 0.0f;
           float* to = scale_smem + (slot * kScalesAhead + b) * BLOCKS * kScalePitch + row0 + (lane >> 3);
           const float* from = p.g.x_scale + kb + b;
-          auto row_scale = [&](int i) {
-            const int r = __shfl_sync(0xffffffffu, i < 8 ? source[0] : source[1], (i & 7) * 4 + (lane >> 3));
-            return there && r >= 0 ? from[static_cast<int64_t>(r) * p.k_blocks] : 0.0f;
-          };
 #pragma unroll 1
-          for (int i0 = 0; i0 < 16; i0 += 8) {
+          for (int half = 0; half < 2; ++half, to += 32) {
+            auto row_scale = [&](int i) {
+              const int r = __shfl_sync(0xffffffffu, half ? source[1] : source[0], i * 4 + (lane >> 3));
+              return there && r >= 0 ? from[static_cast<int64_t>(r) * p.k_blocks] : 0.0f;
+            };
             float x[8];
+            bool any = coarse != 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = row_scale(i0 + i);
+            for (int i = 0; i < 8; ++i) x[i] = row_scale(i) * kHalfFine;
 #pragma unroll
             for (int s = 0; s < BLOCKS; ++s)
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                to[s * kScalePitch + (i0 + i) * 4] = x[i] * w[s];
-                ends |= past_ends(x[i], w[s]);
+                const float v = x[i] * w[s];
+                to[s * kScalePitch + i * 4] = v;
+                any |= !(fabsf(v) < kLargest);
               }
-          }
-          ends = __any_sync(0xffffffffu, ends);
-          if (ends) {
-            const uint32_t row = 0xffu << (lane & 24);
+            any = __any_sync(0xffffffffu, any);
+            if (any) {
+              const uint32_t row = 0xffu << (lane & 24);
 #pragma unroll 1
-            for (int i = 0; i < 16; ++i) {
-              const float x = row_scale(i);
-#pragma unroll
-              for (int s = 0; s < BLOCKS; ++s) {
-                const float v = fabsf(x * w[s]);
-                const bool over = __ballot_sync(0xffffffffu, v == INFINITY) & row;
-                const bool under = __ballot_sync(0xffffffffu, past_ends(x, w[s])) & row;
-                const bool large = __ballot_sync(0xffffffffu, !(v < 1.0f / kHalfFrame)) & row;
-                const int frame = over ? 1 : under && !large ? -1 : 0;
-                const float f = frame > 0 ? 1.0f / kHalfFrame : kHalfFrame;
-                if (frame) to[s * kScalePitch + i * 4] = (x * f) * (w[s] * f);
-                if (b == 0) ctl.frame[slot][s][row0 + (lane >> 3) + i * 4] = static_cast<int8_t>(frame);
+              for (int n = 0; n < 8 * BLOCKS; ++n) {
+                const int i = n & 7, s = n >> 3;
+                const uint32_t bit = 1u << ((s * 2 + half) * 8 + i);
+                const float xs = row_scale(i), ws = there ? *channel_scales(p, at.expert, at.col0 + s * 128, kb + b) : 0.0f;
+                const float v = fine_product(xs, ws);
+                const bool large = fabsf(v) >= kLargest && fabsf(xs) < INFINITY && fabsf(ws) < INFINITY;
+                if (__ballot_sync(0xffffffffu, large) & row) coarse |= bit;
+                to[s * kScalePitch + i * 4] = coarse & bit ? coarse_product(xs, ws) : v;
+                if (b == 0) ctl.coarse[slot][s][row0 + half * 32 + (lane >> 3) + i * 4] = (coarse & bit) != 0;
               }
             }
+            if (lane == 0) ctl.any_coarse[slot][(warp - 2) * 2 + half] = any;
           }
           __syncwarp();
-          if (lane == 0) {
-            ctl.ends[slot][warp - 2] = ends;
-            mbar_arrive(&ctl.scale_full[slot]);
-          }
+          if (lane == 0) mbar_arrive(&ctl.scale_full[slot]);
           if (++slot == kScaleSlots) {
             slot = 0;
             slot_phase ^= 1;
@@ -576,7 +579,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const Fp8Tile at = tiles.at(t, rank, csize);
       const int rows = at.rows - first, col0 = at.col0 + column;
       const bool any = rows > 0 && col0 < p.g.N;
-      int frame = 0;
+      bool coarse = false;
       float total[COLS];
 #pragma unroll
       for (int i = 0; i < COLS; ++i) total[i] = 0.0f;
@@ -585,11 +588,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if (!ok) break;
         const float* scales =
             scale_smem + (slot * kScalesAhead * BLOCKS + (column >> 7)) * kScalePitch + quad * 32 + lane;
-        int next = 0;
-        if (ctl.ends[slot][quad >> 1]) next = ctl.frame[slot][column >> 7][quad * 32 + lane];
-        if (__any_sync(0xffffffffu, next != frame)) {
-          change_frame(total, frame, next);
-          frame = next;
+        bool on = coarse;
+        if (ctl.any_coarse[slot][quad]) on = ctl.coarse[slot][column >> 7][quad * 32 + lane] != 0;
+        if (__any_sync(0xffffffffu, on != coarse)) {
+          scale_totals(total, on != coarse ? kCoarse * kCoarse : 1.0f);
+          coarse = on;
         }
         const int n = min(at.kb1 - kb0, kScalesAhead);
         for (int i = 0; i < n; ++i) {
@@ -635,7 +638,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       if (!ok) break;
-      if (__any_sync(0xffffffffu, frame != 0)) change_frame(total, frame, 0);
+      scale_totals(total, coarse ? kFine : kCoarse);
       if constexpr (S::SPLIT) {
         // every CTA puts its part into shared memory, [row][channel], and adds up every
         // csize-th piece of four channels, the parts in the CTAs' order

@@ -75,7 +75,9 @@ def fp8_matmul(q: torch.Tensor, scale: torch.Tensor, wq: torch.Tensor, wscale: t
 
     ``q`` e4m3 (rows, K) and ``scale`` float32 (rows, ceil(K / 128)) as from
     ``quantize_blocks``; ``wq`` e4m3 (N, K), ``wscale`` float32
-    (ceil(N / 128), ceil(K / 128)). Scales may be any float32 numbers. With a
+    (ceil(N / 128), ceil(K / 128)). Scales may be any float32 numbers (where a
+    row has a product of two scales of 2^36 or more, its terms below 2^-85 may
+    be lost). With a
     ``plan`` the products are grouped by expert as in ``grouped_matmul``:
     ``wq`` and ``wscale`` have a leading num_experts, and with ``gather`` ``q``
     and ``scale`` are by token. Returns (rows, N) of ``out_dtype`` (float32,

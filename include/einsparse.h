@@ -532,7 +532,8 @@ int es_quantize_blocks(const void* x, int dtype, int64_t num_rows, int64_t width
 int es_quantize_block_weights(const void* w, int dtype, int64_t matrices, int64_t N, int64_t K, uint8_t* q,
                               float* scale, void* stream);
 /* y[r, n] = sum_b x_scale[row(r), b] w_scale[e(r), n / 128, b] sum_{k in b} q[row(r), k] wq[e(r), n, k]
- * over the blocks b of the depth, in fp32, rounded once; any fp32 scales. wq:
+ * over the blocks b of the depth, in fp32, rounded once; any fp32 scales (where a
+ * row has a product of two scales of 2^36 or more, its terms below 2^-85 may be lost). wq:
  * (num_experts, N, K) with contiguous k, the scales contiguous. num_experts ==
  * 0: one matrix for all rows (offsets and order NULL). y (num_rows, N)
  * contiguous. */

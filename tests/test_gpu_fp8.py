@@ -385,3 +385,81 @@ def test_output_past_32_bits():
     ref = (q[-200:].double() * s[-200:].double()) @ (wq[1].double() * spread(ws[1], N, K)).t()
     mag = (q[-200:].double() * s[-200:].double()).abs() @ (wq[1].double() * spread(ws[1], N, K)).abs().t()
     check(y[-200:], ref, mag, K, torch.bfloat16)
+
+
+# What a row's blocks of depth hold, eight blocks (the kernel's unit) at a time: ordinary values; zeros with the least scale;
+# products of scales below fp32's normal numbers; above its largest, over zeros and over the smallest values.
+PLAIN, ZERO, TINY_SCALES, OVER_ZERO, OVER_SMALL = range(5)
+
+
+def mixed_rows(g, R, K, kinds):
+    """(q, scale) with rows that hold, from one eight blocks to the next, every order of ``kinds``."""
+    n = blocks(K)
+    kind = (torch.arange(R, device=DEV)[:, None] // len(kinds) ** torch.arange(-(-n // 8), device=DEV)) % len(kinds)
+    kind = torch.tensor(kinds, device=DEV)[kind].repeat_interleave(8, 1)[:, :n]
+    q, s = random8(g, R, n, 128).float(), scales(g, R, n)
+    small = torch.zeros_like(q)
+    small[..., 5] = 2.0 ** -9
+    q = torch.where((kind == PLAIN)[..., None] | (kind == TINY_SCALES)[..., None], q, 0.0)
+    q = torch.where((kind == OVER_SMALL)[..., None], small, q)
+    for k, v in ((ZERO, 2.0 ** -126), (TINY_SCALES, 2.0 ** -118), (OVER_ZERO, 3.0e38), (OVER_SMALL, 1.9 * 2.0 ** 107)):
+        s = torch.where(kind == k, v, s)
+    return q.reshape(R, n * 128)[:, :K].to(E4M3).contiguous(), s
+
+
+@pytest.mark.parametrize("R,K,N,path", [
+    (625, 2500, 10000, L.ES_GROUPED_WIDE), (125, 2304, 19000, L.ES_GROUPED_NARROW),
+    (25, 12100, 300, L.ES_GROUPED_SPLIT), (125, 2200, 9000, L.ES_GROUPED_SPLIT)])
+@pytest.mark.parametrize("kinds", [(PLAIN, ZERO, TINY_SCALES), (PLAIN, ZERO, OVER_ZERO),
+                                   (PLAIN, ZERO, TINY_SCALES, OVER_ZERO, OVER_SMALL)])
+def test_scales_change_along_the_depth(R, K, N, path, kinds):
+    """Blocks whose scales' products are past fp32's ends before, between and after ordinary ones: each counts as what it
+    is. Each block's term is within the usual few roundings of its magnitude, or within what it loses at fp32's lower end:
+    less than 2^-150, and beside a product of scales of 2^36 or more, which is held times 2^-40, half a unit of
+    2^(-149 + 40) times a sum of 128 products of up to 2^17.7, 2^-85.3."""
+    g = gen(K)
+    assert L.lib().es_fp8_matmul_path(0, K, N, R) == path
+    q, s = mixed_rows(g, R, K, kinds)
+    wq = random8(g, N, K).float().clamp(-16, 16).to(E4M3)
+    ws = torch.exp2(20.0 * torch.randint(-1, 2, (blocks(N), blocks(K)), generator=g, device=DEV)) \
+        * (1 + torch.rand(blocks(N), blocks(K), generator=g, device=DEV))
+    y = E.fp8_matmul(q, s, wq, ws, out_dtype=torch.float32)
+    ref, mag = product_ref(q, s, wq, ws)
+    assert float(ref.abs().max()) < torch.finfo(torch.float32).max / 2  # every result is a number
+    large = ((s.double()[:, None] * ws.double()).abs().amax(2) >= 2.0 ** 36).repeat_interleave(128, 1)[:, :N]
+    bound = UNIT[torch.float32] * ref.abs() + (128 + blocks(K) + 3) * 2.0 ** -23 * mag \
+        + blocks(K) * (2.0 ** -150 + 2.0 ** -85 * large)
+    assert bool(((y.double() - ref).abs() <= bound).all())
+    E.check_device_errors()
+
+
+@pytest.mark.parametrize("R", [3, 150, 700])
+@pytest.mark.parametrize("act", [None, "relu"])
+def test_quantized_blocks_of_zeros(R, act):
+    """Zeros in x or in w, as the rounding makes them, behind and before sums above one."""
+    g = gen(R)
+    K, N = 2048 + 128, 3000
+    x, w = randn(g, R, K if act is None else 2 * K, dtype=torch.bfloat16, scale=4.0), randn(g, K, N) * 0.02
+    x[: R // 2, 1024:K] = 0  # of gate, with an activation
+    x[R // 2:, :1024] = 0
+    w[1500:, :200] = 0
+    q, s = E.quantize_blocks(x, activation=act)
+    wq, ws = E.quantize_block_weights(w)
+    ref, mag = product_ref(q, s, wq, ws)
+    assert float(ref.abs().max()) > 4
+    check(E.fp8_matmul(q, s, wq, ws, out_dtype=torch.float32), ref, mag, K, torch.float32)
+
+
+@pytest.mark.parametrize("R", [40, 700])
+def test_a_row_has_its_bits_beside_any_others(R):
+    """A row's result does not depend on what scales the rows beside it have."""
+    g = gen(R + 1)
+    q, s, wq, ws = operands(g, R, 9000, 2200)
+    ws = ws.abs() + 0.001
+    y = E.fp8_matmul(q, s, wq, ws)
+    s2 = s.clone()
+    s2[1::2, 3::4] = 2.0 ** -126
+    s2[2::8, 5] = 3.0e38
+    z = E.fp8_matmul(q, s2, wq, ws)
+    same = (s == s2).all(1)
+    assert torch.equal(y[same], z[same])
