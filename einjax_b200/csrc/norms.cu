@@ -930,7 +930,9 @@ RowForm walked_form(int64_t pieces, int64_t rows) {
   return RowForm{kMostThreads, 0};
 }
 
-constexpr size_t kMostColumnsSmem = 200 * 1024;
+// Shared memory of the columns (dynamic): the most, and what a launch may have without a
+// raised limit, which counts a kernel's own 768 or 1024 bytes too.
+constexpr size_t kMostColumnsSmem = 200 * 1024, kFreeColumnsSmem = 47 * 1024;
 
 size_t columns_bytes(int64_t width, int vec, size_t bytes) {
   return static_cast<size_t>(vec) * (width / vec + 3) * bytes;
@@ -992,7 +994,7 @@ int forward_rows(NormArgs& p, const RowForm& f, size_t smem, cudaStream_t s) {
     constexpr int NP = decltype(np)::value;
     if constexpr (NP > 0) {
       static std::atomic<bool> raised[kMaxAttrDevices];
-      if (smem > 48 * 1024) ES_TRY(raise_smem(norm_rows_kernel<T, W, NP, SHIFT>, raised));
+      if (smem > kFreeColumnsSmem) ES_TRY(raise_smem(norm_rows_kernel<T, W, NP, SHIFT>, raised));
       ES_LAUNCH((norm_rows_kernel<T, W, NP, SHIFT>), blocks, f.threads(), smem, s, p);
     }
     return static_cast<int>(ES_OK);
@@ -1035,7 +1037,7 @@ int backward_rows(NormArgs& p, const RowForm& f, int64_t groups, size_t smem, cu
     constexpr int NP = decltype(np)::value;
     if constexpr (NP > 0) {
       static std::atomic<bool> raised[kMaxAttrDevices];
-      if (smem > 48 * 1024) ES_TRY(raise_smem(norm_grad_rows_kernel<T, W, NP, SHIFT>, raised));
+      if (smem > kFreeColumnsSmem) ES_TRY(raise_smem(norm_grad_rows_kernel<T, W, NP, SHIFT>, raised));
       ES_LAUNCH((norm_grad_rows_kernel<T, W, NP, SHIFT>), static_cast<unsigned>(groups / f.groups()), f.threads(),
                 smem, s, p);
     }

@@ -9,6 +9,9 @@ additions) are fewer than 16. So a value is off by at most ``steps(n) * 2^-24``
 of its terms' magnitudes."""
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -361,3 +364,20 @@ def test_odd_rows_of_many(D, dtype, gate):
     g = gen(D)
     check(make(g, 601, D, dtype, gate, False, True), g=g)
     check(make(g, 601, D, dtype, gate, False, True), grads=False)
+
+
+def test_sizes_at_the_shared_memory_limit():
+    """Rows whose columns take a little less than 48 KB, each the first call of its kernel in a process: bf16 gradients of
+    three and of two columns' sums, and odd rows forwards with their weights and gate in shared memory."""
+    code = ("import test_gpu_norms as t, torch\n"
+            "bf, f32 = torch.bfloat16, torch.float32\n"
+            "for T, D, dtype, gate, weights, grads in ((1000, 1000, bf, 'channel', None, True), (40, 4032, f32, 'channel',"
+            " None, True), (9, 6080, bf, '', f32, True), (5, 8101, bf, 'channel', None, False),"
+            " (5, 6101, bf, '', f32, False), (6, 4032, bf, 'channel', None, True)):\n"
+            "    g = t.gen(D)\n"
+            "    t.check(t.make(g, T, D, dtype, gate, True, True, weights=weights), grads=grads, g=g)\n"
+            "print('passed')\n")
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = {**os.environ, "PYTHONPATH": os.pathsep.join([here, os.path.dirname(here)])}
+    run = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=600)
+    assert run.returncode == 0 and "passed" in run.stdout, run.stdout[-2000:] + run.stderr[-2000:]
