@@ -1173,14 +1173,19 @@ extern "C" int es_residual_norm_grad(const void* x, int64_t x_stride, const void
   p.dh = dh;
   p.dgate = dgate;
   if (num_rows < 0 || width < 0) return ES_ERR_INVALID;
-  if (width == 0) return ES_OK;
+  cudaStream_t s = as_stream(stream);
+  if (width == 0) {  // a gate by token still has a value a row: a sum over no channels
+    if (dgate && gate_kind == ES_GATE_TOKEN && num_rows > 0 &&
+        cudaMemsetAsync(dgate, 0, num_rows * (dtype == ES_F32 ? 4 : 2), s) != cudaSuccess)
+      return ES_ERR_CUDA;
+    return ES_OK;
+  }
   if (num_rows > 0) {  // tensors without values have no addresses
     ES_TRY(check_norm(p, dtype, weight_dtype));
     if ((dy && !norm_in) || (dh && !h) || (dgate && !gate) || (dnorm_in && !norm_in) || (dnorm_out && !norm_out) ||
         !x || ((norm_out || dy) && !stats))
       return ES_ERR_INVALID;
   }
-  cudaStream_t s = as_stream(stream);
   SumArgs sums{};
   sums.width = width;
   p.in_col = p.out_col = p.gate_col = -1;

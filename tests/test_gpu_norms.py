@@ -381,3 +381,15 @@ def test_sizes_at_the_shared_memory_limit():
     env = {**os.environ, "PYTHONPATH": os.pathsep.join([here, os.path.dirname(here)])}
     run = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=600)
     assert run.returncode == 0 and "passed" in run.stdout, run.stdout[-2000:] + run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gate_by_token_of_no_channels(dtype):
+    """A row without channels leaves the gate's gradient a sum of nothing."""
+    T = 5
+    for fill in (math.nan, 3.0):  # memory that the allocator hands out again
+        torch.full((T, 1), fill, dtype=dtype, device=DEV)
+        x, gate = torch.zeros(T, 0, dtype=dtype, device=DEV), torch.ones(T, 1, dtype=dtype, device=DEV).requires_grad_()
+        out, _ = E.residual_norm(x, x, gate=gate)
+        dgate, = torch.autograd.grad(out, gate, torch.ones_like(out))
+        assert dgate.shape == (T, 1) and not dgate.any()
