@@ -1194,14 +1194,16 @@ extern "C" int es_residual_norm_grad(const void* x, int64_t x_stride, const void
     sums.out[sums.columns] = out;
     sums.dtype[sums.columns++] = type;
   };
-  if (dnorm_in) column(p.in_col, dnorm_in, weight_dtype);
+  if (dnorm_in && dy) column(p.in_col, dnorm_in, weight_dtype);
   if (dnorm_out) column(p.out_col, dnorm_out, weight_dtype);
   if (dgate && gate_kind == ES_GATE_CHANNEL) column(p.gate_col, dgate, dtype);
   p.columns = sums.columns;
+  auto clear = [&](void* out, int type) {
+    return cudaMemsetAsync(out, 0, width * (type == ES_F32 ? 4 : 2), s) == cudaSuccess ? ES_OK : ES_ERR_CUDA;
+  };
   if (num_rows == 0) {  // sums of nothing
-    for (int k = 0; k < sums.columns; ++k)
-      if (cudaMemsetAsync(sums.out[k], 0, width * (sums.dtype[k] == ES_F32 ? 4 : 2), s) != cudaSuccess)
-        return ES_ERR_CUDA;
+    for (int k = 0; k < sums.columns; ++k) ES_TRY(clear(sums.out[k], sums.dtype[k]));
+    if (dnorm_in && !dy) ES_TRY(clear(dnorm_in, weight_dtype));
     return ES_OK;
   }
   if (workspace_bytes < es_residual_norm_grad_workspace_size(
@@ -1210,6 +1212,7 @@ extern "C" int es_residual_norm_grad(const void* x, int64_t x_stride, const void
   if (p.columns && !workspace) return ES_ERR_WORKSPACE;
   p.part = static_cast<float*>(workspace);
   sums.part = p.part;
+  if (dnorm_in && !dy) ES_TRY(clear(dnorm_in, weight_dtype));  // no dy: zero, and no column sum
   ES_NORM_CALL(backward, p, sums, s);
   return ES_ERR_UNSUPPORTED;
 }

@@ -17,12 +17,14 @@ import pytest
 import torch
 
 import einjax_b200 as E
+from einjax_b200 import _lib as L
 from test_gpu_experts import TINY, TYPES, UNIT, gen, randn
 
 pytestmark = pytest.mark.gpu
 
 DEV = "cuda"
 NAMES = ("x", "h", "norm_in", "norm_out", "gate")
+L_CODE = {torch.float32: L.ES_F32, torch.bfloat16: L.ES_BF16, torch.float16: L.ES_F16}
 
 
 def steps(n):
@@ -393,3 +395,27 @@ def test_gate_by_token_of_no_channels(dtype):
         out, _ = E.residual_norm(x, x, gate=gate)
         dgate, = torch.autograd.grad(out, gate, torch.ones_like(out))
         assert dgate.shape == (T, 1) and not dgate.any()
+
+
+@pytest.mark.parametrize("D", [64, 1000, 77, 33000])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_entry_point_takes_no_dy_for_zero(D, dtype):
+    """A norm_in's gradient that is asked for without a dy is zero, and the others are as without it."""
+    lib, T = L.lib(), 30
+    g = gen(D)
+    x, h, w, dout = (randn(g, *s, dtype=dtype, scale=1e3) for s in ((T, D), (T, D), (D,), (T, D)))
+    code, stream = L_CODE[dtype], torch.cuda.current_stream().cuda_stream
+    out, y, stats = torch.empty_like(x), torch.empty_like(x), torch.empty(T, 2, device=DEV)
+    head = (x.data_ptr(), D, h.data_ptr(), D, code, T, D, w.data_ptr(), w.data_ptr(), code, None, L.ES_GATE_NONE, 0, 0.7)
+    assert lib.es_residual_norm(*head, 1e-6, out.data_ptr(), y.data_ptr(), stats.data_ptr(), stream) == L.ES_OK
+    nbytes = lib.es_residual_norm_grad_workspace_size(code, T, D, 2)
+    got = []
+    for asked in (False, True):
+        ws = torch.full((nbytes,), 255, dtype=torch.uint8, device=DEV)  # NaN
+        dx, dh, dw_in, dw_out = (torch.full_like(t, math.nan) for t in (x, h, w, w))
+        assert lib.es_residual_norm_grad(*head, stats.data_ptr(), dout.data_ptr(), D, None, 0, dx.data_ptr(),
+                                         dh.data_ptr(), None, dw_in.data_ptr() if asked else None, dw_out.data_ptr(),
+                                         ws.data_ptr(), nbytes, stream) == L.ES_OK
+        got.append((dx, dh, dw_out))
+        assert not asked or not bool(dw_in.any())
+    assert all(torch.equal(a, b) and not bool(a.isnan().any()) for a, b in zip(*got))
