@@ -75,6 +75,12 @@ def _no_tangent(fn: str, *tensors):
         raise NotImplementedError(f"{fn}: no forward-mode derivative; gradients are reverse-mode only")
 
 
+def _number(fn: str, name: str, v):
+    """Raises for a tensor in a number's place whose gradient would be lost."""
+    if isinstance(v, torch.Tensor) and v.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{fn}: {name} is a number and has no gradient; a gate has one")
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` (2-D) with a contiguous last dimension and rows that do not overlap."""
     if t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
@@ -566,6 +572,7 @@ def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, r
         raise TypeError(f"expert_mlp: w_in is {kind}, w_out is {w_out[0].dtype}")
     if activation is not None and kind == torch.int8:
         raise ValueError("expert_mlp: the layer in 8-bit integers has silu alone, activation must be None")
+    _number("expert_mlp", "scale", scale)
     args = (x, router, w_in, w_out, top_k, renormalize, kind, activation, norm_in, norm_out, gate, scale, eps)
     if not quantized:
         return _block(*args)

@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib as L
-from .experts import _DTYPES, _call, _code, _empty, _no_tangent, _on_gpu, _ptr, _rows, _scratch, _together
+from .experts import _DTYPES, _call, _code, _empty, _no_tangent, _number, _on_gpu, _ptr, _rows, _scratch, _together
 
 MIN_EPS = 1e-30
 
@@ -114,6 +114,7 @@ def _run(fn, x, h, norm_in, norm_out, gate, scale, eps):
     T, D = x.shape
     if h is not None and (h.shape != x.shape or h.dtype != x.dtype):
         raise ValueError(f"{fn}: h is {h.dtype} {tuple(h.shape)}, x is {x.dtype} {tuple(x.shape)}")
+    _number(fn, "scale", scale)
     scale, eps = float(scale), float(eps)
     if not MIN_EPS <= eps < math.inf:
         raise ValueError(f"{fn}: eps={eps} is not in [{MIN_EPS}, inf)")
@@ -161,7 +162,7 @@ def residual_norm(x: torch.Tensor, h: torch.Tensor, norm_in: torch.Tensor | None
     None. The norms' weights (width,) have x's type or float32, both the
     same. ``gate`` of x's type: one value a channel (width,), a token
     (num_tokens, 1), or each value's own (num_tokens, width). ``eps`` is at
-    least 1e-30. fp32 throughout, each output rounded once; rows whose squares pass the
+    least 1e-30. ``scale`` and ``eps`` are numbers and have no gradient. fp32 throughout, each output rounded once; rows whose squares pass the
     largest value are normalised all the same. Differentiable in every
     tensor; sums over tokens repeat to the bit."""
     if h is None:

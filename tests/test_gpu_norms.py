@@ -419,3 +419,19 @@ def test_entry_point_takes_no_dy_for_zero(D, dtype):
         got.append((dx, dh, dw_out))
         assert not asked or not bool(dw_in.any())
     assert all(torch.equal(a, b) and not bool(a.isnan().any()) for a, b in zip(*got))
+
+
+def test_scale_that_wants_a_gradient():
+    """The residual's scale is a number. A tensor that wants a gradient would lose it."""
+    x, w = torch.ones(4, 8, device=DEV), torch.ones(8, device=DEV)
+    s = torch.tensor(0.5, device=DEV, requires_grad=True)
+    with pytest.raises(TypeError, match="scale"):
+        E.residual_norm(x, x, w, scale=s)
+    router, w_in, w_out = torch.zeros(8, 2, device=DEV), torch.zeros(2, 8, 16, device=DEV), torch.zeros(2, 8, 8, device=DEV)
+    with pytest.raises(TypeError, match="scale"):
+        E.expert_mlp(x, router, w_in, w_out, 1, activation="silu", scale=s)
+    with pytest.raises(TypeError, match="scale"):
+        E.expert_mlp(x, router, E.quantize_block_weights(w_in), E.quantize_block_weights(w_out), 1, scale=s)
+    with torch.no_grad():
+        out = E.residual_norm(x, x, scale=s)[0]
+    assert torch.equal(out, E.residual_norm(x, x, scale=0.5)[0])
