@@ -251,3 +251,46 @@ def test_one_tensor_in_two_places(dtype):
     assert bool(((dx.double() - (d[0].double() + d[1].double() + d[4].double())).abs() <= 2.01 * unit * size).all())
     both = d[2].double() + d[3].double()
     assert bool(((dw.double() - both).abs() <= 1.01 * unit * both.abs()).all())
+
+
+def routed_ref(p, experts, act, scale, eps):
+    """The block in 64 bits for a routing that is given, differentiable."""
+    x = p["x"]
+    n = rms(x, p["norm_in"], eps)
+    weights = torch.softmax((n @ p["router"]).gather(1, experts), 1)
+    y = torch.zeros_like(x)
+    F = p["w_out"].shape[1]
+    for e in range(p["w_in"].shape[0]):
+        for j in range(experts.shape[1]):
+            at = (experts[:, j] == e).nonzero()[:, 0]
+            h = n[at] @ p["w_in"][e]
+            y = y.index_add(0, at, weights[at, j, None] * ((_Act.apply(h[:, :F], act) * h[:, F:]) @ p["w_out"][e]))
+    return x + scale * p["gate"] * rms(y, p["norm_out"], eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
+def test_training_16_bits_as_routed(dtype, act):
+    """Gradients of a step against the formulas' for the routing that the layer itself took, so that what is left are
+    roundings: of the normalised input, the hidden rows, the experts' rows, their sum and the result, and backwards of
+    the same and of the hidden rows' two halves. Each is at most a unit of its values, in the norm a unit over the square
+    root of three; a dozen in a chain, were all of them alike, are 12 / sqrt(3) = 7 units. relu's derivative jumps: the
+    normalised input's rounding moves a gate of spread s by d, 0.8 s u / sqrt(3) in the mean, and one in d / (s sqrt(2 pi))
+    = 0.18 u of them changes sides of zero, 0.37 u of the half that counts; whole values come or go, so in the norm of the
+    gate's gradient sqrt(0.37 u), whatever else is exact."""
+    g = gen(len(act))
+    p = params(g, 700, 128, 192, 4, dtype, True)
+    for t in p.values():
+        t.requires_grad_()
+    out = call(p, 2, act, 0.5)
+    dout = randn(g, 700, 128, dtype=dtype)
+    got = torch.autograd.grad(out, list(p.values()), dout)
+    with torch.no_grad():
+        experts = E.route_experts(E.rms_norm(p["x"], p["norm_in"]).float() @ p["router"].float(), 2)[1].long()
+    q = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    ref = routed_ref(q, experts, act, 0.5, 1e-6)
+    want = torch.autograd.grad(ref, list(q.values()), dout.double())
+    unit = torch.finfo(dtype).eps / 2
+    for name, a, b in zip(("out", *p), (out.detach(), *got), (ref.detach(), *want)):
+        off = float((a.double() - b).norm() / b.norm())
+        assert off <= 8 * unit + (math.sqrt(0.37 * unit) if act == "relu" else 0.0), (name, off / unit)
