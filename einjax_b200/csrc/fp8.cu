@@ -8,7 +8,10 @@
 // and values NaN. Rows: 128 consecutive values of a row (the last block may be
 // shorter). Weights: 128 x 128 of a matrix.
 // Bound by memory's latency and the conversions alike (B200: 8191 x 4096 bf16 22 us, 4.6 TB/s
-// with 72% of the issue slots; 16400 x 1408 with silu 27 us, 4.4 TB/s, 75%).
+// with 72% of the issue slots; 16400 x 1408 with silu 27 us, 4.4 TB/s, 75%): a thread has
+// the eight values of one block (sixteen with an activation) in flight and no other load.
+// Weights are rounded once: 4096 x 8192 bf16 60 us where they lie along K, 196 us with the
+// transposing copy before it.
 #include <cuda_fp8.h>
 
 #include "activation.cuh"

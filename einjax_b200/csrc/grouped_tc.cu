@@ -414,7 +414,8 @@ __device__ __forceinline__ void gated_block(const TcArgs& p, float (&g)[32], con
   float s[32];
   if (p.activation == ES_ACT_GELU) {
     // rolled, through local memory: 32 times erfc's code keeps the compiler from holding
-    // the other activations' values in registers
+    // the other activations' values in registers (8192 x 4096 x 8192 bf16 1032 us, with silu
+    // 852; 69 rows of 60 experts of 2048 x 1408 153 and 123)
     float a[32], d[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) a[i] = g[i];
@@ -1300,7 +1301,10 @@ int grouped_rows_tc(const GroupedArgs& g, int dtype, const void* x, const void* 
 
 namespace {
 
-// Operands of a gated product: those of the rows' product with the gate, and up.
+// Operands of a gated product: those of the rows' product with the gate, and up. Where F is
+// no multiple of 8, up starts at an address that TMA does not take and is copied in every
+// call, and the gate too where the rows are not: 69 rows of 60 experts, K 2048, F 1408, 1404,
+// 1401: 123, 335, 524 us.
 struct GatedOperands {
   RowsOperands gate;
   Operand up;

@@ -19,10 +19,20 @@
 // once. Column sums stay in shared memory over the rows of a group; each group writes its
 // part, and a second kernel adds the parts in their order, so that results repeat to the
 // bit. Measured on a B200: 16384 x 4096 bf16, both norms and a gate by channel, 114 us
-// forward (537 MB, 4.7 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). The
-// forward pass is near memory's rate; the backward pass is bound by its instructions, with
-// 58% of the issue slots used: 16 warps an SM is what its registers allow. Rows of odd
-// length pay for values that lie at no fixed place: 4099 x 5001 f16 72 us for 164 MB.
+// forward (537 MB, 4.7 TB/s) and 243 us for all of the gradients (805 MB, 3.3 TB/s). Neither
+// memory (6.55 TB/s) nor the issue slots (62% and 58% used) are what bounds them: it is
+// latency that the warps do not cover. Forwards 29 warps an SM wait for the row's loads
+// (a quarter of a warp's cycles), backwards the 16 that registers and column sums allow
+// wait for shared memory (a fifth; its pipe is 68% busy) and for each instruction's own
+// latency (a fifth).
+// Rows of odd length pay for values that lie at no fixed place, and for spills: 4099 x 5001
+// f16 72 us for 164 MB, all gradients with norm_out and a gate by channel 306 us, bf16 243.
+// Spilled bytes (stores / loads of a thread): shifted rows of two pieces forwards f16 220 /
+// 276, bf16 96 / 116 (at the 64 registers of two CTAs an SM), backwards f16 264 / 248, bf16
+// 64 / 76, of four pieces backwards f16 634 / 1044, bf16 192 / 436; whole rows of two pieces
+// forwards f16 56 / 80, bf16 28 / 36. How much of the time is theirs was not measured.
+// Rows longer than 2048 pieces are read again for each step, and their column sums stay in
+// global memory: 2048 x 32768 bf16 192 us forward and 1251 us backward.
 #include <type_traits>
 
 #include "experts.cuh"
@@ -188,6 +198,8 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float (*part)[32], int 
 
 constexpr float kDown = 2.6469779601696886e-23f;  // 2^-75: squares of the largest values, 2^16 of them and more, are finite
 
+// rsqrtf is off by up to 2 units of fp32 and the width's reciprocal by half of one: fp32
+// outputs and gradients are 1.7e-7 off in the norm, torch's elementary operations 1.5e-7.
 __device__ __forceinline__ float inv_rms(float sum, float inv_width, float eps) {
   return rsqrtf(fmaf(sum, inv_width, eps));
 }

@@ -10,7 +10,7 @@ namespace es {
 constexpr uint64_t kTcWaitNs = 2000000000ull;
 constexpr uint64_t kTcDrainNs = 100000000ull;
 
-enum { kKindF16 = 0, kKindI8 = 1, kKindF8 = 2 };
+enum { kKindF16 = 0, kKindI8 = 1 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -194,8 +194,6 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
                : "memory")
   if constexpr (CG == 2 && KIND == kKindF16) ES_MMA(2, f16);
   if constexpr (CG == 2 && KIND == kKindI8) ES_MMA(2, i8);
-  if constexpr (CG == 2 && KIND == kKindF8) ES_MMA(2, f8f6f4);
-  if constexpr (CG == 1 && KIND == kKindF8) ES_MMA(1, f8f6f4);
   if constexpr (CG == 1 && KIND == kKindF16) ES_MMA(1, f16);
   if constexpr (CG == 1 && KIND == kKindI8) ES_MMA(1, i8);
 #undef ES_MMA

@@ -557,8 +557,11 @@ def expert_mlp(x: torch.Tensor, router: torch.Tensor, w_in, w_out, top_k: int, r
     ``quantize_block_weights``, where a gradient through the result raises.
 
     ``activation`` names one of ``gated_matmul``'s. With tensors the gate, its
-    activation and up are then one kernel, rounded once; without it the two
-    products are rounded to x's type before silu. 8-bit integers have silu alone.
+    activation and up are then one kernel, rounded once and faster; without it
+    the two products are rounded to x's type before silu. 8-bit integers have
+    silu alone. In 8-bit floating point gate and up are rounded to x's type
+    between the first product and the activation, whose product is then
+    rounded to 8 bits.
 
     The layer as a block of a network: ``norm_in`` (D,) normalises its input
     (``rms_norm``). With any of ``norm_out`` (D,), ``gate`` and ``scale`` the

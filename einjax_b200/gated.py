@@ -75,7 +75,8 @@ def gated_matmul(x: torch.Tensor, w: torch.Tensor, plan: ExpertPlan | None = Non
     (by erf), ``"gelu_tanh"`` or ``"relu"``. Returns (rows, F) of x's type
     (float32, bfloat16, float16); rows of no expert are zero. Differentiable
     in ``x`` and ``w``; a training step keeps the output's slopes in both
-    products, (rows, 2 F) float32."""
+    products, (rows, 2 F) float32, 8 F bytes a row. F a multiple of 8 (16
+    bits) is fastest: else half of the weights or all are copied in every call."""
     if plan is not None and not isinstance(plan, ExpertPlan):
         raise TypeError(f"gated_matmul: plan must be an ExpertPlan or None, got {type(plan).__name__}")
     if not _together(x, w, x if plan is None else plan.offsets):
