@@ -428,7 +428,7 @@ def test_scales_change_along_the_depth(R, K, N, path, kinds):
     assert float(ref.abs().max()) < torch.finfo(torch.float32).max / 2  # every result is a number
     large = ((s.double()[:, None] * ws.double()).abs().amax(2) >= 2.0 ** 36).repeat_interleave(128, 1)[:, :N]
     bound = UNIT[torch.float32] * ref.abs() + (128 + blocks(K) + 3) * 2.0 ** -23 * mag \
-        + blocks(K) * (2.0 ** -150 + 2.0 ** -85 * large)
+        + blocks(K) * (2.0 ** -150 + 2.0 ** -85 * large.double())
     assert bool(((y.double() - ref).abs() <= bound).all())
     E.check_device_errors()
 
